@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 _LIB_PATH = Path(__file__).resolve().parent / "libasterq.so"
@@ -71,6 +72,11 @@ EXPORTED_SYMBOLS = (
     "asterq_plan_scratch_bytes",
     "asterq_plan_batch",
     "asterq_batch_append",
+    "asterq_kv_append",
+    "asterq_paged_attention_workspace_bytes",
+    "asterq_paged_attention",
+    "asterq_linear_workspace_bytes",
+    "asterq_linear_attention",
 )
 
 
@@ -162,6 +168,120 @@ class PlanBuffers(ctypes.Structure):
     ]
 
 
+class KvAppendParams(ctypes.Structure):
+    """Mirror of ``asterq_kv_append_params``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("n_seqs", ctypes.c_int32),
+        ("n_heads", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("page_tokens", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("n_rows", ctypes.c_int64),
+        ("n_pages", ctypes.c_int64),
+        ("n_positions", ctypes.c_int64),
+        ("q_row_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("k_row_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("v_row_stride", ctypes.c_int64),
+        ("v_head_stride", ctypes.c_int64),
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("cos", ctypes.c_void_p),
+        ("sin", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("row_offsets", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("k_pool", ctypes.c_void_p),
+        ("v_pool", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class PagedAttentionParams(ctypes.Structure):
+    """Mirror of ``asterq_paged_attention_params``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("n_rows", ctypes.c_int32),
+        ("n_heads", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_tokens", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("n_new", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("sink", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float),
+        ("logit_softcap", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("n_pages", ctypes.c_int64),
+        ("q_row_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("q", ctypes.c_void_p),
+        ("k_pool", ctypes.c_void_p),
+        ("v_pool", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class LinearParams(ctypes.Structure):
+    """Mirror of ``asterq_linear_params``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("n_seqs", ctypes.c_int32),
+        ("n_heads", ctypes.c_int32),
+        ("dk", ctypes.c_int32),
+        ("dv", ctypes.c_int32),
+        ("n_slots", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("n_rows", ctypes.c_int64),
+        ("q_row_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("k_row_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("v_row_stride", ctypes.c_int64),
+        ("v_head_stride", ctypes.c_int64),
+        ("decay_row_stride", ctypes.c_int64),
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("log_decay", ctypes.c_void_p),
+        ("state", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("row_offsets", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+def packer(cls) -> struct.Struct:
+    """A ``struct.Struct`` with the layout of a mirror: packing all fields of a call at once costs a
+    fraction of setting them one by one."""
+    codes = {ctypes.c_int32: "i", ctypes.c_int64: "q", ctypes.c_float: "f", ctypes.c_void_p: "P"}
+    return struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_))
+
+
 class AsterqError(RuntimeError):
     """A failed ``asterq_*`` call (status and message from ``asterq_last_error``)."""
 
@@ -234,6 +354,16 @@ def load() -> ctypes.CDLL:
     lib.asterq_plan_batch.argtypes = [ctypes.POINTER(BatchDesc), ctypes.POINTER(PlanBuffers), vp]
     lib.asterq_batch_append.restype = ctypes.c_int
     lib.asterq_batch_append.argtypes = [ctypes.POINTER(BatchDesc), vp, vp, vp, i64, vp, vp, i64, vp, vp]
+    lib.asterq_kv_append.restype = ctypes.c_int
+    lib.asterq_kv_append.argtypes = [vp, vp]  # the parameter struct as packed bytes or byref
+    lib.asterq_paged_attention_workspace_bytes.restype = i64
+    lib.asterq_paged_attention_workspace_bytes.argtypes = [vp]
+    lib.asterq_paged_attention.restype = ctypes.c_int
+    lib.asterq_paged_attention.argtypes = [vp, vp]
+    lib.asterq_linear_workspace_bytes.restype = i64
+    lib.asterq_linear_workspace_bytes.argtypes = [vp]
+    lib.asterq_linear_attention.restype = ctypes.c_int
+    lib.asterq_linear_attention.argtypes = [vp, vp]
     _lib = lib
     return lib
 

@@ -1,0 +1,754 @@
+// Attention of one new token a sequence over a paged grouped-query cache (sm_100a).
+//
+//   out[b, h] = sum_t softmax_t(score) v_t,  score = scale q[b, h] . k_t, softcapped where asked,
+//   over the visible tokens t < L and (t < sink or t >= L - (window - sink)),
+//   with L = lengths[b] + n_new; lse[b, h] = log sum_t exp(score).
+//
+// What bounds it: the visible keys and values are read once (4 Hkv D bytes a token) for 4 H D
+// operations, so H / Hkv operations a byte: memory.  Everything below serves keeping bytes in
+// flight: one persistent CTA per SM, a producer warp that streams 64-token tiles of keys and values
+// into a ring of shared memory by TMA, across the borders of its work, and consumer warps that never
+// wait for one another inside a sequence.
+//
+// Split.  The tiles of all (sequence, kv head, row block) units, laid end to end, are cut into equal
+// contiguous shares, one per CTA, by a prefix sum over `lengths` that every CTA computes for itself:
+// no planning launch, no host copy of the lengths, and a long sequence and a ragged batch are both
+// even to a tile.  A unit that lies in one share is finished there.  A cut unit leaves (o, m, l)
+// records in the workspace, and the CTA that stores its last one joins them, in the order of the
+// shares, so results do not depend on which CTA came last.  No CTA waits for another.
+#include <cuda.h>
+
+#include "asterq_internal.h"
+#include "common.cuh"
+
+namespace asterq {
+namespace pat {
+
+constexpr int kMaxWorkers = 256;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.693147180559945309417f;
+
+struct Args {
+  const void* q;
+  const int* page_table;
+  const int* lengths;
+  void* out;
+  float* lse;
+  float* records;  // o [2 W][NR][D], then m [2 W][NR], then l [2 W][NR]
+  int* counters;   // [2 W], zero between calls
+  int* status;
+  long long q_row_stride, q_head_stride, n_pages, capacity;  // capacity: tokens a row of the table can hold
+  int n_rows, n_heads, n_kv_heads, group, row_blocks;
+  int page_tokens, max_pages, box_rows, n_new, window, sink, out_f32;
+  float scale, softcap, cap_in;  // cap_in: 2 log2(e) scale / softcap
+};
+
+// D: head dim.  NR: query rows of a block (the query heads of one kv head, in eights).
+template <bool kF16_, int D_, int NR_>
+struct Cfg {
+  static constexpr bool kF16 = kF16_;
+  static constexpr int D = D_, NR = NR_, NT = NR_ / 8;
+  // A warp takes 16 tokens of a tile.  Two teams of warps take alternate tiles, so one team's
+  // softmax runs beside the other's products.  256-wide heads use 32-token tiles: the stage keeps
+  // its 32 KB and the ring its depth.
+  static constexpr int kTile = D == 256 ? 32 : 64;
+  static constexpr int kTeamWarps = kTile / 16, kWarps = 2 * kTeamWarps, kThreads = 32 * kWarps + 32;
+  static constexpr int kColBoxes = D / 64;
+  static constexpr int kHalfBytes = kTile * D * 2, kStageBytes = 2 * kHalfBytes;
+  // an even count, so that a stage and its barrier always serve the same team
+  static constexpr int kStages = D == 64 ? 12 : 6;
+  static constexpr int kSlice = NR == 16 ? 32 : 64, kPad = kSlice + 4;  // dims joined at a time
+  static constexpr int kMergeFloats = kWarps * NR * kPad > kMaxWorkers * NR ? kWarps * NR * kPad : kMaxWorkers * NR;
+  static constexpr int kSmem = 1024 + kStages * kStageBytes + (kMergeFloats + 2 * kWarps * NR) * 4 + 256;
+};
+
+ASTERQ_DEVICE void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+// the transpose of an 8 x 8 matrix of 16-bit values held as MMA fragments
+ASTERQ_DEVICE uint32_t transpose8(uint32_t x) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+  return d;
+}
+
+// The visible tiles of one sequence.  Tile k of its list is tokens [kTile j, kTile (j + 1)) with
+// j = k below sink_tiles and first + k - sink_tiles from there on.
+struct Span {
+  int length, sink, from, sink_tiles, first, tiles;
+  ASTERQ_DEVICE int tile(int k) const { return k < sink_tiles ? k : first + (k - sink_tiles); }
+  ASTERQ_DEVICE bool visible(int t) const { return t < length && (t < sink || t >= from); }
+};
+template <int kTile>
+ASTERQ_DEVICE Span span_of(const Args& a, int row) {
+  Span s;
+  const int n = __ldg(a.lengths + row);
+  long long want = n < 0 ? 0 : (long long)n + a.n_new;
+  s.length = (int)min(want, a.capacity);
+  s.sink = 0;
+  s.from = 0;
+  s.sink_tiles = 0;
+  s.first = 0;
+  const int last = (s.length + kTile - 1) / kTile;
+  if (a.window > 0 && s.length > a.window) {
+    s.sink = min(a.sink, a.window);
+    s.from = s.length - (a.window - s.sink);
+    s.sink_tiles = (s.sink + kTile - 1) / kTile;
+    s.first = s.from >= s.length ? last : max(s.from / kTile, s.sink_tiles);
+  }
+  s.tiles = s.sink_tiles + max(0, last - s.first);
+  return s;
+}
+
+// One CTA's share [x, end) of all tiles, walked unit by unit; every warp walks it for itself.
+template <int kTile>
+struct Walk {
+  long long x, end, row_start;
+  int row;
+  Span span;
+  // of the current piece
+  int unit, k0, n;          // unit within the row, its first tile here, tiles here
+  long long unit_start;
+  template <class A>
+  ASTERQ_DEVICE bool next(const A& a, int units_per_row) {
+    if (x >= end) return false;
+    while (x >= row_start + (long long)span.tiles * units_per_row) {
+      row_start += (long long)span.tiles * units_per_row;
+      span = span_of<kTile>(a, ++row);
+    }
+    const long long in_row = x - row_start;
+    unit = (int)(in_row / span.tiles);
+    unit_start = row_start + (long long)unit * span.tiles;
+    k0 = (int)(x - unit_start);
+    n = (int)min((long long)(span.tiles - k0), end - x);
+    x += n;
+    return true;
+  }
+};
+
+struct Start {
+  long long row_start, total;
+  int row;
+};
+
+template <class C>
+__global__ void __launch_bounds__(C::kThreads, 1)
+    attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                     const __grid_constant__ Args a) {
+  constexpr int D = C::D, NR = C::NR, NT = C::NT, kTile = C::kTile;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* merge = reinterpret_cast<float*>(smem + C::kStages * C::kStageBytes);
+  float* warp_m = merge + C::kMergeFloats;
+  float* warp_l = warp_m + C::kWarps * NR;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(warp_l + C::kWarps * NR);
+  __shared__ Start start_s;
+  __shared__ long long scan_s[32];
+  __shared__ int abort_s, last_s;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * C::kStages;
+  const int units_per_row = a.n_kv_heads * a.row_blocks;
+
+  if (tid == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(full0 + 8 * i, 1);
+      mbar_init(empty0 + 8 * i, C::kTeamWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    abort_s = 0;
+  }
+
+  // The share: thread t sums the tiles of rows [t R, (t + 1) R), the block scans the sums.
+  const int strip = (a.n_rows + C::kThreads - 1) / C::kThreads;
+  const int r0 = min(tid * strip, a.n_rows), r1 = min(r0 + strip, a.n_rows);
+  long long sum = 0;
+  for (int r = r0; r < r1; ++r) sum += span_of<kTile>(a, r).tiles;
+  sum *= units_per_row;
+  long long scan = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const long long up = __shfl_up_sync(0xffffffffu, scan, d);
+    if (lane >= d) scan += up;
+  }
+  if (lane == 31) scan_s[warp] = scan;
+  __syncthreads();
+  long long before = scan - sum, total = 0;
+  for (int w = 0; w <= C::kWarps; ++w) {
+    if (w < warp) before += scan_s[w];
+    total += scan_s[w];
+  }
+  const int W = (int)min((long long)gridDim.x, max(total, 1ll)), me = blockIdx.x;
+  Walk<kTile> walk;
+  walk.x = total * me / W;
+  walk.end = me < W ? total * (me + 1) / W : walk.x;
+  if (walk.x < walk.end && before <= walk.x && walk.x < before + sum) {
+    Start s;
+    s.row = r0;
+    s.row_start = before;
+    while (true) {
+      const long long here = (long long)span_of<kTile>(a, s.row).tiles * units_per_row;
+      if (walk.x < s.row_start + here) break;
+      s.row_start += here;
+      ++s.row;
+    }
+    start_s = s;
+  }
+  // rows that see nothing: zeros, and a log-sum of -inf
+  for (int r = me; r < a.n_rows; r += gridDim.x) {
+    if (span_of<kTile>(a, r).tiles > 0) continue;
+    for (int i = tid; i < a.n_heads * D; i += C::kThreads) {
+      const long long at = (long long)r * a.n_heads * D + i;
+      if (a.out_f32) static_cast<float*>(a.out)[at] = 0.0f;
+      else static_cast<uint16_t*>(a.out)[at] = 0;
+    }
+    if (a.lse)
+      for (int i = tid; i < a.n_heads; i += C::kThreads) a.lse[(long long)r * a.n_heads + i] = -INFINITY;
+  }
+  __syncthreads();
+  if (walk.x >= walk.end) return;
+  const long long my_start = walk.x;
+  walk.row = start_s.row;
+  walk.row_start = start_s.row_start;
+  walk.span = span_of<kTile>(a, walk.row);
+
+  if (warp == C::kWarps) {
+    // ------------------------------------------------------------------ producer
+    // Boxes of box_rows tokens (a divisor of the page and of the tile) by 64 dims.  Lane i holds
+    // the page of the i-th of the next 32 boxes, fetched by one load for all of them.
+    const int boxes = kTile / a.box_rows;
+    const uint32_t box_bytes = a.box_rows * 128;
+    int it = 0;
+    while (walk.next(a, units_per_row)) {
+      const int head = walk.unit / a.row_blocks;
+      const int* table = a.page_table + (long long)walk.row * a.max_pages;
+      int held = -32, page = 0;
+      for (int j = 0; j < walk.n; ++j, ++it) {
+        const int stage = it % C::kStages;
+        if (it >= C::kStages && !mbar_wait(empty0 + 8 * stage, ((it / C::kStages) - 1) & 1, &abort_s)) return;
+        const uint32_t dst = smem_u32(smem) + stage * C::kStageBytes, bar = full0 + 8 * stage;
+        const int token = walk.span.tile(walk.k0 + j) * kTile;
+        uint32_t wanted = 0;
+        for (int b = 0; b < boxes; ++b) {
+          const int t = token + b * a.box_rows;
+          const bool use = t < walk.span.length && (t < walk.span.sink || t + a.box_rows > walk.span.from);
+          wanted |= (uint32_t)use << b;
+        }
+        if (lane == 0) mbar_expect_tx(bar, __popc(wanted) * box_bytes * C::kColBoxes * 2);
+        for (int b = 0; b < boxes; ++b) {
+          const int i = j * boxes + b;
+          if (i >= held + 32) {
+            held = i;
+            const int ti = i + lane;  // the box this lane looks up
+            const int jj = ti / boxes;
+            page = 0;
+            if (jj < walk.n) {
+              const int t = walk.span.tile(walk.k0 + jj) * kTile + (ti - jj * boxes) * a.box_rows;
+              if (t < walk.span.length && (t < walk.span.sink || t + a.box_rows > walk.span.from)) {
+                page = __ldg(table + t / a.page_tokens);
+                if (page < 0 || page >= a.n_pages) {
+                  if (a.status) atomicMax(a.status, 1);
+                  page = 0;
+                }
+              }
+            }
+          }
+          const int pg = __shfl_sync(0xffffffffu, page, i - held);
+          if (lane == 0 && (wanted >> b & 1)) {
+            const int t = token + b * a.box_rows, y = t % a.page_tokens;
+            const int z = pg * a.n_kv_heads + head;
+#pragma unroll
+            for (int c = 0; c < C::kColBoxes; ++c) {
+              const uint32_t to = dst + c * kTile * 128 + b * box_bytes;
+              tma_3d(to, &k_map, c * 64, y, z, bar);
+              tma_3d(to + C::kHalfBytes, &v_map, c * 64, y, z, bar);
+            }
+          }
+        }
+      }
+    }
+    return;
+  }
+
+  // -------------------------------------------------------------------- consumers
+  // Scores are computed transposed, S^T = K Q^T with tokens as the MMA's 16 rows and query heads as
+  // its 8 columns, so a group of 8 heads or fewer wastes nothing; then O^T += V^T P^T with dims as
+  // rows.  Each warp keeps its own running maximum and sum over the tokens it saw; the warps join
+  // once a unit.
+  const int team = warp / C::kTeamWarps, g = lane >> 2, qd = lane & 3;
+  const int row16 = (warp % C::kTeamWarps) * 16;
+  const int k_row = row16 + (lane & 15), k_chunk = lane >> 4;
+  const int v_row = row16 + (lane & 7) + ((lane >> 4) << 3), v_chunk = (lane >> 3) & 1;
+  const float scale2 = a.scale * kLog2e;
+  const long long n_slots = 2ll * gridDim.x;
+  int it = 0;
+  while (walk.next(a, units_per_row)) {
+    const int head = walk.unit / a.row_blocks, block = walk.unit - head * a.row_blocks;
+    const int rows = min(NR, a.group - block * NR);
+    const long long h0 = (long long)head * a.group + block * NR;  // query head of the block's row 0
+    uint32_t qf[D / 16][NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int r = t * 8 + g;
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.q) +
+                                                              walk.row * a.q_row_stride + (h0 + r) * a.q_head_stride);
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {
+        qf[s][t][0] = r < rows ? __ldg(src + s * 8 + qd) : 0u;
+        qf[s][t][1] = r < rows ? __ldg(src + s * 8 + qd + 4) : 0u;
+      }
+    }
+    float acc[D / 16][NT][4];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      m[t][0] = m[t][1] = -INFINITY;
+      l[t][0] = l[t][1] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][t][e] = 0.0f;
+    }
+
+    for (int j = 0; j < walk.n; ++j, ++it) {
+      if ((it & 1) != team) continue;
+      const int stage = it % C::kStages;
+      const uint32_t k_base = smem_u32(smem) + stage * C::kStageBytes, v_base = k_base + C::kHalfBytes;
+      if (!mbar_wait(full0 + 8 * stage, (it / C::kStages) & 1, &abort_s)) break;
+      const int token = walk.span.tile(walk.k0 + j) * kTile + row16;
+      const bool whole = token + 15 < walk.span.length && (token >= walk.span.from || token + 15 < walk.span.sink);
+      const bool any = whole || (token < walk.span.length && (token < walk.span.sink || token + 15 >= walk.span.from));
+      if (any) {
+        float sc[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+          uint32_t f[4];
+          ldmatrix_x4(f, k_base + (s / 4) * kTile * 128 + k_row * 128 + ((((s % 4) * 2 + k_chunk) ^ (k_row & 7)) << 4));
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            if constexpr (C::kF16) mma_f16(sc[t], f, qf[s][t][0], qf[s][t][1]);
+            else mma_bf16(sc[t], f, qf[s][t][0], qf[s][t][1]);
+          }
+        }
+        // this thread's tokens: g and g + 8; its query rows: 8 t + 2 qd + {0, 1}
+        const bool see0 = whole || walk.span.visible(token + g), see1 = whole || walk.span.visible(token + g + 8);
+        uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if (a.softcap > 0.0f) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              // cap tanh(x / cap) with tanh(y) = 1 - 2 / (1 + e^2y), good to a few 1e-7 of cap
+              const float e2y = ex2_ftz(sc[t][e] * a.cap_in);
+              sc[t][e] = a.softcap * kLog2e * (1.0f - __fdividef(2.0f, 1.0f + e2y));
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[t][e] *= scale2;
+          }
+          if (!see0) sc[t][0] = sc[t][1] = -INFINITY;
+          if (!see1) sc[t][2] = sc[t][3] = -INFINITY;
+          float hi[2] = {fmaxf(sc[t][0], sc[t][2]), fmaxf(sc[t][1], sc[t][3])};
+#pragma unroll
+          for (int d = 4; d < 32; d *= 2) {
+            hi[0] = fmaxf(hi[0], __shfl_xor_sync(0xffffffffu, hi[0], d));
+            hi[1] = fmaxf(hi[1], __shfl_xor_sync(0xffffffffu, hi[1], d));
+          }
+          if (__any_sync(0xffffffffu, hi[0] > m[t][0] || hi[1] > m[t][1])) {
+            float turn[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float now = fmaxf(m[t][e], hi[e]);
+              turn[e] = now == -INFINITY ? 1.0f : ex2_ftz(m[t][e] - now);
+              m[t][e] = now;
+              l[t][e] *= turn[e];
+            }
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              acc[i][t][0] *= turn[0];
+              acc[i][t][1] *= turn[1];
+              acc[i][t][2] *= turn[0];
+              acc[i][t][3] *= turn[1];
+            }
+          }
+          // a row whose scores so far are all -inf keeps weights exp2(-inf - 0) = 0
+          const float m0 = m[t][0] == -INFINITY ? 0.0f : m[t][0], m1 = m[t][1] == -INFINITY ? 0.0f : m[t][1];
+          const float p0 = see0 ? ex2_ftz(sc[t][0] - m0) : 0.0f, p1 = see0 ? ex2_ftz(sc[t][1] - m1) : 0.0f;
+          const float p2 = see1 ? ex2_ftz(sc[t][2] - m0) : 0.0f, p3 = see1 ? ex2_ftz(sc[t][3] - m1) : 0.0f;
+          l[t][0] += p0 + p2;
+          l[t][1] += p1 + p3;
+          // The weights go to the second product as two 16-bit parts: one rounding would cost the
+          // output as much as its own type does, and the second product's time is hidden behind
+          // the loads (2 x 8 MMAs of 350 cycles a warp at D = 128).
+          uint32_t h01, h23;
+          float2 b01, b23;
+          if constexpr (C::kF16) {
+            h01 = pack_half2(p0, p1), h23 = pack_half2(p2, p3);
+            b01 = unpack_half2(h01), b23 = unpack_half2(h23);
+            pl[t][0] = transpose8(pack_half2(p0 - b01.x, p1 - b01.y));
+            pl[t][1] = transpose8(pack_half2(p2 - b23.x, p3 - b23.y));
+          } else {
+            h01 = pack_bf162(p0, p1), h23 = pack_bf162(p2, p3);
+            b01 = unpack_bf162(h01), b23 = unpack_bf162(h23);
+            pl[t][0] = transpose8(pack_bf162(p0 - b01.x, p1 - b01.y));
+            pl[t][1] = transpose8(pack_bf162(p2 - b23.x, p3 - b23.y));
+          }
+          ph[t][0] = transpose8(h01);
+          ph[t][1] = transpose8(h23);
+        }
+        // In a tile with tokens that are not seen, their values are cleared as well: 0 times an
+        // infinity or NaN that a page happens to hold past a sequence's end is not 0.
+        uint32_t keep_lo = 0xffffffffu, keep_hi = 0xffffffffu;
+        if (!whole) {
+          keep_lo = (walk.span.visible(token + 2 * qd) ? 0xffffu : 0u) |
+                    (walk.span.visible(token + 2 * qd + 1) ? 0xffff0000u : 0u);
+          keep_hi = (walk.span.visible(token + 2 * qd + 8) ? 0xffffu : 0u) |
+                    (walk.span.visible(token + 2 * qd + 9) ? 0xffff0000u : 0u);
+        }
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t f[4];
+          ldmatrix_x4_trans(f, v_base + (i / 4) * kTile * 128 + v_row * 128 +
+                                   ((((i % 4) * 2 + v_chunk) ^ (v_row & 7)) << 4));
+          if (!whole) {
+            f[0] &= keep_lo;
+            f[1] &= keep_lo;
+            f[2] &= keep_hi;
+            f[3] &= keep_hi;
+          }
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            if constexpr (C::kF16) {
+              mma_f16(acc[i][t], f, ph[t][0], ph[t][1]);
+              mma_f16(acc[i][t], f, pl[t][0], pl[t][1]);
+            } else {
+              mma_bf16(acc[i][t], f, ph[t][0], ph[t][1]);
+              mma_bf16(acc[i][t], f, pl[t][0], pl[t][1]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty0 + 8 * stage);
+    }
+
+    // ------------------------------------------------------------------ the warps join
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], d);
+        if (g == 0) {
+          warp_m[warp * NR + t * 8 + 2 * qd + e] = m[t][e];
+          warp_l[warp * NR + t * 8 + 2 * qd + e] = l[t][e];
+        }
+      }
+    named_sync(1, C::kWarps * 32);
+    const bool cut = walk.n < walk.span.tiles;
+    // slot of this piece: a share's first piece may be the tail or middle of a unit, its last the head
+    const long long slot = 2ll * me + (walk.unit_start > my_start ? 1 : 0);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float top = -INFINITY;
+        for (int w = 0; w < C::kWarps; ++w) top = fmaxf(top, warp_m[w * NR + t * 8 + 2 * qd + e]);
+        const float turn = m[t][e] == -INFINITY ? 0.0f : ex2_ftz(m[t][e] - top);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          acc[i][t][e] *= turn;
+          acc[i][t][e + 2] *= turn;
+        }
+      }
+#pragma unroll
+    for (int part = 0; part < D / C::kSlice; ++part) {
+#pragma unroll
+      for (int i = 0; i < C::kSlice / 16; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            merge[(warp * NR + t * 8 + 2 * qd + (e & 1)) * C::kPad + i * 16 + g + (e >> 1) * 8] =
+                acc[part * (C::kSlice / 16) + i][t][e];
+      named_sync(1, C::kWarps * 32);
+      for (int i = tid; i < NR * C::kSlice; i += C::kWarps * 32) {
+        const int r = i / C::kSlice, d = i % C::kSlice;
+        float sum = 0.0f, top = -INFINITY, total_l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < C::kWarps; ++w) {
+          sum += merge[(w * NR + r) * C::kPad + d];
+          top = fmaxf(top, warp_m[w * NR + r]);
+        }
+#pragma unroll
+        for (int w = 0; w < C::kWarps; ++w) {
+          const float mw = warp_m[w * NR + r];
+          total_l += mw == -INFINITY ? warp_l[w * NR + r] : warp_l[w * NR + r] * ex2_ftz(mw - top);
+        }
+        const int dim = part * C::kSlice + d;
+        if (cut) {
+          a.records[(slot * NR + r) * D + dim] = sum;
+          if (dim == 0) {
+            a.records[n_slots * NR * D + slot * NR + r] = top;
+            a.records[n_slots * NR * (D + 1) + slot * NR + r] = total_l;
+          }
+        } else if (r < rows) {
+          const long long at = ((long long)walk.row * a.n_heads + h0 + r) * D + dim;
+          const float o = sum / total_l;
+          if (a.out_f32) static_cast<float*>(a.out)[at] = o;
+          else if constexpr (C::kF16) static_cast<__half*>(a.out)[at] = __float2half_rn(o);
+          else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(o);
+          if (a.lse && dim == 0)
+            a.lse[(long long)walk.row * a.n_heads + h0 + r] = (top + log2f(total_l)) * kLn2;
+        }
+      }
+      named_sync(1, C::kWarps * 32);
+    }
+    if (!cut) continue;
+
+    // ------------------------------------------------------------------ the pieces of a cut unit join
+    const long long u0 = walk.unit_start, u1 = u0 + walk.span.tiles;
+    const int w0 = (int)(((u0 + 1) * W - 1) / total), w1 = (int)((u1 * W - 1) / total);
+    const int pieces = w1 - w0 + 1;
+    const long long slot0 = 2ll * w0 + (u0 > total * w0 / W ? 1 : 0);  // pieces after the first are at 2 w
+    __threadfence();
+    named_sync(1, C::kWarps * 32);
+    if (tid == 0) last_s = atomicAdd(a.counters + slot0, 1) == pieces - 1;
+    named_sync(1, C::kWarps * 32);
+    if (!last_s) continue;
+    __threadfence();
+    if (tid == 0) a.counters[slot0] = 0;
+    const float* rec_m = a.records + n_slots * NR * D;
+    const float* rec_l = rec_m + n_slots * NR;
+    for (int r = warp; r < NR; r += C::kWarps) {
+      float top = -INFINITY, sum = 0.0f;
+      for (int w = lane; w < pieces; w += 32)
+        top = fmaxf(top, __ldcg(rec_m + (w == 0 ? slot0 : 2ll * (w0 + w)) * NR + r));
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      for (int w = lane; w < pieces; w += 32) {
+        const long long at = (w == 0 ? slot0 : 2ll * (w0 + w)) * NR + r;
+        const float mw = __ldcg(rec_m + at), f = mw == -INFINITY ? 1.0f : ex2_ftz(mw - top);
+        merge[w * NR + r] = f;
+        sum += f * __ldcg(rec_l + at);
+      }
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (lane == 0) {
+        warp_l[r] = sum;
+        if (a.lse && r < rows) a.lse[(long long)walk.row * a.n_heads + h0 + r] = (top + log2f(sum)) * kLn2;
+      }
+    }
+    named_sync(1, C::kWarps * 32);
+    for (int i = tid; i < NR * D / 4; i += C::kWarps * 32) {
+      const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+      if (r >= rows) continue;
+      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+      for (int w = 0; w < pieces; ++w) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(
+            a.records + ((w == 0 ? slot0 : 2ll * (w0 + w)) * NR + r) * D + d));
+        const float f = merge[w * NR + r];
+        o.x += f * v.x;
+        o.y += f * v.y;
+        o.z += f * v.z;
+        o.w += f * v.w;
+      }
+      const float sum = warp_l[r];
+      o.x /= sum;
+      o.y /= sum;
+      o.z /= sum;
+      o.w /= sum;
+      const long long at = ((long long)walk.row * a.n_heads + h0 + r) * D + d;
+      if (a.out_f32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = o;
+      } else {
+        uint2 w;
+        if constexpr (C::kF16) w = make_uint2(pack_half2(o.x, o.y), pack_half2(o.z, o.w));
+        else w = make_uint2(pack_bf162(o.x, o.y), pack_bf162(o.z, o.w));
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = w;
+      }
+    }
+    named_sync(1, C::kWarps * 32);
+  }
+  // a wait that ran into its limit (about two seconds): the outputs are not valid
+  if (tid == 0 && ld_shared_volatile(&abort_s) && a.status) atomicMax(a.status, 2);
+}
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  if (!fn) {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(ptr);
+  }
+  return fn;
+}
+
+// [n_pages * n_kv_heads][page_tokens][D] 16-bit values, read in boxes of [box_rows][64 dims] with the
+// 128-byte swizzle
+static int make_map(CUtensorMap* map, const void* base, const asterq_paged_attention_params* p, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return set_error(ASTERQ_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled unavailable");
+  const cuuint64_t dims[3] = {(cuuint64_t)p->head_dim, (cuuint64_t)p->page_tokens,
+                              (cuuint64_t)(p->n_pages > 0 ? p->n_pages * p->n_kv_heads : 1)};
+  const cuuint64_t strides[2] = {(cuuint64_t)p->head_dim * 2, (cuuint64_t)p->head_dim * 2 * p->page_tokens};
+  const cuuint32_t box[3] = {64u, (cuuint32_t)box_rows, 1u}, step[3] = {1u, 1u, 1u};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, step,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(ASTERQ_ERR_CUDA, "paged_attention: tensor map encoding failed (%d)", (int)r);
+  return ASTERQ_OK;
+}
+
+// SMs of the current device, read once per device
+static int sm_count(int* dev) {
+  static int counts[64] = {0};
+  if (cudaGetDevice(dev) != cudaSuccess) return 0;
+  if (*dev < 64 && counts[*dev]) return counts[*dev];
+  int n = 0;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, *dev) != cudaSuccess) return 0;
+  n = n < kMaxWorkers ? n : kMaxWorkers;
+  if (*dev < 64) counts[*dev] = n;
+  return n;
+}
+
+static int rows_of_block(int group) { return group <= 8 ? 8 : 16; }
+
+static int64_t workspace_bytes(int workers, int rows, int head_dim) {
+  return 2ll * workers * rows * (head_dim + 2) * 4 + (2ll * workers * 4 + 15) / 16 * 16;
+}
+
+template <class C>
+static int launch(const CUtensorMap& k_map, const CUtensorMap& v_map, const Args& a, int workers, int dev,
+                  cudaStream_t s) {
+  static unsigned long long configured = 0;  // one bit per device ordinal
+  if (dev >= 64 || !(configured & (1ull << dev))) {
+    const cudaError_t e = cudaFuncSetAttribute(attention_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess)
+      return set_error(ASTERQ_ERR_CUDA, "paged_attention: shared memory opt-in: %s", cudaGetErrorString(e));
+    if (dev < 64) configured |= 1ull << dev;
+  }
+  attention_kernel<C><<<workers, C::kThreads, C::kSmem, s>>>(k_map, v_map, a);
+  return check_launch("paged_attention");
+}
+
+template <bool kF16, int D>
+static int by_rows(const CUtensorMap& k_map, const CUtensorMap& v_map, const Args& a, int workers, int dev,
+                   cudaStream_t s) {
+  if (rows_of_block(a.group) == 8) return launch<Cfg<kF16, D, 8>>(k_map, v_map, a, workers, dev, s);
+  return launch<Cfg<kF16, D, 16>>(k_map, v_map, a, workers, dev, s);
+}
+
+static int check(const asterq_paged_attention_params* p) {
+  if (!p) return set_error(ASTERQ_ERR_INVALID_ARGUMENT, "paged_attention: null parameters");
+  if (p->n_rows < 0 || p->n_heads <= 0 || p->n_kv_heads <= 0 || p->n_heads % p->n_kv_heads || p->page_tokens <= 0 ||
+      p->max_pages < 0 || p->n_pages < 0 || p->n_new < 0 || p->window < 0 || p->sink < 0)
+    return set_error(ASTERQ_ERR_INVALID_ARGUMENT, "paged_attention: bad sizes");
+  if (p->dtype != ASTERQ_DTYPE_BF16 && p->dtype != ASTERQ_DTYPE_F16)
+    return set_error(ASTERQ_ERR_UNSUPPORTED, "paged_attention: dtype %d: bf16 or f16", p->dtype);
+  if (p->out_dtype != p->dtype && p->out_dtype != ASTERQ_DTYPE_F32)
+    return set_error(ASTERQ_ERR_UNSUPPORTED, "paged_attention: the output is of the queries' type or f32");
+  if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)
+    return set_error(ASTERQ_ERR_UNSUPPORTED, "paged_attention: head_dim %d: 64, 128 or 256", p->head_dim);
+  if (p->page_tokens % 16)
+    return set_error(ASTERQ_ERR_UNSUPPORTED, "paged_attention: page_tokens %d must be a multiple of 16", p->page_tokens);
+  if (p->n_pages * p->n_kv_heads > 0x7fffffffLL || (int64_t)p->max_pages * p->page_tokens > 0x7fff0000LL)
+    return set_error(ASTERQ_ERR_UNSUPPORTED, "paged_attention: more than 2^31 pages or tokens of a sequence");
+  return ASTERQ_OK;
+}
+
+}  // namespace pat
+}  // namespace asterq
+
+using namespace asterq;
+
+extern "C" int64_t asterq_paged_attention_workspace_bytes(const asterq_paged_attention_params* p) {
+  clear_error();
+  if (pat::check(p) != ASTERQ_OK) return 0;
+  int dev = 0;
+  const int workers = pat::sm_count(&dev);
+  return pat::workspace_bytes(workers > 0 ? workers : pat::kMaxWorkers, pat::rows_of_block(p->n_heads / p->n_kv_heads),
+                              p->head_dim);
+}
+
+extern "C" int asterq_paged_attention(const asterq_paged_attention_params* p, void* stream) {
+  clear_error();
+  int st = pat::check(p);
+  if (st != ASTERQ_OK) return st;
+  if (p->n_rows == 0) return ASTERQ_OK;
+  if (!p->q || !p->lengths || !p->out || (p->max_pages > 0 && p->n_pages > 0 && (!p->k_pool || !p->v_pool)) ||
+      (p->max_pages > 0 && !p->page_table))
+    return set_error(ASTERQ_ERR_INVALID_ARGUMENT, "paged_attention: null pointer");
+  const void* vec[] = {p->k_pool, p->v_pool, p->out, p->workspace};
+  for (const void* ptr : vec)
+    if (reinterpret_cast<uintptr_t>(ptr) & 15)
+      return set_error(ASTERQ_ERR_MISALIGNED, "paged_attention: pools, output and workspace must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(p->q) & 3) || p->q_row_stride % 2 || p->q_head_stride % 2)
+    return set_error(ASTERQ_ERR_MISALIGNED, "paged_attention: queries must be 4-byte aligned, their strides even");
+  int dev = 0;
+  const int workers = pat::sm_count(&dev);
+  if (workers <= 0) return set_error(ASTERQ_ERR_CUDA, "paged_attention: no CUDA device");
+  pat::Args a;
+  a.group = p->n_heads / p->n_kv_heads;
+  const int rows = pat::rows_of_block(a.group);
+  if (!p->workspace || p->workspace_bytes < pat::workspace_bytes(workers, rows, p->head_dim))
+    return set_error(ASTERQ_ERR_WORKSPACE, "paged_attention: workspace of %lld bytes, %lld needed",
+                     (long long)p->workspace_bytes, (long long)pat::workspace_bytes(workers, rows, p->head_dim));
+  a.row_blocks = (a.group + rows - 1) / rows;
+  a.q = p->q;
+  a.page_table = p->page_table;
+  a.lengths = p->lengths;
+  a.out = p->out;
+  a.lse = p->lse;
+  // counters first: their place does not depend on the call's geometry, so one workspace serves calls
+  // of different heads in turn
+  a.counters = static_cast<int*>(p->workspace);
+  a.records = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + (2ll * workers * 4 + 15) / 16 * 16);
+  a.status = p->status;
+  a.q_row_stride = p->q_row_stride;
+  a.q_head_stride = p->q_head_stride;
+  a.n_pages = p->n_pages;
+  a.capacity = p->n_pages > 0 ? (long long)p->max_pages * p->page_tokens : 0;
+  a.n_rows = p->n_rows;
+  a.n_heads = p->n_heads;
+  a.n_kv_heads = p->n_kv_heads;
+  a.page_tokens = p->page_tokens;
+  a.max_pages = p->max_pages;
+  a.n_new = p->n_new;
+  a.window = p->window;
+  a.sink = p->sink;
+  a.out_f32 = p->out_dtype == ASTERQ_DTYPE_F32;
+  a.scale = p->softmax_scale;
+  a.softcap = p->logit_softcap > 0.0f ? p->logit_softcap : 0.0f;
+  a.cap_in = a.softcap > 0.0f ? 2.0f * pat::kLog2e * a.scale / a.softcap : 0.0f;
+  // boxes of a tile lie in one page each: the largest of 64, 32 and 16 tokens that divides the page
+  a.box_rows = p->page_tokens % 64 == 0 ? 64 : p->page_tokens % 32 == 0 ? 32 : 16;
+  if (p->head_dim == 256 && a.box_rows > 32) a.box_rows = 32;
+  CUtensorMap k_map, v_map;
+  const bool pools = a.capacity > 0;  // with none, nothing is visible and the maps are never read
+  if ((st = pat::make_map(&k_map, pools ? p->k_pool : p->workspace, p, a.box_rows)) != ASTERQ_OK) return st;
+  if ((st = pat::make_map(&v_map, pools ? p->v_pool : p->workspace, p, a.box_rows)) != ASTERQ_OK) return st;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const bool f16 = p->dtype == ASTERQ_DTYPE_F16;
+  switch (p->head_dim) {
+    case 64: return f16 ? pat::by_rows<true, 64>(k_map, v_map, a, workers, dev, s)
+                        : pat::by_rows<false, 64>(k_map, v_map, a, workers, dev, s);
+    case 128: return f16 ? pat::by_rows<true, 128>(k_map, v_map, a, workers, dev, s)
+                         : pat::by_rows<false, 128>(k_map, v_map, a, workers, dev, s);
+    default: return f16 ? pat::by_rows<true, 256>(k_map, v_map, a, workers, dev, s)
+                        : pat::by_rows<false, 256>(k_map, v_map, a, workers, dev, s);
+  }
+}

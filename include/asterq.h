@@ -380,6 +380,154 @@ int asterq_cp_combine_wait(const void* mailbox, int32_t world, int32_t n_blocks,
                            int32_t latent_dim, void* out, int32_t out_dtype, int64_t wait_limit_cycles,
                            int32_t* status, void* stream);
 
+/*
+ * Paged grouped-query cache: the keys and values of an ordinary attention layer beside the latent
+ * layers of a hybrid model, in pools
+ *   k_pool, v_pool  dtype [n_pages, n_kv_heads, page_tokens, head_dim], 16-byte aligned
+ * with int32 page tables page_table [n_seqs][max_pages] (the pages of a sequence, oldest first) and
+ * lengths [n_seqs] (cached tokens; negative: an empty slot) on the device.  No counterpart in the
+ * reference, whose cache holds latents only.
+ *
+ * asterq_kv_append writes a step's or a prompt chunk's new keys and values at the end of each
+ * sequence, rotated by position on the way, and writes the rotated queries beside them:
+ * row r of sequence s, row_offsets[s] <= r < row_offsets[s + 1], has position
+ * lengths[s] + r - row_offsets[s].  The first rotary_dim dims of each head turn in pairs
+ * (j, j + rotary_dim / 2), or (2j, 2j + 1) with `interleaved`, by cos[position][j] and
+ * sin[position][j]: x' = x cos - y sin, y' = y cos + x sin in fp32, rounded once to dtype; the other
+ * dims are copied.  `lengths` is not advanced (the layers of a model share it).  A row whose position
+ * has no page in the table, a page id outside [0, n_pages) or (rotary_dim > 0) no row in cos / sin is
+ * left out with its query and sets *status to 1; rows of an empty slot or of no sequence are left out.
+ * q may be NULL (keys and values only).  q_out must not overlap the inputs.
+ * head_dim: a multiple of 16 up to 512; rotary_dim: a multiple of 16 up to head_dim, 0 for no rotation.
+ */
+typedef struct asterq_kv_append_params {
+  int32_t dtype; /* ASTERQ_DTYPE_BF16 or ASTERQ_DTYPE_F16, of q, k, v and the pools */
+  int32_t n_seqs;
+  int32_t n_heads;
+  int32_t n_kv_heads;
+  int32_t head_dim;
+  int32_t rotary_dim;
+  int32_t interleaved;
+  int32_t page_tokens;
+  int32_t max_pages; /* row stride of page_table */
+  int32_t reserved;
+  int64_t n_rows;      /* rows of q, k and v */
+  int64_t n_pages;     /* pages of the pools */
+  int64_t n_positions; /* rows of cos and sin */
+  int64_t q_row_stride, q_head_stride; /* in elements, multiples of 8; a head's dims are contiguous */
+  int64_t k_row_stride, k_head_stride;
+  int64_t v_row_stride, v_head_stride;
+  const void* q;
+  const void* k;
+  const void* v;
+  const float* cos; /* [n_positions][rotary_dim / 2] */
+  const float* sin;
+  const int32_t* page_table;
+  const int32_t* lengths;
+  const int32_t* row_offsets; /* [n_seqs + 1], not decreasing */
+  void* q_out;                /* [n_rows][n_heads][head_dim] */
+  void* k_pool;
+  void* v_pool;
+  int32_t* status; /* may be NULL */
+} asterq_kv_append_params;
+
+int asterq_kv_append(const asterq_kv_append_params* p, void* stream);
+
+/*
+ * Attention of one new token a sequence over such a cache:
+ *   out[b][h] = sum over visible t of softmax(score) v_t,  score = softmax_scale q[b][h] . k_t
+ *   (softcapped to logit_softcap tanh(score / logit_softcap) when logit_softcap > 0),
+ * heads h of kv head h / (n_heads / n_kv_heads).  Sequence b has L = lengths[b] + n_new tokens
+ * (n_new = 1: the step's own token, appended while `lengths` has not advanced yet); with window > 0
+ * token t is visible when t < min(sink, window) or t >= L - (window - min(sink, window)), otherwise
+ * all are.  lse[b][h] = log(sum of exp(score)) in natural logarithms, optional.  A sequence without
+ * tokens (lengths[b] < 0, or L = 0) gets zeros and -inf.  Pages with no visible token may have any id;
+ * where a needed id is outside [0, n_pages) the row's output is not valid and *status becomes 1.
+ * Products of the weights are taken in two 16-bit parts, softmax statistics and sums in fp32.
+ * head_dim 64, 128 or 256; page_tokens a multiple of 16.
+ *
+ * workspace: asterq_paged_attention_workspace_bytes bytes, zeroed once before its first use; every
+ * call leaves it ready for the next one on the same stream.  Calls that overlap on the GPU need a
+ * workspace each.  A workspace serves calls of any shape that need no more bytes than it has.
+ */
+typedef struct asterq_paged_attention_params {
+  int32_t dtype;     /* of q and the pools: ASTERQ_DTYPE_BF16 or ASTERQ_DTYPE_F16 */
+  int32_t out_dtype; /* the same or ASTERQ_DTYPE_F32 */
+  int32_t n_rows;    /* sequences */
+  int32_t n_heads;
+  int32_t n_kv_heads;
+  int32_t head_dim;
+  int32_t page_tokens;
+  int32_t max_pages;
+  int32_t n_new;
+  int32_t window; /* 0: none */
+  int32_t sink;
+  float softmax_scale;
+  float logit_softcap; /* <= 0: off */
+  int32_t reserved;
+  int64_t n_pages;
+  int64_t q_row_stride, q_head_stride; /* in elements, even; a head's dims are contiguous */
+  const void* q;
+  const void* k_pool;
+  const void* v_pool;
+  const int32_t* page_table;
+  const int32_t* lengths;
+  void* out;  /* [n_rows][n_heads][head_dim] */
+  float* lse; /* [n_rows][n_heads] or NULL */
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* status; /* may be NULL */
+} asterq_paged_attention_params;
+
+int64_t asterq_paged_attention_workspace_bytes(const asterq_paged_attention_params* p);
+int asterq_paged_attention(const asterq_paged_attention_params* p, void* stream);
+
+/*
+ * Linear attention with a decay for each head: the recurrent layers beside the latent ones.  Each
+ * (slot, head) has a state S fp32 [dk][dv] in `state` [n_slots][n_heads][dk][dv], updated in place:
+ *   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   out_t = scale q_t S_t
+ * for the rows row_offsets[s] <= t < row_offsets[s + 1] of sequence s, whose state is slots[s]
+ * (row_offsets NULL: one token a sequence, row s).  g_t = log_decay[t * decay_row_stride + head]
+ * (decay_row_stride 0: one constant for each head), not above 0.  lengths (may be NULL): sequences with
+ * lengths[s] <= 0 start from a state of zeros, whatever their slot holds.  A slot below 0 is an empty
+ * one: its rows are written as zeros; one at or above n_slots is taken the same way and sets *status
+ * to 1, and so do row offsets outside [0, n_rows], whose sequence is left out.  Sequences of a call
+ * have slots of their own.
+ * dk, dv: 64 or 128.  q, k, v, out of one type: bf16, f16 or f32.
+ * workspace: asterq_linear_workspace_bytes bytes (0: none needed), not kept between calls; calls that
+ * overlap on the GPU need one each.
+ */
+typedef struct asterq_linear_params {
+  int32_t dtype;
+  int32_t n_seqs;
+  int32_t n_heads;
+  int32_t dk;
+  int32_t dv;
+  int32_t n_slots;
+  float scale;
+  int32_t reserved;
+  int64_t n_rows;
+  int64_t q_row_stride, q_head_stride; /* in elements, multiples of 8; a head's dims are contiguous */
+  int64_t k_row_stride, k_head_stride;
+  int64_t v_row_stride, v_head_stride;
+  int64_t decay_row_stride;
+  const void* q;
+  const void* k;
+  const void* v;
+  const float* log_decay;
+  float* state;
+  const int32_t* slots;
+  const int32_t* lengths;
+  const int32_t* row_offsets;
+  void* out; /* [n_rows][n_heads][dv] */
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* status; /* may be NULL */
+} asterq_linear_params;
+
+int64_t asterq_linear_workspace_bytes(const asterq_linear_params* p);
+int asterq_linear_attention(const asterq_linear_params* p, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
