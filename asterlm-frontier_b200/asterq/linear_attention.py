@@ -9,7 +9,9 @@ slot, float32 [n_slots, n_heads, dk, dv], updated in place:
 * ``linear_attention_prefill``: ragged prompt chunks, rows ``row_offsets[s]`` and on for sequence s;
 * ``linear_attention_step``: one new token a sequence.
 
-Both call ``asterq_linear_attention``; nothing waits for the GPU or reads from it.
+Both call ``asterq_linear_attention``; nothing waits for the GPU or reads from it, so calls can be
+recorded in a CUDA graph (the first prompt call on a stream allocates that stream's workspace: make it
+before the capture).
 """
 from __future__ import annotations
 
@@ -37,10 +39,31 @@ def _rows(x: torch.Tensor, name: str, q: torch.Tensor, dim: int) -> torch.Tensor
     return x
 
 
-_workspaces: dict[tuple[int, int], torch.Tensor] = {}
+class LinearAttentionWorkspace:
+    """Device memory for the states between the SMs that share a prompt; its contents are of one call.
+    One serves any sequence of calls on one stream; calls that overlap on the GPU need one each."""
+
+    def __init__(self, device="cuda") -> None:
+        device = torch.device(device)
+        p = _lib.LinearParams()  # the most any geometry needs
+        p.dtype, p.n_seqs, p.n_heads, p.dk, p.dv, p.n_rows, p.row_offsets = _lib.DTYPE_BF16, 1, 1, 128, 128, 1 << 20, 1
+        with torch.cuda.device(device):
+            self.nbytes = int(_lib.load().asterq_linear_workspace_bytes(_lib.ctypes.byref(p)))
+            self.buffer = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
 
 
-def _run(state, slots, lengths, row_offsets, q, k, v, log_decay, scale, out, status):
+_workspaces: dict[tuple[int, int], LinearAttentionWorkspace] = {}
+
+
+def _workspace(device: torch.device, stream: int) -> LinearAttentionWorkspace:
+    """The workspace that calls on this stream share when the caller brings none."""
+    ws = _workspaces.get((device.index, stream))
+    if ws is None:
+        ws = _workspaces[(device.index, stream)] = LinearAttentionWorkspace(device)
+    return ws
+
+
+def _run(state, slots, lengths, row_offsets, q, k, v, log_decay, scale, out, workspace, status):
     if q.dim() != 3 or state.dim() != 4:
         raise ValueError("q must be [rows, n_heads, dk] and state [n_slots, n_heads, dk, dv]")
     if q.dtype not in _DTYPES:
@@ -77,6 +100,10 @@ def _run(state, slots, lengths, row_offsets, q, k, v, log_decay, scale, out, sta
         raise ValueError(f"out must be a contiguous {q.dtype} tensor {(rows, heads, dv)}")
     device = q.device
     stream = torch.cuda.current_stream(device).cuda_stream
+    ws_ptr = ws_bytes = 0
+    if row_offsets is not None:
+        ws = _workspace(device, stream) if workspace is None else workspace
+        ws_ptr, ws_bytes = ws.buffer.data_ptr(), ws.nbytes
     q_row, q_head, _ = q.stride()
     k_row, k_head, _ = k.stride()
     v_row, v_head, _ = v.stride()
@@ -86,7 +113,7 @@ def _run(state, slots, lengths, row_offsets, q, k, v, log_decay, scale, out, sta
                        log_decay.stride(0) if log_decay.dim() == 2 else 0, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                        log_decay.data_ptr(), state.data_ptr(), slots.data_ptr(),
                        0 if lengths is None else lengths.data_ptr(),
-                       0 if row_offsets is None else row_offsets.data_ptr(), out.data_ptr(), 0, 0,
+                       0 if row_offsets is None else row_offsets.data_ptr(), out.data_ptr(), ws_ptr, ws_bytes,
                        0 if status is None else status.data_ptr()),
           device, stream)
     return out
@@ -104,6 +131,7 @@ def linear_attention_prefill(
     *,
     scale: float | None = None,
     out: torch.Tensor | None = None,
+    workspace: LinearAttentionWorkspace | None = None,
     status: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """Outputs [rows, n_heads, dv] of ragged prompt chunks; the slots' states move to the chunks' ends.
@@ -115,7 +143,7 @@ def linear_attention_prefill(
     stride.  log_decay float32 [n_heads] or [rows, n_heads], not above 0.  scale: 1 / sqrt(dk) unless
     given.  status int32 [1]: set to 1 when a slot or row offset was out of range.
     """
-    return _run(state, slots, lengths, row_offsets, q, k, v, log_decay, scale, out, status)
+    return _run(state, slots, lengths, row_offsets, q, k, v, log_decay, scale, out, workspace, status)
 
 
 def linear_attention_step(
@@ -133,4 +161,4 @@ def linear_attention_step(
 ) -> torch.Tensor:
     """One new token a sequence: row i updates slot ``slots[i]`` and reads it; arguments as for
     ``linear_attention_prefill``."""
-    return _run(state, slots, lengths, None, q, k, v, log_decay, scale, out, status)
+    return _run(state, slots, lengths, None, q, k, v, log_decay, scale, out, None, status)

@@ -2,30 +2,12 @@
 //
 //   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t,   S [Dk][Dv] per (slot, head)
 //
-// scan_kernel walks the recurrence token by token: the form for single tokens, and for chunks too
-// short for the chunked form.
-#include "asterq_internal.h"
-#include "common.cuh"
+// scan_kernel walks the recurrence token by token: the form for single tokens, for prompts too short
+// for the chunked form (csrc/linear_chunk.cu) and for the types that it does not take.
+#include "linear.cuh"
 
 namespace asterq {
 namespace lin {
-
-struct Args {
-  const void* q;
-  const void* k;
-  const void* v;
-  const float* log_decay;
-  float* state;
-  const int* slots;
-  const int* lengths;      // NULL: every sequence continues from its state
-  const int* row_offsets;  // NULL: row s is sequence s's one token
-  void* out;
-  int* status;
-  long long q_row, q_head, k_row, k_head, v_row, v_head, decay_row;  // strides in elements
-  long long n_rows;
-  int n_seqs, n_heads, n_slots;
-  float scale;
-};
 
 template <int kType>
 ASTERQ_DEVICE float load1(const void* p, long long i) {
@@ -152,14 +134,21 @@ static void scan_by_dims(const Args& a, int dk, int dv, int sms, cudaStream_t s)
   else scan<kType, 128, 128>(a, sms, s);
 }
 
-static int sm_count() {
+// SMs of the current device, read once per device
+static int sm_count(int* device) {
   static int counts[64] = {0};
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  if (dev < 64 && counts[dev]) return counts[dev];
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  if (dev < 64) counts[dev] = n;
+  int n = 0;
+  if (cudaGetDevice(device) != cudaSuccess) return 0;
+  if (*device < 64 && counts[*device]) return counts[*device];
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, *device) != cudaSuccess) return 0;
+  if (*device < 64) counts[*device] = n;
   return n;
+}
+
+// The chunked form takes bf16 prompts of 24 tokens a sequence or more on average: it needs about 20 us
+// for any of them up to one chunk a CTA, the scan 0.5 us a token.
+static bool in_chunks(const asterq_linear_params* p) {
+  return p->dtype == ASTERQ_DTYPE_BF16 && p->row_offsets && p->n_rows >= 24ll * p->n_seqs;
 }
 
 static int check(const asterq_linear_params* p) {
@@ -182,8 +171,9 @@ using namespace asterq;
 
 extern "C" int64_t asterq_linear_workspace_bytes(const asterq_linear_params* p) {
   clear_error();
-  if (lin::check(p) != ASTERQ_OK) return 0;
-  return 0;
+  if (lin::check(p) != ASTERQ_OK || !lin::in_chunks(p)) return 0;
+  int device = 0;
+  return lin::chunk_workspace_bytes(p->dk, p->dv, lin::sm_count(&device));
 }
 
 extern "C" int asterq_linear_attention(const asterq_linear_params* p, void* stream) {
@@ -204,7 +194,8 @@ extern "C" int asterq_linear_attention(const asterq_linear_params* p, void* stre
                              p->v_head_stride};
   for (int64_t s : strides)
     if (s % 8) return set_error(ASTERQ_ERR_MISALIGNED, "linear_attention: row and head strides must be multiples of 8");
-  const int sms = lin::sm_count();
+  int device = 0;
+  const int sms = lin::sm_count(&device);
   if (sms <= 0) return set_error(ASTERQ_ERR_CUDA, "linear_attention: no CUDA device");
   lin::Args a;
   a.q = p->q;
@@ -230,6 +221,14 @@ extern "C" int asterq_linear_attention(const asterq_linear_params* p, void* stre
   a.n_slots = p->n_slots;
   a.scale = p->scale;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (lin::in_chunks(p)) {
+    const int64_t need = lin::chunk_workspace_bytes(p->dk, p->dv, sms);
+    if (!p->workspace || p->workspace_bytes < need)
+      return set_error(ASTERQ_ERR_WORKSPACE, "linear_attention: workspace of %lld bytes, %lld needed",
+                       (long long)p->workspace_bytes, (long long)need);
+    const int done = lin::chunk_launch(a, p->dk, p->dv, sms, device, p->workspace, s);
+    if (done != ASTERQ_ERR_UNSUPPORTED) return done;  // else strides that the copy engine cannot follow
+  }
   switch (p->dtype) {
     case ASTERQ_DTYPE_F32: lin::scan_by_dims<ASTERQ_DTYPE_F32>(a, p->dk, p->dv, sms, s); break;
     case ASTERQ_DTYPE_F16: lin::scan_by_dims<ASTERQ_DTYPE_F16>(a, p->dk, p->dv, sms, s); break;
