@@ -18,9 +18,11 @@
 // a first pass computes what each such piece adds to a state of zeros (keys and values only), a small
 // kernel chains the pieces of a (sequence, head), and the main pass starts each piece from its state.
 //
-// Roles in a CTA (448 threads): warps 0-3 turn Q K^T into A (row i = thread i) and write the output;
+// Roles in a CTA (512 threads): warps 0-3 turn Q K^T into A (row i = thread i) and write the output;
 // warps 4-11 hold S in registers (thread = key dim, half of the value dims), scale and split the keys
-// and update S; warp 12 loads by TMA; one thread of warp 13 issues all products.
+// and update S; warp 12 loads by TMA; warp 13 issues all products; warp 14 sums the decays, a chunk
+// ahead; warp 15 stores whole chunks of outputs by TMA.  Warps 4-11 take registers of the last four (at
+// 128 a thread S would spill to local memory).
 #include <cuda.h>
 
 #include "linear.cuh"
@@ -32,8 +34,10 @@ namespace {
 
 constexpr int kChunk = 128;
 constexpr int kSlots = 5;       // tiles of 128 tokens in flight or in use
-constexpr int kThreads = 448;
+constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
+constexpr int kRegsA = 96, kRegsS = 168, kRegsIssue = 80;
+static_assert(kRegsA + 2 * kRegsS + kRegsIssue <= 4 * 128, "the split draws on the block's registers at launch");
 constexpr int kBoxBytes = kChunk * 128;
 constexpr int kMinShare = 4;    // chunks: below that the first pass costs more than another SM saves
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -54,8 +58,7 @@ struct Work {
 };
 
 struct Seq {
-  long long row0;
-  int rows, slot, chunks, fresh;
+  int row0, rows, slot, chunks, fresh;
 };
 ASTERQ_DEVICE Seq seq_of(const Args& a, int s) {
   Seq q;
@@ -69,21 +72,21 @@ ASTERQ_DEVICE Seq seq_of(const Args& a, int s) {
   return q;
 }
 
+// The launch sees to it that all chunks of a call count up to less than 2^31.
 struct Walk {
-  long long x, end, seq_start;
+  int x, end, seq_start;
   int s;
   Seq seq;
   int head, k0, n;  // the current piece: chunks [k0, k0 + n) of (sequence s, head)
   ASTERQ_DEVICE bool next(const Args& a) {
     if (x >= end) return false;
-    while (x >= seq_start + (long long)seq.chunks * a.n_heads) {
-      seq_start += (long long)seq.chunks * a.n_heads;
+    while (x >= seq_start + seq.chunks * a.n_heads) {
+      seq_start += seq.chunks * a.n_heads;
       seq = seq_of(a, ++s);
     }
-    const long long in = x - seq_start;
-    head = (int)(in / seq.chunks);
-    k0 = (int)(in - (long long)head * seq.chunks);
-    n = (int)min((long long)(seq.chunks - k0), end - x);
+    head = (x - seq_start) / seq.chunks;
+    k0 = x - seq_start - head * seq.chunks;
+    n = min(seq.chunks - k0, end - x);
     x += n;
     return true;
   }
@@ -97,9 +100,11 @@ struct Cfg {
   static constexpr int kStateBytes = kStateOnly ? 0 : kDk * kDv * 2;  // one bf16 part
   // barriers
   static constexpr int kFull = 0, kEmpty = kSlots, kQk = 2 * kSlots, kQs = kQk + 1, kULo = kQk + 2, kU = kQk + 3,
-                       kO = kQk + 4, kDecay = kQk + 5, kKeys = kQk + 6, kKeysHi = kQk + 7, kS = kQk + 8,
-                       kA = kQk + 9, kOFree = kQk + 10, kDrain = kQk + 11, kBars = kQk + 12;
-  static constexpr int kMiscBytes = 2 * kChunk * 4 + kChunk * 4 + 16 + kBars * 8 + 16 * 8 + 32 + 32;
+                       kO = kQk + 4, kKeys = kQk + 5, kKeysHi = kQk + 6, kS = kQk + 7, kA = kQk + 8,
+                       kOFree = kQk + 9, kOut = kQk + 10, kDrain = kQk + 11, kDecay = kQk + 12,
+                       kDecayFree = kQk + 14, kBars = kQk + 16;
+  static constexpr int kMiscBytes = 4 * kChunk * 4 + 2 * 12 * 4 + kBars * 8 + 24 * 4;
+  static_assert(kWarps <= 16, "scan_s");
   static constexpr int kSmem = kSlots * kSlotBytes + 2 * kStateBytes + kMiscBytes;
 };
 
@@ -111,79 +116,100 @@ ASTERQ_DEVICE void tma_rows(uint32_t dst, const CUtensorMap* map, int x, int hea
       : "memory");
 }
 
-// x as a sum of bf16 parts, two values at a time
+// A wait of a whole warp in as few instructions as its limit allows: the roles' loops together have to fit
+// the instruction cache (unrolled, and with longer waits, they did not, and half of all issue slots went
+// by without an instruction).  A round suspends for up to 20 us, so the limit is some seconds.
+ASTERQ_DEVICE bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  uint32_t done;
+  int rounds = 0;
+  while ((done = mbar_try_sleep(bar, parity, 20000u)) == 0) {
+    if (++rounds > (1 << 18)) *abort_flag = 1;
+    if (ld_shared_volatile(abort_flag)) break;
+  }
+  return __all_sync(0xffffffffu, (int)done) != 0;
+}
+
+// x as a sum of bf16 parts, two values at a time, by cutting off: the next eight bits of each, packed, and
+// the rest, which is exact.  Rounding instead would take cvt, a quarter-rate conversion of which this
+// kernel would need 67,000 a chunk: it was what bound it.  Three parts leave less than 2^-24 of x, two
+// less than 2^-16, towards zero.
+ASTERQ_DEVICE uint32_t last_part(float x, float y) { return prmt(__float_as_uint(x), __float_as_uint(y), 0x7632); }
 ASTERQ_DEVICE uint32_t split_part(float& x, float& y) {
-  const uint32_t p = pack_bf162(x, y);
-  x -= bf16lo_to_f32(p);
-  y -= bf16hi_to_f32(p);
+  const uint32_t p = last_part(x, y);
+  x -= __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+  y -= __uint_as_float(__float_as_uint(y) & 0xffff0000u);
   return p;
 }
 
 template <int kDk, int kDv, bool kStateOnly>
 __global__ void __launch_bounds__(kThreads, 1)
     chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
-                 const __grid_constant__ CUtensorMap v_map, const __grid_constant__ Args a,
-                 const __grid_constant__ Work work) {
+                 const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap o_map,
+                 const __grid_constant__ Args a, const __grid_constant__ Work work) {
   using C = Cfg<kDk, kDv, kStateOnly>;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
   const uint32_t s_hi = base + kSlots * C::kSlotBytes, s_lo = s_hi + C::kStateBytes;
   float* g_s = reinterpret_cast<float*>(smem + kSlots * C::kSlotBytes + 2 * C::kStateBytes);  // [2][kChunk]
-  float* w_s = g_s + 2 * kChunk;
-  float* tot_s = w_s + kChunk;  // [4]
-  uint64_t* bars_s = reinterpret_cast<uint64_t*>(tot_s + 4);
-  long long* scan_s = reinterpret_cast<long long*>(bars_s + C::kBars);  // [16]
-  long long* start_s = scan_s + 16;                                     // sequence, its first chunk
-  int* abort_s = reinterpret_cast<int*>(start_s + 2);
-  uint32_t* tmem_s = reinterpret_cast<uint32_t*>(abort_s + 1);
+  float* f_s = g_s + 2 * kChunk;     // [2][kChunk] 2^(decay from a token to the end of its 32)
+  float* far_s = f_s + 2 * kChunk;   // [2][12]: 2^(decay from each 32's end to the chunk's end), 2^(each 32's decay),
+                                     // the chunk's decay
+  uint64_t* bars_s = reinterpret_cast<uint64_t*>(far_s + 24);
+  int* scan_s = reinterpret_cast<int*>(bars_s + C::kBars);  // [16]
+  int* start_s = scan_s + 16;                               // sequence, its first chunk
+  int* abort_s = start_s + 2;
+  int* never_s = abort_s + 1;  // stays 0: the flag of waits that an abort must not cut short
+  uint32_t* tmem_s = reinterpret_cast<uint32_t*>(abort_s + 2);
   const uint32_t bars = smem_u32(bars_s);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   auto bar = [&](int i) { return bars + 8 * i; };
-  // A wait that runs into its limit raises the abort flag and every other wait returns at once: the
-  // walk goes on to its end over whatever is there, within bounds, and nothing hangs.
-  auto wait = [&](int i, int phase) { (void)mbar_wait(bar(i), phase & 1, abort_s); };
+  // A wait that runs into its limit raises the abort flag, every other wait then returns at once, and
+  // each warp leaves its work as a whole and waits (again with a limit) for what it has in flight.
+  auto wait = [&](int i, int phase) { return wait_for(bar(i), phase & 1, abort_s); };
+  bool ok = true;
 
   if (tid == 0) {
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(bar(C::kFull + i), 1);
       mbar_init(bar(C::kEmpty + i), 1);
     }
-    for (int i : {C::kQk, C::kQs, C::kULo, C::kU, C::kO, C::kDecay, C::kDrain}) mbar_init(bar(i), 1);
+    for (int i : {C::kQk, C::kQs, C::kULo, C::kU, C::kO, C::kDrain, C::kDecay, C::kDecay + 1}) mbar_init(bar(i), 1);
     for (int i : {C::kKeys, C::kKeysHi, C::kS}) mbar_init(bar(i), 8);
-    for (int i : {C::kA, C::kOFree}) mbar_init(bar(i), 4);
+    for (int i : {C::kA, C::kOFree, C::kOut}) mbar_init(bar(i), 4);
+    for (int i : {C::kDecayFree, C::kDecayFree + 1}) mbar_init(bar(i), kStateOnly ? 8 : 12);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     *abort_s = 0;
+    *never_s = 0;
   }
 
   // this CTA's share: a prefix sum over the sequences' chunks, thread t summing a strip of them
   const int strip = (a.n_seqs + kThreads - 1) / kThreads;
   const int s0 = min(tid * strip, a.n_seqs), s1 = min(s0 + strip, a.n_seqs);
-  long long sum = 0;
+  int sum = 0;
   for (int s = s0; s < s1; ++s) sum += seq_of(a, s).chunks;
   sum *= a.n_heads;
-  long long scan = sum;
+  int scan = sum;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
-    const long long up = __shfl_up_sync(0xffffffffu, scan, d);
+    const int up = __shfl_up_sync(0xffffffffu, scan, d);
     if (lane >= d) scan += up;
   }
   if (lane == 31) scan_s[warp] = scan;
   __syncthreads();
-  long long before = scan - sum, total = 0;
+  int before = scan - sum, total = 0;
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) before += scan_s[w];
     total += scan_s[w];
   }
   const int me = blockIdx.x;
-  const int W = (int)max(1ll, min((long long)gridDim.x, (total + kMinShare - 1) / kMinShare));
+  const int W = max(1, min((int)gridDim.x, (total + kMinShare - 1) / kMinShare));
   Walk walk;
-  walk.x = me < W ? total * me / W : total;
-  walk.end = me < W ? total * (me + 1) / W : total;
+  walk.x = me < W ? (int)((long long)total * me / W) : total;
+  walk.end = me < W ? (int)((long long)total * (me + 1) / W) : total;
   if (walk.x < walk.end && before <= walk.x && walk.x < before + sum) {
-    int s = s0;
-    long long at = before;
+    int s = s0, at = before;
     while (true) {
-      const long long here = (long long)seq_of(a, s).chunks * a.n_heads;
+      const int here = seq_of(a, s).chunks * a.n_heads;
       if (walk.x < at + here) break;
       at += here;
       ++s;
@@ -199,14 +225,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int begin = __ldg(a.row_offsets + s), end = __ldg(a.row_offsets + s + 1);
       if (tid == 0 && a.status && (begin < 0 || end > a.n_rows || (q.rows > 0 && q.slot >= a.n_slots)))
         atomicMax(a.status, 1);
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + q.row0 * a.n_heads * kDv);
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (long long)q.row0 * a.n_heads * kDv);
       for (long long i = tid; i < (long long)q.rows * a.n_heads * (kDv / 8); i += kThreads)
         dst[i] = make_uint4(0, 0, 0, 0);
     }
   }
   __syncthreads();
   if (walk.x < walk.end) {
-    walk.s = (int)start_s[0];
+    walk.s = start_s[0];
     walk.seq_start = start_s[1];
     walk.seq = seq_of(a, walk.s);
   }
@@ -237,171 +263,300 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_after();
   const uint32_t tmem = *tmem_s;
 
-  if (warp == 12) {
-    // ---------------------------------------------------------------- loads
-    if (lane == 0) {
+  // Registers of a thread by role: 128 (kRegsA + 2 kRegsS + kRegsIssue) of the 512 x 128 that the block was
+  // launched with.
+  if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+    if (warp == 12) {
+      // -------------------------------------------------------------- loads
       int n = 0;
       auto load = [&](const CUtensorMap* map, int boxes, int row, int head) {
         const int slot = n % kSlots;
-        if (n >= kSlots) wait(C::kEmpty + slot, n / kSlots - 1);
-        mbar_expect_tx(bar(C::kFull + slot), boxes * kBoxBytes);
-        for (int b = 0; b < boxes; ++b)
-          tma_rows(base + slot * C::kSlotBytes + b * kBoxBytes, map, b * 64, head, row, bar(C::kFull + slot));
+        if (n >= kSlots) ok = ok && wait(C::kEmpty + slot, n / kSlots - 1);
+        if (!ok) return;
+        if (lane == 0) {
+          mbar_expect_tx(bar(C::kFull + slot), boxes * kBoxBytes);
+          for (int b = 0; b < boxes; ++b)
+            tma_rows(base + slot * C::kSlotBytes + b * kBoxBytes, map, b * 64, head, row, bar(C::kFull + slot));
+        }
         ++n;
       };
-      while (walk.next(a))
-        for (int j = 0; j < walk.n; ++j) {
-          const int row = (int)walk.seq.row0 + (walk.k0 + j) * kChunk;
+      while (ok && walk.next(a))
+        for (int j = 0; j < walk.n && ok; ++j) {
+          const int row = walk.seq.row0 + (walk.k0 + j) * kChunk;
           load(&k_map, kDk / 64, row, walk.head);
           if (!kStateOnly) load(&q_map, kDk / 64, row, walk.head);
           load(&v_map, kDv / 64, row, walk.head);
         }
-      // after a wait ran out nobody may have waited for the last copies: they land before the exit
-      if (ld_shared_volatile(abort_s)) {
-        int none = 0;
-        for (int t = max(0, n - kSlots); t < n; ++t)
-          (void)mbar_wait(bar(C::kFull + t % kSlots), (t / kSlots) & 1, &none, 20000000);
-      }
-    }
-    __syncwarp();
-  } else if (warp == 13) {
-    // ---------------------------------------------------------------- products
-    if (lane == 0) {
+      // the last copies have landed before the exit, also when nobody waits for them any more
+      for (int t = max(0, n - kSlots); t < n; ++t)
+        (void)mbar_wait(bar(C::kFull + t % kSlots), (t / kSlots) & 1, never_s, 200000000);
+    } else if (warp == 13) {
+      // -------------------------------------------------------------- products
       constexpr uint32_t kQkDesc = tc::idesc_bf16(kChunk, false), kVDesc = tc::idesc_bf16(kDv, true);
+      // steps of 16 tokens: eight of them but in a sequence's last chunk
+      auto over_tokens = [&](int steps, auto step) {
+        int s = 0;
+#pragma unroll 1
+        for (; s + 4 <= steps; s += 4) {
+          step(s);
+          step(s + 1);
+          step(s + 2);
+          step(s + 3);
+        }
+#pragma unroll 1
+        for (; s < steps; ++s) step(s);
+      };
       int c = 0;
-      while (walk.next(a))
+      while (ok && walk.next(a))
         for (int j = 0; j < walk.n; ++j, ++c) {
           const int rows = min(kChunk, walk.seq.rows - (walk.k0 + j) * kChunk), steps = (rows + 15) / 16;
           const int t = c * C::kTiles, tv = t + C::kTiles - 1;
           const uint32_t k_at = base + (t % kSlots) * C::kSlotBytes, v_at = base + (tv % kSlots) * C::kSlotBytes;
+          const uint32_t v_desc = tc::desc_mn_major(v_at, kBoxBytes);
           const bool carried = walk.k0 + j > 0 || !walk.seq.fresh;  // S is not zero by construction
           if constexpr (!kStateOnly) {
             const int tq = t + 1;
             const uint32_t q_at = base + (tq % kSlots) * C::kSlotBytes;
-            wait(C::kFull + t % kSlots, t / kSlots);
-            wait(C::kFull + tq % kSlots, tq / kSlots);
-#pragma unroll
-            for (int s = 0; s < kDk / 16; ++s) {
-              const uint32_t at = (s / 4) * kBoxBytes + (s % 4) * 32;
-              tc::mma_ss(tmem + kColA, tc::desc_k_major(q_at + at), tc::desc_k_major(k_at + at), kQkDesc, s > 0);
-            }
-            tc::commit(bar(C::kQk));
-            wait(C::kS, c);
-            if (c > 0) wait(C::kOFree, c - 1);
-            tc::fence_after();
-            if (carried) {
+            const uint32_t q_desc = tc::desc_k_major(q_at), k_desc = tc::desc_k_major(k_at);
+            ok = ok && wait(C::kFull + t % kSlots, t / kSlots) && wait(C::kFull + tq % kSlots, tq / kSlots);
+            if (!ok) break;
+            if (tc::elect()) {
 #pragma unroll
               for (int s = 0; s < kDk / 16; ++s) {
-                const uint64_t q_desc = tc::desc_k_major(q_at + (s / 4) * kBoxBytes + (s % 4) * 32);
-                tc::mma_ss(tmem + kColO, q_desc, tc::desc_mn_major(s_hi + s * 2048, kDk * 128), kVDesc, s > 0);
-                tc::mma_ss(tmem + kColO, q_desc, tc::desc_mn_major(s_lo + s * 2048, kDk * 128), kVDesc, true);
+                const uint32_t at = ((s / 4) * kBoxBytes + (s % 4) * 32) >> 4;
+                tc::mma_ss(tmem + kColA, q_desc + at, k_desc + at, kQkDesc, s > 0);
               }
+              tc::commit(bar(C::kQk));
             }
-            tc::commit(bar(C::kQs));
-            tc::commit(bar(C::kEmpty + tq % kSlots));
+            ok = wait(C::kS, c) && (c == 0 || wait(C::kOFree, c - 1));
+            if (!ok) break;
+            tc::fence_after();
+            if (tc::elect()) {
+              if (carried) {
+                const uint32_t hi_desc = tc::desc_mn_major(s_hi, kDk * 128), lo_desc = tc::desc_mn_major(s_lo, kDk * 128);
+#pragma unroll
+                for (int s = 0; s < kDk / 16; ++s) {
+                  const uint32_t at = ((s / 4) * kBoxBytes + (s % 4) * 32) >> 4;
+                  tc::mma_ss(tmem + kColO, q_desc + at, hi_desc + s * 128, kVDesc, s > 0);
+                  tc::mma_ss(tmem + kColO, q_desc + at, lo_desc + s * 128, kVDesc, true);
+                }
+              }
+              tc::commit(bar(C::kQs));
+            }
           } else {
-            wait(C::kS, c);
+            ok = wait(C::kS, c);
+            if (!ok) break;
             tc::fence_after();
           }
-          wait(C::kFull + tv % kSlots, tv / kSlots);
-          wait(C::kKeys, c);
+          ok = wait(C::kFull + tv % kSlots, tv / kSlots) && wait(C::kKeys, c);
+          if (!ok) break;
           tc::fence_after();
-          for (int s = 0; s < steps; ++s)
-            tc::mma_ts(tmem + kColU, tmem + kColK + 8 * s, tc::desc_mn_major(v_at + s * 2048, kBoxBytes), kVDesc, s > 0);
-          tc::commit(bar(C::kULo));
-          for (int s = 0; s < steps; ++s)
-            tc::mma_ts(tmem + kColU, tmem + kColK + 64 + 8 * s, tc::desc_mn_major(v_at + s * 2048, kBoxBytes), kVDesc, true);
-          wait(C::kKeysHi, c);
+          if (tc::elect()) {
+            over_tokens(steps, [&](int s) { tc::mma_ts(tmem + kColU, tmem + kColK + 8 * s, v_desc + s * 128, kVDesc, s > 0); });
+            tc::commit(bar(C::kULo));
+            over_tokens(steps, [&](int s) { tc::mma_ts(tmem + kColU, tmem + kColK + 64 + 8 * s, v_desc + s * 128, kVDesc, true); });
+          }
+          ok = wait(C::kKeysHi, c);
+          if (!ok) break;
           tc::fence_after();
-          for (int s = 0; s < steps; ++s)
-            tc::mma_ts(tmem + kColU, tmem + kColK + 8 * s, tc::desc_mn_major(v_at + s * 2048, kBoxBytes), kVDesc, true);
-          tc::commit(bar(C::kU));
-          tc::commit(bar(C::kEmpty + t % kSlots));
+          if (tc::elect()) {
+            over_tokens(steps, [&](int s) { tc::mma_ts(tmem + kColU, tmem + kColK + 8 * s, v_desc + s * 128, kVDesc, true); });
+            tc::commit(bar(C::kU));
+            tc::commit(bar(C::kEmpty + t % kSlots));
+            if (kStateOnly) tc::commit(bar(C::kEmpty + tv % kSlots));
+          }
           if constexpr (!kStateOnly) {
-            wait(C::kA, c);
+            ok = wait(C::kA, c);
+            if (!ok) break;
             tc::fence_after();
-            for (int s = 0; s < steps; ++s) {
-              const uint32_t at = tmem + kColA + 32 * (s / 2) + 8 * (s % 2);
-              const uint64_t v_desc = tc::desc_mn_major(v_at + s * 2048, kBoxBytes);
-              tc::mma_ts(tmem + kColO, at, v_desc, kVDesc, carried || s > 0);
-              tc::mma_ts(tmem + kColO, at + 16, v_desc, kVDesc, true);
+            if (tc::elect()) {
+              over_tokens(steps, [&](int s) {
+                const uint32_t at = tmem + kColA + 32 * (s / 2) + 8 * (s % 2);
+                if (s == 0) tc::mma_ts(tmem + kColO, at, v_desc, kVDesc, carried);
+                else tc::mma_ts(tmem + kColO, at, v_desc + s * 128, kVDesc, true);
+                tc::mma_ts(tmem + kColO, at + 16, v_desc + s * 128, kVDesc, true);
+              });
+              tc::commit(bar(C::kO));
+              tc::commit(bar(C::kEmpty + tv % kSlots));
             }
-            tc::commit(bar(C::kO));
           }
-          tc::commit(bar(C::kEmpty + tv % kSlots));
         }
       // every product and every arrival above is done before the tensor memory goes back
-      tc::commit(bar(C::kDrain));
-      int none = 0;
-      (void)mbar_wait(bar(C::kDrain), 0, &none);
+      if (tc::elect()) tc::commit(bar(C::kDrain));
+      (void)mbar_wait(bar(C::kDrain), 0, never_s);
+    } else if (warp == 14) {
+      // -------------------------------------------------------------- decays
+      // Lane i has tokens 4 i .. 4 i + 3, eight lanes a 32.  Everything is a sum of what follows, never a
+      // difference: a decay of -inf, or one that outweighs the others, costs the tokens after it nothing.
+      double decay = 0.0;
+      int c = 0;
+      while (ok && walk.next(a)) {
+        float next[4];
+        auto read = [&](int j) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int at = (walk.k0 + j) * kChunk + 4 * lane + e;
+            next[e] = j < walk.n && at < walk.seq.rows
+                          ? __ldg(a.log_decay + (long long)(walk.seq.row0 + at) * a.decay_row + walk.head) : 0.0f;
+          }
+        };
+        read(0);
+        for (int j = 0; j < walk.n; ++j, ++c) {
+          float g[4], after[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) g[e] = next[e] * kLog2e;
+          read(j + 1);
+          after[3] = 0.0f;
+#pragma unroll
+          for (int e = 2; e >= 0; --e) after[e] = after[e + 1] + g[e + 1];
+          float sum = after[0] + g[0];  // from this lane's first token to the end of its 32
+#pragma unroll
+          for (int d = 1; d < 8; d *= 2) {
+            const float down = __shfl_down_sync(0xffffffffu, sum, d);
+            if ((lane & 7) + d < 8) sum += down;
+          }
+          float later = __shfl_down_sync(0xffffffffu, sum, 1);
+          if ((lane & 7) == 7) later = 0.0f;
+          const float all = __shfl_sync(0xffffffffu, sum, 8 * (lane & 3));  // the decay of 32 number lane % 4
+          float beyond = 0.0f;                                              // of the 32s after it
+#pragma unroll
+          for (int e = 1; e < 4; ++e) {
+            const float x = __shfl_sync(0xffffffffu, all, (lane & 3) + e < 4 ? (lane & 3) + e : 0);
+            if ((lane & 3) + e < 4) beyond += x;
+          }
+          double whole = ((double)g[0] + g[1]) + ((double)g[2] + g[3]);
+#pragma unroll
+          for (int d = 16; d > 0; d /= 2) whole += __shfl_xor_sync(0xffffffffu, whole, d);
+          decay += whole;
+          const int buf = c & 1;
+          if (c >= 2) {
+            ok = wait(C::kDecayFree + buf, c / 2 - 1);
+            if (!ok) break;
+          }
+          reinterpret_cast<float4*>(g_s + buf * kChunk)[lane] = make_float4(g[0], g[1], g[2], g[3]);
+          reinterpret_cast<float4*>(f_s + buf * kChunk)[lane] =
+              make_float4(exp2f(after[0] + later), exp2f(after[1] + later), exp2f(after[2] + later), exp2f(after[3] + later));
+          if (lane < 4) {
+            far_s[buf * 12 + lane] = exp2f(beyond);
+            far_s[buf * 12 + 4 + lane] = exp2f(all);
+          }
+          // in 64 bits: a constant decay's error would add up over all the chunks it acts on
+          if (lane == 4) far_s[buf * 12 + 8] = (float)exp2(whole);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(C::kDecay + buf));
+        }
+        if (kStateOnly && lane == 0) {
+          Header h;
+          h.decay = decay;
+          h.kind = walk.k0 == 0 ? 1 : 2;
+          h.slot = walk.seq.slot;
+          h.head = walk.head;
+          h.fresh = walk.seq.fresh;
+          work.headers[me] = h;
+        }
+      }
+    } else {
+      // -------------------------------------------------------------- whole chunks of outputs
+      // They are staged where the chunk's queries were, which nothing reads any more.
+      if constexpr (!kStateOnly) {
+        int c = 0;
+        while (ok && walk.next(a))
+          for (int j = 0; j < walk.n; ++j, ++c) {
+            const int slot = (c * C::kTiles + 1) % kSlots, row = walk.seq.row0 + (walk.k0 + j) * kChunk;
+            ok = wait(C::kOut, c);
+            if (!ok) break;
+            if (lane == 0) {
+              if (walk.seq.rows - (walk.k0 + j) * kChunk >= kChunk) {
+                for (int b = 0; b < kDv / 64; ++b)
+                  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
+                                   &o_map),
+                               "r"(b * 64), "r"(walk.head), "r"(row), "r"(base + slot * C::kSlotBytes + b * kBoxBytes)
+                               : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+              }
+              mbar_arrive(bar(C::kEmpty + slot));
+            }
+          }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        __syncwarp();
+      }
     }
-    __syncwarp();
   } else if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsA));
     // ---------------------------------------------------------------- A and the output
     if constexpr (!kStateOnly) {
       const uint32_t lanes = tmem + ((uint32_t)warp << 21);  // this warp's 32 lanes
       const int i = warp * 32 + lane;                        // row of the chunk
       int c = 0;
-      while (walk.next(a))
+      while (ok && walk.next(a))
         for (int j = 0; j < walk.n; ++j, ++c) {
           const int rows = min(kChunk, walk.seq.rows - (walk.k0 + j) * kChunk);
           const bool carried = walk.k0 + j > 0 || !walk.seq.fresh;
           const float* g = g_s + (c & 1) * kChunk;
-          if (c == 0) wait(C::kDecay, 0);
-          wait(C::kQk, c);
+          const float* f = f_s + (c & 1) * kChunk;
+          const float* p32 = far_s + (c & 1) * 12 + 4;
+          ok = wait(C::kDecay + (c & 1), c / 2) && wait(C::kQk, c);
+          if (!ok) break;
           tc::fence_after();
-          // From the row's own token back: sum = G_ij, exact where it matters, whatever came before.
+          // The row's own 32 columns: 2^G_ij from the diagonal back, sums that are exact where they matter.
+          uint32_t r[32], out[32];
+          tc::ld32(r, lanes + kColA + 32 * warp);
           float sum = 0.0f;
-#pragma unroll 1
-          for (int group = 3; group >= 0; --group) {
-            uint32_t r[32];
-            if (group > warp) {
-              if (32 * group >= rows) continue;  // no product reads these columns
+          tc::wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) r[e] = 0;
-              tc::st32(lanes + kColA + 32 * group, r);
-              continue;
+          for (int e = 15; e >= 0; --e) {
+            float x[2];
+#pragma unroll
+            for (int h = 1; h >= 0; --h) {
+              const int col = 2 * e + h;
+              if (col < lane) sum += g[32 * warp + col + 1];
+              x[h] = col <= lane ? __uint_as_float(r[col]) * (ex2_ftz(sum) * a.scale) : 0.0f;
             }
+            out[e] = split_part(x[0], x[1]);
+            out[16 + e] = last_part(x[0], x[1]);
+          }
+          tc::st32(lanes + kColA + 32 * warp, out);
+          // The 32s before it: 2^(from the 32's end to the row) times 2^(from the column to the 32's end).
+          float far = ex2_ftz(sum + g[32 * warp]) * a.scale;
+#pragma unroll 1
+          for (int group = warp - 1; group >= 0; --group) {
             tc::ld32(r, lanes + kColA + 32 * group);
+            const float4* fg = reinterpret_cast<const float4*>(f + 32 * group);
             tc::wait_ld();
-            uint32_t out[32];
-            if (group == warp) {
 #pragma unroll
-              for (int e = 15; e >= 0; --e) {
-                float x[2];
-#pragma unroll
-                for (int h = 1; h >= 0; --h) {
-                  const int col = 2 * e + h;
-                  if (col < lane) sum += g[32 * group + col + 1];
-                  x[h] = col <= lane ? __uint_as_float(r[col]) * ex2_ftz(sum) : 0.0f;
-                }
-                out[e] = split_part(x[0], x[1]);
-                out[16 + e] = pack_bf162(x[0], x[1]);
-              }
-            } else {
-#pragma unroll
-              for (int e = 15; e >= 0; --e) {
-                sum += g[32 * group + 2 * e + 2];
-                float x1 = __uint_as_float(r[2 * e + 1]) * ex2_ftz(sum);
-                sum += g[32 * group + 2 * e + 1];
-                float x0 = __uint_as_float(r[2 * e]) * ex2_ftz(sum);
-                out[e] = split_part(x0, x1);
-                out[16 + e] = pack_bf162(x0, x1);
-              }
+            for (int e = 0; e < 8; ++e) {
+              const float4 w = fg[e];
+              float x0 = __uint_as_float(r[4 * e]) * far * w.x, x1 = __uint_as_float(r[4 * e + 1]) * far * w.y;
+              float x2 = __uint_as_float(r[4 * e + 2]) * far * w.z, x3 = __uint_as_float(r[4 * e + 3]) * far * w.w;
+              out[2 * e] = split_part(x0, x1);
+              out[16 + 2 * e] = last_part(x0, x1);
+              out[2 * e + 1] = split_part(x2, x3);
+              out[16 + 2 * e + 1] = last_part(x2, x3);
             }
             tc::st32(lanes + kColA + 32 * group, out);
+            far *= p32[group];
           }
-          const float from_start = exp2f(sum + g[0]);
-          wait(C::kQs, c);
+#pragma unroll 1
+          for (int group = warp + 1; group < 4; ++group) {
+            if (32 * group >= rows) break;  // no product reads these columns
+#pragma unroll
+            for (int e = 0; e < 32; ++e) r[e] = 0;
+            tc::st32(lanes + kColA + 32 * group, r);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(C::kDecayFree + (c & 1)));
+          ok = wait(C::kQs, c);
+          if (!ok) break;
           tc::fence_after();
           if (carried) {
 #pragma unroll 1
             for (int d = 0; d < kDv; d += 32) {
-              uint32_t r[32];
               tc::ld32(r, lanes + kColO + d);
               tc::wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * from_start);
+              for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * far);
               tc::st32(lanes + kColO + d, r);
             }
           }
@@ -409,50 +564,56 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(C::kA));
-          wait(C::kO, c);
+          ok = wait(C::kO, c);
+          if (!ok) break;
           tc::fence_after();
           const long long row = walk.seq.row0 + (walk.k0 + j) * kChunk + i;
           uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (row * a.n_heads + walk.head) * kDv);
+          const uint32_t stage = base + ((c * C::kTiles + 1) % kSlots) * C::kSlotBytes + i * 128;
 #pragma unroll 1
           for (int d = 0; d < kDv; d += 32) {
-            uint32_t r[32];
             tc::ld32(r, lanes + kColO + d);
             tc::wait_ld();
             if (d + 32 == kDv) {
-              // The next chunk's decays are waited for before the products may go on: the warps that
-              // write them could otherwise run two chunks ahead of this barrier's phase.
-              if (j + 1 < walk.n || walk.x < walk.end) wait(C::kDecay, c + 1);
               tc::fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(bar(C::kOFree));
             }
-            if (i < rows) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                uint32_t p[4];
+            for (int e = 0; e < 4; ++e) {
+              uint32_t p[4];
 #pragma unroll
-                for (int h = 0; h < 4; ++h)
-                  p[h] = pack_bf162(__uint_as_float(r[8 * e + 2 * h]) * a.scale,
-                                    __uint_as_float(r[8 * e + 2 * h + 1]) * a.scale);
+              for (int h = 0; h < 4; ++h)
+                p[h] = pack_bf162(__uint_as_float(r[8 * e + 2 * h]), __uint_as_float(r[8 * e + 2 * h + 1]));
+              if (rows == kChunk) {
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                                 stage + (d / 64) * kBoxBytes + ((((d % 64) / 8 + e) ^ (i & 7)) << 4)),
+                             "r"(p[0]), "r"(p[1]), "r"(p[2]), "r"(p[3])
+                             : "memory");
+              } else if (i < rows) {
                 dst[d / 8 + e] = make_uint4(p[0], p[1], p[2], p[3]);
               }
             }
           }
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(C::kOut));
         }
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsS));
     // ---------------------------------------------------------------- keys and state
     constexpr int kCols = kDv / 2;
     const int part = (warp - 4) >> 2;               // tokens 64 part .., value dims kCols part ..
     const int dk = (warp & 3) * 32 + lane;          // key dim
     const bool has = kDk == 128 || (warp & 3) < 2;  // whole warps
-    const int t = (warp & 3) * 32 + lane;           // token whose decay a thread of the first part reads
     const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
-    const uint32_t k_col = (dk / 64) * kBoxBytes + (dk & 7) * 2;
-    const int k_unit = (dk % 64) >> 3;
+    // ldmatrix rows: lane -> token lane % 8 of an 8-token block, 8 key dims lane / 8 of the warp's 32
+    const uint32_t k_row = ((warp & 3) / 2) * kBoxBytes + (part * 64 + (lane & 7)) * 128 +
+                           (((((warp & 3) % 2) * 4 + (lane >> 3)) ^ (lane & 7)) << 4);
     float s[kCols];
     int c = 0;
-    while (walk.next(a)) {
+    while (ok && walk.next(a)) {
       const Seq q = walk.seq;
       const bool ends = walk.k0 + walk.n == q.chunks;
       const long long slot_at = (((long long)q.slot * a.n_heads + walk.head) * kDk + dk) * kDv + part * kCols;
@@ -472,12 +633,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         s[e + 2] = x.z;
         s[e + 3] = x.w;
       }
-      double decay = 0.0;
-      auto read_decay = [&](int j) {
-        const int at = (walk.k0 + j) * kChunk + t;
-        return part == 0 && j < walk.n && at < q.rows ? __ldg(a.log_decay + (q.row0 + at) * a.decay_row + walk.head) : 0.0f;
-      };
-      float g_next = read_decay(0);
       for (int j = 0; j < walk.n; ++j, ++c) {
         const int rows = min(kChunk, q.rows - (walk.k0 + j) * kChunk), steps = (rows + 15) / 16;
         // S for this chunk's outputs; the products of the last chunk that read the old one are done
@@ -492,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int h = 0; h < 4; ++h) {
               float x = s[8 * e + 2 * h], y = s[8 * e + 2 * h + 1];
               hi[h] = split_part(x, y);
-              lo[h] = pack_bf162(x, y);
+              lo[h] = last_part(x, y);
             }
             const uint32_t at = row_at + (((unit0 + e) ^ (dk & 7)) << 4);
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(s_hi + at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]),
@@ -508,68 +663,58 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(C::kS));
 
-        // decays: this token's, and the weight from it to the chunk's end
-        const float g = g_next * kLog2e;
-        g_next = read_decay(j + 1);
-        float after = g;  // inclusive from this token on, within the warp
-        if (part == 0) {
-          g_s[(c & 1) * kChunk + t] = g;
-#pragma unroll
-          for (int d = 1; d < 32; d *= 2) {
-            const float down = __shfl_down_sync(0xffffffffu, after, d);
-            if (lane + d < 32) after += down;
-          }
-          if (lane == 0) tot_s[warp & 3] = after;
-          after = __shfl_down_sync(0xffffffffu, after, 1);
-          if (lane == 31) after = 0.0f;
-        }
-        named_sync(2, 256);
-        if (tid == 128) mbar_arrive(bar(C::kDecay));
-        if (part == 0) {
-#pragma unroll
-          for (int w = 3; w > 0; --w)
-            if (w > (warp & 3)) after += tot_s[w];
-          w_s[t] = exp2f(after);
-        }
-        const double chunk_decay = ((double)tot_s[0] + tot_s[1]) + ((double)tot_s[2] + tot_s[3]);
-        decay += chunk_decay;
-        // in 64 bits: a constant decay's error would add up over all the chunks it acts on
-        const float whole = (float)exp2(chunk_decay);
-        named_sync(2, 256);
-
-        // the keys, weighted and split
+        // the keys, weighted and split: thread t has key dims t / 4 + 8 m and tokens 2 (t % 4), + 1 of each block
         const int tk = c * C::kTiles, tv = tk + C::kTiles - 1;
-        const uint32_t k_at = base + (tk % kSlots) * C::kSlotBytes + k_col;
-        uint32_t hi[32];
-        wait(C::kFull + tk % kSlots, tk / kSlots);
-        if (has) {
+        const uint32_t k_at = base + (tk % kSlots) * C::kSlotBytes + k_row;
+        const float2* weight = reinterpret_cast<const float2*>(f_s + (c & 1) * kChunk + part * 64) + (lane & 3);
+        const float* far = far_s + (c & 1) * 12;
+        ok = wait(C::kDecay + (c & 1), c / 2) && wait(C::kFull + tk % kSlots, tk / kSlots);
+        if (!ok) break;
+        const float whole = far[8];
+        // eight tokens of the warp's 32 key dims, weighted: x and y are tokens tok and tok + 1
+        auto weighted = [&](int block, auto put) {
+          uint32_t f[4];
+          ldmatrix_x4_trans(f, k_at + block * 1024);
+          const float2 w = weight[block * 4];
+          const float to_end = far[part * 2 + block / 4], wx = w.x * to_end, wy = w.y * to_end;
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
+          for (int m = 0; m < 4; ++m) put(m, bf16lo_to_f32(f[m]) * wx, bf16hi_to_f32(f[m]) * wy);
+        };
+        const int units = has ? min(4, (rows - part * 64 + 15) / 16) : 0;  // steps of 16 tokens here; may be < 0
+        if (rows < kChunk && has) {
+          // keys past the sequence's end, where this warp would read them: zeros (a weight of zero would
+          // not clear a NaN)
+          for (int e = lane + 4 * max(0, rows - part * 64); e < 4 * 64; e += 32) {
+            const int tok = part * 64 + e / 4, unit = ((warp & 3) % 2) * 4 + e % 4;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                             base + (tk % kSlots) * C::kSlotBytes + ((warp & 3) / 2) * kBoxBytes + tok * 128 +
+                             ((unit ^ (tok & 7)) << 4)),
+                         "r"(0)
+                         : "memory");
+          }
+          __syncwarp();
+        }
+        {
+#pragma unroll 1
+          for (int u = 0; u < units; ++u) {
             const int t0 = part * 64 + u * 16;
-            if (t0 >= rows) continue;
             uint32_t mid[8], lo[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              float x[2];
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int tok = t0 + 2 * e + h;
-                uint16_t raw;
-                asm volatile("ld.shared.u16 %0, [%1];"
-                             : "=h"(raw)
-                             : "r"(k_at + tok * 128 + ((k_unit ^ (tok & 7)) << 4)));
-                x[h] = __uint_as_float((uint32_t)raw << 16) * w_s[tok];
-                if (tok >= rows) x[h] = 0.0f;
-              }
-              hi[u * 8 + e] = split_part(x[0], x[1]);
-              mid[e] = split_part(x[0], x[1]);
-              lo[e] = pack_bf162(x[0], x[1]);
-            }
-            tc::st8(lanes + kColK + t0 / 2, lo);
-            tc::st8(lanes + kColK + 64 + t0 / 2, mid);
+            for (int h = 0; h < 2; ++h)
+              weighted(2 * u + h, [&](int m, float x, float y) {
+                (void)split_part(x, y);
+                mid[h * 4 + m] = split_part(x, y);
+                lo[h * 4 + m] = last_part(x, y);
+              });
+            const uint32_t to = lanes + kColK + t0 / 2;
+            tc::st_16x128b_x2(to, lo[0], lo[1], lo[4], lo[5]);
+            tc::st_16x128b_x2(to + (16u << 16), lo[2], lo[3], lo[6], lo[7]);
+            tc::st_16x128b_x2(to + 64, mid[0], mid[1], mid[4], mid[5]);
+            tc::st_16x128b_x2(to + 64 + (16u << 16), mid[2], mid[3], mid[6], mid[7]);
           }
         }
-        wait(C::kFull + tv % kSlots, tv / kSlots);
+        ok = wait(C::kFull + tv % kSlots, tv / kSlots);
+        if (!ok) break;
         if (rows < steps * 16) {
           // the last chunk's products run over whole steps of 16 tokens: values past the end are zeros
           const uint32_t v_at = base + (tv % kSlots) * C::kSlotBytes;
@@ -586,25 +731,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(C::kKeys));
-        wait(C::kULo, c);
+        ok = wait(C::kULo, c);
+        if (!ok) break;
         tc::fence_after();
-        if (has) {
+        // the leading parts, in the place of the smallest: computed again rather than held, which would not
+        // leave S enough registers
+#pragma unroll 1
+        for (int u = 0; u < units; ++u) {
+          uint32_t p[8];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int t0 = part * 64 + u * 16;
-            if (t0 >= rows) continue;
-            uint32_t r[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) r[e] = hi[u * 8 + e];
-            tc::st8(lanes + kColK + t0 / 2, r);
-          }
+          for (int h = 0; h < 2; ++h)
+            weighted(2 * u + h, [&](int m, float x, float y) { p[h * 4 + m] = last_part(x, y); });
+          const uint32_t to = lanes + kColK + (part * 64 + u * 16) / 2;
+          tc::st_16x128b_x2(to, p[0], p[1], p[4], p[5]);
+          tc::st_16x128b_x2(to + (16u << 16), p[2], p[3], p[6], p[7]);
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::kDecayFree + (c & 1)));
         tc::wait_st();
         tc::fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(C::kKeysHi));
 
-        wait(C::kU, c);
+        ok = wait(C::kU, c);
+        if (!ok) break;
         tc::fence_after();
         if (has) {
 #pragma unroll
@@ -617,18 +767,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+      if (!ok) break;
       float* to = nullptr;
       if (kStateOnly) {
         to = work.pieces + (long long)me * kDk * kDv + piece_at;
-        if (tid == 128) {
-          Header h;
-          h.decay = decay;
-          h.kind = walk.k0 == 0 ? 1 : 2;
-          h.slot = q.slot;
-          h.head = walk.head;
-          h.fresh = q.fresh;
-          work.headers[me] = h;
-        }
       } else if (ends) {
         to = a.state + slot_at;
       }
@@ -695,6 +837,7 @@ EncodeTiledFn encode_fn() {
 // rows of bf16 heads [n_rows][n_heads][dim] with any strides, read in boxes of 128 rows x 64 dims
 bool make_map(CUtensorMap* map, const void* base, const Args& a, int dim, long long row_stride, long long head_stride) {
   EncodeTiledFn fn = encode_fn();
+  if ((a.n_rows / kChunk + a.n_seqs) * a.n_heads > 0x7fffffff) return false;  // Walk counts in 32 bits
   if (!fn || row_stride <= 0 || head_stride <= 0) return false;
   const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)a.n_heads, (cuuint64_t)a.n_rows};
   const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)row_stride * 2};
@@ -708,9 +851,10 @@ template <int kDk, int kDv>
 int launch(const Args& a, int workers, int device, void* workspace, cudaStream_t s) {
   using First = Cfg<kDk, kDv, true>;
   using Main = Cfg<kDk, kDv, false>;
-  CUtensorMap q_map, k_map, v_map;
+  CUtensorMap q_map, k_map, v_map, o_map;
   if (!make_map(&q_map, a.q, a, kDk, a.q_row, a.q_head) || !make_map(&k_map, a.k, a, kDk, a.k_row, a.k_head) ||
-      !make_map(&v_map, a.v, a, kDv, a.v_row, a.v_head))
+      !make_map(&v_map, a.v, a, kDv, a.v_row, a.v_head) ||
+      !make_map(&o_map, a.out, a, kDv, (long long)a.n_heads * kDv, kDv))
     return ASTERQ_ERR_UNSUPPORTED;
   static unsigned long long configured = 0;  // one bit per device ordinal
   if (device >= 64 || !(configured & (1ull << device))) {
@@ -726,9 +870,9 @@ int launch(const Args& a, int workers, int device, void* workspace, cudaStream_t
   work.headers = static_cast<Header*>(workspace);
   work.pieces = reinterpret_cast<float*>(static_cast<char*>(workspace) + (workers * sizeof(Header) + 255) / 256 * 256);
   work.starts = work.pieces + (long long)workers * kDk * kDv;
-  chunk_kernel<kDk, kDv, true><<<workers, kThreads, First::kSmem, s>>>(q_map, k_map, v_map, a, work);
+  chunk_kernel<kDk, kDv, true><<<workers, kThreads, First::kSmem, s>>>(q_map, k_map, v_map, o_map, a, work);
   chain_kernel<kDk, kDv><<<dim3(workers, kDk * kDv / 1024), 256, 0, s>>>(a, work, workers);
-  chunk_kernel<kDk, kDv, false><<<workers, kThreads, Main::kSmem, s>>>(q_map, k_map, v_map, a, work);
+  chunk_kernel<kDk, kDv, false><<<workers, kThreads, Main::kSmem, s>>>(q_map, k_map, v_map, o_map, a, work);
   return check_launch("linear_attention");
 }
 

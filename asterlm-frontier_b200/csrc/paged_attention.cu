@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(warp_l + C::kWarps * NR);
   __shared__ Start start_s;
   __shared__ long long scan_s[32];
-  __shared__ int abort_s, last_s;
+  __shared__ int abort_s, never_s, last_s;  // never_s stays 0: for waits that an abort must not cut short
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * C::kStages;
   const int units_per_row = a.n_kv_heads * a.row_blocks;
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       mbar_init(empty0 + 8 * i, C::kTeamWarps);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    abort_s = 0;
+    abort_s = never_s = 0;
   }
 
   // The share: thread t sums the tiles of rows [t R, (t + 1) R), the block scans the sums.
@@ -222,13 +222,17 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     const int boxes = kTile / a.box_rows;
     const uint32_t box_bytes = a.box_rows * 128;
     int it = 0;
-    while (walk.next(a, units_per_row)) {
+    bool ok = true;
+    while (ok && walk.next(a, units_per_row)) {
       const int head = walk.unit / a.row_blocks;
       const int* table = a.page_table + (long long)walk.row * a.max_pages;
       int held = -32, page = 0;
       for (int j = 0; j < walk.n; ++j, ++it) {
         const int stage = it % C::kStages;
-        if (it >= C::kStages && !mbar_wait(empty0 + 8 * stage, ((it / C::kStages) - 1) & 1, &abort_s)) return;
+        if (it >= C::kStages) {
+          ok = __all_sync(0xffffffffu, (int)mbar_wait(empty0 + 8 * stage, ((it / C::kStages) - 1) & 1, &abort_s)) != 0;
+          if (!ok) break;
+        }
         const uint32_t dst = smem_u32(smem) + stage * C::kStageBytes, bar = full0 + 8 * stage;
         const int token = walk.span.tile(walk.k0 + j) * kTile;
         uint32_t wanted = 0;
@@ -270,6 +274,9 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         }
       }
     }
+    // the last copies have landed before the exit, also when a wait ran out and nobody waits for them
+    for (int t = max(0, it - C::kStages); t < it; ++t)
+      (void)mbar_wait(full0 + 8 * (t % C::kStages), (t / C::kStages) & 1, &never_s, 200000000);
     return;
   }
 
@@ -317,7 +324,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       if ((it & 1) != team) continue;
       const int stage = it % C::kStages;
       const uint32_t k_base = smem_u32(smem) + stage * C::kStageBytes, v_base = k_base + C::kHalfBytes;
-      if (!mbar_wait(full0 + 8 * stage, (it / C::kStages) & 1, &abort_s)) break;
+      if (!__all_sync(0xffffffffu, (int)mbar_wait(full0 + 8 * stage, (it / C::kStages) & 1, &abort_s))) break;
       const int token = walk.span.tile(walk.k0 + j) * kTile + row16;
       const bool whole = token + 15 < walk.span.length && (token >= walk.span.from || token + 15 < walk.span.sink);
       const bool any = whole || (token < walk.span.length && (token < walk.span.sink || token + 15 >= walk.span.from));

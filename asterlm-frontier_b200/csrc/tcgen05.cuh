@@ -46,9 +46,11 @@ ASTERQ_DEVICE void st32(uint32_t addr, const uint32_t (&r)[32]) {
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
-ASTERQ_DEVICE void st8(uint32_t addr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(r[0]),
-               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+// 16 lanes from the address's on, four columns twice over: thread t <-> lanes t / 4 and t / 4 + 8, column
+// t % 4 (r[0], r[1]), then the next four columns (r[2], r[3]): the layout of ldmatrix's 8 x 8 matrices
+ASTERQ_DEVICE void st_16x128b_x2(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r0), "r"(r1), "r"(r2),
+               "r"(r3)
                : "memory");
 }
 
@@ -59,12 +61,12 @@ ASTERQ_DEVICE void st8(uint32_t addr, const uint32_t (&r)[8]) {
 //             with a descriptor of its own
 //   mn_major  rows are K, the 64 values run along M or N; boxes of the next 64 are `box_bytes` on
 // ---------------------------------------------------------------------------
-ASTERQ_DEVICE uint64_t desc_base(uint32_t lbo_bytes) {
-  return ((uint64_t)(lbo_bytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-ASTERQ_DEVICE uint64_t desc_k_major(uint32_t smem) { return desc_base(16) | ((smem & 0x3ffff) >> 4); }
-ASTERQ_DEVICE uint64_t desc_mn_major(uint32_t smem, uint32_t box_bytes) {
-  return desc_base(box_bytes) | ((smem & 0x3ffff) >> 4);
+// A descriptor here is its low word: the start address and the stride between boxes, in 16-byte units.
+// The high word is the same for all of them: 1024 bytes between groups of eight rows, the swizzle.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+ASTERQ_DEVICE uint32_t desc_k_major(uint32_t smem) { return ((smem & 0x3ffff) >> 4) | (1u << 16); }
+ASTERQ_DEVICE uint32_t desc_mn_major(uint32_t smem, uint32_t box_bytes) {
+  return ((smem & 0x3ffff) >> 4) | ((box_bytes >> 4) << 16);
 }
 // bf16 x bf16 -> fp32, A K-major, M = 128
 constexpr uint32_t idesc_bf16(int n, bool b_mn_major) {
@@ -72,18 +74,28 @@ constexpr uint32_t idesc_bf16(int n, bool b_mn_major) {
          ((128u / 16) << 24);
 }
 
+// one lane of a converged warp; products are issued under it so that their operands stay in uniform
+// registers (issued from a divergent thread in a rolled loop they took 110 cycles each instead of 64)
+ASTERQ_DEVICE bool elect() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p;
+}
+
 // D[tmem] (+)= A B, both operands in shared memory; issued by one thread
-ASTERQ_DEVICE void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+ASTERQ_DEVICE void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.u32 p, %4, 0;\n mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "r"(kDescHigh)
       : "memory");
 }
 // A in tensor memory: lane = row, 32-bit column = two consecutive k
-ASTERQ_DEVICE void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+ASTERQ_DEVICE void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      "{\n .reg .pred p;\n .reg .b64 b;\n setp.ne.u32 p, %4, 0;\n mov.b64 b, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "r"(kDescHigh)
       : "memory");
 }
 // the mbarrier gets one arrival when all MMAs issued so far by this thread are done
