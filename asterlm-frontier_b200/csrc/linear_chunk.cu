@@ -6,12 +6,16 @@
 //   S <- 2^{G} S + sum_j (w_j k_j) v_j^T.
 // Four products of 128 x 128 x 128 a chunk and head of 128 dims; q, k, v are read once and o written
 // once (128 KB a chunk and head).  At one head-chunk a CTA, an SM's share of the memory bandwidth
-// takes 5,700 cycles for them; the products below take 3,600 to 4,100 on the tensor core.
+// takes 5,700 cycles for them; the products below take 4,600 on the tensor core.
 //
 // Rounding.  Products take bf16 operands and sum in fp32.  A and S enter as two bf16 parts (16 bits:
 // beside the output's own rounding they vanish).  The state is an fp32 output, so its update must not
-// round w_j k_j to less: it enters as three bf16 parts (24 bits), smallest first, each chunk's sum is
-// formed from zero on the tensor core and added to S in fp32 registers.
+// round w_j k_j to less.  The weight is split into bf16 parts w = w1 + w2 + w3 and the key's bf16 products
+// with them, exact in two parts each by one multiplication and one fused one, give four operands,
+//   k w1 = p1 + p2,   k w2 = m + r,   l = k w3 + r:   p1, p2, m and l,
+// for five packed operations a pair of values (splitting the fp32 product instead took twenty).  They are
+// summed smallest first; each chunk's sum is formed from zero on the tensor core and added to S in fp32
+// registers.
 //
 // Work.  One persistent CTA an SM takes an equal, contiguous share of all (sequence, head, chunk)s.
 // Where a share ends inside a (sequence, head), the state there has to come from the chunks before:
@@ -102,8 +106,8 @@ struct Cfg {
   static constexpr int kFull = 0, kEmpty = kSlots, kQk = 2 * kSlots, kQs = kQk + 1, kULo = kQk + 2, kU = kQk + 3,
                        kO = kQk + 4, kKeys = kQk + 5, kKeysHi = kQk + 6, kS = kQk + 7, kA = kQk + 8,
                        kOFree = kQk + 9, kOut = kQk + 10, kDrain = kQk + 11, kDecay = kQk + 12,
-                       kDecayFree = kQk + 14, kBars = kQk + 16;
-  static constexpr int kMiscBytes = 4 * kChunk * 4 + 2 * 12 * 4 + kBars * 8 + 24 * 4;
+                       kDecayFree = kQk + 14, kW = kQk + 16, kWFree = kQk + 17, kBars = kQk + 18;
+  static constexpr int kMiscBytes = 2 * (kChunk + 96) * 4 + 2 * 4 * 4 + 3 * kChunk * 2 + 16 + kBars * 8 + 24 * 4;
   static_assert(kWarps <= 16, "scan_s");
   static constexpr int kSmem = kSlots * kSlotBytes + 2 * kStateBytes + kMiscBytes;
 };
@@ -141,6 +145,17 @@ ASTERQ_DEVICE uint32_t split_part(float& x, float& y) {
   return p;
 }
 
+// 2^x of a whole chunk's decay to fp32's last bit: a constant decay's error would add up over all the chunks
+// it acts on.  x = n + r with |r| <= 1/2, 2^r by the series of e^(r ln 2), whose tenth term is below 2^-36.
+ASTERQ_DEVICE float exp2_once(double x) {
+  if (x < -160.0) return 0.0f;
+  const double n = rint(x), r = (x - n) * 0.69314718055994530942;
+  double y = 1.0;
+#pragma unroll
+  for (int i = 9; i > 0; --i) y = fma(y, r * (1.0 / i), 1.0);
+  return ldexpf((float)y, (int)n);
+}
+
 template <int kDk, int kDv, bool kStateOnly>
 __global__ void __launch_bounds__(kThreads, 1)
     chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
@@ -150,11 +165,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
   const uint32_t s_hi = base + kSlots * C::kSlotBytes, s_lo = s_hi + C::kStateBytes;
+  // decays of a chunk (log2 of a token's, and what follows from them), by warp 14
   float* g_s = reinterpret_cast<float*>(smem + kSlots * C::kSlotBytes + 2 * C::kStateBytes);  // [2][kChunk]
-  float* f_s = g_s + 2 * kChunk;     // [2][kChunk] 2^(decay from a token to the end of its 32)
-  float* far_s = f_s + 2 * kChunk;   // [2][12]: 2^(decay from each 32's end to the chunk's end), 2^(each 32's decay),
-                                     // the chunk's decay
-  uint64_t* bars_s = reinterpret_cast<uint64_t*>(far_s + 24);
+  float* f_s = g_s + 2 * kChunk;  // [2][96]: 2^(from a token of the first three 32s to the end of its 32)
+  float* p32_s = f_s + 2 * 96;    // [2][4]: 2^(each 32's decay)
+  uint16_t* w_s = reinterpret_cast<uint16_t*>(p32_s + 8);        // [3][kChunk]: bf16 parts of the weight to the chunk's end
+  float* whole_s = reinterpret_cast<float*>(w_s + 3 * kChunk);  // [4], one used: 2^(the chunk's decay)
+  uint64_t* bars_s = reinterpret_cast<uint64_t*>(whole_s + 4);
   int* scan_s = reinterpret_cast<int*>(bars_s + C::kBars);  // [16]
   int* start_s = scan_s + 16;                               // sequence, its first chunk
   int* abort_s = start_s + 2;
@@ -173,10 +190,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar(C::kFull + i), 1);
       mbar_init(bar(C::kEmpty + i), 1);
     }
-    for (int i : {C::kQk, C::kQs, C::kULo, C::kU, C::kO, C::kDrain, C::kDecay, C::kDecay + 1}) mbar_init(bar(i), 1);
-    for (int i : {C::kKeys, C::kKeysHi, C::kS}) mbar_init(bar(i), 8);
+    for (int i : {C::kQk, C::kQs, C::kULo, C::kU, C::kO, C::kDrain, C::kDecay, C::kDecay + 1, C::kW}) mbar_init(bar(i), 1);
+    for (int i : {C::kKeys, C::kKeysHi, C::kS, C::kWFree}) mbar_init(bar(i), 8);
     for (int i : {C::kA, C::kOFree, C::kOut}) mbar_init(bar(i), 4);
-    for (int i : {C::kDecayFree, C::kDecayFree + 1}) mbar_init(bar(i), kStateOnly ? 8 : 12);
+    for (int i : {C::kDecayFree, C::kDecayFree + 1}) mbar_init(bar(i), 4);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     *abort_s = 0;
     *never_s = 0;
@@ -270,23 +287,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 12) {
       // -------------------------------------------------------------- loads
       int n = 0;
-      auto load = [&](const CUtensorMap* map, int boxes, int row, int head) {
-        const int slot = n % kSlots;
-        if (n >= kSlots) ok = ok && wait(C::kEmpty + slot, n / kSlots - 1);
-        if (!ok) return;
-        if (lane == 0) {
-          mbar_expect_tx(bar(C::kFull + slot), boxes * kBoxBytes);
-          for (int b = 0; b < boxes; ++b)
-            tma_rows(base + slot * C::kSlotBytes + b * kBoxBytes, map, b * 64, head, row, bar(C::kFull + slot));
-        }
-        ++n;
-      };
       while (ok && walk.next(a))
         for (int j = 0; j < walk.n && ok; ++j) {
           const int row = walk.seq.row0 + (walk.k0 + j) * kChunk;
-          load(&k_map, kDk / 64, row, walk.head);
-          if (!kStateOnly) load(&q_map, kDk / 64, row, walk.head);
-          load(&v_map, kDv / 64, row, walk.head);
+#pragma unroll 1
+          for (int tile = 0; tile < C::kTiles; ++tile, ++n) {
+            const bool is_v = tile == C::kTiles - 1;
+            const CUtensorMap* map = is_v ? &v_map : tile == 0 ? &k_map : &q_map;
+            const int slot = n % kSlots, boxes = is_v ? kDv / 64 : kDk / 64;
+            if (n >= kSlots) ok = wait(C::kEmpty + slot, n / kSlots - 1);
+            if (!ok) break;
+            if (lane == 0) {
+              mbar_expect_tx(bar(C::kFull + slot), boxes * kBoxBytes);
+#pragma unroll 1
+              for (int b = 0; b < boxes; ++b)
+                tma_rows(base + slot * C::kSlotBytes + b * kBoxBytes, map, b * 64, walk.head, row, bar(C::kFull + slot));
+            }
+          }
         }
       // the last copies have landed before the exit, also when nobody waits for them any more
       for (int t = max(0, n - kSlots); t < n; ++t)
@@ -294,18 +311,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 13) {
       // -------------------------------------------------------------- products
       constexpr uint32_t kQkDesc = tc::idesc_bf16(kChunk, false), kVDesc = tc::idesc_bf16(kDv, true);
-      // steps of 16 tokens: eight of them but in a sequence's last chunk
+      // steps of 16 tokens: eight of them but in a sequence's last chunk.  Rolled: under elect an unrolled loop
+      // issues no faster, and the instruction cache is short.
       auto over_tokens = [&](int steps, auto step) {
-        int s = 0;
 #pragma unroll 1
-        for (; s + 4 <= steps; s += 4) {
-          step(s);
-          step(s + 1);
-          step(s + 2);
-          step(s + 3);
-        }
-#pragma unroll 1
-        for (; s < steps; ++s) step(s);
+        for (int s = 0; s < steps; ++s) step(s);
       };
       int c = 0;
       while (ok && walk.next(a))
@@ -315,27 +325,38 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t k_at = base + (t % kSlots) * C::kSlotBytes, v_at = base + (tv % kSlots) * C::kSlotBytes;
           const uint32_t v_desc = tc::desc_mn_major(v_at, kBoxBytes);
           const bool carried = walk.k0 + j > 0 || !walk.seq.fresh;  // S is not zero by construction
+          const int tq = t + 1;
+          const uint32_t q_desc = tc::desc_k_major(base + (tq % kSlots) * C::kSlotBytes), k_desc = tc::desc_k_major(k_at);
           if constexpr (!kStateOnly) {
-            const int tq = t + 1;
-            const uint32_t q_at = base + (tq % kSlots) * C::kSlotBytes;
-            const uint32_t q_desc = tc::desc_k_major(q_at), k_desc = tc::desc_k_major(k_at);
-            ok = ok && wait(C::kFull + t % kSlots, t / kSlots) && wait(C::kFull + tq % kSlots, tq / kSlots);
+            // the columns that Q K^T goes to are free when the last chunk's A has been read
+            ok = wait(C::kFull + t % kSlots, t / kSlots) && wait(C::kFull + tq % kSlots, tq / kSlots) &&
+                 (c == 0 || wait(C::kO, c - 1));
             if (!ok) break;
             if (tc::elect()) {
-#pragma unroll
+#pragma unroll 1
               for (int s = 0; s < kDk / 16; ++s) {
                 const uint32_t at = ((s / 4) * kBoxBytes + (s % 4) * 32) >> 4;
                 tc::mma_ss(tmem + kColA, q_desc + at, k_desc + at, kQkDesc, s > 0);
               }
               tc::commit(bar(C::kQk));
             }
+          }
+          ok = wait(C::kFull + tv % kSlots, tv / kSlots) && wait(C::kKeys, c);
+          if (!ok) break;
+          tc::fence_after();
+          if (tc::elect()) {
+            over_tokens(steps, [&](int s) { tc::mma_ts(tmem + kColU, tmem + kColK + 8 * s, v_desc + s * 128, kVDesc, s > 0); });
+            over_tokens(steps, [&](int s) { tc::mma_ts(tmem + kColU, tmem + kColK + 64 + 8 * s, v_desc + s * 128, kVDesc, true); });
+            tc::commit(bar(C::kULo));
+          }
+          if constexpr (!kStateOnly) {
             ok = wait(C::kS, c) && (c == 0 || wait(C::kOFree, c - 1));
             if (!ok) break;
             tc::fence_after();
             if (tc::elect()) {
               if (carried) {
                 const uint32_t hi_desc = tc::desc_mn_major(s_hi, kDk * 128), lo_desc = tc::desc_mn_major(s_lo, kDk * 128);
-#pragma unroll
+#pragma unroll 1
                 for (int s = 0; s < kDk / 16; ++s) {
                   const uint32_t at = ((s / 4) * kBoxBytes + (s % 4) * 32) >> 4;
                   tc::mma_ss(tmem + kColO, q_desc + at, hi_desc + s * 128, kVDesc, s > 0);
@@ -344,24 +365,13 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               tc::commit(bar(C::kQs));
             }
-          } else {
-            ok = wait(C::kS, c);
-            if (!ok) break;
-            tc::fence_after();
-          }
-          ok = wait(C::kFull + tv % kSlots, tv / kSlots) && wait(C::kKeys, c);
-          if (!ok) break;
-          tc::fence_after();
-          if (tc::elect()) {
-            over_tokens(steps, [&](int s) { tc::mma_ts(tmem + kColU, tmem + kColK + 8 * s, v_desc + s * 128, kVDesc, s > 0); });
-            tc::commit(bar(C::kULo));
-            over_tokens(steps, [&](int s) { tc::mma_ts(tmem + kColU, tmem + kColK + 64 + 8 * s, v_desc + s * 128, kVDesc, true); });
           }
           ok = wait(C::kKeysHi, c);
           if (!ok) break;
           tc::fence_after();
           if (tc::elect()) {
             over_tokens(steps, [&](int s) { tc::mma_ts(tmem + kColU, tmem + kColK + 8 * s, v_desc + s * 128, kVDesc, true); });
+            over_tokens(steps, [&](int s) { tc::mma_ts(tmem + kColU, tmem + kColK + 64 + 8 * s, v_desc + s * 128, kVDesc, true); });
             tc::commit(bar(C::kU));
             tc::commit(bar(C::kEmpty + t % kSlots));
             if (kStateOnly) tc::commit(bar(C::kEmpty + tv % kSlots));
@@ -372,10 +382,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc::fence_after();
             if (tc::elect()) {
               over_tokens(steps, [&](int s) {
-                const uint32_t at = tmem + kColA + 32 * (s / 2) + 8 * (s % 2);
-                if (s == 0) tc::mma_ts(tmem + kColO, at, v_desc, kVDesc, carried);
-                else tc::mma_ts(tmem + kColO, at, v_desc + s * 128, kVDesc, true);
-                tc::mma_ts(tmem + kColO, at + 16, v_desc + s * 128, kVDesc, true);
+                const uint32_t at = tmem + kColA + 16 * s;
+                tc::mma_ts(tmem + kColO, at, v_desc + s * 128, kVDesc, carried || s > 0);
+                tc::mma_ts(tmem + kColO, at + 8, v_desc + s * 128, kVDesc, true);
               });
               tc::commit(bar(C::kO));
               tc::commit(bar(C::kEmpty + tv % kSlots));
@@ -429,22 +438,37 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int d = 16; d > 0; d /= 2) whole += __shfl_xor_sync(0xffffffffu, whole, d);
           decay += whole;
-          const int buf = c & 1;
-          if (c >= 2) {
-            ok = wait(C::kDecayFree + buf, c / 2 - 1);
+          if constexpr (!kStateOnly) {
+            const int buf = c & 1;
+            if (c >= 2) {
+              ok = wait(C::kDecayFree + buf, c / 2 - 1);
+              if (!ok) break;
+            }
+            reinterpret_cast<float4*>(g_s + buf * kChunk)[lane] = make_float4(g[0], g[1], g[2], g[3]);
+            if (lane < 24)
+              reinterpret_cast<float4*>(f_s + buf * 96)[lane] = make_float4(
+                  ex2_ftz(after[0] + later), ex2_ftz(after[1] + later), ex2_ftz(after[2] + later),
+                  ex2_ftz(after[3] + later));
+            if (lane < 4) p32_s[buf * 4 + lane] = ex2_ftz(all);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(C::kDecay + buf));
+          }
+          later += __shfl_sync(0xffffffffu, beyond, lane / 8);
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = ex2_ftz(after[e] + later);
+          if (c >= 1) {
+            ok = wait(C::kWFree, c - 1);
             if (!ok) break;
           }
-          reinterpret_cast<float4*>(g_s + buf * kChunk)[lane] = make_float4(g[0], g[1], g[2], g[3]);
-          reinterpret_cast<float4*>(f_s + buf * kChunk)[lane] =
-              make_float4(exp2f(after[0] + later), exp2f(after[1] + later), exp2f(after[2] + later), exp2f(after[3] + later));
-          if (lane < 4) {
-            far_s[buf * 12 + lane] = exp2f(beyond);
-            far_s[buf * 12 + 4 + lane] = exp2f(all);
+#pragma unroll
+          for (int part = 0; part < 3; ++part) {
+            const uint32_t w01 = split_part(w[0], w[1]), w23 = split_part(w[2], w[3]);
+            reinterpret_cast<uint2*>(w_s + part * kChunk)[lane] = make_uint2(w01, w23);
           }
-          // in 64 bits: a constant decay's error would add up over all the chunks it acts on
-          if (lane == 4) far_s[buf * 12 + 8] = (float)exp2(whole);
+          if (lane == 0) *whole_s = exp2_once(whole);
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(C::kDecay + buf));
+          if (lane == 0) mbar_arrive(bar(C::kW));
         }
         if (kStateOnly && lane == 0) {
           Header h;
@@ -492,59 +516,63 @@ __global__ void __launch_bounds__(kThreads, 1)
       int c = 0;
       while (ok && walk.next(a))
         for (int j = 0; j < walk.n; ++j, ++c) {
-          const int rows = min(kChunk, walk.seq.rows - (walk.k0 + j) * kChunk);
+          const int rows = min(kChunk, walk.seq.rows - (walk.k0 + j) * kChunk), steps = (rows + 15) / 16;
           const bool carried = walk.k0 + j > 0 || !walk.seq.fresh;
+          uint32_t r[32];
           const float* g = g_s + (c & 1) * kChunk;
-          const float* f = f_s + (c & 1) * kChunk;
-          const float* p32 = far_s + (c & 1) * 12 + 4;
+          const float* f = f_s + (c & 1) * 96;
+          const float* p32 = p32_s + (c & 1) * 4;
           ok = wait(C::kDecay + (c & 1), c / 2) && wait(C::kQk, c);
           if (!ok) break;
           tc::fence_after();
+          // A step of 16 columns at a time, in place: eight columns of leading parts, eight of the rest.
           // The row's own 32 columns: 2^G_ij from the diagonal back, sums that are exact where they matter.
-          uint32_t r[32], out[32];
-          tc::ld32(r, lanes + kColA + 32 * warp);
+          uint32_t x[16];
           float sum = 0.0f;
-          tc::wait_ld();
+#pragma unroll 1
+          for (int half = 1; half >= 0; --half) {
+            const uint32_t at = lanes + kColA + 32 * warp + 16 * half;
+            const float* next = g + 32 * warp + 16 * half + 1;
+            const int left = lane - 16 * half;  // columns of this step before the row's own
+            tc::ld16(x, at);
+            tc::wait_ld();
+            uint32_t out[16];
 #pragma unroll
-          for (int e = 15; e >= 0; --e) {
-            float x[2];
-#pragma unroll
-            for (int h = 1; h >= 0; --h) {
-              const int col = 2 * e + h;
-              if (col < lane) sum += g[32 * warp + col + 1];
-              x[h] = col <= lane ? __uint_as_float(r[col]) * (ex2_ftz(sum) * a.scale) : 0.0f;
+            for (int e = 7; e >= 0; --e) {
+              if (2 * e + 1 < left) sum += next[2 * e + 1];
+              float b = 2 * e + 1 <= left ? __uint_as_float(x[2 * e + 1]) * (ex2_ftz(sum) * a.scale) : 0.0f;
+              if (2 * e < left) sum += next[2 * e];
+              float f0 = 2 * e <= left ? __uint_as_float(x[2 * e]) * (ex2_ftz(sum) * a.scale) : 0.0f;
+              out[e] = split_part(f0, b);
+              out[8 + e] = last_part(f0, b);
             }
-            out[e] = split_part(x[0], x[1]);
-            out[16 + e] = last_part(x[0], x[1]);
+            tc::st16(at, out);
           }
-          tc::st32(lanes + kColA + 32 * warp, out);
           // The 32s before it: 2^(from the 32's end to the row) times 2^(from the column to the 32's end).
           float far = ex2_ftz(sum + g[32 * warp]) * a.scale;
 #pragma unroll 1
-          for (int group = warp - 1; group >= 0; --group) {
-            tc::ld32(r, lanes + kColA + 32 * group);
-            const float4* fg = reinterpret_cast<const float4*>(f + 32 * group);
+          for (int step = 2 * warp - 1; step >= 0; --step) {
+            tc::ld16(x, lanes + kColA + 16 * step);
+            const float4* fg = reinterpret_cast<const float4*>(f + 16 * step);
             tc::wait_ld();
+            uint32_t out[16];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < 4; ++e) {
               const float4 w = fg[e];
-              float x0 = __uint_as_float(r[4 * e]) * far * w.x, x1 = __uint_as_float(r[4 * e + 1]) * far * w.y;
-              float x2 = __uint_as_float(r[4 * e + 2]) * far * w.z, x3 = __uint_as_float(r[4 * e + 3]) * far * w.w;
+              float x0 = __uint_as_float(x[4 * e]) * far * w.x, x1 = __uint_as_float(x[4 * e + 1]) * far * w.y;
+              float x2 = __uint_as_float(x[4 * e + 2]) * far * w.z, x3 = __uint_as_float(x[4 * e + 3]) * far * w.w;
               out[2 * e] = split_part(x0, x1);
-              out[16 + 2 * e] = last_part(x0, x1);
+              out[8 + 2 * e] = last_part(x0, x1);
               out[2 * e + 1] = split_part(x2, x3);
-              out[16 + 2 * e + 1] = last_part(x2, x3);
+              out[8 + 2 * e + 1] = last_part(x2, x3);
             }
-            tc::st32(lanes + kColA + 32 * group, out);
-            far *= p32[group];
+            tc::st16(lanes + kColA + 16 * step, out);
+            if (step % 2 == 0) far *= p32[step / 2];
           }
-#pragma unroll 1
-          for (int group = warp + 1; group < 4; ++group) {
-            if (32 * group >= rows) break;  // no product reads these columns
 #pragma unroll
-            for (int e = 0; e < 32; ++e) r[e] = 0;
-            tc::st32(lanes + kColA + 32 * group, r);
-          }
+          for (int e = 0; e < 16; ++e) x[e] = 0;
+#pragma unroll 1
+          for (int step = 2 * warp + 2; step < steps; ++step) tc::st16(lanes + kColA + 16 * step, x);
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(C::kDecayFree + (c & 1)));
           ok = wait(C::kQs, c);
@@ -635,8 +663,73 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int j = 0; j < walk.n; ++j, ++c) {
         const int rows = min(kChunk, q.rows - (walk.k0 + j) * kChunk), steps = (rows + 15) / 16;
-        // S for this chunk's outputs; the products of the last chunk that read the old one are done
-        // (they were issued before the update that was waited for)
+        // the keys, weighted and split: thread t has key dims t / 4 + 8 m and tokens 2 (t % 4), + 1 of each block
+        const int tk = c * C::kTiles, tv = tk + C::kTiles - 1;
+        const uint32_t k_at = base + (tk % kSlots) * C::kSlotBytes + k_row;
+        const uint32_t* weight = reinterpret_cast<const uint32_t*>(w_s) + part * 32 + (lane & 3);
+        ok = wait(C::kW, c) && wait(C::kFull + tk % kSlots, tk / kSlots);
+        if (!ok) break;
+        const float whole = *whole_s;
+        const int units = has ? min(4, (rows - part * 64 + 15) / 16) : 0;  // steps of 16 tokens here; may be < 0
+        if (rows < kChunk && has) {
+          // keys past the sequence's end, where this warp would read them: zeros (a weight of zero would
+          // not clear a NaN)
+          for (int e = lane + 4 * max(0, rows - part * 64); e < 4 * 64; e += 32) {
+            const int tok = part * 64 + e / 4, unit = ((warp & 3) % 2) * 4 + e % 4;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                             base + (tk % kSlots) * C::kSlotBytes + ((warp & 3) / 2) * kBoxBytes + tok * 128 +
+                             ((unit ^ (tok & 7)) << 4)),
+                         "r"(0)
+                         : "memory");
+          }
+          __syncwarp();
+        }
+        {
+#pragma unroll 1
+          for (int u = 0; u < units; ++u) {
+            const int t0 = part * 64 + u * 16;
+            uint32_t m[8], l[8];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t k[4];
+              ldmatrix_x4_trans(k, k_at + (2 * u + h) * 1024);
+              const uint32_t w2 = weight[64 + (2 * u + h) * 4], w3 = weight[128 + (2 * u + h) * 4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                m[h * 4 + e] = tc::mul_bf162(k[e], w2);
+                l[h * 4 + e] = tc::fma_bf162(k[e], w3, tc::fma_bf162(k[e], w2, tc::neg_bf162(m[h * 4 + e])));
+              }
+            }
+            const uint32_t to = lanes + kColK + t0 / 2;
+            tc::st_16x128b_x2(to, l[0], l[1], l[4], l[5]);
+            tc::st_16x128b_x2(to + (16u << 16), l[2], l[3], l[6], l[7]);
+            tc::st_16x128b_x2(to + 64, m[0], m[1], m[4], m[5]);
+            tc::st_16x128b_x2(to + 64 + (16u << 16), m[2], m[3], m[6], m[7]);
+          }
+        }
+        ok = wait(C::kFull + tv % kSlots, tv / kSlots);
+        if (!ok) break;
+        if (rows < steps * 16) {
+          // the last chunk's products run over whole steps of 16 tokens: values past the end are zeros
+          const uint32_t v_at = base + (tv % kSlots) * C::kSlotBytes;
+          for (int e = tid - 128; e < (steps * 16 - rows) * (kDv / 8); e += 256) {
+            const int row = rows + e / (kDv / 8), unit = e % (kDv / 8);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_at + (unit / 8) * kBoxBytes + row * 128 +
+                                                                          (unit % 8) * 16),
+                         "r"(0)
+                         : "memory");
+          }
+          fence_async_shared();
+        }
+        tc::wait_st();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::kKeys));
+        // S for this chunk's outputs, over the one that the last chunk's have read
+        if (!kStateOnly) {
+          if (c > 0) ok = wait(C::kQs, c - 1);
+          if (!ok) break;
+        }
         if (!kStateOnly && has) {
           const uint32_t row_at = ((part * kCols) / 64) * (kDk * 128) + dk * 128;
           const int unit0 = ((part * kCols) % 64) / 8;
@@ -659,95 +752,36 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           fence_async_shared();
         }
-        tc::fence_before();  // after the reads of U
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::kS));
-
-        // the keys, weighted and split: thread t has key dims t / 4 + 8 m and tokens 2 (t % 4), + 1 of each block
-        const int tk = c * C::kTiles, tv = tk + C::kTiles - 1;
-        const uint32_t k_at = base + (tk % kSlots) * C::kSlotBytes + k_row;
-        const float2* weight = reinterpret_cast<const float2*>(f_s + (c & 1) * kChunk + part * 64) + (lane & 3);
-        const float* far = far_s + (c & 1) * 12;
-        ok = wait(C::kDecay + (c & 1), c / 2) && wait(C::kFull + tk % kSlots, tk / kSlots);
-        if (!ok) break;
-        const float whole = far[8];
-        // eight tokens of the warp's 32 key dims, weighted: x and y are tokens tok and tok + 1
-        auto weighted = [&](int block, auto put) {
-          uint32_t f[4];
-          ldmatrix_x4_trans(f, k_at + block * 1024);
-          const float2 w = weight[block * 4];
-          const float to_end = far[part * 2 + block / 4], wx = w.x * to_end, wy = w.y * to_end;
-#pragma unroll
-          for (int m = 0; m < 4; ++m) put(m, bf16lo_to_f32(f[m]) * wx, bf16hi_to_f32(f[m]) * wy);
-        };
-        const int units = has ? min(4, (rows - part * 64 + 15) / 16) : 0;  // steps of 16 tokens here; may be < 0
-        if (rows < kChunk && has) {
-          // keys past the sequence's end, where this warp would read them: zeros (a weight of zero would
-          // not clear a NaN)
-          for (int e = lane + 4 * max(0, rows - part * 64); e < 4 * 64; e += 32) {
-            const int tok = part * 64 + e / 4, unit = ((warp & 3) % 2) * 4 + e % 4;
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
-                             base + (tk % kSlots) * C::kSlotBytes + ((warp & 3) / 2) * kBoxBytes + tok * 128 +
-                             ((unit ^ (tok & 7)) << 4)),
-                         "r"(0)
-                         : "memory");
-          }
+        if (!kStateOnly) {
           __syncwarp();
+          if (lane == 0) mbar_arrive(bar(C::kS));
         }
-        {
-#pragma unroll 1
-          for (int u = 0; u < units; ++u) {
-            const int t0 = part * 64 + u * 16;
-            uint32_t mid[8], lo[8];
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              weighted(2 * u + h, [&](int m, float x, float y) {
-                (void)split_part(x, y);
-                mid[h * 4 + m] = split_part(x, y);
-                lo[h * 4 + m] = last_part(x, y);
-              });
-            const uint32_t to = lanes + kColK + t0 / 2;
-            tc::st_16x128b_x2(to, lo[0], lo[1], lo[4], lo[5]);
-            tc::st_16x128b_x2(to + (16u << 16), lo[2], lo[3], lo[6], lo[7]);
-            tc::st_16x128b_x2(to + 64, mid[0], mid[1], mid[4], mid[5]);
-            tc::st_16x128b_x2(to + 64 + (16u << 16), mid[2], mid[3], mid[6], mid[7]);
-          }
-        }
-        ok = wait(C::kFull + tv % kSlots, tv / kSlots);
-        if (!ok) break;
-        if (rows < steps * 16) {
-          // the last chunk's products run over whole steps of 16 tokens: values past the end are zeros
-          const uint32_t v_at = base + (tv % kSlots) * C::kSlotBytes;
-          for (int e = tid - 128; e < (steps * 16 - rows) * (kDv / 8); e += 256) {
-            const int row = rows + e / (kDv / 8), unit = e % (kDv / 8);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_at + (unit / 8) * kBoxBytes + row * 128 +
-                                                                          (unit % 8) * 16),
-                         "r"(0)
-                         : "memory");
-          }
-          fence_async_shared();
-        }
-        tc::wait_st();
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::kKeys));
         ok = wait(C::kULo, c);
         if (!ok) break;
         tc::fence_after();
-        // the leading parts, in the place of the smallest: computed again rather than held, which would not
-        // leave S enough registers
+        // the larger parts in their place
 #pragma unroll 1
         for (int u = 0; u < units; ++u) {
-          uint32_t p[8];
+          uint32_t p1[8], p2[8];
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            weighted(2 * u + h, [&](int m, float x, float y) { p[h * 4 + m] = last_part(x, y); });
+          for (int h = 0; h < 2; ++h) {
+            uint32_t k[4];
+            ldmatrix_x4_trans(k, k_at + (2 * u + h) * 1024);
+            const uint32_t w1 = weight[(2 * u + h) * 4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              p1[h * 4 + e] = tc::mul_bf162(k[e], w1);
+              p2[h * 4 + e] = tc::fma_bf162(k[e], w1, tc::neg_bf162(p1[h * 4 + e]));
+            }
+          }
           const uint32_t to = lanes + kColK + (part * 64 + u * 16) / 2;
-          tc::st_16x128b_x2(to, p[0], p[1], p[4], p[5]);
-          tc::st_16x128b_x2(to + (16u << 16), p[2], p[3], p[6], p[7]);
+          tc::st_16x128b_x2(to, p2[0], p2[1], p2[4], p2[5]);
+          tc::st_16x128b_x2(to + (16u << 16), p2[2], p2[3], p2[6], p2[7]);
+          tc::st_16x128b_x2(to + 64, p1[0], p1[1], p1[4], p1[5]);
+          tc::st_16x128b_x2(to + 64 + (16u << 16), p1[2], p1[3], p1[6], p1[7]);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::kDecayFree + (c & 1)));
+        if (lane == 0) mbar_arrive(bar(C::kWFree));
         tc::wait_st();
         tc::fence_before();
         __syncwarp();

@@ -23,7 +23,7 @@ ASTERQ_DEVICE void fence_after() { asm volatile("tcgen05.fence::after_thread_syn
 ASTERQ_DEVICE void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 ASTERQ_DEVICE void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// thread i of the warp <-> lane i, 32 (16, 8) consecutive columns
+// thread i of the warp <-> lane i, 32 or 16 consecutive columns
 ASTERQ_DEVICE void ld32(uint32_t (&r)[32], uint32_t addr) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -44,6 +44,20 @@ ASTERQ_DEVICE void st32(uint32_t addr, const uint32_t (&r)[32]) {
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
       "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+ASTERQ_DEVICE void ld16(uint32_t (&r)[16], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+ASTERQ_DEVICE void st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 // 16 lanes from the address's on, four columns twice over: thread t <-> lanes t / 4 and t / 4 + 8, column
@@ -68,6 +82,19 @@ ASTERQ_DEVICE uint32_t desc_k_major(uint32_t smem) { return ((smem & 0x3ffff) >>
 ASTERQ_DEVICE uint32_t desc_mn_major(uint32_t smem, uint32_t box_bytes) {
   return ((smem & 0x3ffff) >> 4) | ((box_bytes >> 4) << 16);
 }
+// packed bf16 arithmetic, rounded once
+ASTERQ_DEVICE uint32_t mul_bf162(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+ASTERQ_DEVICE uint32_t fma_bf162(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+ASTERQ_DEVICE uint32_t neg_bf162(uint32_t a) { return a ^ 0x80008000u; }
+
 // bf16 x bf16 -> fp32, A K-major, M = 128
 constexpr uint32_t idesc_bf16(int n, bool b_mn_major) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n / 8) << 17) |
