@@ -19,14 +19,15 @@
 //
 // Work.  One persistent CTA an SM takes an equal, contiguous share of all (sequence, head, chunk)s.
 // Where a share ends inside a (sequence, head), the state there has to come from the chunks before:
-// a first pass computes what each such piece adds to a state of zeros (keys and values only), a small
-// kernel chains the pieces of a (sequence, head), and the main pass starts each piece from its state.
+// a first pass computes what these chunks add to a state of zeros (keys and values only), itself cut into
+// equal shares, a small kernel chains the parts of each (sequence, head), and the main pass starts each of
+// its pieces from its state.
 //
 // Roles in a CTA (512 threads): warps 0-3 turn Q K^T into A (row i = thread i) and write the output;
 // warps 4-11 hold S in registers (thread = key dim, half of the value dims), scale and split the keys
 // and update S; warp 12 loads by TMA; warp 13 issues all products; warp 14 sums the decays, a chunk
-// ahead; warp 15 stores whole chunks of outputs by TMA.  Warps 4-11 take registers of the last four (at
-// 128 a thread S would spill to local memory).
+// ahead; warp 15 completes the warpgroup whose registers warps 4-11 take (at 128 a thread S would spill to
+// local memory).
 #include <cuda.h>
 
 #include "linear.cuh"
@@ -37,7 +38,8 @@ namespace lin {
 namespace {
 
 constexpr int kChunk = 128;
-constexpr int kSlots = 5;       // tiles of 128 tokens in flight or in use
+constexpr int kSlots = 5;       // tiles of 128 tokens in shared memory: two of keys, two of values, one of queries
+constexpr int kQSlot = 4;
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kRegsA = 96, kRegsS = 168, kRegsIssue = 80;
@@ -48,17 +50,22 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // tensor memory columns
 constexpr uint32_t kColA = 0, kColO = 128, kColU = 256, kColK = 384;
 
-// what the first pass leaves of each worker's last piece, when that ends inside a (sequence, head)
-struct Header {
-  double decay;  // log2 of the piece's whole decay
-  int kind;      // 0: no such piece, 1: the (sequence, head)'s first piece, 2: a later one
+// A part of the first pass: some chunks of one (sequence, head), from a state of zeros.
+struct Part {
+  float decay;   // over all of them
   int slot, head, fresh;
+  int next;      // the (sequence, head)'s next part, or -1
+  int border;    // the border of shares that the part reaches, or -1
 };
 
+// Border w is between the main pass's shares w - 1 and w.
 struct Work {
-  Header* headers;  // [workers]
-  float* pieces;    // [workers][Dk][Dv]: the pieces' own sums, then the states after them
-  float* starts;    // [workers][Dk][Dv]: first pieces' initial states (their slot may be rewritten meanwhile)
+  Part* parts;     // [2 workers]
+  int* first;      // [workers] the first part of the (sequence, head) whose first cut is border w, or -1
+  float* sums;     // [2 workers][Dk][Dv]: what the parts add
+  float* borders;  // [workers][Dk][Dv]: the state at border w
+  float* starts;   // [workers][Dk][Dv]: the initial state of the (sequence, head) whose first cut is border w (its
+                   // slot may be rewritten while the main pass still wants it)
 };
 
 struct Seq {
@@ -96,21 +103,60 @@ struct Walk {
   }
 };
 
+// The same for the first pass: the chunks before each border that is inside a (sequence, head), back to the
+// border before or the (sequence, head)'s start, laid end to end.
+struct FirstWalk {
+  int x, end;  // this CTA's share
+  const int* before;     // [W + 1] chunks in front of those of border w
+  const int* position;   // [W] the borders themselves
+  const int* sequence;   // [W] the sequence that border w is in, and its first chunk
+  const int* seq_start;
+  int w;       // the border that the current piece belongs to
+  Seq seq;
+  int head, k0, n;
+  ASTERQ_DEVICE bool next(const Args& a) {
+    if (x >= end) return false;
+    while (x >= before[w + 1]) ++w;
+    seq = seq_of(a, sequence[w]);
+    const int at = position[w] - (before[w + 1] - x) - seq_start[w];
+    head = at / seq.chunks;
+    k0 = at - head * seq.chunks;
+    n = min(before[w + 1], end) - x;
+    x += n;
+    return true;
+  }
+};
+template <bool kStateOnly>
+struct WalkOf {
+  using type = Walk;
+};
+template <>
+struct WalkOf<true> {
+  using type = FirstWalk;
+};
+
 template <int kDk, int kDv, bool kStateOnly>
 struct Cfg {
-  static constexpr int kTiles = kStateOnly ? 2 : 3;  // tiles of a chunk: K, (Q,) V
   static constexpr int kMaxD = kDk > kDv ? kDk : kDv;
   static constexpr int kSlotBytes = kMaxD / 64 * kBoxBytes;
   static constexpr int kStateBytes = kStateOnly ? 0 : kDk * kDv * 2;  // one bf16 part
   // barriers
   static constexpr int kFull = 0, kEmpty = kSlots, kQk = 2 * kSlots, kQs = kQk + 1, kULo = kQk + 2, kU = kQk + 3,
                        kO = kQk + 4, kKeys = kQk + 5, kKeysHi = kQk + 6, kS = kQk + 7, kA = kQk + 8,
-                       kOFree = kQk + 9, kOut = kQk + 10, kDrain = kQk + 11, kDecay = kQk + 12,
-                       kDecayFree = kQk + 14, kW = kQk + 16, kWFree = kQk + 17, kBars = kQk + 18;
-  static constexpr int kMiscBytes = 2 * (kChunk + 96) * 4 + 2 * 4 * 4 + 3 * kChunk * 2 + 16 + kBars * 8 + 24 * 4;
+                       kOFree = kQk + 9, kDrain = kQk + 10, kW = kQk + 11, kWFree = kQk + 12, kDecay = kQk + 13,
+                       kDecayFree = kQk + 15, kBars = kQk + 17;
+  static constexpr int kMiscBytes = 2 * (kChunk + 96) * 4 + 4 * 4 * 4 + 3 * kChunk * 2 + 16 + kBars * 8 + 24 * 4;
   static_assert(kWarps <= 16, "scan_s");
-  static constexpr int kSmem = kSlots * kSlotBytes + 2 * kStateBytes + kMiscBytes;
+  static constexpr int kTableBytes = kStateOnly ? (4 * kThreads + 2) * 4 : 0;  // FirstWalk's arrays
+  static constexpr int kSmem = kSlots * kSlotBytes + 2 * kStateBytes + kMiscBytes + kTableBytes;
 };
+
+// The slot of a chunk's keys or values, and how many tiles it held before.  (Queries: slot kQSlot, use c.)
+struct Place {
+  int slot, use;
+};
+ASTERQ_DEVICE Place keys_of(int c) { return {2 * (c & 1), c / 2}; }
+ASTERQ_DEVICE Place values_of(int c) { return {2 * (c & 1) + 1, c / 2}; }
 
 ASTERQ_DEVICE void tma_rows(uint32_t dst, const CUtensorMap* map, int x, int head, int row, uint32_t bar) {
   asm volatile(
@@ -145,6 +191,12 @@ ASTERQ_DEVICE uint32_t split_part(float& x, float& y) {
   return p;
 }
 
+ASTERQ_DEVICE void st_global_32(void* p, const uint32_t (&r)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
 // 2^x of a whole chunk's decay to fp32's last bit: a constant decay's error would add up over all the chunks
 // it acts on.  x = n + r with |r| <= 1/2, 2^r by the series of e^(r ln 2), whose tenth term is below 2^-36.
 ASTERQ_DEVICE float exp2_once(double x) {
@@ -159,17 +211,18 @@ ASTERQ_DEVICE float exp2_once(double x) {
 template <int kDk, int kDv, bool kStateOnly>
 __global__ void __launch_bounds__(kThreads, 1)
     chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
-                 const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap o_map,
-                 const __grid_constant__ Args a, const __grid_constant__ Work work) {
+                 const __grid_constant__ CUtensorMap v_map, const __grid_constant__ Args a,
+                 const __grid_constant__ Work work) {
   using C = Cfg<kDk, kDv, kStateOnly>;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
   const uint32_t s_hi = base + kSlots * C::kSlotBytes, s_lo = s_hi + C::kStateBytes;
   // decays of a chunk (log2 of a token's, and what follows from them), by warp 14
-  float* g_s = reinterpret_cast<float*>(smem + kSlots * C::kSlotBytes + 2 * C::kStateBytes);  // [2][kChunk]
+  float* g_s = reinterpret_cast<float*>(smem + kSlots * C::kSlotBytes + 2 * C::kStateBytes);  // [2][kChunk], of the token after
   float* f_s = g_s + 2 * kChunk;  // [2][96]: 2^(from a token of the first three 32s to the end of its 32)
   float* p32_s = f_s + 2 * 96;    // [2][4]: 2^(each 32's decay)
-  uint16_t* w_s = reinterpret_cast<uint16_t*>(p32_s + 8);        // [3][kChunk]: bf16 parts of the weight to the chunk's end
+  float* first_s = p32_s + 8;     // [2][4]: decays (log2) of each 32's first token
+  uint16_t* w_s = reinterpret_cast<uint16_t*>(first_s + 8);      // [3][kChunk]: bf16 parts of the weight to the chunk's end
   float* whole_s = reinterpret_cast<float*>(w_s + 3 * kChunk);  // [4], one used: 2^(the chunk's decay)
   uint64_t* bars_s = reinterpret_cast<uint64_t*>(whole_s + 4);
   int* scan_s = reinterpret_cast<int*>(bars_s + C::kBars);  // [16]
@@ -177,6 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int* abort_s = start_s + 2;
   int* never_s = abort_s + 1;  // stays 0: the flag of waits that an abort must not cut short
   uint32_t* tmem_s = reinterpret_cast<uint32_t*>(abort_s + 2);
+  [[maybe_unused]] int* table_s = abort_s + 6;
   const uint32_t bars = smem_u32(bars_s);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   auto bar = [&](int i) { return bars + 8 * i; };
@@ -192,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i : {C::kQk, C::kQs, C::kULo, C::kU, C::kO, C::kDrain, C::kDecay, C::kDecay + 1, C::kW}) mbar_init(bar(i), 1);
     for (int i : {C::kKeys, C::kKeysHi, C::kS, C::kWFree}) mbar_init(bar(i), 8);
-    for (int i : {C::kA, C::kOFree, C::kOut}) mbar_init(bar(i), 4);
+    for (int i : {C::kA, C::kOFree}) mbar_init(bar(i), 4);
     for (int i : {C::kDecayFree, C::kDecayFree + 1}) mbar_init(bar(i), 4);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     *abort_s = 0;
@@ -220,21 +274,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   const int me = blockIdx.x;
   const int W = max(1, min((int)gridDim.x, (total + kMinShare - 1) / kMinShare));
-  Walk walk;
-  walk.x = me < W ? (int)((long long)total * me / W) : total;
-  walk.end = me < W ? (int)((long long)total * (me + 1) / W) : total;
-  if (walk.x < walk.end && before <= walk.x && walk.x < before + sum) {
-    int s = s0, at = before;
-    while (true) {
-      const int here = seq_of(a, s).chunks * a.n_heads;
-      if (walk.x < at + here) break;
-      at += here;
-      ++s;
+  auto border = [&](int w) { return (int)((long long)total * w / W); };
+  typename WalkOf<kStateOnly>::type walk;
+  if constexpr (!kStateOnly) {
+    walk.x = me < W ? border(me) : total;
+    walk.end = me < W ? border(me + 1) : total;
+    if (walk.x < walk.end && before <= walk.x && walk.x < before + sum) {
+      int s = s0, at = before;
+      while (true) {
+        const int here = seq_of(a, s).chunks * a.n_heads;
+        if (walk.x < at + here) break;
+        at += here;
+        ++s;
+      }
+      start_s[0] = s;
+      start_s[1] = at;
     }
-    start_s[0] = s;
-    start_s[1] = at;
-  }
-  if (!kStateOnly) {
     // rows of empty slots are zeros; ranges out of bounds are reported
     for (int s = me; s < a.n_seqs; s += gridDim.x) {
       const Seq q = seq_of(a, s);
@@ -246,32 +301,71 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (long long i = tid; i < (long long)q.rows * a.n_heads * (kDv / 8); i += kThreads)
         dst[i] = make_uint4(0, 0, 0, 0);
     }
-  }
-  __syncthreads();
-  if (walk.x < walk.end) {
+    __syncthreads();
+    if (walk.x >= walk.end) return;
     walk.s = start_s[0];
     walk.seq_start = start_s[1];
     walk.seq = seq_of(a, walk.s);
-  }
-  if (kStateOnly) {
-    // only the share's last piece, when its (sequence, head) goes on in the next share
-    bool cut = false;
-    if (walk.x < walk.end) {
-      Walk last = walk;
-      while (true) {
-        Walk step = last;
-        if (!step.next(a)) break;
-        walk = last;
-        last = step;
-        cut = step.k0 + step.n < step.seq.chunks;
+  } else {
+    // Thread w looks where border w is and how many chunks before it the first pass needs.
+    int* strips = reinterpret_cast<int*>(smem);  // the tiles' place, not used yet: [kThreads]
+    int* tables = table_s;                       // 4 arrays of kThreads + 1
+    strips[tid] = before;
+    __syncthreads();
+    const int w = tid;
+    int need = 0, s = 0, at = 0, unit = 0;
+    if (w > 0 && w < W) {
+      const int pos = border(w);
+      int lo = 0, hi = kThreads - 1;
+      while (lo < hi) {  // the last strip that starts at pos or before
+        const int mid = (lo + hi + 1) / 2;
+        if (strips[mid] <= pos) lo = mid;
+        else hi = mid - 1;
       }
+      s = lo * strip;
+      at = strips[lo];
+      int chunks;
+      while (true) {
+        chunks = seq_of(a, s).chunks;
+        if (pos < at + chunks * a.n_heads) break;
+        at += chunks * a.n_heads;
+        ++s;
+      }
+      unit = pos - (pos - at) % chunks;
+      if (unit < pos) need = pos - max(border(w - 1), unit);
     }
-    if (!cut) {
-      if (tid == 0) work.headers[me].kind = 0;
-      return;
+    scan = need;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int up = __shfl_up_sync(0xffffffffu, scan, d);
+      if (lane >= d) scan += up;
     }
-  } else if (walk.x >= walk.end) {
-    return;
+    if (lane == 31) scan_s[warp] = scan;
+    __syncthreads();
+    int ahead = scan - need, all = 0;
+    for (int i = 0; i < kWarps; ++i) {
+      if (i < warp) ahead += scan_s[i];
+      all += scan_s[i];
+    }
+    tables[w] = ahead;
+    if (w == kThreads - 1) tables[kThreads] = all;
+    tables[kThreads + 1 + w] = border(min(w, W));
+    tables[2 * kThreads + 1 + w] = s;
+    tables[3 * kThreads + 1 + w] = at;
+    // part i of worker m at border w is number w + m: both go up together along the chunks
+    if (w == me && w < (int)gridDim.x) {
+      const bool starts = need > 0 && unit >= border(w - 1);
+      work.first[w] = starts ? w + (int)(((long long)(ahead + 1) * W - 1) / all) : -1;
+    }
+    __syncthreads();
+    walk.x = me < W ? (int)((long long)all * me / W) : all;
+    walk.end = me < W ? (int)((long long)all * (me + 1) / W) : all;
+    if (walk.x >= walk.end) return;
+    walk.before = tables;
+    walk.position = tables + kThreads + 1;
+    walk.sequence = tables + 2 * kThreads + 1;
+    walk.seq_start = tables + 3 * kThreads + 1;
+    walk.w = 0;
   }
 
   if (warp == 13) tc::alloc512(smem_u32(tmem_s));
@@ -286,28 +380,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
     if (warp == 12) {
       // -------------------------------------------------------------- loads
-      int n = 0;
+      int c = 0;
       while (ok && walk.next(a))
-        for (int j = 0; j < walk.n && ok; ++j) {
+        for (int j = 0; j < walk.n && ok; ++j, ++c) {
           const int row = walk.seq.row0 + (walk.k0 + j) * kChunk;
 #pragma unroll 1
-          for (int tile = 0; tile < C::kTiles; ++tile, ++n) {
-            const bool is_v = tile == C::kTiles - 1;
-            const CUtensorMap* map = is_v ? &v_map : tile == 0 ? &k_map : &q_map;
-            const int slot = n % kSlots, boxes = is_v ? kDv / 64 : kDk / 64;
-            if (n >= kSlots) ok = wait(C::kEmpty + slot, n / kSlots - 1);
+          for (int tile = 0; tile < (kStateOnly ? 2 : 3); ++tile) {
+            const Place at = tile == 0 ? keys_of(c) : tile == 1 ? values_of(c) : Place{kQSlot, c};
+            const CUtensorMap* map = tile == 0 ? &k_map : tile == 1 ? &v_map : &q_map;
+            const int boxes = tile == 1 ? kDv / 64 : kDk / 64;
+            if (at.use > 0) ok = wait(C::kEmpty + at.slot, at.use - 1);
             if (!ok) break;
             if (lane == 0) {
-              mbar_expect_tx(bar(C::kFull + slot), boxes * kBoxBytes);
+              mbar_expect_tx(bar(C::kFull + at.slot), boxes * kBoxBytes);
 #pragma unroll 1
               for (int b = 0; b < boxes; ++b)
-                tma_rows(base + slot * C::kSlotBytes + b * kBoxBytes, map, b * 64, walk.head, row, bar(C::kFull + slot));
+                tma_rows(base + at.slot * C::kSlotBytes + b * kBoxBytes, map, b * 64, walk.head, row,
+                         bar(C::kFull + at.slot));
             }
           }
         }
-      // the last copies have landed before the exit, also when nobody waits for them any more
-      for (int t = max(0, n - kSlots); t < n; ++t)
-        (void)mbar_wait(bar(C::kFull + t % kSlots), (t / kSlots) & 1, never_s, 200000000);
+      // the last copies have landed before the exit, also when nobody waits for them any more (the slots'
+      // last uses: of the chunk before this one, whichever was reached)
+      if (!ok) {
+        for (int last = max(0, c - 2); last <= c; ++last) {
+          (void)mbar_wait(bar(C::kFull + keys_of(last).slot), keys_of(last).use & 1, never_s, 200000000);
+          (void)mbar_wait(bar(C::kFull + values_of(last).slot), values_of(last).use & 1, never_s, 200000000);
+          if (!kStateOnly) (void)mbar_wait(bar(C::kFull + kQSlot), last & 1, never_s, 200000000);
+        }
+      }
     } else if (warp == 13) {
       // -------------------------------------------------------------- products
       constexpr uint32_t kQkDesc = tc::idesc_bf16(kChunk, false), kVDesc = tc::idesc_bf16(kDv, true);
@@ -317,31 +418,32 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int s = 0; s < steps; ++s) step(s);
       };
+      // The order of a chunk's products follows the state warps, on whose loop everything waits: the smaller
+      // parts of the keys; A V of the chunk before (its A is made by now) while they make the larger parts;
+      // those; and Q K^T and Q S while they update S and weigh the next keys.
+      int last_steps = 0, last_carried = 0;
+      auto a_times_v = [&](int c) {
+        ok = wait(C::kA, c);
+        if (!ok) return;
+        tc::fence_after();
+        if (tc::elect()) {
+          const uint32_t v_desc = tc::desc_mn_major(base + values_of(c).slot * C::kSlotBytes, kBoxBytes);
+          over_tokens(last_steps, [&](int s) {
+            const uint32_t at = tmem + kColA + 16 * s;
+            tc::mma_ts(tmem + kColO, at, v_desc + s * 128, kVDesc, last_carried || s > 0);
+            tc::mma_ts(tmem + kColO, at + 8, v_desc + s * 128, kVDesc, true);
+          });
+          tc::commit(bar(C::kO));
+          tc::commit(bar(C::kEmpty + values_of(c).slot));
+        }
+      };
       int c = 0;
       while (ok && walk.next(a))
         for (int j = 0; j < walk.n; ++j, ++c) {
           const int rows = min(kChunk, walk.seq.rows - (walk.k0 + j) * kChunk), steps = (rows + 15) / 16;
-          const int t = c * C::kTiles, tv = t + C::kTiles - 1;
-          const uint32_t k_at = base + (t % kSlots) * C::kSlotBytes, v_at = base + (tv % kSlots) * C::kSlotBytes;
-          const uint32_t v_desc = tc::desc_mn_major(v_at, kBoxBytes);
-          const bool carried = walk.k0 + j > 0 || !walk.seq.fresh;  // S is not zero by construction
-          const int tq = t + 1;
-          const uint32_t q_desc = tc::desc_k_major(base + (tq % kSlots) * C::kSlotBytes), k_desc = tc::desc_k_major(k_at);
-          if constexpr (!kStateOnly) {
-            // the columns that Q K^T goes to are free when the last chunk's A has been read
-            ok = wait(C::kFull + t % kSlots, t / kSlots) && wait(C::kFull + tq % kSlots, tq / kSlots) &&
-                 (c == 0 || wait(C::kO, c - 1));
-            if (!ok) break;
-            if (tc::elect()) {
-#pragma unroll 1
-              for (int s = 0; s < kDk / 16; ++s) {
-                const uint32_t at = ((s / 4) * kBoxBytes + (s % 4) * 32) >> 4;
-                tc::mma_ss(tmem + kColA, q_desc + at, k_desc + at, kQkDesc, s > 0);
-              }
-              tc::commit(bar(C::kQk));
-            }
-          }
-          ok = wait(C::kFull + tv % kSlots, tv / kSlots) && wait(C::kKeys, c);
+          const Place kp = keys_of(c), vp = values_of(c);
+          const uint32_t v_desc = tc::desc_mn_major(base + vp.slot * C::kSlotBytes, kBoxBytes);
+          ok = wait(C::kFull + vp.slot, vp.use) && wait(C::kKeys, c);
           if (!ok) break;
           tc::fence_after();
           if (tc::elect()) {
@@ -349,7 +451,37 @@ __global__ void __launch_bounds__(kThreads, 1)
             over_tokens(steps, [&](int s) { tc::mma_ts(tmem + kColU, tmem + kColK + 64 + 8 * s, v_desc + s * 128, kVDesc, true); });
             tc::commit(bar(C::kULo));
           }
+          if (!kStateOnly && c > 0) a_times_v(c - 1);
+          ok = ok && wait(C::kKeysHi, c);
+          if (!ok) break;
+          tc::fence_after();
+          if (tc::elect()) {
+            over_tokens(steps, [&](int s) { tc::mma_ts(tmem + kColU, tmem + kColK + 8 * s, v_desc + s * 128, kVDesc, true); });
+            over_tokens(steps, [&](int s) { tc::mma_ts(tmem + kColU, tmem + kColK + 64 + 8 * s, v_desc + s * 128, kVDesc, true); });
+            tc::commit(bar(C::kU));
+            if (kStateOnly) {
+              tc::commit(bar(C::kEmpty + kp.slot));
+              tc::commit(bar(C::kEmpty + vp.slot));
+            }
+          }
+          const uint32_t q_desc = tc::desc_k_major(base + kQSlot * C::kSlotBytes);
           if constexpr (!kStateOnly) {
+            // the columns that Q K^T goes to are free when the last chunk's A has been read
+            ok = wait(C::kFull + kp.slot, kp.use) && wait(C::kFull + kQSlot, c) && (c == 0 || wait(C::kO, c - 1));
+            if (!ok) break;
+            if (tc::elect()) {
+              const uint32_t k_desc = tc::desc_k_major(base + kp.slot * C::kSlotBytes);
+#pragma unroll 1
+              for (int s = 0; s < kDk / 16; ++s) {
+                const uint32_t at = ((s / 4) * kBoxBytes + (s % 4) * 32) >> 4;
+                tc::mma_ss(tmem + kColA, q_desc + at, k_desc + at, kQkDesc, s > 0);
+              }
+              tc::commit(bar(C::kQk));
+              tc::commit(bar(C::kEmpty + kp.slot));
+            }
+          }
+          if constexpr (!kStateOnly) {
+            const bool carried = walk.k0 + j > 0 || !walk.seq.fresh;  // S is not zero by construction
             ok = wait(C::kS, c) && (c == 0 || wait(C::kOFree, c - 1));
             if (!ok) break;
             tc::fence_after();
@@ -364,33 +496,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
               }
               tc::commit(bar(C::kQs));
+              tc::commit(bar(C::kEmpty + kQSlot));
             }
-          }
-          ok = wait(C::kKeysHi, c);
-          if (!ok) break;
-          tc::fence_after();
-          if (tc::elect()) {
-            over_tokens(steps, [&](int s) { tc::mma_ts(tmem + kColU, tmem + kColK + 8 * s, v_desc + s * 128, kVDesc, true); });
-            over_tokens(steps, [&](int s) { tc::mma_ts(tmem + kColU, tmem + kColK + 64 + 8 * s, v_desc + s * 128, kVDesc, true); });
-            tc::commit(bar(C::kU));
-            tc::commit(bar(C::kEmpty + t % kSlots));
-            if (kStateOnly) tc::commit(bar(C::kEmpty + tv % kSlots));
-          }
-          if constexpr (!kStateOnly) {
-            ok = wait(C::kA, c);
-            if (!ok) break;
-            tc::fence_after();
-            if (tc::elect()) {
-              over_tokens(steps, [&](int s) {
-                const uint32_t at = tmem + kColA + 16 * s;
-                tc::mma_ts(tmem + kColO, at, v_desc + s * 128, kVDesc, carried || s > 0);
-                tc::mma_ts(tmem + kColO, at + 8, v_desc + s * 128, kVDesc, true);
-              });
-              tc::commit(bar(C::kO));
-              tc::commit(bar(C::kEmpty + tv % kSlots));
-            }
+            last_steps = steps;
+            last_carried = carried;
           }
         }
+      if (!kStateOnly && ok) a_times_v(c - 1);
       // every product and every arrival above is done before the tensor memory goes back
       if (tc::elect()) tc::commit(bar(C::kDrain));
       (void)mbar_wait(bar(C::kDrain), 0, never_s);
@@ -444,7 +556,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               ok = wait(C::kDecayFree + buf, c / 2 - 1);
               if (!ok) break;
             }
-            reinterpret_cast<float4*>(g_s + buf * kChunk)[lane] = make_float4(g[0], g[1], g[2], g[3]);
+            const float after_lane = __shfl_down_sync(0xffffffffu, g[0], 1);
+            reinterpret_cast<float4*>(g_s + buf * kChunk)[lane] = make_float4(g[1], g[2], g[3], after_lane);
+            if (lane % 8 == 0) first_s[buf * 4 + lane / 8] = g[0];
             if (lane < 24)
               reinterpret_cast<float4*>(f_s + buf * 96)[lane] = make_float4(
                   ex2_ftz(after[0] + later), ex2_ftz(after[1] + later), ex2_ftz(after[2] + later),
@@ -470,41 +584,29 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(C::kW));
         }
-        if (kStateOnly && lane == 0) {
-          Header h;
-          h.decay = decay;
-          h.kind = walk.k0 == 0 ? 1 : 2;
-          h.slot = walk.seq.slot;
-          h.head = walk.head;
-          h.fresh = walk.seq.fresh;
-          work.headers[me] = h;
-        }
-      }
-    } else {
-      // -------------------------------------------------------------- whole chunks of outputs
-      // They are staged where the chunk's queries were, which nothing reads any more.
-      if constexpr (!kStateOnly) {
-        int c = 0;
-        while (ok && walk.next(a))
-          for (int j = 0; j < walk.n; ++j, ++c) {
-            const int slot = (c * C::kTiles + 1) % kSlots, row = walk.seq.row0 + (walk.k0 + j) * kChunk;
-            ok = wait(C::kOut, c);
-            if (!ok) break;
-            if (lane == 0) {
-              if (walk.seq.rows - (walk.k0 + j) * kChunk >= kChunk) {
-                for (int b = 0; b < kDv / 64; ++b)
-                  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
-                                   &o_map),
-                               "r"(b * 64), "r"(walk.head), "r"(row), "r"(base + slot * C::kSlotBytes + b * kBoxBytes)
-                               : "memory");
-                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-              }
-              mbar_arrive(bar(C::kEmpty + slot));
+        if constexpr (kStateOnly) {
+          if (lane == 0) {
+            const int w = walk.w, at_border = walk.x == walk.before[w + 1];
+            Part p;
+            p.decay = exp2_once(decay);
+            p.slot = walk.seq.slot;
+            p.head = walk.head;
+            p.fresh = walk.seq.fresh;
+            p.border = at_border ? w : -1;
+            const int all = walk.before[kThreads];
+            auto worker_of = [&](int x) { return (int)(((long long)(x + 1) * W - 1) / all); };
+            p.next = at_border ? -1 : w + worker_of(walk.x);
+            if (at_border) {
+              // the (sequence, head) goes on to the next border, or ends before it
+              const int unit = walk.position[w] - walk.k0 - walk.n;
+              const bool more = w + 1 < W && walk.before[w + 2] > walk.before[w + 1] &&
+                                walk.position[w + 1] < unit + walk.seq.chunks;
+              p.next = more ? w + 1 + worker_of(walk.x) : -1;
             }
+            work.parts[w + me] = p;
           }
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-        __syncwarp();
+          decay = 0.0;
+        }
       }
     }
   } else if (warp < 4) {
@@ -532,24 +634,32 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
           for (int half = 1; half >= 0; --half) {
             const uint32_t at = lanes + kColA + 32 * warp + 16 * half;
-            const float* next = g + 32 * warp + 16 * half + 1;
+            const float4* next = reinterpret_cast<const float4*>(g + 32 * warp + 16 * half);
             const int left = lane - 16 * half;  // columns of this step before the row's own
             tc::ld16(x, at);
-            tc::wait_ld();
             uint32_t out[16];
+            tc::wait_ld();
 #pragma unroll
-            for (int e = 7; e >= 0; --e) {
-              if (2 * e + 1 < left) sum += next[2 * e + 1];
-              float b = 2 * e + 1 <= left ? __uint_as_float(x[2 * e + 1]) * (ex2_ftz(sum) * a.scale) : 0.0f;
-              if (2 * e < left) sum += next[2 * e];
-              float f0 = 2 * e <= left ? __uint_as_float(x[2 * e]) * (ex2_ftz(sum) * a.scale) : 0.0f;
-              out[e] = split_part(f0, b);
-              out[8 + e] = last_part(f0, b);
+            for (int e = 3; e >= 0; --e) {
+              const float4 w = next[e];
+              float y[4];
+              const float step[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+              for (int h = 3; h >= 0; --h) {
+                const int col = 4 * e + h;
+                sum += col < left ? step[h] : 0.0f;
+                const float product = __uint_as_float(x[col]) * (ex2_ftz(sum) * a.scale);
+                y[h] = col <= left ? product : 0.0f;
+              }
+              out[2 * e] = split_part(y[0], y[1]);
+              out[8 + 2 * e] = last_part(y[0], y[1]);
+              out[2 * e + 1] = split_part(y[2], y[3]);
+              out[8 + 2 * e + 1] = last_part(y[2], y[3]);
             }
             tc::st16(at, out);
           }
           // The 32s before it: 2^(from the 32's end to the row) times 2^(from the column to the 32's end).
-          float far = ex2_ftz(sum + g[32 * warp]) * a.scale;
+          float far = ex2_ftz(sum + first_s[(c & 1) * 4 + warp]) * a.scale;
 #pragma unroll 1
           for (int step = 2 * warp - 1; step >= 0; --step) {
             tc::ld16(x, lanes + kColA + 16 * step);
@@ -596,8 +706,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           tc::fence_after();
           const long long row = walk.seq.row0 + (walk.k0 + j) * kChunk + i;
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (row * a.n_heads + walk.head) * kDv);
-          const uint32_t stage = base + ((c * C::kTiles + 1) % kSlots) * C::kSlotBytes + i * 128;
+          uint16_t* dst = static_cast<uint16_t*>(a.out) + (row * a.n_heads + walk.head) * kDv;
 #pragma unroll 1
           for (int d = 0; d < kDv; d += 32) {
             tc::ld32(r, lanes + kColO + d);
@@ -607,25 +716,17 @@ __global__ void __launch_bounds__(kThreads, 1)
               __syncwarp();
               if (lane == 0) mbar_arrive(bar(C::kOFree));
             }
+            if (i >= rows) continue;
+            // whole sectors of a row at a time
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              uint32_t p[4];
+            for (int e = 0; e < 2; ++e) {
+              uint32_t p[8];
 #pragma unroll
-              for (int h = 0; h < 4; ++h)
-                p[h] = pack_bf162(__uint_as_float(r[8 * e + 2 * h]), __uint_as_float(r[8 * e + 2 * h + 1]));
-              if (rows == kChunk) {
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                                 stage + (d / 64) * kBoxBytes + ((((d % 64) / 8 + e) ^ (i & 7)) << 4)),
-                             "r"(p[0]), "r"(p[1]), "r"(p[2]), "r"(p[3])
-                             : "memory");
-              } else if (i < rows) {
-                dst[d / 8 + e] = make_uint4(p[0], p[1], p[2], p[3]);
-              }
+              for (int h = 0; h < 8; ++h)
+                p[h] = pack_bf162(__uint_as_float(r[16 * e + 2 * h]), __uint_as_float(r[16 * e + 2 * h + 1]));
+              st_global_32(dst + d + 16 * e, p);
             }
           }
-          fence_async_shared();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(C::kOut));
         }
     }
   } else {
@@ -649,9 +750,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the state at the piece's start
       const float* from = nullptr;
       if (!kStateOnly) {
-        if (walk.k0 > 0) from = work.pieces + (long long)(me - 1) * kDk * kDv + piece_at;
+        if (walk.k0 > 0) from = work.borders + (long long)me * kDk * kDv + piece_at;
         else if (q.fresh) from = nullptr;
-        else from = ends ? a.state + slot_at : work.starts + (long long)me * kDk * kDv + piece_at;
+        else from = ends ? a.state + slot_at : work.starts + (long long)(me + 1) * kDk * kDv + piece_at;
       }
 #pragma unroll
       for (int e = 0; e < kCols; e += 4) {
@@ -664,20 +765,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = 0; j < walk.n; ++j, ++c) {
         const int rows = min(kChunk, q.rows - (walk.k0 + j) * kChunk), steps = (rows + 15) / 16;
         // the keys, weighted and split: thread t has key dims t / 4 + 8 m and tokens 2 (t % 4), + 1 of each block
-        const int tk = c * C::kTiles, tv = tk + C::kTiles - 1;
-        const uint32_t k_at = base + (tk % kSlots) * C::kSlotBytes + k_row;
+        const Place kp = keys_of(c), vp = values_of(c);
+        const uint32_t k_at = base + kp.slot * C::kSlotBytes + k_row;
         const uint32_t* weight = reinterpret_cast<const uint32_t*>(w_s) + part * 32 + (lane & 3);
-        ok = wait(C::kW, c) && wait(C::kFull + tk % kSlots, tk / kSlots);
+        ok = wait(C::kW, c) && wait(C::kFull + kp.slot, kp.use);
         if (!ok) break;
         const float whole = *whole_s;
-        const int units = has ? min(4, (rows - part * 64 + 15) / 16) : 0;  // steps of 16 tokens here; may be < 0
+        // 32 tokens of the warp's 32 key dims: values 4 h + m are key dims 8 m .. of tokens 8 h ..
+        auto put = [&](uint32_t to, const uint32_t (&p)[16]) {
+          tc::st_16x128b_x4(to, p[0], p[1], p[4], p[5], p[8], p[9], p[12], p[13]);
+          tc::st_16x128b_x4(to + (16u << 16), p[2], p[3], p[6], p[7], p[10], p[11], p[14], p[15]);
+        };
+        const int units = has ? min(2, (rows - part * 64 + 31) / 32) : 0;  // 32s of tokens here; may be < 0
         if (rows < kChunk && has) {
           // keys past the sequence's end, where this warp would read them: zeros (a weight of zero would
           // not clear a NaN)
           for (int e = lane + 4 * max(0, rows - part * 64); e < 4 * 64; e += 32) {
             const int tok = part * 64 + e / 4, unit = ((warp & 3) % 2) * 4 + e % 4;
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
-                             base + (tk % kSlots) * C::kSlotBytes + ((warp & 3) / 2) * kBoxBytes + tok * 128 +
+                             base + kp.slot * C::kSlotBytes + ((warp & 3) / 2) * kBoxBytes + tok * 128 +
                              ((unit ^ (tok & 7)) << 4)),
                          "r"(0)
                          : "memory");
@@ -687,31 +793,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         {
 #pragma unroll 1
           for (int u = 0; u < units; ++u) {
-            const int t0 = part * 64 + u * 16;
-            uint32_t m[8], l[8];
+            uint32_t m[16], l[16];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < 4; ++h) {
               uint32_t k[4];
-              ldmatrix_x4_trans(k, k_at + (2 * u + h) * 1024);
-              const uint32_t w2 = weight[64 + (2 * u + h) * 4], w3 = weight[128 + (2 * u + h) * 4];
+              ldmatrix_x4_trans(k, k_at + (4 * u + h) * 1024);
+              const uint32_t w2 = weight[64 + (4 * u + h) * 4], w3 = weight[128 + (4 * u + h) * 4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 m[h * 4 + e] = tc::mul_bf162(k[e], w2);
                 l[h * 4 + e] = tc::fma_bf162(k[e], w3, tc::fma_bf162(k[e], w2, tc::neg_bf162(m[h * 4 + e])));
               }
             }
-            const uint32_t to = lanes + kColK + t0 / 2;
-            tc::st_16x128b_x2(to, l[0], l[1], l[4], l[5]);
-            tc::st_16x128b_x2(to + (16u << 16), l[2], l[3], l[6], l[7]);
-            tc::st_16x128b_x2(to + 64, m[0], m[1], m[4], m[5]);
-            tc::st_16x128b_x2(to + 64 + (16u << 16), m[2], m[3], m[6], m[7]);
+            put(lanes + kColK + part * 32 + u * 16, l);
+            put(lanes + kColK + 64 + part * 32 + u * 16, m);
           }
         }
-        ok = wait(C::kFull + tv % kSlots, tv / kSlots);
+        ok = wait(C::kFull + vp.slot, vp.use);
         if (!ok) break;
         if (rows < steps * 16) {
           // the last chunk's products run over whole steps of 16 tokens: values past the end are zeros
-          const uint32_t v_at = base + (tv % kSlots) * C::kSlotBytes;
+          const uint32_t v_at = base + vp.slot * C::kSlotBytes;
           for (int e = tid - 128; e < (steps * 16 - rows) * (kDv / 8); e += 256) {
             const int row = rows + e / (kDv / 8), unit = e % (kDv / 8);
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_at + (unit / 8) * kBoxBytes + row * 128 +
@@ -725,6 +827,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(C::kKeys));
+        ok = wait(C::kULo, c);
+        if (!ok) break;
+        tc::fence_after();
+        // the larger parts in their place
+#pragma unroll 1
+        for (int u = 0; u < units; ++u) {
+          uint32_t p1[16], p2[16];
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            uint32_t k[4];
+            ldmatrix_x4_trans(k, k_at + (4 * u + h) * 1024);
+            const uint32_t w1 = weight[(4 * u + h) * 4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              p1[h * 4 + e] = tc::mul_bf162(k[e], w1);
+              p2[h * 4 + e] = tc::fma_bf162(k[e], w1, tc::neg_bf162(p1[h * 4 + e]));
+            }
+          }
+          put(lanes + kColK + part * 32 + u * 16, p2);
+          put(lanes + kColK + 64 + part * 32 + u * 16, p1);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::kWFree));
+        tc::wait_st();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::kKeysHi));
+
         // S for this chunk's outputs, over the one that the last chunk's have read
         if (!kStateOnly) {
           if (c > 0) ok = wait(C::kQs, c - 1);
@@ -756,36 +886,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(C::kS));
         }
-        ok = wait(C::kULo, c);
-        if (!ok) break;
-        tc::fence_after();
-        // the larger parts in their place
-#pragma unroll 1
-        for (int u = 0; u < units; ++u) {
-          uint32_t p1[8], p2[8];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t k[4];
-            ldmatrix_x4_trans(k, k_at + (2 * u + h) * 1024);
-            const uint32_t w1 = weight[(2 * u + h) * 4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              p1[h * 4 + e] = tc::mul_bf162(k[e], w1);
-              p2[h * 4 + e] = tc::fma_bf162(k[e], w1, tc::neg_bf162(p1[h * 4 + e]));
-            }
-          }
-          const uint32_t to = lanes + kColK + (part * 64 + u * 16) / 2;
-          tc::st_16x128b_x2(to, p2[0], p2[1], p2[4], p2[5]);
-          tc::st_16x128b_x2(to + (16u << 16), p2[2], p2[3], p2[6], p2[7]);
-          tc::st_16x128b_x2(to + 64, p1[0], p1[1], p1[4], p1[5]);
-          tc::st_16x128b_x2(to + 64 + (16u << 16), p1[2], p1[3], p1[6], p1[7]);
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::kWFree));
-        tc::wait_st();
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::kKeysHi));
 
         ok = wait(C::kU, c);
         if (!ok) break;
@@ -803,11 +903,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       float* to = nullptr;
-      if (kStateOnly) {
-        to = work.pieces + (long long)me * kDk * kDv + piece_at;
-      } else if (ends) {
-        to = a.state + slot_at;
-      }
+      if constexpr (kStateOnly) to = work.sums + (long long)(walk.w + me) * kDk * kDv + piece_at;
+      else if (ends) to = a.state + slot_at;
       if (to && has) {
 #pragma unroll
         for (int e = 0; e < kCols; e += 4)
@@ -824,31 +921,42 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0 && *abort_s && a.status) atomicMax(a.status, 2);
 }
 
-// The states between the pieces of a (sequence, head), one thread for four values: worker w's piece
-// becomes the state after it.  A chain is as long as the (sequence, head) has shares.
+// The states at the borders inside a (sequence, head), one thread for four values: block b follows the
+// parts of the one whose first cut is border b.
 template <int kDk, int kDv>
-__global__ void __launch_bounds__(256) chain_kernel(const __grid_constant__ Args a, const __grid_constant__ Work work,
-                                                    int workers) {
-  int w = blockIdx.x;
-  Header h = work.headers[w];
-  if (h.kind != 1) return;
+__global__ void __launch_bounds__(256) chain_kernel(const __grid_constant__ Args a, const __grid_constant__ Work work) {
+  __shared__ Part parts[2 * kThreads];
+  __shared__ int list[2 * kThreads], count;
+  const int first = work.first[blockIdx.x];
+  if (first < 0) return;
+  // the parts that may belong to it, then their order: a chain of loads from memory would take longer than
+  // all the rest
+  for (int i = first + threadIdx.x; i < 2 * (int)gridDim.x; i += 256) parts[i] = work.parts[i];
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int n = 0;
+    for (int i = first; i >= 0 && n < 2 * (int)gridDim.x; i = parts[i].next) list[n++] = i;
+    count = n;
+  }
+  __syncthreads();
   const long long at = ((long long)blockIdx.y * 256 + threadIdx.x) * 4;
-  if (at >= kDk * kDv) return;
+  const Part p0 = parts[first];
   float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (!h.fresh) s = *reinterpret_cast<const float4*>(a.state + ((long long)h.slot * a.n_heads + h.head) * kDk * kDv + at);
-  *reinterpret_cast<float4*>(work.starts + (long long)w * kDk * kDv + at) = s;
-  while (true) {
-    float4* p = reinterpret_cast<float4*>(work.pieces + (long long)w * kDk * kDv + at);
-    const float f = (float)exp2(h.decay);
-    const float4 u = *p;
+  if (!p0.fresh)
+    s = *reinterpret_cast<const float4*>(a.state + ((long long)p0.slot * a.n_heads + p0.head) * kDk * kDv + at);
+  *reinterpret_cast<float4*>(work.starts + (long long)blockIdx.x * kDk * kDv + at) = s;
+  const int n = count;
+#pragma unroll 4
+  for (int k = 0; k < n; ++k) {
+    const int i = list[k];
+    const float4 u = __ldcg(reinterpret_cast<const float4*>(work.sums + (long long)i * kDk * kDv + at));
+    const float f = parts[i].decay;
     s.x = fmaf(f, s.x, u.x);
     s.y = fmaf(f, s.y, u.y);
     s.z = fmaf(f, s.z, u.z);
     s.w = fmaf(f, s.w, u.w);
-    *p = s;
-    if (++w >= workers) break;
-    h = work.headers[w];
-    if (h.kind != 2) break;
+    if (parts[i].border >= 0)
+      *reinterpret_cast<float4*>(work.borders + (long long)parts[i].border * kDk * kDv + at) = s;
   }
 }
 
@@ -871,6 +979,7 @@ EncodeTiledFn encode_fn() {
 // rows of bf16 heads [n_rows][n_heads][dim] with any strides, read in boxes of 128 rows x 64 dims
 bool make_map(CUtensorMap* map, const void* base, const Args& a, int dim, long long row_stride, long long head_stride) {
   EncodeTiledFn fn = encode_fn();
+  if (reinterpret_cast<uintptr_t>(a.out) & 31) return false;  // outputs are stored 32 bytes at a time
   if ((a.n_rows / kChunk + a.n_seqs) * a.n_heads > 0x7fffffff) return false;  // Walk counts in 32 bits
   if (!fn || row_stride <= 0 || head_stride <= 0) return false;
   const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)a.n_heads, (cuuint64_t)a.n_rows};
@@ -881,14 +990,17 @@ bool make_map(CUtensorMap* map, const void* base, const Args& a, int dim, long l
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+int64_t table_bytes(int workers) {
+  return (2 * workers * (int64_t)sizeof(Part) + workers * (int64_t)sizeof(int) + 255) / 256 * 256;
+}
+
 template <int kDk, int kDv>
 int launch(const Args& a, int workers, int device, void* workspace, cudaStream_t s) {
   using First = Cfg<kDk, kDv, true>;
   using Main = Cfg<kDk, kDv, false>;
-  CUtensorMap q_map, k_map, v_map, o_map;
+  CUtensorMap q_map, k_map, v_map;
   if (!make_map(&q_map, a.q, a, kDk, a.q_row, a.q_head) || !make_map(&k_map, a.k, a, kDk, a.k_row, a.k_head) ||
-      !make_map(&v_map, a.v, a, kDv, a.v_row, a.v_head) ||
-      !make_map(&o_map, a.out, a, kDv, (long long)a.n_heads * kDv, kDv))
+      !make_map(&v_map, a.v, a, kDv, a.v_row, a.v_head))
     return ASTERQ_ERR_UNSUPPORTED;
   static unsigned long long configured = 0;  // one bit per device ordinal
   if (device >= 64 || !(configured & (1ull << device))) {
@@ -901,22 +1013,26 @@ int launch(const Args& a, int workers, int device, void* workspace, cudaStream_t
     if (device < 64) configured |= 1ull << device;
   }
   Work work;
-  work.headers = static_cast<Header*>(workspace);
-  work.pieces = reinterpret_cast<float*>(static_cast<char*>(workspace) + (workers * sizeof(Header) + 255) / 256 * 256);
-  work.starts = work.pieces + (long long)workers * kDk * kDv;
-  chunk_kernel<kDk, kDv, true><<<workers, kThreads, First::kSmem, s>>>(q_map, k_map, v_map, o_map, a, work);
-  chain_kernel<kDk, kDv><<<dim3(workers, kDk * kDv / 1024), 256, 0, s>>>(a, work, workers);
-  chunk_kernel<kDk, kDv, false><<<workers, kThreads, Main::kSmem, s>>>(q_map, k_map, v_map, o_map, a, work);
+  char* at = static_cast<char*>(workspace);
+  work.parts = reinterpret_cast<Part*>(at);
+  work.first = reinterpret_cast<int*>(at + 2 * workers * sizeof(Part));
+  work.sums = reinterpret_cast<float*>(at + table_bytes(workers));
+  work.borders = work.sums + 2ll * workers * kDk * kDv;
+  work.starts = work.borders + (long long)workers * kDk * kDv;
+  chunk_kernel<kDk, kDv, true><<<workers, kThreads, First::kSmem, s>>>(q_map, k_map, v_map, a, work);
+  chain_kernel<kDk, kDv><<<dim3(workers, kDk * kDv / 1024), 256, 0, s>>>(a, work);
+  chunk_kernel<kDk, kDv, false><<<workers, kThreads, Main::kSmem, s>>>(q_map, k_map, v_map, a, work);
   return check_launch("linear_attention");
 }
 
 }  // namespace
 
 int64_t chunk_workspace_bytes(int dk, int dv, int workers) {
-  return (workers * (int64_t)sizeof(Header) + 255) / 256 * 256 + 2ll * workers * dk * dv * 4;
+  return table_bytes(min(workers, kThreads)) + 4ll * min(workers, kThreads) * dk * dv * 4;
 }
 
 int chunk_launch(const Args& a, int dk, int dv, int workers, int device, void* workspace, cudaStream_t s) {
+  workers = min(workers, kThreads);  // the first pass looks each share's border up with a thread
   if (dk == 64 && dv == 64) return launch<64, 64>(a, workers, device, workspace, s);
   if (dk == 64) return launch<64, 128>(a, workers, device, workspace, s);
   if (dv == 64) return launch<128, 64>(a, workers, device, workspace, s);

@@ -60,11 +60,13 @@ ASTERQ_DEVICE void st16(uint32_t addr, const uint32_t (&r)[16]) {
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-// 16 lanes from the address's on, four columns twice over: thread t <-> lanes t / 4 and t / 4 + 8, column
-// t % 4 (r[0], r[1]), then the next four columns (r[2], r[3]): the layout of ldmatrix's 8 x 8 matrices
-ASTERQ_DEVICE void st_16x128b_x2(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
-  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r0), "r"(r1), "r"(r2),
-               "r"(r3)
+// 16 lanes from the address's on, four columns four times over: thread t <-> lanes t / 4 and t / 4 + 8,
+// column t % 4 (r0, r1), then the next four columns (r2, r3), ..: the layout of ldmatrix's 8 x 8 matrices.
+// A store takes a warp some 40 cycles whatever its width.
+ASTERQ_DEVICE void st_16x128b_x4(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3, uint32_t r4,
+                                 uint32_t r5, uint32_t r6, uint32_t r7) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(r0), "r"(r1),
+               "r"(r2), "r"(r3), "r"(r4), "r"(r5), "r"(r6), "r"(r7)
                : "memory");
 }
 
