@@ -10,12 +10,14 @@
 // into a ring of shared memory by TMA, across the borders of its work, and consumer warps that never
 // wait for one another inside a sequence.
 //
-// Split.  The tiles of all (sequence, kv head, row block) units, laid end to end, are cut into equal
-// contiguous shares, one per CTA, by a prefix sum over `lengths` that every CTA computes for itself:
-// no planning launch, no host copy of the lengths, and a long sequence and a ragged batch are both
-// even to a tile.  A unit that lies in one share is finished there.  A cut unit leaves (o, m, l)
-// records in the workspace, and the CTA that stores its last one joins them, in the order of the
-// shares, so results do not depend on which CTA came last.  No CTA waits for another.
+// Split.  The tiles of all (sequence, kv head, row block) units, laid end to end with a few tiles' worth
+// in front of each unit for what it costs by itself, are cut into equal contiguous shares, one per CTA,
+// by a prefix sum over `lengths` that every CTA computes for itself: no planning launch, no host copy of
+// the lengths, and a long sequence and a ragged batch are both even to a tile.  A unit that lies in one
+// share is finished there; a short one by half of the CTA's warps, while the other half has the next.  A
+// cut unit leaves (o, m, l) records in the workspace, and the CTA that stores its last one joins them, in
+// the order of the shares, so results do not depend on which CTA came last; of many records groups are
+// joined first, each by the CTA that stores its last one.  No CTA waits for another.
 #include <cuda.h>
 
 #include "asterq_internal.h"
@@ -35,7 +37,7 @@ struct Args {
   void* out;
   float* lse;
   float* records;  // o [2 W][NR][D], then m [2 W][NR], then l [2 W][NR]
-  int* counters;   // [2 W], zero between calls
+  int* counters;   // [4 W], zero between calls: records stored of a unit or of a group, groups joined of a unit
   int* status;
   long long q_row_stride, q_head_stride, n_pages, capacity;  // capacity: tokens a row of the table can hold
   int n_rows, n_heads, n_kv_heads, group, row_blocks;
@@ -55,11 +57,19 @@ struct Cfg {
   static constexpr int kTeamWarps = kTile / 16, kWarps = 2 * kTeamWarps, kThreads = 32 * kWarps + 32;
   static constexpr int kColBoxes = D / 64;
   static constexpr int kHalfBytes = kTile * D * 2, kStageBytes = 2 * kHalfBytes;
-  // an even count, so that a stage and its barrier always serve the same team
   static constexpr int kStages = D == 64 ? 12 : 6;
+  // queries of the next units, rows padded against conflicts
+  static constexpr int kQSlots = NR * D >= 2048 ? 2 : 4, kQPitch = D * 2 + 16;
+  static constexpr int kQBytes = NR * kQPitch;
   static constexpr int kSlice = NR == 16 ? 32 : 64, kPad = kSlice + 4;  // dims joined at a time
-  static constexpr int kMergeFloats = kWarps * NR * kPad > kMaxWorkers * NR ? kWarps * NR * kPad : kMaxWorkers * NR;
-  static constexpr int kSmem = 1024 + kStages * kStageBytes + (kMergeFloats + 2 * kWarps * NR) * 4 + 256;
+  static constexpr int kMergeFloats = kWarps * NR * kPad;
+  static_assert(kMergeFloats >= 24 * NR, "weights of the records that are joined at once");
+  // What a unit costs beside its tiles, in tiles (a unit by itself takes about a microsecond, two at a time;
+  // a tile's share of the memory bandwidth 0.4 us at 64 dims, 0.75 us above).
+  static constexpr int kUnitCost = D == 64 ? 2 : 1;
+  static constexpr int kSoloTiles = 8;  // units up to this long are taken by one team
+  static constexpr int kSmem =
+      1024 + kStages * kStageBytes + kQSlots * kQBytes + (kMergeFloats + 2 * kWarps * NR) * 4 + (3 * kStages + 2 * kQSlots) * 8;
 };
 
 ASTERQ_DEVICE void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
@@ -104,29 +114,35 @@ ASTERQ_DEVICE Span span_of(const Args& a, int row) {
   return s;
 }
 
-// One CTA's share [x, end) of all tiles, walked unit by unit; every warp walks it for itself.
-template <int kTile>
+// One CTA's share [x, end) of all units' costs, walked piece by piece; every warp walks it for itself.
+template <int kTile, int kUnitCost>
 struct Walk {
   long long x, end, row_start;
   int row;
   Span span;
   // of the current piece
-  int unit, k0, n;          // unit within the row, its first tile here, tiles here
-  long long unit_start;
+  int unit, k0, n;        // unit within the row, its first tile here, tiles here
+  long long first_tile;   // where the unit's first tile is
   template <class A>
   ASTERQ_DEVICE bool next(const A& a, int units_per_row) {
-    if (x >= end) return false;
-    while (x >= row_start + (long long)span.tiles * units_per_row) {
-      row_start += (long long)span.tiles * units_per_row;
-      span = span_of<kTile>(a, ++row);
+    while (x < end) {
+      const int per_unit = span.tiles + kUnitCost;
+      if (span.tiles == 0 || x >= row_start + (long long)per_unit * units_per_row) {
+        if (span.tiles > 0) row_start += (long long)per_unit * units_per_row;
+        span = span_of<kTile>(a, ++row);
+        continue;
+      }
+      const long long in_row = x - row_start;
+      unit = in_row < 0x7fffffff ? (int)in_row / per_unit : (int)(in_row / per_unit);
+      const long long unit_start = row_start + (long long)unit * per_unit;
+      const int at = (int)(x - unit_start), cost = (int)min((long long)(per_unit - at), end - x);
+      first_tile = unit_start + kUnitCost;
+      k0 = max(at - kUnitCost, 0);
+      n = max(at + cost - kUnitCost, 0) - k0;
+      x += cost;
+      if (n > 0) return true;
     }
-    const long long in_row = x - row_start;
-    unit = (int)(in_row / span.tiles);
-    unit_start = row_start + (long long)unit * span.tiles;
-    k0 = (int)(x - unit_start);
-    n = (int)min((long long)(span.tiles - k0), end - x);
-    x += n;
-    return true;
+    return false;
   }
 };
 
@@ -142,32 +158,43 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   constexpr int D = C::D, NR = C::NR, NT = C::NT, kTile = C::kTile;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* merge = reinterpret_cast<float*>(smem + C::kStages * C::kStageBytes);
+  const uint32_t q_ring = smem_u32(smem) + C::kStages * C::kStageBytes;
+  float* merge = reinterpret_cast<float*>(smem + C::kStages * C::kStageBytes + C::kQSlots * C::kQBytes);
   float* warp_m = merge + C::kMergeFloats;
   float* warp_l = warp_m + C::kWarps * NR;
   uint64_t* bars = reinterpret_cast<uint64_t*>(warp_l + C::kWarps * NR);
   __shared__ Start start_s;
   __shared__ long long scan_s[32];
-  __shared__ int abort_s, never_s, last_s;  // never_s stays 0: for waits that an abort must not cut short
+  __shared__ int abort_s, never_s, last_s, group_s;  // never_s stays 0: for waits that an abort must not cut short
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * C::kStages;
+  // a full barrier for each stage and the team that its tile is for: a barrier's waiters see each of its phases
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 16 * C::kStages, q_full0 = empty0 + 8 * C::kStages,
+                 q_empty0 = q_full0 + 8 * C::kQSlots;
   const int units_per_row = a.n_kv_heads * a.row_blocks;
 
   if (tid == 0) {
     for (int i = 0; i < C::kStages; ++i) {
-      mbar_init(full0 + 8 * i, 1);
+      mbar_init(full0 + 16 * i, 1);
+      mbar_init(full0 + 16 * i + 8, 1);
       mbar_init(empty0 + 8 * i, C::kTeamWarps);
+    }
+    for (int i = 0; i < C::kQSlots; ++i) {
+      mbar_init(q_full0 + 8 * i, 1);
+      mbar_init(q_empty0 + 8 * i, C::kWarps);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     abort_s = never_s = 0;
   }
 
-  // The share: thread t sums the tiles of rows [t R, (t + 1) R), the block scans the sums.
+  // The share: thread t sums the costs of rows [t R, (t + 1) R), the block scans the sums.
   const int strip = (a.n_rows + C::kThreads - 1) / C::kThreads;
   const int r0 = min(tid * strip, a.n_rows), r1 = min(r0 + strip, a.n_rows);
   long long sum = 0;
-  for (int r = r0; r < r1; ++r) sum += span_of<kTile>(a, r).tiles;
-  sum *= units_per_row;
+  auto cost_of = [&](int row) {
+    const int tiles = span_of<kTile>(a, row).tiles;
+    return tiles > 0 ? (long long)(tiles + C::kUnitCost) * units_per_row : 0ll;
+  };
+  for (int r = r0; r < r1; ++r) sum += cost_of(r);
   long long scan = sum;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
@@ -182,7 +209,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     total += scan_s[w];
   }
   const int W = (int)min((long long)gridDim.x, max(total, 1ll)), me = blockIdx.x;
-  Walk<kTile> walk;
+  Walk<kTile, C::kUnitCost> walk;
   walk.x = total * me / W;
   walk.end = me < W ? total * (me + 1) / W : walk.x;
   if (walk.x < walk.end && before <= walk.x && walk.x < before + sum) {
@@ -190,7 +217,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     s.row = r0;
     s.row_start = before;
     while (true) {
-      const long long here = (long long)span_of<kTile>(a, s.row).tiles * units_per_row;
+      const long long here = cost_of(s.row);
       if (walk.x < s.row_start + here) break;
       s.row_start += here;
       ++s.row;
@@ -221,19 +248,36 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     // the page of the i-th of the next 32 boxes, fetched by one load for all of them.
     const int boxes = kTile / a.box_rows;
     const uint32_t box_bytes = a.box_rows * 128;
-    int it = 0;
+    int it = 0, piece = 0;
+    uint32_t used[2] = {0, 0};  // uses of each stage by each team, modulo 2
     bool ok = true;
-    while (ok && walk.next(a, units_per_row)) {
-      const int head = walk.unit / a.row_blocks;
+    for (; ok && walk.next(a, units_per_row); ++piece) {
+      const int head = walk.unit / a.row_blocks, block = walk.unit - head * a.row_blocks;
+      const int rows = min(NR, a.group - block * NR);
+      const bool solo = walk.n == walk.span.tiles && walk.n <= C::kSoloTiles;
+      const int q_slot = piece % C::kQSlots;
+      if (piece >= C::kQSlots) {
+        ok = __all_sync(0xffffffffu, (int)mbar_wait(q_empty0 + 8 * q_slot, ((piece / C::kQSlots) - 1) & 1, &abort_s)) != 0;
+        if (!ok) break;
+      }
+      if (lane == 0) mbar_expect_tx(q_full0 + 8 * q_slot, rows * D * 2);
+      __syncwarp();
+      if (lane < rows)
+        bulk_1d(q_ring + q_slot * C::kQBytes + lane * C::kQPitch,
+                static_cast<const uint16_t*>(a.q) + walk.row * a.q_row_stride +
+                    ((long long)head * a.group + block * NR + lane) * a.q_head_stride,
+                D * 2, q_full0 + 8 * q_slot);
       const int* table = a.page_table + (long long)walk.row * a.max_pages;
       int held = -32, page = 0;
       for (int j = 0; j < walk.n; ++j, ++it) {
-        const int stage = it % C::kStages;
+        const int stage = it % C::kStages, team = solo ? piece & 1 : j & 1;
         if (it >= C::kStages) {
           ok = __all_sync(0xffffffffu, (int)mbar_wait(empty0 + 8 * stage, ((it / C::kStages) - 1) & 1, &abort_s)) != 0;
           if (!ok) break;
         }
-        const uint32_t dst = smem_u32(smem) + stage * C::kStageBytes, bar = full0 + 8 * stage;
+        used[0] ^= (uint32_t)(team == 0) << stage;
+        used[1] ^= (uint32_t)team << stage;
+        const uint32_t dst = smem_u32(smem) + stage * C::kStageBytes, bar = full0 + 16 * stage + 8 * team;
         const int token = walk.span.tile(walk.k0 + j) * kTile;
         uint32_t wanted = 0;
         for (int b = 0; b < boxes; ++b) {
@@ -275,8 +319,12 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       }
     }
     // the last copies have landed before the exit, also when a wait ran out and nobody waits for them
-    for (int t = max(0, it - C::kStages); t < it; ++t)
-      (void)mbar_wait(full0 + 8 * (t % C::kStages), (t / C::kStages) & 1, &never_s, 200000000);
+    if (!ok) {
+      for (int i = 0; i < 2 * C::kStages; ++i)
+        (void)mbar_wait(full0 + 8 * i, (used[i & 1] >> (i / 2) & 1) ^ 1, &never_s, 200000000);
+      for (int i = max(0, piece - C::kQSlots); i <= piece; ++i)
+        (void)mbar_wait(q_full0 + 8 * (i % C::kQSlots), (i / C::kQSlots) & 1, &never_s, 200000000);
+    }
     return;
   }
 
@@ -292,22 +340,36 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   const float scale2 = a.scale * kLog2e;
   const long long n_slots = 2ll * gridDim.x;
   int it = 0;
-  while (walk.next(a, units_per_row)) {
+  uint32_t phase = 0;  // of each stage's barrier of this team
+  for (int piece = 0; walk.next(a, units_per_row); ++piece) {
     const int head = walk.unit / a.row_blocks, block = walk.unit - head * a.row_blocks;
     const int rows = min(NR, a.group - block * NR);
     const long long h0 = (long long)head * a.group + block * NR;  // query head of the block's row 0
+    const bool cut = walk.n < walk.span.tiles, solo = !cut && walk.n <= C::kSoloTiles;
+    const int q_slot = piece % C::kQSlots;
+    // Every warp follows the queries of every unit, so that none falls a phase behind.  (After a wait has run
+    // out all go on to the end, waits returning at once, since they still meet at barriers.)
+    (void)mbar_wait(q_full0 + 8 * q_slot, (piece / C::kQSlots) & 1, &abort_s);
+    __syncwarp();
+    if (solo && (piece & 1) != team) {
+      it += walk.n;
+      if (lane == 0) mbar_arrive(q_empty0 + 8 * q_slot);
+      continue;
+    }
     uint32_t qf[D / 16][NT][2];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int r = t * 8 + g;
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.q) +
-                                                              walk.row * a.q_row_stride + (h0 + r) * a.q_head_stride);
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s) {
-        qf[s][t][0] = r < rows ? __ldg(src + s * 8 + qd) : 0u;
-        qf[s][t][1] = r < rows ? __ldg(src + s * 8 + qd + 4) : 0u;
+      for (int s = 0; s < D / 16; s += 2) {
+        uint32_t f[4];
+        ldmatrix_x4(f, q_ring + q_slot * C::kQBytes + (t * 8 + (lane & 7)) * C::kQPitch + s * 32 + (lane >> 3) * 16);
+        qf[s][t][0] = f[0];
+        qf[s][t][1] = f[1];
+        qf[s + 1][t][0] = f[2];
+        qf[s + 1][t][1] = f[3];
       }
-    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(q_empty0 + 8 * q_slot);
     float acc[D / 16][NT][4];
     float m[NT][2], l[NT][2];
 #pragma unroll
@@ -321,10 +383,11 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     }
 
     for (int j = 0; j < walk.n; ++j, ++it) {
-      if ((it & 1) != team) continue;
+      if (!solo && (j & 1) != team) continue;
       const int stage = it % C::kStages;
       const uint32_t k_base = smem_u32(smem) + stage * C::kStageBytes, v_base = k_base + C::kHalfBytes;
-      if (!__all_sync(0xffffffffu, (int)mbar_wait(full0 + 8 * stage, (it / C::kStages) & 1, &abort_s))) break;
+      if (!__all_sync(0xffffffffu, (int)mbar_wait(full0 + 16 * stage + 8 * team, phase >> stage & 1, &abort_s))) break;
+      phase ^= 1u << stage;
       const int token = walk.span.tile(walk.k0 + j) * kTile + row16;
       const bool whole = token + 15 < walk.span.length && (token >= walk.span.from || token + 15 < walk.span.sink);
       const bool any = whole || (token < walk.span.length && (token < walk.span.sink || token + 15 >= walk.span.from));
@@ -445,6 +508,10 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     }
 
     // ------------------------------------------------------------------ the warps join
+    // the team's, or all; either way with barriers that only they use
+    const int wa = solo ? team * C::kTeamWarps : 0, wn = solo ? C::kTeamWarps : C::kWarps;
+    const int me_in = tid - wa * 32, threads = wn * 32;
+    auto sync = [&]() { named_sync(solo ? 1 + team : 3, threads); };
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -456,16 +523,15 @@ __global__ void __launch_bounds__(C::kThreads, 1)
           warp_l[warp * NR + t * 8 + 2 * qd + e] = l[t][e];
         }
       }
-    named_sync(1, C::kWarps * 32);
-    const bool cut = walk.n < walk.span.tiles;
+    sync();
     // slot of this piece: a share's first piece may be the tail or middle of a unit, its last the head
-    const long long slot = 2ll * me + (walk.unit_start > my_start ? 1 : 0);
+    const long long slot = 2ll * me + (walk.first_tile > my_start ? 1 : 0);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float top = -INFINITY;
-        for (int w = 0; w < C::kWarps; ++w) top = fmaxf(top, warp_m[w * NR + t * 8 + 2 * qd + e]);
+        for (int w = wa; w < wa + wn; ++w) top = fmaxf(top, warp_m[w * NR + t * 8 + 2 * qd + e]);
         const float turn = m[t][e] == -INFINITY ? 0.0f : ex2_ftz(m[t][e] - top);
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
@@ -483,17 +549,15 @@ __global__ void __launch_bounds__(C::kThreads, 1)
           for (int e = 0; e < 4; ++e)
             merge[(warp * NR + t * 8 + 2 * qd + (e & 1)) * C::kPad + i * 16 + g + (e >> 1) * 8] =
                 acc[part * (C::kSlice / 16) + i][t][e];
-      named_sync(1, C::kWarps * 32);
-      for (int i = tid; i < NR * C::kSlice; i += C::kWarps * 32) {
+      sync();
+      for (int i = me_in; i < (cut ? NR : rows) * C::kSlice; i += threads) {
         const int r = i / C::kSlice, d = i % C::kSlice;
         float sum = 0.0f, top = -INFINITY, total_l = 0.0f;
-#pragma unroll
-        for (int w = 0; w < C::kWarps; ++w) {
+        for (int w = wa; w < wa + wn; ++w) {
           sum += merge[(w * NR + r) * C::kPad + d];
           top = fmaxf(top, warp_m[w * NR + r]);
         }
-#pragma unroll
-        for (int w = 0; w < C::kWarps; ++w) {
+        for (int w = wa; w < wa + wn; ++w) {
           const float mw = warp_m[w * NR + r];
           total_l += mw == -INFINITY ? warp_l[w * NR + r] : warp_l[w * NR + r] * ex2_ftz(mw - top);
         }
@@ -504,7 +568,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             a.records[n_slots * NR * D + slot * NR + r] = top;
             a.records[n_slots * NR * (D + 1) + slot * NR + r] = total_l;
           }
-        } else if (r < rows) {
+        } else {
           const long long at = ((long long)walk.row * a.n_heads + h0 + r) * D + dim;
           const float o = sum / total_l;
           if (a.out_f32) static_cast<float*>(a.out)[at] = o;
@@ -514,74 +578,102 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             a.lse[(long long)walk.row * a.n_heads + h0 + r] = (top + log2f(total_l)) * kLn2;
         }
       }
-      named_sync(1, C::kWarps * 32);
+      sync();
     }
     if (!cut) continue;
 
     // ------------------------------------------------------------------ the pieces of a cut unit join
-    const long long u0 = walk.unit_start, u1 = u0 + walk.span.tiles;
+    const long long u0 = walk.first_tile, u1 = u0 + walk.span.tiles;
     const int w0 = (int)(((u0 + 1) * W - 1) / total), w1 = (int)((u1 * W - 1) / total);
     const int pieces = w1 - w0 + 1;
-    const long long slot0 = 2ll * w0 + (u0 > total * w0 / W ? 1 : 0);  // pieces after the first are at 2 w
+    const int slot0 = 2 * w0 + (u0 > total * w0 / W ? 1 : 0);  // pieces after the first are at 2 w
+    auto slot_of = [&](int i) { return i == 0 ? slot0 : 2 * (w0 + i); };
+    // beyond 24 records, groups of about their square root are joined first
+    const int size = pieces <= 24 ? pieces : pieces <= 64 ? 8 : pieces <= 160 ? 12 : 16;
+    const int groups = (pieces + size - 1) / size, group = (me - w0) / size;
     __threadfence();
-    named_sync(1, C::kWarps * 32);
-    if (tid == 0) last_s = atomicAdd(a.counters + slot0, 1) == pieces - 1;
-    named_sync(1, C::kWarps * 32);
+    sync();
+    if (tid == 0) last_s = atomicAdd(a.counters + slot_of(group * size), 1) == min(size, pieces - group * size) - 1;
+    sync();
     if (!last_s) continue;
     __threadfence();
-    if (tid == 0) a.counters[slot0] = 0;
-    const float* rec_m = a.records + n_slots * NR * D;
-    const float* rec_l = rec_m + n_slots * NR;
-    for (int r = warp; r < NR; r += C::kWarps) {
-      float top = -INFINITY, sum = 0.0f;
-      for (int w = lane; w < pieces; w += 32)
-        top = fmaxf(top, __ldcg(rec_m + (w == 0 ? slot0 : 2ll * (w0 + w)) * NR + r));
+    if (tid == 0) a.counters[slot_of(group * size)] = 0;
+    float* rec_m = a.records + n_slots * NR * D;
+    float* rec_l = rec_m + n_slots * NR;
+    // records first, first + step, .. (n of them): to the output, or into the first one's place
+    auto join = [&](int first, int n, int step, bool whole) {
+      for (int r = warp; r < NR; r += C::kWarps) {
+        float top = -INFINITY, sum = 0.0f;
+        for (int i = lane; i < n; i += 32) top = fmaxf(top, __ldcg(rec_m + slot_of(first + i * step) * NR + r));
 #pragma unroll
-      for (int d = 1; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      for (int w = lane; w < pieces; w += 32) {
-        const long long at = (w == 0 ? slot0 : 2ll * (w0 + w)) * NR + r;
-        const float mw = __ldcg(rec_m + at), f = mw == -INFINITY ? 1.0f : ex2_ftz(mw - top);
-        merge[w * NR + r] = f;
-        sum += f * __ldcg(rec_l + at);
-      }
+        for (int d = 1; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        for (int i = lane; i < n; i += 32) {
+          const int at = slot_of(first + i * step) * NR + r;
+          const float mw = __ldcg(rec_m + at), f = mw == -INFINITY ? 1.0f : ex2_ftz(mw - top);
+          merge[i * NR + r] = f;
+          sum += f * __ldcg(rec_l + at);
+        }
 #pragma unroll
-      for (int d = 1; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      if (lane == 0) {
-        warp_l[r] = sum;
-        if (a.lse && r < rows) a.lse[(long long)walk.row * a.n_heads + h0 + r] = (top + log2f(sum)) * kLn2;
+        for (int d = 1; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane == 0) {
+          warp_m[r] = top;
+          warp_l[r] = sum;
+        }
       }
-    }
-    named_sync(1, C::kWarps * 32);
-    for (int i = tid; i < NR * D / 4; i += C::kWarps * 32) {
-      const int r = i / (D / 4), d = (i % (D / 4)) * 4;
-      if (r >= rows) continue;
-      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      sync();
+      for (int i = tid; i < NR * D / 4; i += C::kWarps * 32) {
+        const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+        if (r >= rows) continue;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
-      for (int w = 0; w < pieces; ++w) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(
-            a.records + ((w == 0 ? slot0 : 2ll * (w0 + w)) * NR + r) * D + d));
-        const float f = merge[w * NR + r];
-        o.x += f * v.x;
-        o.y += f * v.y;
-        o.z += f * v.z;
-        o.w += f * v.w;
+        for (int k = 0; k < n; ++k) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(
+              a.records + ((long long)slot_of(first + k * step) * NR + r) * D + d));
+          const float f = merge[k * NR + r];
+          o.x += f * v.x;
+          o.y += f * v.y;
+          o.z += f * v.z;
+          o.w += f * v.w;
+        }
+        if (!whole) {
+          *reinterpret_cast<float4*>(a.records + ((long long)slot_of(first) * NR + r) * D + d) = o;
+          continue;
+        }
+        const float sum = warp_l[r];
+        o.x /= sum;
+        o.y /= sum;
+        o.z /= sum;
+        o.w /= sum;
+        const long long at = ((long long)walk.row * a.n_heads + h0 + r) * D + d;
+        if (a.out_f32) {
+          *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = o;
+        } else {
+          uint2 w;
+          if constexpr (C::kF16) w = make_uint2(pack_half2(o.x, o.y), pack_half2(o.z, o.w));
+          else w = make_uint2(pack_bf162(o.x, o.y), pack_bf162(o.z, o.w));
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = w;
+        }
       }
-      const float sum = warp_l[r];
-      o.x /= sum;
-      o.y /= sum;
-      o.z /= sum;
-      o.w /= sum;
-      const long long at = ((long long)walk.row * a.n_heads + h0 + r) * D + d;
-      if (a.out_f32) {
-        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = o;
-      } else {
-        uint2 w;
-        if constexpr (C::kF16) w = make_uint2(pack_half2(o.x, o.y), pack_half2(o.z, o.w));
-        else w = make_uint2(pack_bf162(o.x, o.y), pack_bf162(o.z, o.w));
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = w;
+      if (tid < NR) {
+        if (!whole) {
+          rec_m[slot_of(first) * NR + tid] = warp_m[tid];
+          rec_l[slot_of(first) * NR + tid] = warp_l[tid];
+        } else if (a.lse && tid < rows) {
+          a.lse[(long long)walk.row * a.n_heads + h0 + tid] = (warp_m[tid] + log2f(warp_l[tid])) * kLn2;
+        }
       }
-    }
-    named_sync(1, C::kWarps * 32);
+      sync();
+    };
+    join(group * size, min(size, pieces - group * size), 1, groups == 1);
+    if (groups == 1) continue;
+    __threadfence();
+    sync();
+    if (tid == 0) group_s = atomicAdd(a.counters + n_slots + slot0, 1) == groups - 1;
+    sync();
+    if (!group_s) continue;
+    __threadfence();
+    if (tid == 0) a.counters[n_slots + slot0] = 0;
+    join(0, groups, size, true);
   }
   // a wait that ran into its limit (about two seconds): the outputs are not valid
   if (tid == 0 && ld_shared_volatile(&abort_s) && a.status) atomicMax(a.status, 2);
@@ -635,7 +727,7 @@ static int sm_count(int* dev) {
 static int rows_of_block(int group) { return group <= 8 ? 8 : 16; }
 
 static int64_t workspace_bytes(int workers, int rows, int head_dim) {
-  return 2ll * workers * rows * (head_dim + 2) * 4 + (2ll * workers * 4 + 15) / 16 * 16;
+  return 2ll * workers * rows * (head_dim + 2) * 4 + (4ll * workers * 4 + 15) / 16 * 16;
 }
 
 template <class C>
@@ -699,12 +791,12 @@ extern "C" int asterq_paged_attention(const asterq_paged_attention_params* p, vo
   if (!p->q || !p->lengths || !p->out || (p->max_pages > 0 && p->n_pages > 0 && (!p->k_pool || !p->v_pool)) ||
       (p->max_pages > 0 && !p->page_table))
     return set_error(ASTERQ_ERR_INVALID_ARGUMENT, "paged_attention: null pointer");
-  const void* vec[] = {p->k_pool, p->v_pool, p->out, p->workspace};
+  const void* vec[] = {p->q, p->k_pool, p->v_pool, p->out, p->workspace};
   for (const void* ptr : vec)
     if (reinterpret_cast<uintptr_t>(ptr) & 15)
-      return set_error(ASTERQ_ERR_MISALIGNED, "paged_attention: pools, output and workspace must be 16-byte aligned");
-  if ((reinterpret_cast<uintptr_t>(p->q) & 3) || p->q_row_stride % 2 || p->q_head_stride % 2)
-    return set_error(ASTERQ_ERR_MISALIGNED, "paged_attention: queries must be 4-byte aligned, their strides even");
+      return set_error(ASTERQ_ERR_MISALIGNED, "paged_attention: arrays must be 16-byte aligned");
+  if (p->q_row_stride % 8 || p->q_head_stride % 8)
+    return set_error(ASTERQ_ERR_MISALIGNED, "paged_attention: the queries' strides must be multiples of 8");
   int dev = 0;
   const int workers = pat::sm_count(&dev);
   if (workers <= 0) return set_error(ASTERQ_ERR_CUDA, "paged_attention: no CUDA device");
@@ -723,7 +815,7 @@ extern "C" int asterq_paged_attention(const asterq_paged_attention_params* p, vo
   // counters first: their place does not depend on the call's geometry, so one workspace serves calls
   // of different heads in turn
   a.counters = static_cast<int*>(p->workspace);
-  a.records = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + (2ll * workers * 4 + 15) / 16 * 16);
+  a.records = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + (4ll * workers * 4 + 15) / 16 * 16);
   a.status = p->status;
   a.q_row_stride = p->q_row_stride;
   a.q_head_stride = p->q_head_stride;

@@ -466,7 +466,7 @@ typedef struct asterq_paged_attention_params {
   float logit_softcap; /* <= 0: off */
   int32_t reserved;
   int64_t n_pages;
-  int64_t q_row_stride, q_head_stride; /* in elements, even; a head's dims are contiguous */
+  int64_t q_row_stride, q_head_stride; /* in elements, multiples of 8; a head's dims are contiguous */
   const void* q;
   const void* k_pool;
   const void* v_pool;
