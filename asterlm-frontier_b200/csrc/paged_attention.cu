@@ -50,33 +50,32 @@ template <bool kF16_, int D_, int NR_>
 struct Cfg {
   static constexpr bool kF16 = kF16_;
   static constexpr int D = D_, NR = NR_, NT = NR_ / 8;
-  // A warp takes 16 tokens of a tile.  Two teams of warps take alternate tiles, so one team's
-  // softmax runs beside the other's products.  256-wide heads use 32-token tiles: the stage keeps
-  // its 32 KB and the ring its depth.
-  static constexpr int kTile = D == 256 ? 32 : 64;
-  static constexpr int kTeamWarps = kTile / 16, kWarps = 2 * kTeamWarps, kThreads = 32 * kWarps + 32;
-  static constexpr int kColBoxes = D / 64;
+  // Tiles of 32 KB.  A warp takes kSub times 16 tokens of a tile.  Two teams of warps take alternate tiles,
+  // so one team's softmax runs beside the other's products.
+  static constexpr int kTile = 8192 / D, kSub = D == 64 ? 2 : 1;
+  static constexpr int kTeamWarps = kTile / 16 / kSub, kWarps = 2 * kTeamWarps, kThreads = 32 * kWarps + 32;
+  static constexpr int kSubTokens = 16 * kTeamWarps;  // from one of a warp's 16 tokens to its next
   static constexpr int kHalfBytes = kTile * D * 2, kStageBytes = 2 * kHalfBytes;
-  static constexpr int kStages = D == 64 ? 12 : 6;
+  static constexpr int kStages = 6;
   // queries of the next units, rows padded against conflicts
   static constexpr int kQSlots = NR * D >= 2048 ? 2 : 4, kQPitch = D * 2 + 16;
   static constexpr int kQBytes = NR * kQPitch;
   static constexpr int kSlice = NR == 16 ? 32 : 64, kPad = kSlice + 4;  // dims joined at a time
   static constexpr int kMergeFloats = kWarps * NR * kPad;
   static_assert(kMergeFloats >= 24 * NR, "weights of the records that are joined at once");
-  // What a unit costs beside its tiles, in tiles (a unit by itself takes about a microsecond, two at a time;
-  // a tile's share of the memory bandwidth 0.4 us at 64 dims, 0.75 us above).
-  static constexpr int kUnitCost = D == 64 ? 2 : 1;
-  static constexpr int kSoloTiles = 8;  // units up to this long are taken by one team
+  // What a unit costs beside its tiles, in tiles: a unit by itself takes 1.5 us, two at a time, a tile's share of
+  // the memory bandwidth 0.75 us.
+  static constexpr int kUnitCost = 1;
+  static constexpr int kSoloTiles = 4;  // units up to this long are taken by one team
   static constexpr int kSmem =
       1024 + kStages * kStageBytes + kQSlots * kQBytes + (kMergeFloats + 2 * kWarps * NR) * 4 + (3 * kStages + 2 * kQSlots) * 8;
 };
 
-ASTERQ_DEVICE void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+ASTERQ_DEVICE void tma_box(uint32_t dst, const CUtensorMap* map, int token, int z, uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          dst),
-      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %2, %4}], "
+      "[%5];" ::"r"(dst),
+      "l"(map), "r"(0), "r"(token), "r"(z), "r"(bar)
       : "memory");
 }
 // the transpose of an 8 x 8 matrix of 16-bit values held as MMA fragments
@@ -244,18 +243,52 @@ __global__ void __launch_bounds__(C::kThreads, 1)
 
   if (warp == C::kWarps) {
     // ------------------------------------------------------------------ producer
-    // Boxes of box_rows tokens (a divisor of the page and of the tile) by 64 dims.  Lane i holds
-    // the page of the i-th of the next 32 boxes, fetched by one load for all of them.
-    const int boxes = kTile / a.box_rows;
-    const uint32_t box_bytes = a.box_rows * 128;
-    int it = 0, piece = 0;
+    // A tile comes in boxes of box_rows tokens (a divisor of the page and of the tile), one lane a box of keys
+    // or values: it looks its page up and issues its copy.
+    const int box = lane / 2, is_v = lane & 1;
+    const CUtensorMap* map = is_v ? &v_map : &k_map;
+    const uint32_t box_bytes = a.box_rows * D * 2;
+    const uint32_t box_at = is_v * C::kHalfBytes + box * box_bytes;
+    // Lookups run ahead of the copies, by a tile within a unit and by a unit's first tile across units: this
+    // warp by itself has to stay below the time that a tile takes to arrive.
+    struct Piece {
+      int k0, n, row, head, block, solo;
+      Span span;
+      int token, column, offset, page;  // this lane's box of the next tile: its page's place in the table, and id
+      bool use;
+    };
+    auto look_up = [&](Piece& p) {
+      p.use = box * a.box_rows < kTile && p.token < p.span.length &&
+              (p.token < p.span.sink || p.token + a.box_rows > p.span.from);
+      p.page = p.use ? __ldg(a.page_table + (long long)p.row * a.max_pages + p.column) : 0;
+    };
+    auto place = [&](Piece& p, int k) {
+      p.token = p.span.tile(k) * kTile + box * a.box_rows;
+      p.column = p.token / a.page_tokens;
+      p.offset = p.token - p.column * a.page_tokens;
+      look_up(p);
+    };
+    auto next_piece = [&](Piece& p) {
+      if (!walk.next(a, units_per_row)) return false;
+      p.k0 = walk.k0;
+      p.n = walk.n;
+      p.row = walk.row;
+      p.head = walk.unit / a.row_blocks;
+      p.block = walk.unit - p.head * a.row_blocks;
+      p.span = walk.span;
+      p.solo = walk.n == walk.span.tiles && walk.n <= C::kSoloTiles;
+      place(p, p.k0);
+      return true;
+    };
     uint32_t used[2] = {0, 0};  // uses of each stage by each team, modulo 2
     bool ok = true;
-    for (; ok && walk.next(a, units_per_row); ++piece) {
-      const int head = walk.unit / a.row_blocks, block = walk.unit - head * a.row_blocks;
-      const int rows = min(NR, a.group - block * NR);
-      const bool solo = walk.n == walk.span.tiles && walk.n <= C::kSoloTiles;
-      const int q_slot = piece % C::kQSlots;
+    int stage = 0, round = 0, piece = 0;
+    Piece p, ahead;
+    bool more = next_piece(ahead);
+    for (; ok && more; ++piece) {
+      p = ahead;
+      more = next_piece(ahead);
+      const int q_slot = piece % C::kQSlots, rows = min(NR, a.group - p.block * NR);
       if (piece >= C::kQSlots) {
         ok = __all_sync(0xffffffffu, (int)mbar_wait(q_empty0 + 8 * q_slot, ((piece / C::kQSlots) - 1) & 1, &abort_s)) != 0;
         if (!ok) break;
@@ -264,57 +297,43 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       __syncwarp();
       if (lane < rows)
         bulk_1d(q_ring + q_slot * C::kQBytes + lane * C::kQPitch,
-                static_cast<const uint16_t*>(a.q) + walk.row * a.q_row_stride +
-                    ((long long)head * a.group + block * NR + lane) * a.q_head_stride,
+                static_cast<const uint16_t*>(a.q) + p.row * a.q_row_stride +
+                    ((long long)p.head * a.group + p.block * NR + lane) * a.q_head_stride,
                 D * 2, q_full0 + 8 * q_slot);
-      const int* table = a.page_table + (long long)walk.row * a.max_pages;
-      int held = -32, page = 0;
-      for (int j = 0; j < walk.n; ++j, ++it) {
-        const int stage = it % C::kStages, team = solo ? piece & 1 : j & 1;
-        if (it >= C::kStages) {
-          ok = __all_sync(0xffffffffu, (int)mbar_wait(empty0 + 8 * stage, ((it / C::kStages) - 1) & 1, &abort_s)) != 0;
+      for (int j = 0; j < p.n; ++j) {
+        const int team = (p.solo ? piece : j) & 1;
+        int page = p.page;
+        const int offset = p.offset;
+        const bool use = p.use;
+        if (j + 1 < p.n) {
+          if (p.k0 + j + 1 == p.span.sink_tiles) {
+            place(p, p.k0 + j + 1);
+          } else {
+            p.token += kTile;
+            for (p.offset += kTile; p.offset >= a.page_tokens; p.offset -= a.page_tokens) ++p.column;
+            look_up(p);
+          }
+        }
+        if (round > 0) {
+          ok = __all_sync(0xffffffffu, (int)mbar_wait(empty0 + 8 * stage, (round - 1) & 1, &abort_s)) != 0;
           if (!ok) break;
+        }
+        const uint32_t bar = full0 + 16 * stage + 8 * team;
+        const uint32_t wanted = __ballot_sync(0xffffffffu, use);
+        if (lane == 0) mbar_expect_tx(bar, __popc(wanted) * box_bytes);
+        __syncwarp();
+        if (use) {
+          if (page < 0 || page >= a.n_pages) {
+            if (a.status) atomicMax(a.status, 1);
+            page = 0;
+          }
+          tma_box(smem_u32(smem) + stage * C::kStageBytes + box_at, map, offset, page * a.n_kv_heads + p.head, bar);
         }
         used[0] ^= (uint32_t)(team == 0) << stage;
         used[1] ^= (uint32_t)team << stage;
-        const uint32_t dst = smem_u32(smem) + stage * C::kStageBytes, bar = full0 + 16 * stage + 8 * team;
-        const int token = walk.span.tile(walk.k0 + j) * kTile;
-        uint32_t wanted = 0;
-        for (int b = 0; b < boxes; ++b) {
-          const int t = token + b * a.box_rows;
-          const bool use = t < walk.span.length && (t < walk.span.sink || t + a.box_rows > walk.span.from);
-          wanted |= (uint32_t)use << b;
-        }
-        if (lane == 0) mbar_expect_tx(bar, __popc(wanted) * box_bytes * C::kColBoxes * 2);
-        for (int b = 0; b < boxes; ++b) {
-          const int i = j * boxes + b;
-          if (i >= held + 32) {
-            held = i;
-            const int ti = i + lane;  // the box this lane looks up
-            const int jj = ti / boxes;
-            page = 0;
-            if (jj < walk.n) {
-              const int t = walk.span.tile(walk.k0 + jj) * kTile + (ti - jj * boxes) * a.box_rows;
-              if (t < walk.span.length && (t < walk.span.sink || t + a.box_rows > walk.span.from)) {
-                page = __ldg(table + t / a.page_tokens);
-                if (page < 0 || page >= a.n_pages) {
-                  if (a.status) atomicMax(a.status, 1);
-                  page = 0;
-                }
-              }
-            }
-          }
-          const int pg = __shfl_sync(0xffffffffu, page, i - held);
-          if (lane == 0 && (wanted >> b & 1)) {
-            const int t = token + b * a.box_rows, y = t % a.page_tokens;
-            const int z = pg * a.n_kv_heads + head;
-#pragma unroll
-            for (int c = 0; c < C::kColBoxes; ++c) {
-              const uint32_t to = dst + c * kTile * 128 + b * box_bytes;
-              tma_3d(to, &k_map, c * 64, y, z, bar);
-              tma_3d(to + C::kHalfBytes, &v_map, c * 64, y, z, bar);
-            }
-          }
+        if (++stage == C::kStages) {
+          stage = 0;
+          ++round;
         }
       }
     }
@@ -337,6 +356,15 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   const int row16 = (warp % C::kTeamWarps) * 16;
   const int k_row = row16 + (lane & 15), k_chunk = lane >> 4;
   const int v_row = row16 + (lane & 7) + ((lane >> 4) << 3), v_chunk = (lane >> 3) & 1;
+  // a box's rows of 64 dims, then the same rows of the next 64
+  const uint32_t col_bytes = a.box_rows * 128;
+  uint32_t k_at[C::kSub], v_at[C::kSub];
+#pragma unroll
+  for (int u = 0; u < C::kSub; ++u) {
+    const int k = k_row + u * C::kSubTokens, v = v_row + u * C::kSubTokens;
+    k_at[u] = k / a.box_rows * (a.box_rows * D * 2) + k % a.box_rows * 128;
+    v_at[u] = v / a.box_rows * (a.box_rows * D * 2) + v % a.box_rows * 128;
+  }
   const float scale2 = a.scale * kLog2e;
   const long long n_slots = 2ll * gridDim.x;
   int it = 0;
@@ -388,42 +416,62 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       const uint32_t k_base = smem_u32(smem) + stage * C::kStageBytes, v_base = k_base + C::kHalfBytes;
       if (!__all_sync(0xffffffffu, (int)mbar_wait(full0 + 16 * stage + 8 * team, phase >> stage & 1, &abort_s))) break;
       phase ^= 1u << stage;
-      const int token = walk.span.tile(walk.k0 + j) * kTile + row16;
-      const bool whole = token + 15 < walk.span.length && (token >= walk.span.from || token + 15 < walk.span.sink);
-      const bool any = whole || (token < walk.span.length && (token < walk.span.sink || token + 15 >= walk.span.from));
+      const int token0 = walk.span.tile(walk.k0 + j) * kTile + row16;
+      // all of the warp's tokens are seen / some are
+      bool whole = true, any = false;
+#pragma unroll
+      for (int u = 0; u < C::kSub; ++u) {
+        const int first = token0 + u * C::kSubTokens, last = first + 15;
+        whole = whole && last < walk.span.length && (first >= walk.span.from || last < walk.span.sink);
+        any = any || (first < walk.span.length && (first < walk.span.sink || last >= walk.span.from));
+      }
       if (any) {
-        float sc[NT][4];
+        float sc[C::kSub][NT][4];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.0f;
+        for (int u = 0; u < C::kSub; ++u)
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-          uint32_t f[4];
-          ldmatrix_x4(f, k_base + (s / 4) * kTile * 128 + k_row * 128 + ((((s % 4) * 2 + k_chunk) ^ (k_row & 7)) << 4));
+          for (int t = 0; t < NT; ++t) sc[u][t][0] = sc[u][t][1] = sc[u][t][2] = sc[u][t][3] = 0.0f;
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            if constexpr (C::kF16) mma_f16(sc[t], f, qf[s][t][0], qf[s][t][1]);
-            else mma_bf16(sc[t], f, qf[s][t][0], qf[s][t][1]);
+        for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+          for (int u = 0; u < C::kSub; ++u) {
+            uint32_t f[4];
+            ldmatrix_x4(f, k_base + k_at[u] + (s / 4) * col_bytes + ((((s % 4) * 2 + k_chunk) ^ (k_row & 7)) << 4));
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              if constexpr (C::kF16) mma_f16(sc[u][t], f, qf[s][t][0], qf[s][t][1]);
+              else mma_bf16(sc[u][t], f, qf[s][t][0], qf[s][t][1]);
+            }
           }
+        // this thread's tokens: g and g + 8 of each 16; its query rows: 8 t + 2 qd + {0, 1}
+        bool see[C::kSub][2];
+#pragma unroll
+        for (int u = 0; u < C::kSub; ++u) {
+          see[u][0] = whole || walk.span.visible(token0 + u * C::kSubTokens + g);
+          see[u][1] = whole || walk.span.visible(token0 + u * C::kSubTokens + g + 8);
         }
-        // this thread's tokens: g and g + 8; its query rows: 8 t + 2 qd + {0, 1}
-        const bool see0 = whole || walk.span.visible(token + g), see1 = whole || walk.span.visible(token + g + 8);
-        uint32_t ph[NT][2], pl[NT][2];
+        uint32_t ph[C::kSub][NT][2], pl[C::kSub][NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          if (a.softcap > 0.0f) {
+          float hi[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              // cap tanh(x / cap) with tanh(y) = 1 - 2 / (1 + e^2y), good to a few 1e-7 of cap
-              const float e2y = ex2_ftz(sc[t][e] * a.cap_in);
-              sc[t][e] = a.softcap * kLog2e * (1.0f - __fdividef(2.0f, 1.0f + e2y));
+          for (int u = 0; u < C::kSub; ++u) {
+            if (a.softcap > 0.0f) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                // cap tanh(x / cap) with tanh(y) = 1 - 2 / (1 + e^2y), good to a few 1e-7 of cap
+                const float e2y = ex2_ftz(sc[u][t][e] * a.cap_in);
+                sc[u][t][e] = a.softcap * kLog2e * (1.0f - __fdividef(2.0f, 1.0f + e2y));
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sc[u][t][e] *= scale2;
             }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[t][e] *= scale2;
+            if (!see[u][0]) sc[u][t][0] = sc[u][t][1] = -INFINITY;
+            if (!see[u][1]) sc[u][t][2] = sc[u][t][3] = -INFINITY;
+            hi[0] = fmaxf(hi[0], fmaxf(sc[u][t][0], sc[u][t][2]));
+            hi[1] = fmaxf(hi[1], fmaxf(sc[u][t][1], sc[u][t][3]));
           }
-          if (!see0) sc[t][0] = sc[t][1] = -INFINITY;
-          if (!see1) sc[t][2] = sc[t][3] = -INFINITY;
-          float hi[2] = {fmaxf(sc[t][0], sc[t][2]), fmaxf(sc[t][1], sc[t][3])};
 #pragma unroll
           for (int d = 4; d < 32; d *= 2) {
             hi[0] = fmaxf(hi[0], __shfl_xor_sync(0xffffffffu, hi[0], d));
@@ -448,60 +496,65 @@ __global__ void __launch_bounds__(C::kThreads, 1)
           }
           // a row whose scores so far are all -inf keeps weights exp2(-inf - 0) = 0
           const float m0 = m[t][0] == -INFINITY ? 0.0f : m[t][0], m1 = m[t][1] == -INFINITY ? 0.0f : m[t][1];
-          const float p0 = see0 ? ex2_ftz(sc[t][0] - m0) : 0.0f, p1 = see0 ? ex2_ftz(sc[t][1] - m1) : 0.0f;
-          const float p2 = see1 ? ex2_ftz(sc[t][2] - m0) : 0.0f, p3 = see1 ? ex2_ftz(sc[t][3] - m1) : 0.0f;
-          l[t][0] += p0 + p2;
-          l[t][1] += p1 + p3;
-          // The weights go to the second product as two 16-bit parts: one rounding would cost the
-          // output as much as its own type does, and the second product's time is hidden behind
-          // the loads (2 x 8 MMAs of 350 cycles a warp at D = 128).
-          uint32_t h01, h23;
-          float2 b01, b23;
-          if constexpr (C::kF16) {
-            h01 = pack_half2(p0, p1), h23 = pack_half2(p2, p3);
-            b01 = unpack_half2(h01), b23 = unpack_half2(h23);
-            pl[t][0] = transpose8(pack_half2(p0 - b01.x, p1 - b01.y));
-            pl[t][1] = transpose8(pack_half2(p2 - b23.x, p3 - b23.y));
-          } else {
-            h01 = pack_bf162(p0, p1), h23 = pack_bf162(p2, p3);
-            b01 = unpack_bf162(h01), b23 = unpack_bf162(h23);
-            pl[t][0] = transpose8(pack_bf162(p0 - b01.x, p1 - b01.y));
-            pl[t][1] = transpose8(pack_bf162(p2 - b23.x, p3 - b23.y));
+#pragma unroll
+          for (int u = 0; u < C::kSub; ++u) {
+            const float p0 = see[u][0] ? ex2_ftz(sc[u][t][0] - m0) : 0.0f, p1 = see[u][0] ? ex2_ftz(sc[u][t][1] - m1) : 0.0f;
+            const float p2 = see[u][1] ? ex2_ftz(sc[u][t][2] - m0) : 0.0f, p3 = see[u][1] ? ex2_ftz(sc[u][t][3] - m1) : 0.0f;
+            l[t][0] += p0 + p2;
+            l[t][1] += p1 + p3;
+            // The weights go to the second product as two 16-bit parts: one rounding would cost the output as
+            // much as its own type does, and the second product's time is hidden behind the loads.
+            uint32_t h01, h23;
+            float2 b01, b23;
+            if constexpr (C::kF16) {
+              h01 = pack_half2(p0, p1), h23 = pack_half2(p2, p3);
+              b01 = unpack_half2(h01), b23 = unpack_half2(h23);
+              pl[u][t][0] = transpose8(pack_half2(p0 - b01.x, p1 - b01.y));
+              pl[u][t][1] = transpose8(pack_half2(p2 - b23.x, p3 - b23.y));
+            } else {
+              h01 = pack_bf162(p0, p1), h23 = pack_bf162(p2, p3);
+              b01 = unpack_bf162(h01), b23 = unpack_bf162(h23);
+              pl[u][t][0] = transpose8(pack_bf162(p0 - b01.x, p1 - b01.y));
+              pl[u][t][1] = transpose8(pack_bf162(p2 - b23.x, p3 - b23.y));
+            }
+            ph[u][t][0] = transpose8(h01);
+            ph[u][t][1] = transpose8(h23);
           }
-          ph[t][0] = transpose8(h01);
-          ph[t][1] = transpose8(h23);
         }
         // In a tile with tokens that are not seen, their values are cleared as well: 0 times an
         // infinity or NaN that a page happens to hold past a sequence's end is not 0.
-        uint32_t keep_lo = 0xffffffffu, keep_hi = 0xffffffffu;
-        if (!whole) {
-          keep_lo = (walk.span.visible(token + 2 * qd) ? 0xffffu : 0u) |
-                    (walk.span.visible(token + 2 * qd + 1) ? 0xffff0000u : 0u);
-          keep_hi = (walk.span.visible(token + 2 * qd + 8) ? 0xffffu : 0u) |
-                    (walk.span.visible(token + 2 * qd + 9) ? 0xffff0000u : 0u);
-        }
+        uint32_t keep[C::kSub][2];
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          uint32_t f[4];
-          ldmatrix_x4_trans(f, v_base + (i / 4) * kTile * 128 + v_row * 128 +
-                                   ((((i % 4) * 2 + v_chunk) ^ (v_row & 7)) << 4));
-          if (!whole) {
-            f[0] &= keep_lo;
-            f[1] &= keep_lo;
-            f[2] &= keep_hi;
-            f[3] &= keep_hi;
+        for (int u = 0; u < C::kSub; ++u)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int at = token0 + u * C::kSubTokens + 2 * qd + 8 * h;
+            keep[u][h] = whole ? 0xffffffffu
+                               : (walk.span.visible(at) ? 0xffffu : 0u) | (walk.span.visible(at + 1) ? 0xffff0000u : 0u);
           }
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            if constexpr (C::kF16) {
-              mma_f16(acc[i][t], f, ph[t][0], ph[t][1]);
-              mma_f16(acc[i][t], f, pl[t][0], pl[t][1]);
-            } else {
-              mma_bf16(acc[i][t], f, ph[t][0], ph[t][1]);
-              mma_bf16(acc[i][t], f, pl[t][0], pl[t][1]);
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int u = 0; u < C::kSub; ++u) {
+            uint32_t f[4];
+            ldmatrix_x4_trans(f, v_base + v_at[u] + (i / 4) * col_bytes + ((((i % 4) * 2 + v_chunk) ^ (v_row & 7)) << 4));
+            if (!whole) {
+              f[0] &= keep[u][0];
+              f[1] &= keep[u][0];
+              f[2] &= keep[u][1];
+              f[3] &= keep[u][1];
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              if constexpr (C::kF16) {
+                mma_f16(acc[i][t], f, ph[u][t][0], ph[u][t][1]);
+                mma_f16(acc[i][t], f, pl[u][t][0], pl[u][t][1]);
+              } else {
+                mma_bf16(acc[i][t], f, ph[u][t][0], ph[u][t][1]);
+                mma_bf16(acc[i][t], f, pl[u][t][0], pl[u][t][1]);
+              }
             }
           }
-        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(empty0 + 8 * stage);
@@ -695,16 +748,16 @@ static EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// [n_pages * n_kv_heads][page_tokens][D] 16-bit values, read in boxes of [box_rows][64 dims] with the
+// [n_pages * n_kv_heads][page_tokens][D] 16-bit values, read in boxes of [D / 64][box_rows][64 dims] with the
 // 128-byte swizzle
 static int make_map(CUtensorMap* map, const void* base, const asterq_paged_attention_params* p, int box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return set_error(ASTERQ_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled unavailable");
-  const cuuint64_t dims[3] = {(cuuint64_t)p->head_dim, (cuuint64_t)p->page_tokens,
+  const cuuint64_t dims[4] = {64u, (cuuint64_t)p->page_tokens, (cuuint64_t)p->head_dim / 64,
                               (cuuint64_t)(p->n_pages > 0 ? p->n_pages * p->n_kv_heads : 1)};
-  const cuuint64_t strides[2] = {(cuuint64_t)p->head_dim * 2, (cuuint64_t)p->head_dim * 2 * p->page_tokens};
-  const cuuint32_t box[3] = {64u, (cuuint32_t)box_rows, 1u}, step[3] = {1u, 1u, 1u};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, step,
+  const cuuint64_t strides[3] = {(cuuint64_t)p->head_dim * 2, 128u, (cuuint64_t)p->head_dim * 2 * p->page_tokens};
+  const cuuint32_t box[4] = {64u, (cuuint32_t)box_rows, (cuuint32_t)p->head_dim / 64, 1u}, step[4] = {1u, 1u, 1u, 1u};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides, box, step,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
@@ -833,9 +886,9 @@ extern "C" int asterq_paged_attention(const asterq_paged_attention_params* p, vo
   a.scale = p->softmax_scale;
   a.softcap = p->logit_softcap > 0.0f ? p->logit_softcap : 0.0f;
   a.cap_in = a.softcap > 0.0f ? 2.0f * pat::kLog2e * a.scale / a.softcap : 0.0f;
-  // boxes of a tile lie in one page each: the largest of 64, 32 and 16 tokens that divides the page
-  a.box_rows = p->page_tokens % 64 == 0 ? 64 : p->page_tokens % 32 == 0 ? 32 : 16;
-  if (p->head_dim == 256 && a.box_rows > 32) a.box_rows = 32;
+  // a box of a tile lies in one page: the largest of the tile, its half, .. down to 16 tokens that divides the page
+  a.box_rows = 8192 / p->head_dim;
+  while (p->page_tokens % a.box_rows) a.box_rows /= 2;
   CUtensorMap k_map, v_map;
   const bool pools = a.capacity > 0;  // with none, nothing is visible and the maps are never read
   if ((st = pat::make_map(&k_map, pools ? p->k_pool : p->workspace, p, a.box_rows)) != ASTERQ_OK) return st;
