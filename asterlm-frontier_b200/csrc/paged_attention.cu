@@ -60,8 +60,10 @@ struct Cfg {
   // queries of the next units, rows padded against conflicts
   static constexpr int kQSlots = NR * D >= 2048 ? 2 : 4, kQPitch = D * 2 + 16;
   static constexpr int kQBytes = NR * kQPitch;
-  static constexpr int kSlice = NR == 16 ? 32 : 64, kPad = kSlice + 4;  // dims joined at a time
-  static constexpr int kMergeFloats = kWarps * NR * kPad;
+  // dims joined at a time, in two buffers taken in turn; their count is even, so a unit ends with the second
+  static constexpr int kSlice = NR == 16 ? 16 : 32, kPad = kSlice + 4;
+  static constexpr int kBufFloats = kWarps * NR * kPad, kMergeFloats = 2 * kBufFloats;
+  static_assert(D / kSlice % 2 == 0, "the two buffers alternate across units");
   static_assert(kMergeFloats >= 24 * NR, "weights of the records that are joined at once");
   // What a unit costs beside its tiles, in tiles: a unit by itself takes 1.5 us, two at a time, a tile's share of
   // the memory bandwidth 0.75 us.
@@ -116,24 +118,32 @@ ASTERQ_DEVICE Span span_of(const Args& a, int row) {
 // One CTA's share [x, end) of all units' costs, walked piece by piece; every warp walks it for itself.
 template <int kTile, int kUnitCost>
 struct Walk {
-  long long x, end, row_start;
+  long long x, end, unit_start;  // unit_start: of the unit that x is in, or has just passed
   int row;
   Span span;
   // of the current piece
   int unit, k0, n;        // unit within the row, its first tile here, tiles here
   long long first_tile;   // where the unit's first tile is
   template <class A>
+  ASTERQ_DEVICE void start(const A& a, int at_row, long long row_start) {
+    row = at_row;
+    span = span_of<kTile>(a, row);
+    unit = (int)((x - row_start) / (span.tiles + kUnitCost));
+    unit_start = row_start + (long long)unit * (span.tiles + kUnitCost);
+  }
+  template <class A>
   ASTERQ_DEVICE bool next(const A& a, int units_per_row) {
     while (x < end) {
-      const int per_unit = span.tiles + kUnitCost;
-      if (span.tiles == 0 || x >= row_start + (long long)per_unit * units_per_row) {
-        if (span.tiles > 0) row_start += (long long)per_unit * units_per_row;
-        span = span_of<kTile>(a, ++row);
-        continue;
+      int per_unit = span.tiles + kUnitCost;
+      if (x >= unit_start + per_unit) {
+        unit_start += per_unit;
+        if (++unit == units_per_row) {
+          unit = 0;
+          do span = span_of<kTile>(a, ++row);
+          while (span.tiles == 0);
+          per_unit = span.tiles + kUnitCost;
+        }
       }
-      const long long in_row = x - row_start;
-      unit = in_row < 0x7fffffff ? (int)in_row / per_unit : (int)(in_row / per_unit);
-      const long long unit_start = row_start + (long long)unit * per_unit;
       const int at = (int)(x - unit_start), cost = (int)min((long long)(per_unit - at), end - x);
       first_tile = unit_start + kUnitCost;
       k0 = max(at - kUnitCost, 0);
@@ -237,9 +247,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   __syncthreads();
   if (walk.x >= walk.end) return;
   const long long my_start = walk.x;
-  walk.row = start_s.row;
-  walk.row_start = start_s.row_start;
-  walk.span = span_of<kTile>(a, walk.row);
+  walk.start(a, start_s.row, start_s.row_start);
 
   if (warp == C::kWarps) {
     // ------------------------------------------------------------------ producer
@@ -257,16 +265,17 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       int token, column, offset, page;  // this lane's box of the next tile: its page's place in the table, and id
       bool use;
     };
-    auto look_up = [&](Piece& p) {
+    auto look_up = [&](Piece& p, bool same_page) {
       p.use = box * a.box_rows < kTile && p.token < p.span.length &&
               (p.token < p.span.sink || p.token + a.box_rows > p.span.from);
-      p.page = p.use ? __ldg(a.page_table + (long long)p.row * a.max_pages + p.column) : 0;
+      if (p.use && !same_page) p.page = __ldg(a.page_table + (long long)p.row * a.max_pages + p.column);
     };
     auto place = [&](Piece& p, int k) {
       p.token = p.span.tile(k) * kTile + box * a.box_rows;
       p.column = p.token / a.page_tokens;
       p.offset = p.token - p.column * a.page_tokens;
-      look_up(p);
+      p.page = 0;
+      look_up(p, false);
     };
     auto next_piece = [&](Piece& p) {
       if (!walk.next(a, units_per_row)) return false;
@@ -309,9 +318,11 @@ __global__ void __launch_bounds__(C::kThreads, 1)
           if (p.k0 + j + 1 == p.span.sink_tiles) {
             place(p, p.k0 + j + 1);
           } else {
+            const int column = p.column;
+            const bool had = p.use;
             p.token += kTile;
             for (p.offset += kTile; p.offset >= a.page_tokens; p.offset -= a.page_tokens) ++p.column;
-            look_up(p);
+            look_up(p, had && p.column == column);
           }
         }
         if (round > 0) {
@@ -451,9 +462,10 @@ __global__ void __launch_bounds__(C::kThreads, 1)
           see[u][1] = whole || walk.span.visible(token0 + u * C::kSubTokens + g + 8);
         }
         uint32_t ph[C::kSub][NT][2], pl[C::kSub][NT][2];
+        float hi[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          float hi[2] = {-INFINITY, -INFINITY};
+          hi[t][0] = hi[t][1] = -INFINITY;
 #pragma unroll
           for (int u = 0; u < C::kSub; ++u) {
             if (a.softcap > 0.0f) {
@@ -469,19 +481,27 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             }
             if (!see[u][0]) sc[u][t][0] = sc[u][t][1] = -INFINITY;
             if (!see[u][1]) sc[u][t][2] = sc[u][t][3] = -INFINITY;
-            hi[0] = fmaxf(hi[0], fmaxf(sc[u][t][0], sc[u][t][2]));
-            hi[1] = fmaxf(hi[1], fmaxf(sc[u][t][1], sc[u][t][3]));
+            hi[t][0] = fmaxf(hi[t][0], fmaxf(sc[u][t][0], sc[u][t][2]));
+            hi[t][1] = fmaxf(hi[t][1], fmaxf(sc[u][t][1], sc[u][t][3]));
           }
+        }
 #pragma unroll
-          for (int d = 4; d < 32; d *= 2) {
-            hi[0] = fmaxf(hi[0], __shfl_xor_sync(0xffffffffu, hi[0], d));
-            hi[1] = fmaxf(hi[1], __shfl_xor_sync(0xffffffffu, hi[1], d));
+        for (int d = 4; d < 32; d *= 2)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            hi[t][0] = fmaxf(hi[t][0], __shfl_xor_sync(0xffffffffu, hi[t][0], d));
+            hi[t][1] = fmaxf(hi[t][1], __shfl_xor_sync(0xffffffffu, hi[t][1], d));
           }
-          if (__any_sync(0xffffffffu, hi[0] > m[t][0] || hi[1] > m[t][1])) {
+        bool higher = false;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) higher = higher || hi[t][0] > m[t][0] || hi[t][1] > m[t][1];
+        if (__any_sync(0xffffffffu, higher)) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
             float turn[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float now = fmaxf(m[t][e], hi[e]);
+              const float now = fmaxf(m[t][e], hi[t][e]);
               turn[e] = now == -INFINITY ? 1.0f : ex2_ftz(m[t][e] - now);
               m[t][e] = now;
               l[t][e] *= turn[e];
@@ -494,6 +514,9 @@ __global__ void __launch_bounds__(C::kThreads, 1)
               acc[i][t][3] *= turn[1];
             }
           }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
           // a row whose scores so far are all -inf keeps weights exp2(-inf - 0) = 0
           const float m0 = m[t][0] == -INFINITY ? 0.0f : m[t][0], m1 = m[t][1] == -INFINITY ? 0.0f : m[t][1];
 #pragma unroll
@@ -565,6 +588,8 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     const int wa = solo ? team * C::kTeamWarps : 0, wn = solo ? C::kTeamWarps : C::kWarps;
     const int me_in = tid - wa * 32, threads = wn * 32;
     auto sync = [&]() { named_sync(solo ? 1 + team : 3, threads); };
+    // slot of this piece: a share's first piece may be the tail or middle of a unit, its last the head
+    const long long slot = 2ll * me + (walk.first_tile > my_start ? 1 : 0);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -576,62 +601,61 @@ __global__ void __launch_bounds__(C::kThreads, 1)
           warp_l[warp * NR + t * 8 + 2 * qd + e] = l[t][e];
         }
       }
-    sync();
-    // slot of this piece: a share's first piece may be the tail or middle of a unit, its last the head
-    const long long slot = 2ll * me + (walk.first_tile > my_start ? 1 : 0);
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float top = -INFINITY;
-        for (int w = wa; w < wa + wn; ++w) top = fmaxf(top, warp_m[w * NR + t * 8 + 2 * qd + e]);
-        const float turn = m[t][e] == -INFINITY ? 0.0f : ex2_ftz(m[t][e] - top);
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          acc[i][t][e] *= turn;
-          acc[i][t][e + 2] *= turn;
-        }
-      }
+    // Each thread sums the same rows of every slice, so the warps' factors are looked up once, behind the
+    // first barrier; with the second slice's barrier passed nobody reads warp_m and warp_l any more.
+    constexpr int kOwn = NR * C::kSlice / (C::kTeamWarps * 32);  // of a team; half as many with all warps
+    float factor[kOwn][C::kWarps], weight_sum[kOwn];
 #pragma unroll
     for (int part = 0; part < D / C::kSlice; ++part) {
+      float* buf = merge + (part & 1) * C::kBufFloats;
 #pragma unroll
       for (int i = 0; i < C::kSlice / 16; ++i)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            merge[(warp * NR + t * 8 + 2 * qd + (e & 1)) * C::kPad + i * 16 + g + (e >> 1) * 8] =
+            buf[(warp * NR + t * 8 + 2 * qd + (e & 1)) * C::kPad + i * 16 + g + (e >> 1) * 8] =
                 acc[part * (C::kSlice / 16) + i][t][e];
       sync();
-      for (int i = me_in; i < (cut ? NR : rows) * C::kSlice; i += threads) {
-        const int r = i / C::kSlice, d = i % C::kSlice;
-        float sum = 0.0f, top = -INFINITY, total_l = 0.0f;
-        for (int w = wa; w < wa + wn; ++w) {
-          sum += merge[(w * NR + r) * C::kPad + d];
-          top = fmaxf(top, warp_m[w * NR + r]);
-        }
-        for (int w = wa; w < wa + wn; ++w) {
-          const float mw = warp_m[w * NR + r];
-          total_l += mw == -INFINITY ? warp_l[w * NR + r] : warp_l[w * NR + r] * ex2_ftz(mw - top);
-        }
-        const int dim = part * C::kSlice + d;
-        if (cut) {
-          a.records[(slot * NR + r) * D + dim] = sum;
-          if (dim == 0) {
+#pragma unroll
+      for (int k = 0; k < kOwn; ++k) {
+        const int i = me_in + k * threads, r = i / C::kSlice, d = i % C::kSlice, dim = part * C::kSlice + d;
+        if (r >= (cut ? NR : rows)) continue;
+        if (part == 0) {
+          float top = -INFINITY, total_l = 0.0f;
+#pragma unroll
+          for (int w = 0; w < C::kWarps; ++w)
+            if (w < wn) top = fmaxf(top, factor[k][w] = warp_m[(wa + w) * NR + r]);
+#pragma unroll
+          for (int w = 0; w < C::kWarps; ++w)
+            if (w < wn) {
+              const float lw = warp_l[(wa + w) * NR + r];  // not 0 although the maximum is -inf: NaN scores
+              const bool none = factor[k][w] == -INFINITY;
+              factor[k][w] = none ? 0.0f : ex2_ftz(factor[k][w] - top);
+              total_l += none ? lw : lw * factor[k][w];
+            }
+          weight_sum[k] = total_l;
+          if (d == 0 && cut) {
             a.records[n_slots * NR * D + slot * NR + r] = top;
             a.records[n_slots * NR * (D + 1) + slot * NR + r] = total_l;
+          } else if (d == 0 && a.lse) {
+            a.lse[(long long)walk.row * a.n_heads + h0 + r] = (top + log2f(total_l)) * kLn2;
           }
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < C::kWarps; ++w)
+          if (w < wn) sum = fmaf(factor[k][w], buf[((wa + w) * NR + r) * C::kPad + d], sum);
+        if (cut) {
+          a.records[(slot * NR + r) * D + dim] = sum;
         } else {
           const long long at = ((long long)walk.row * a.n_heads + h0 + r) * D + dim;
-          const float o = sum / total_l;
+          const float o = sum / weight_sum[k];
           if (a.out_f32) static_cast<float*>(a.out)[at] = o;
           else if constexpr (C::kF16) static_cast<__half*>(a.out)[at] = __float2half_rn(o);
           else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(o);
-          if (a.lse && dim == 0)
-            a.lse[(long long)walk.row * a.n_heads + h0 + r] = (top + log2f(total_l)) * kLn2;
         }
       }
-      sync();
     }
     if (!cut) continue;
 
