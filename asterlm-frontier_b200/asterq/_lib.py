@@ -282,6 +282,26 @@ def packer(cls) -> struct.Struct:
     return struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_))
 
 
+_calls = None
+
+
+def quick_calls():
+    """The extension module ``_calls`` bound to the loaded library, or None where it is not built: the
+    callers' own checks then make every call."""
+    global _calls
+    if _calls is None:
+        try:
+            from . import _calls as module
+        except ImportError:
+            _calls = False
+            return None
+        lib = load()
+        module.bind(*(ctypes.cast(f, ctypes.c_void_p).value
+                      for f in (lib.asterq_kv_append, lib.asterq_paged_attention, lib.asterq_linear_attention)))
+        _calls = module
+    return _calls or None
+
+
 class AsterqError(RuntimeError):
     """A failed ``asterq_*`` call (status and message from ``asterq_last_error``)."""
 

@@ -4,6 +4,8 @@
 ``__graft_entry__.build()`` compiles every ``csrc/*.cu`` for sm_100a with nvcc
 and links one shared library next to this file.  The library depends only on
 the CUDA runtime (linked statically), so it loads without PyTorch.
+``build_calls`` compiles ``csrc/torch_calls.cpp`` against torch's headers: an
+extension module that shortens the calls a decode step makes for every layer.
 """
 from __future__ import annotations
 
@@ -11,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -19,6 +22,8 @@ CSRC = PROJECT_DIR / "csrc"
 INCLUDE = PROJECT_DIR.parent / "include"
 LIB_NAME = "libasterq.so"
 LIB_PATH = PKG_DIR / LIB_NAME
+CALLS_SRC = CSRC / "torch_calls.cpp"
+CALLS_PATH = PKG_DIR / ("_calls" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 BUILD_DIR = PROJECT_DIR / "_build"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -90,6 +95,32 @@ def build(verbose: bool = False, force: bool = False, ptxas_verbose: bool = Fals
     return LIB_PATH
 
 
+def build_calls(verbose: bool = False, force: bool = False) -> Path:
+    """Compile ``asterq/_calls`` (the quick way from torch tensors to the library's calls, g++)."""
+    if not force and not _stale(CALLS_PATH, [CALLS_SRC, *sorted(INCLUDE.glob("*.h"))]):
+        return CALLS_PATH
+    import torch
+    from torch.utils import cpp_extension
+
+    tmp = CALLS_PATH.with_name(CALLS_PATH.name + ".tmp")
+    libs = Path(torch.__file__).resolve().parent / "lib"
+    cuda = Path(nvcc_path()).resolve().parent.parent
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-I{p}" for p in cpp_extension.include_paths()), f"-I{cuda / 'include'}",
+           f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}", str(CALLS_SRC), "-o", str(tmp), f"-L{libs}",
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError("g++ failed on torch_calls.cpp")
+    os.replace(tmp, CALLS_PATH)
+    return CALLS_PATH
+
+
 if __name__ == "__main__":
     build(verbose=True, force="--force" in sys.argv, ptxas_verbose="--ptxas" in sys.argv)
     print(LIB_PATH)
+    print(build_calls(verbose=True, force="--force" in sys.argv))

@@ -20,7 +20,7 @@ import math
 import torch
 
 from . import _lib
-from .paged_kv import _call, _check_int
+from .paged_kv import _call, _check_int, _quick
 
 _PARAMS = _lib.packer(_lib.LinearParams)
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
@@ -60,10 +60,18 @@ def _workspace(device: torch.device, stream: int) -> LinearAttentionWorkspace:
     ws = _workspaces.get((device.index, stream))
     if ws is None:
         ws = _workspaces[(device.index, stream)] = LinearAttentionWorkspace(device)
+        if _quick() is not None:
+            _quick().workspace(1, device.index, stream, ws.buffer.data_ptr(), ws.nbytes)
     return ws
 
 
 def _run(state, slots, lengths, row_offsets, q, k, v, log_decay, scale, out, workspace, status):
+    quick = _quick()
+    if quick is not None and workspace is None:
+        done = quick.linear(state, slots, lengths, row_offsets, q, k, v, log_decay,
+                            q.shape[-1] ** -0.5 if scale is None else scale, out, status)
+        if done is not NotImplemented:
+            return done
     if q.dim() != 3 or state.dim() != 4:
         raise ValueError("q must be [rows, n_heads, dk] and state [n_slots, n_heads, dk, dv]")
     if q.dtype not in _DTYPES:

@@ -31,6 +31,16 @@ _ATTEND = _lib.packer(_lib.PagedAttentionParams)
 ATTENTION_HEAD_DIMS = (64, 128, 256)
 
 
+_quick_module = 0  # not looked for yet
+
+
+def _quick():
+    global _quick_module
+    if _quick_module == 0:
+        _quick_module = _lib.quick_calls()
+    return _quick_module
+
+
 class PagedKVPools:
     """Page pools of one layer: ``k`` and ``v`` [n_pages, n_kv_heads, page_tokens, head_dim], contiguous,
     bfloat16 or float16 on the GPU."""
@@ -38,6 +48,10 @@ class PagedKVPools:
     __slots__ = ("k", "v")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor) -> None:
+        self.k, self.v = k, v
+        quick = _quick()
+        if quick is not None and quick.check_pools(k, v) is True:
+            return
         if k.dim() != 4 or v.shape != k.shape:
             raise ValueError("k and v must be [n_pages, n_kv_heads, page_tokens, head_dim]")
         if k.dtype not in _DTYPES or v.dtype != k.dtype:
@@ -46,7 +60,6 @@ class PagedKVPools:
             raise RuntimeError("asterq caches live on the GPU; there is no CPU path")
         if not (k.is_contiguous() and v.is_contiguous()):
             raise ValueError("the pools must be contiguous")
-        self.k, self.v = k, v
 
     @staticmethod
     def empty(n_pages: int, n_kv_heads: int, page_tokens: int, head_dim: int, *, dtype=torch.bfloat16,
@@ -78,6 +91,8 @@ def _workspace(device: torch.device, stream: int) -> PagedAttentionWorkspace:
     ws = _workspaces.get((device.index, stream))
     if ws is None:
         ws = _workspaces[(device.index, stream)] = PagedAttentionWorkspace(device)
+        if _quick() is not None:
+            _quick().workspace(0, device.index, stream, ws.buffer.data_ptr(), ws.nbytes)
     return ws
 
 
@@ -140,6 +155,11 @@ def append_kv(
     (``q_out``, not overlapping q, if given); rows left out leave it unwritten.  status int32 [1]: set to
     1 when a row had no page in the table or no row in cos / sin and was left out.
     """
+    quick = _quick()
+    if quick is not None:
+        done = quick.append(pools.k, pools.v, page_table, lengths, row_offsets, k, v, q, cos, sin, interleaved, q_out, status)
+        if done is not NotImplemented:
+            return done
     n_kv, page, dim = pools.k.shape[1:]
     if row_offsets.dim() != 1 or page_table.dim() != 2:
         raise ValueError("page_table must be [n_seqs, max_pages] and row_offsets [n_seqs + 1]")
@@ -220,6 +240,13 @@ def paged_attention(
     ``softmax_scale`` (1 / sqrt(head_dim)) q . k, softcapped to ``logit_softcap`` if given.  ``out``: the
     queries' type or float32.  status int32 [1]: set to 1 when a needed page id was outside the pool.
     """
+    quick = _quick()
+    if quick is not None and workspace is None and window_size != 0:
+        done = quick.attend(pools.k, pools.v, page_table, lengths, q, n_new, window_size or 0, sink_tokens,
+                            pools.k.shape[3] ** -0.5 if softmax_scale is None else softmax_scale, logit_softcap or 0.0,
+                            out, return_lse, status)
+        if done is not NotImplemented:
+            return done
     if q.dim() != 3 or page_table.dim() != 2:
         raise ValueError("q must be [n_seqs, n_heads, head_dim] and page_table [n_seqs, max_pages]")
     n_pages, n_kv, page, dim = pools.k.shape
