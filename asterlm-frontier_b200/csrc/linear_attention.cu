@@ -35,7 +35,9 @@ constexpr int kThreads = 256;
 // One CTA: kCols columns of one (sequence, head)'s state, in registers from the first token to the
 // last.  A single token reads and writes 8 Dk Dv bytes of state for 5 Dk Dv operations: bound by
 // memory.  Each thread has four columns of Dk kCols / 1024 rows, all of whose loads are in flight at
-// once, and kCols / 4 lanes read a row's columns together.
+// once, and kCols / 4 lanes read a row's columns together.  Measured: 256 rows of 32 heads of 128 x 128, one
+// token each, 164 us, 6.5 TB/s; 4 rows of 16 heads 2.9 us.  Several tokens add about 0.45 us each, the latency of
+// the next token's loads and of the sum over the key dims.
 template <int kType, int kDk, int kDv, int kCols>
 __global__ void __launch_bounds__(kThreads) scan_kernel(const __grid_constant__ Args a) {
   constexpr int kLanes = kCols / 4;              // threads of a row
@@ -117,14 +119,19 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(const __grid_constant__ 
 
 template <int kType, int kDk, int kDv>
 static void scan(const Args& a, int sms, cudaStream_t s) {
-  // Columns of a CTA: the whole width, whose loads are the longest runs, once (sequence, head) pairs
-  // fill the SMs twice over; below that 32 columns, so that more SMs share the traffic.
+  // Columns of a CTA: the whole width, whose loads are the longest runs, but 32 of 128 while the (sequence,
+  // head) pairs do not fill the SMs twice over.  Measured at 128 x 128 dims, 32 columns against all 128:
+  // one token, 64 pairs 2.9 against 3.5 us, 288 pairs 6.2 against 5.9, 8192 pairs 173 against 164; 24 tokens,
+  // 64 pairs 14.7 against 17.2, 512 pairs 72 against 58.  Of 64 columns the whole is as good or better
+  // throughout: 64 pairs of 2 tokens 3.3 against 3.4 us, 4096 of 24 tokens 156 against 238.
   const dim3 grid(a.n_seqs, a.n_heads, 1);
-  if ((long long)a.n_seqs * a.n_heads >= 2ll * sms) {
-    scan_kernel<kType, kDk, kDv, kDv><<<grid, kThreads, 0, s>>>(a);
-  } else {
-    scan_kernel<kType, kDk, kDv, 32><<<dim3(a.n_seqs, a.n_heads, kDv / 32), kThreads, 0, s>>>(a);
+  if constexpr (kDv == 128) {
+    if ((long long)a.n_seqs * a.n_heads < 2ll * sms) {
+      scan_kernel<kType, kDk, kDv, 32><<<dim3(a.n_seqs, a.n_heads, kDv / 32), kThreads, 0, s>>>(a);
+      return;
+    }
   }
+  scan_kernel<kType, kDk, kDv, kDv><<<grid, kThreads, 0, s>>>(a);
 }
 template <int kType>
 static void scan_by_dims(const Args& a, int dk, int dv, int sms, cudaStream_t s) {
@@ -145,8 +152,11 @@ static int sm_count(int* device) {
   return n;
 }
 
-// The chunked form takes bf16 prompts of 24 tokens a sequence or more on average: it needs about 20 us
-// for any of them up to one chunk a CTA, the scan 0.5 us a token.
+// The chunked form takes bf16 prompts of 24 tokens a sequence or more on average.  Measured at 128 x 128
+// dims, chunked against the scan: 24 tokens, 16 heads of one sequence 21 against 12.5 us, 128 (sequence, head)
+// pairs 22 against 23, 512 pairs 48 against 58, 4096 pairs 232 against 451; 128 tokens, 16 pairs 23 against 57,
+// 4096 pairs 296 against 2147.  At 64 x 64 dims: 24 tokens, 128 pairs 17 against 18 us, 4096 pairs 130 against
+// 155; 128 tokens, 18 against 87 and 135 against 753.
 static bool in_chunks(const asterq_linear_params* p) {
   return p->dtype == ASTERQ_DTYPE_BF16 && p->row_offsets && p->n_rows >= 24ll * p->n_seqs;
 }

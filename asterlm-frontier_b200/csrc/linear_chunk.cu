@@ -8,6 +8,12 @@
 // once (128 KB a chunk and head).  At one head-chunk a CTA, an SM's share of the memory bandwidth
 // takes 5,700 cycles for them; the products below take 4,600 on the tensor core.
 //
+// Measured (128 x 128 dims): 32777 tokens of 12 sequences and 32 heads 440 us, 2.5 TB/s (the bytes alone: 170 us).
+// A CTA's 55 chunks take 6.2 us each: the chain of a chunk, from keys through weighted parts, tensor memory
+// and products to the state, hides only in part behind the next one's, with shared memory 60% busy.  8192
+// tokens of one sequence and 16 heads: 104 us, of which the first pass takes 41 and the chain of states 8.  One
+// chunk of 16 heads: 23 us, three launches and the latency of one chunk.
+//
 // Rounding.  Products take bf16 operands and sum in fp32.  A and S enter as two bf16 parts (16 bits:
 // beside the output's own rounding they vanish).  The state is an fp32 output, so its update must not
 // round w_j k_j to less.  The weight is split into bf16 parts w = w1 + w2 + w3 and the key's bf16 products
@@ -26,8 +32,8 @@
 // Roles in a CTA (512 threads): warps 0-3 turn Q K^T into A (row i = thread i) and write the output;
 // warps 4-11 hold S in registers (thread = key dim, half of the value dims), scale and split the keys
 // and update S; warp 12 loads by TMA; warp 13 issues all products; warp 14 sums the decays, a chunk
-// ahead; warp 15 completes the warpgroup whose registers warps 4-11 take (at 128 a thread S would spill to
-// local memory).
+// ahead; warp 15 looks for values that are not finite.  Warps 4-11 take registers from the other groups (at
+// 128 a thread S would spill to local memory).
 #include <cuda.h>
 
 #include "linear.cuh"
@@ -45,7 +51,6 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kRegsA = 96, kRegsS = 168, kRegsIssue = 80;
 static_assert(kRegsA + 2 * kRegsS + kRegsIssue <= 4 * 128, "the split draws on the block's registers at launch");
 constexpr int kBoxBytes = kChunk * 128;
-constexpr int kMinShare = 4;    // chunks: below that the first pass costs more than another SM saves
 constexpr float kLog2e = 1.44269504088896340736f;
 // tensor memory columns
 constexpr uint32_t kColA = 0, kColO = 128, kColU = 256, kColK = 384;
@@ -66,6 +71,7 @@ struct Work {
   float* borders;  // [workers][Dk][Dv]: the state at border w
   float* starts;   // [workers][Dk][Dv]: the initial state of the (sequence, head) whose first cut is border w (its
                    // slot may be rewritten while the main pass still wants it)
+  uint32_t* bad;   // [workers][4][Dv]: the first row of chunk c % 4 whose value is not finite
 };
 
 struct Seq {
@@ -144,8 +150,8 @@ struct Cfg {
   static constexpr int kFull = 0, kEmpty = kSlots, kQk = 2 * kSlots, kQs = kQk + 1, kULo = kQk + 2, kU = kQk + 3,
                        kO = kQk + 4, kKeys = kQk + 5, kKeysHi = kQk + 6, kS = kQk + 7, kA = kQk + 8,
                        kOFree = kQk + 9, kDrain = kQk + 10, kW = kQk + 11, kWFree = kQk + 12, kDecay = kQk + 13,
-                       kDecayFree = kQk + 15, kBars = kQk + 17;
-  static constexpr int kMiscBytes = 2 * (kChunk + 96) * 4 + 4 * 4 * 4 + 3 * kChunk * 2 + 16 + kBars * 8 + 24 * 4;
+                       kDecayFree = kQk + 15, kChecked = kQk + 17, kBars = kQk + 19;
+  static constexpr int kMiscBytes = 2 * (kChunk + 96) * 4 + 4 * 4 * 4 + 3 * kChunk * 2 + 16 + kBars * 8 + 28 * 4;
   static_assert(kWarps <= 16, "scan_s");
   static constexpr int kTableBytes = kStateOnly ? (4 * kThreads + 2) * 4 : 0;  // FirstWalk's arrays
   static constexpr int kSmem = kSlots * kSlotBytes + 2 * kStateBytes + kMiscBytes + kTableBytes;
@@ -191,9 +197,23 @@ ASTERQ_DEVICE uint32_t split_part(float& x, float& y) {
   return p;
 }
 
+// per bf16: the larger magnitude (its sign means nothing), or NaN
+ASTERQ_DEVICE uint32_t max_abs_bf162(uint32_t x, uint32_t y) {
+  uint32_t r;
+  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+  return r;
+}
+
 ASTERQ_DEVICE void st_global_32(void* p, const uint32_t (&r)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
                "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+ASTERQ_DEVICE void ld_global_32(float* r, const float* p) {
+  asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7])
+               : "l"(p)
                : "memory");
 }
 
@@ -230,7 +250,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   int* abort_s = start_s + 2;
   int* never_s = abort_s + 1;  // stays 0: the flag of waits that an abort must not cut short
   uint32_t* tmem_s = reinterpret_cast<uint32_t*>(abort_s + 2);
-  [[maybe_unused]] int* table_s = abort_s + 6;
+  int* bad_s = abort_s + 3;  // [4]: whether chunk c % 4 has values that are not finite
+  [[maybe_unused]] int* table_s = abort_s + 10;
   const uint32_t bars = smem_u32(bars_s);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   auto bar = [&](int i) { return bars + 8 * i; };
@@ -244,7 +265,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar(C::kFull + i), 1);
       mbar_init(bar(C::kEmpty + i), 1);
     }
-    for (int i : {C::kQk, C::kQs, C::kULo, C::kU, C::kO, C::kDrain, C::kDecay, C::kDecay + 1, C::kW}) mbar_init(bar(i), 1);
+    for (int i : {C::kQk, C::kQs, C::kULo, C::kU, C::kO, C::kDrain, C::kDecay, C::kDecay + 1, C::kChecked, C::kChecked + 1, C::kW})
+      mbar_init(bar(i), 1);
     for (int i : {C::kKeys, C::kKeysHi, C::kS, C::kWFree}) mbar_init(bar(i), 8);
     for (int i : {C::kA, C::kOFree}) mbar_init(bar(i), 4);
     for (int i : {C::kDecayFree, C::kDecayFree + 1}) mbar_init(bar(i), 4);
@@ -273,7 +295,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     total += scan_s[w];
   }
   const int me = blockIdx.x;
-  const int W = max(1, min((int)gridDim.x, (total + kMinShare - 1) / kMinShare));
+  // As many shares as the longest needs: fewer cuts inside a (sequence, head).
+  const int longest = max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+  const int W = max(1, (total + longest - 1) / longest);
   auto border = [&](int w) { return (int)((long long)total * w / W); };
   typename WalkOf<kStateOnly>::type walk;
   if constexpr (!kStateOnly) {
@@ -381,7 +405,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 12) {
       // -------------------------------------------------------------- loads
       int c = 0;
-      while (ok && walk.next(a))
+      while (ok && walk.next(a)) {
+        // the state that the piece starts from, for the warps that will want it about a chunk later
+        if (!kStateOnly && walk.k0 == 0 && !walk.seq.fresh && lane == 0)
+          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(
+                           a.state + ((long long)walk.seq.slot * a.n_heads + walk.head) * kDk * kDv),
+                       "r"(kDk * kDv * 4)
+                       : "memory");
         for (int j = 0; j < walk.n && ok; ++j, ++c) {
           const int row = walk.seq.row0 + (walk.k0 + j) * kChunk;
 #pragma unroll 1
@@ -400,6 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
+      }
       // the last copies have landed before the exit, also when nobody waits for them any more (the slots'
       // last uses: of the chunk before this one, whichever was reached)
       if (!ok) {
@@ -443,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int rows = min(kChunk, walk.seq.rows - (walk.k0 + j) * kChunk), steps = (rows + 15) / 16;
           const Place kp = keys_of(c), vp = values_of(c);
           const uint32_t v_desc = tc::desc_mn_major(base + vp.slot * C::kSlotBytes, kBoxBytes);
-          ok = wait(C::kFull + vp.slot, vp.use) && wait(C::kKeys, c);
+          ok = wait(C::kFull + vp.slot, vp.use) && (kStateOnly || wait(C::kChecked + (c & 1), c / 2)) && wait(C::kKeys, c);
           if (!ok) break;
           tc::fence_after();
           if (tc::elect()) {
@@ -608,6 +639,51 @@ __global__ void __launch_bounds__(kThreads, 1)
           decay = 0.0;
         }
       }
+    } else if (!kStateOnly) {
+      // -------------------------------------------------------------- values that are not finite
+      // A's zeros above the diagonal do not cancel them, so rows before them would become NaN.  They are
+      // taken out here; the warps of the output and of the state write NaN in their column from their row on.
+      int c = 0;
+      while (ok && walk.next(a))
+        for (int j = 0; j < walk.n; ++j, ++c) {
+          const int rows = min(kChunk, walk.seq.rows - (walk.k0 + j) * kChunk);
+          const Place vp = values_of(c);
+          uint8_t* tile = smem + vp.slot * C::kSlotBytes;
+          ok = wait(C::kFull + vp.slot, vp.use);
+          if (!ok) break;
+          uint32_t most = 0;
+#pragma unroll 1
+          for (int at = lane * 16; at < kDv / 64 * kBoxBytes; at += 4 * 512) {
+            uint4 x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              x[u] = (at + u * 512) % kBoxBytes < rows * 128 ? *reinterpret_cast<const uint4*>(tile + at + u * 512)
+                                                             : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              most = max_abs_bf162(max_abs_bf162(max_abs_bf162(max_abs_bf162(most, x[u].x), x[u].y), x[u].z), x[u].w);
+          }
+          const bool any = __any_sync(0xffffffffu, (most & 0x7fffu) >= 0x7f80u || (most >> 16 & 0x7fffu) >= 0x7f80u);
+          if (any) {
+#pragma unroll 1
+            for (int d = lane; d < kDv; d += 32) {
+              uint32_t first = 0;  // or NaN with the column's first row in its last bits
+#pragma unroll 1
+              for (int row = rows - 1; row >= 0; --row) {
+                uint16_t* x = reinterpret_cast<uint16_t*>(tile + d / 64 * kBoxBytes + row * 128 +
+                                                          (((d % 64 / 8) ^ (row & 7)) << 4)) + d % 8;
+                if ((*x & 0x7f80) != 0x7f80) continue;
+                *x = 0;
+                first = 0x7fc00000u | row;
+              }
+              work.bad[(me * 4 + (c & 3)) * kDv + d] = first;
+            }
+            fence_async_shared();
+          }
+          if (lane == 0) bad_s[c & 3] = any;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(C::kChecked + (c & 1)));
+        }
     }
   } else if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsA));
@@ -685,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int step = 2 * warp + 2; step < steps; ++step) tc::st16(lanes + kColA + 16 * step, x);
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(C::kDecayFree + (c & 1)));
-          ok = wait(C::kQs, c);
+          ok = wait(C::kQs, c) && wait(C::kChecked + (c & 1), c / 2);
           if (!ok) break;
           tc::fence_after();
           if (carried) {
@@ -727,6 +803,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               st_global_32(dst + d + 16 * e, p);
             }
           }
+          if (bad_s[c & 3] && i < rows) {
+            const uint32_t* bad = work.bad + (me * 4 + (c & 3)) * kDv;
+#pragma unroll 1
+            for (int d = 0; d < kDv; ++d)
+              if (bad[d] && (int)(bad[d] & (kChunk - 1)) <= i) dst[d] = 0x7fff;
+          }
         }
     }
   } else {
@@ -754,13 +836,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         else if (q.fresh) from = nullptr;
         else from = ends ? a.state + slot_at : work.starts + (long long)(me + 1) * kDk * kDv + piece_at;
       }
+      if (from && has) {
 #pragma unroll
-      for (int e = 0; e < kCols; e += 4) {
-        const float4 x = from && has ? *reinterpret_cast<const float4*>(from + e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        s[e] = x.x;
-        s[e + 1] = x.y;
-        s[e + 2] = x.z;
-        s[e + 3] = x.w;
+        for (int e = 0; e < kCols; e += 8) ld_global_32(s + e, from + e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) s[e] = 0.0f;
       }
       for (int j = 0; j < walk.n; ++j, ++c) {
         const int rows = min(kChunk, q.rows - (walk.k0 + j) * kChunk), steps = (rows + 15) / 16;
@@ -827,7 +908,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(C::kKeys));
-        ok = wait(C::kULo, c);
+        ok = wait(C::kULo, c) && (kStateOnly || wait(C::kChecked + (c & 1), c / 2));
         if (!ok) break;
         tc::fence_after();
         // the larger parts in their place
@@ -899,6 +980,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 32; ++e) s[d + e] = fmaf(whole, s[d + e], __uint_as_float(r[e]));
           }
+          if (!kStateOnly && bad_s[c & 3]) {
+            const uint32_t* bad = work.bad + (me * 4 + (c & 3)) * kDv + part * kCols;
+#pragma unroll
+            for (int d = 0; d < kCols; d += 4) {
+              const uint4 x = *reinterpret_cast<const uint4*>(bad + d);
+              s[d] += __uint_as_float(x.x);
+              s[d + 1] += __uint_as_float(x.y);
+              s[d + 2] += __uint_as_float(x.z);
+              s[d + 3] += __uint_as_float(x.w);
+            }
+          }
         }
       }
       if (!ok) break;
@@ -907,8 +999,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       else if (ends) to = a.state + slot_at;
       if (to && has) {
 #pragma unroll
-        for (int e = 0; e < kCols; e += 4)
-          *reinterpret_cast<float4*>(to + e) = make_float4(s[e], s[e + 1], s[e + 2], s[e + 3]);
+        for (int e = 0; e < kCols; e += 8) {
+          uint32_t p[8];
+#pragma unroll
+          for (int h = 0; h < 8; ++h) p[h] = __float_as_uint(s[e + h]);
+          st_global_32(to + e, p);
+        }
       }
     }
   }
@@ -979,7 +1075,8 @@ EncodeTiledFn encode_fn() {
 // rows of bf16 heads [n_rows][n_heads][dim] with any strides, read in boxes of 128 rows x 64 dims
 bool make_map(CUtensorMap* map, const void* base, const Args& a, int dim, long long row_stride, long long head_stride) {
   EncodeTiledFn fn = encode_fn();
-  if (reinterpret_cast<uintptr_t>(a.out) & 31) return false;  // outputs are stored 32 bytes at a time
+  // outputs and states are read and written 32 bytes at a time
+  if ((reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.state)) & 31) return false;
   if ((a.n_rows / kChunk + a.n_seqs) * a.n_heads > 0x7fffffff) return false;  // Walk counts in 32 bits
   if (!fn || row_stride <= 0 || head_stride <= 0) return false;
   const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)a.n_heads, (cuuint64_t)a.n_rows};
@@ -1000,7 +1097,7 @@ int launch(const Args& a, int workers, int device, void* workspace, cudaStream_t
   using Main = Cfg<kDk, kDv, false>;
   CUtensorMap q_map, k_map, v_map;
   if (!make_map(&q_map, a.q, a, kDk, a.q_row, a.q_head) || !make_map(&k_map, a.k, a, kDk, a.k_row, a.k_head) ||
-      !make_map(&v_map, a.v, a, kDv, a.v_row, a.v_head))
+      !make_map(&v_map, a.v, a, kDv, a.v_row, a.v_head) || (reinterpret_cast<uintptr_t>(workspace) & 31))
     return ASTERQ_ERR_UNSUPPORTED;
   static unsigned long long configured = 0;  // one bit per device ordinal
   if (device >= 64 || !(configured & (1ull << device))) {
@@ -1019,6 +1116,7 @@ int launch(const Args& a, int workers, int device, void* workspace, cudaStream_t
   work.sums = reinterpret_cast<float*>(at + table_bytes(workers));
   work.borders = work.sums + 2ll * workers * kDk * kDv;
   work.starts = work.borders + (long long)workers * kDk * kDv;
+  work.bad = reinterpret_cast<uint32_t*>(work.starts + (long long)workers * kDk * kDv);
   chunk_kernel<kDk, kDv, true><<<workers, kThreads, First::kSmem, s>>>(q_map, k_map, v_map, a, work);
   chain_kernel<kDk, kDv><<<dim3(workers, kDk * kDv / 1024), 256, 0, s>>>(a, work);
   chunk_kernel<kDk, kDv, false><<<workers, kThreads, Main::kSmem, s>>>(q_map, k_map, v_map, a, work);
@@ -1028,7 +1126,7 @@ int launch(const Args& a, int workers, int device, void* workspace, cudaStream_t
 }  // namespace
 
 int64_t chunk_workspace_bytes(int dk, int dv, int workers) {
-  return table_bytes(min(workers, kThreads)) + 4ll * min(workers, kThreads) * dk * dv * 4;
+  return table_bytes(min(workers, kThreads)) + 4ll * min(workers, kThreads) * (dk * dv + dv) * 4;
 }
 
 int chunk_launch(const Args& a, int dk, int dv, int workers, int device, void* workspace, cudaStream_t s) {

@@ -442,7 +442,8 @@ int asterq_kv_append(const asterq_kv_append_params* p, void* stream);
  * token t is visible when t < min(sink, window) or t >= L - (window - min(sink, window)), otherwise
  * all are.  lse[b][h] = log(sum of exp(score)) in natural logarithms, optional.  A sequence without
  * tokens (lengths[b] < 0, or L = 0) gets zeros and -inf.  Pages with no visible token may have any id;
- * where a needed id is outside [0, n_pages) the row's output is not valid and *status becomes 1.
+ * where a needed id is outside [0, n_pages) the row's output is not valid and *status becomes 1.  A sequence
+ * longer than its row of the table (max_pages * page_tokens) ends there.
  * Products of the weights are taken in two 16-bit parts, softmax statistics and sums in fp32.
  * head_dim 64, 128 or 256; page_tokens a multiple of 16.
  *
@@ -492,10 +493,12 @@ int asterq_paged_attention(const asterq_paged_attention_params* p, void* stream)
  * lengths[s] <= 0 start from a state of zeros, whatever their slot holds.  A slot below 0 is an empty
  * one: its rows are written as zeros; one at or above n_slots is taken the same way and sets *status
  * to 1, and so do row offsets outside [0, n_rows], whose sequence is left out.  Sequences of a call
- * have slots of their own.
+ * have slots of their own.  A value of v that is not finite reaches its column of the state, and of the outputs
+ * from its row on (where an infinity may become NaN), and nothing else.
  * dk, dv: 64 or 128.  q, k, v, out of one type: bf16, f16 or f32.
  * workspace: asterq_linear_workspace_bytes bytes (0: none needed), not kept between calls; calls that
- * overlap on the GPU need one each.
+ * overlap on the GPU need one each.  bf16 prompts run in chunks where state, out and workspace are 32-byte aligned
+ * and strides are positive, and token by token otherwise.
  */
 typedef struct asterq_linear_params {
   int32_t dtype;
