@@ -18,6 +18,12 @@
 // cut unit leaves (o, m, l) records in the workspace, and the CTA that stores its last one joins them, in
 // the order of the shares, so results do not depend on which CTA came last; of many records groups are
 // joined first, each by the CTA that stores its last one.  No CTA waits for another.
+//
+// Measured (bf16, 128 dims, 8 kv heads, pages of 64): 64 sequences of 1k to 32k tokens 358 us, 6.7 TB/s of keys
+// and values.  One sequence of 8192 tokens of 4 kv heads takes 17 us, of which the bytes are 2.6: launch, table
+// lookups, the pipeline's filling and the join of 37 pieces a head are the rest.  256 sequences of at most 512
+// visible tokens, 16 kv heads of 64: 91 us against 25 of bytes, 4096 units of some 1.7 us of fixed cost each on
+// 296 teams.
 #include <cuda.h>
 
 #include "asterq_internal.h"
@@ -67,8 +73,13 @@ struct Cfg {
   static_assert(kMergeFloats >= 24 * NR, "weights of the records that are joined at once");
   // What a unit costs beside its tiles, in tiles: a unit by itself takes 1.5 us, two at a time, a tile's share of
   // the memory bandwidth 0.75 us.
+  // kUnitCost: what a unit costs by itself, in tiles.  Measured with 0, 1 and 2: 64 rows of 1 to 2048 tokens,
+  // 8 kv heads of 128, 40.5, 32.4 and 30.6 us; 256 rows of at most 512 visible tokens, 16 kv heads of 64, 99.9, 91.7
+  // and 101.5; 64 rows of 1k to 32k tokens 372, 367 and 365.
+  // kSoloTiles: units up to this long are taken by one team.  Measured with 0, 4 and 8: the same three 34.2, 32.4 and
+  // 33.5 us; 99.1, 91.7 and 91.4; 372, 367 and 367.  (64 rows of 1 to 512 tokens, 20.7, 22.3 and 24.1, would have all.)
   static constexpr int kUnitCost = 1;
-  static constexpr int kSoloTiles = 4;  // units up to this long are taken by one team
+  static constexpr int kSoloTiles = 4;
   static constexpr int kSmem =
       1024 + kStages * kStageBytes + kQSlots * kQBytes + (kMergeFloats + 2 * kWarps * NR) * 4 + (3 * kStages + 2 * kQSlots) * 8;
 };
@@ -174,7 +185,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(warp_l + C::kWarps * NR);
   __shared__ Start start_s;
   __shared__ long long scan_s[32];
-  __shared__ int abort_s, never_s, last_s, group_s;  // never_s stays 0: for waits that an abort must not cut short
+  __shared__ int abort_s, never_s, last_s;  // never_s stays 0: for waits that an abort must not cut short
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // a full barrier for each stage and the team that its tile is for: a barrier's waiters see each of its phases
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 16 * C::kStages, q_full0 = empty0 + 8 * C::kStages,
@@ -584,9 +595,16 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     }
 
     // ------------------------------------------------------------------ the warps join
+    // What the joins compute from these must not be kept in registers over the loop above, which has none to
+    // spare: the compiler is not told that they are still the same.
+    int tid_j = tid;
+    float *merge_j = merge, *records = a.records;
+    asm volatile("" : "+r"(tid_j), "+l"(merge_j), "+l"(records));
+    const int lane_j = tid_j & 31, warp_j = tid_j >> 5;
+    float *m_j = merge_j + C::kMergeFloats, *l_j = m_j + C::kWarps * NR;
     // the team's, or all; either way with barriers that only they use
     const int wa = solo ? team * C::kTeamWarps : 0, wn = solo ? C::kTeamWarps : C::kWarps;
-    const int me_in = tid - wa * 32, threads = wn * 32;
+    const int me_in = tid_j - wa * 32, threads = wn * 32;
     auto sync = [&]() { named_sync(solo ? 1 + team : 3, threads); };
     // slot of this piece: a share's first piece may be the tail or middle of a unit, its last the head
     const long long slot = 2ll * me + (walk.first_tile > my_start ? 1 : 0);
@@ -596,61 +614,70 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], d);
-        if (g == 0) {
-          warp_m[warp * NR + t * 8 + 2 * qd + e] = m[t][e];
-          warp_l[warp * NR + t * 8 + 2 * qd + e] = l[t][e];
+        if ((lane_j >> 2) == 0) {
+          m_j[warp_j * NR + t * 8 + 2 * (lane_j & 3) + e] = m[t][e];
+          l_j[warp_j * NR + t * 8 + 2 * (lane_j & 3) + e] = l[t][e];
         }
       }
     // Each thread sums the same rows of every slice, so the warps' factors are looked up once, behind the
-    // first barrier; with the second slice's barrier passed nobody reads warp_m and warp_l any more.
+    // first barrier; with the second slice's barrier passed nobody reads m_j and l_j any more.
     constexpr int kOwn = NR * C::kSlice / (C::kTeamWarps * 32);  // of a team; half as many with all warps
-    float factor[kOwn][C::kWarps], weight_sum[kOwn];
+    float factor[kOwn][C::kWarps], inverse[kOwn];
 #pragma unroll
     for (int part = 0; part < D / C::kSlice; ++part) {
-      float* buf = merge + (part & 1) * C::kBufFloats;
+      float* buf = merge_j + (part & 1) * C::kBufFloats;
 #pragma unroll
       for (int i = 0; i < C::kSlice / 16; ++i)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            buf[(warp * NR + t * 8 + 2 * qd + (e & 1)) * C::kPad + i * 16 + g + (e >> 1) * 8] =
+            buf[(warp_j * NR + t * 8 + 2 * (lane_j & 3) + (e & 1)) * C::kPad + i * 16 + (lane_j >> 2) + (e >> 1) * 8] =
                 acc[part * (C::kSlice / 16) + i][t][e];
       sync();
 #pragma unroll
       for (int k = 0; k < kOwn; ++k) {
+        if (!solo && k >= kOwn / 2) continue;
         const int i = me_in + k * threads, r = i / C::kSlice, d = i % C::kSlice, dim = part * C::kSlice + d;
-        if (r >= (cut ? NR : rows)) continue;
         if (part == 0) {
-          float top = -INFINITY, total_l = 0.0f;
+          // A row's weights, a warp_j's by each of kWarps lanes: every thread for itself took 850 cycles of a
+          // unit's 3,000.
+          const int w = lane_j % C::kWarps;
+          const float mw = w < wn ? m_j[(wa + w) * NR + r] : -INFINITY;
+          const float lw = w < wn ? l_j[(wa + w) * NR + r] : 0.0f;  // not 0 although mw is -inf: NaN scores
+          float top = mw;
 #pragma unroll
-          for (int w = 0; w < C::kWarps; ++w)
-            if (w < wn) top = fmaxf(top, factor[k][w] = warp_m[(wa + w) * NR + r]);
+          for (int e = 1; e < C::kWarps; e *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, e));
+          const float f = mw == -INFINITY ? 0.0f : ex2_ftz(mw - top);
+          float total_l = mw == -INFINITY ? lw : lw * f;
 #pragma unroll
-          for (int w = 0; w < C::kWarps; ++w)
-            if (w < wn) {
-              const float lw = warp_l[(wa + w) * NR + r];  // not 0 although the maximum is -inf: NaN scores
-              const bool none = factor[k][w] == -INFINITY;
-              factor[k][w] = none ? 0.0f : ex2_ftz(factor[k][w] - top);
-              total_l += none ? lw : lw * factor[k][w];
+          for (int e = 1; e < C::kWarps; e *= 2) total_l += __shfl_xor_sync(0xffffffffu, total_l, e);
+#pragma unroll
+          for (int e = 0; e < C::kWarps; ++e) factor[k][e] = __shfl_sync(0xffffffffu, f, (lane_j & ~(C::kWarps - 1)) + e);
+          if (d == 0 && r < rows) {
+            if (cut) {
+              records[n_slots * NR * D + slot * NR + r] = top;
+              records[n_slots * NR * (D + 1) + slot * NR + r] = total_l;
+            } else if (a.lse) {
+              a.lse[(long long)walk.row * a.n_heads + h0 + r] = (top + log2f(total_l)) * kLn2;
             }
-          weight_sum[k] = total_l;
-          if (d == 0 && cut) {
-            a.records[n_slots * NR * D + slot * NR + r] = top;
-            a.records[n_slots * NR * (D + 1) + slot * NR + r] = total_l;
-          } else if (d == 0 && a.lse) {
-            a.lse[(long long)walk.row * a.n_heads + h0 + r] = (top + log2f(total_l)) * kLn2;
           }
+          inverse[k] = 1.0f / total_l;
         }
+        if (r >= rows) continue;
         float sum = 0.0f;
+        const float* from = buf + (wa * NR + r) * C::kPad + d;
 #pragma unroll
-        for (int w = 0; w < C::kWarps; ++w)
-          if (w < wn) sum = fmaf(factor[k][w], buf[((wa + w) * NR + r) * C::kPad + d], sum);
+        for (int w = 0; w < C::kTeamWarps; ++w) sum = fmaf(factor[k][w], from[w * NR * C::kPad], sum);
+        if (!solo) {
+#pragma unroll
+          for (int w = C::kTeamWarps; w < C::kWarps; ++w) sum = fmaf(factor[k][w], from[w * NR * C::kPad], sum);
+        }
         if (cut) {
-          a.records[(slot * NR + r) * D + dim] = sum;
+          records[(slot * NR + r) * D + dim] = sum;
         } else {
           const long long at = ((long long)walk.row * a.n_heads + h0 + r) * D + dim;
-          const float o = sum / weight_sum[k];
+          const float o = sum * inverse[k];
           if (a.out_f32) static_cast<float*>(a.out)[at] = o;
           else if constexpr (C::kF16) static_cast<__half*>(a.out)[at] = __float2half_rn(o);
           else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(o);
@@ -668,89 +695,115 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     // beyond 24 records, groups of about their square root are joined first
     const int size = pieces <= 24 ? pieces : pieces <= 64 ? 8 : pieces <= 160 ? 12 : 16;
     const int groups = (pieces + size - 1) / size, group = (me - w0) / size;
-    __threadfence();
-    sync();
-    if (tid == 0) last_s = atomicAdd(a.counters + slot_of(group * size), 1) == min(size, pieces - group * size) - 1;
-    sync();
-    if (!last_s) continue;
-    __threadfence();
-    if (tid == 0) a.counters[slot_of(group * size)] = 0;
-    float* rec_m = a.records + n_slots * NR * D;
+    float* rec_m = records + n_slots * NR * D;
     float* rec_l = rec_m + n_slots * NR;
-    // records first, first + step, .. (n of them): to the output, or into the first one's place
-    auto join = [&](int first, int n, int step, bool whole) {
-      for (int r = warp; r < NR; r += C::kWarps) {
-        float top = -INFINITY, sum = 0.0f;
-        for (int i = lane; i < n; i += 32) top = fmaxf(top, __ldcg(rec_m + slot_of(first + i * step) * NR + r));
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        for (int i = lane; i < n; i += 32) {
-          const int at = slot_of(first + i * step) * NR + r;
-          const float mw = __ldcg(rec_m + at), f = mw == -INFINITY ? 1.0f : ex2_ftz(mw - top);
-          merge[i * NR + r] = f;
-          sum += f * __ldcg(rec_l + at);
-        }
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        if (lane == 0) {
-          warp_m[r] = top;
-          warp_l[r] = sum;
-        }
+    // Records first, first + step, .. (n of them) become the output, or take the first one's place.  This runs once or
+    // twice a launch, so what it takes is the latency of its loads (all that fit are on their way before the
+    // first is needed) and of fetching its instructions: one copy of them for both levels.
+    int first = group * size, n = min(size, pieces - first), step = 1;
+    int* counter = a.counters + slot_of(first);
+    bool whole = groups == 1;
+#pragma unroll 1
+    while (true) {
+      sync();
+      if (tid_j == 0) {
+        __threadfence();
+        last_s = atomicAdd(counter, 1) == n - 1;
+        if (last_s) *counter = 0;
+        __threadfence();
       }
       sync();
-      for (int i = tid; i < NR * D / 4; i += C::kWarps * 32) {
-        const int r = i / (D / 4), d = (i % (D / 4)) * 4;
-        if (r >= rows) continue;
+      if (!last_s) break;
+      constexpr int kAhead = 8;
+      auto record = [&](int k) { return slot_of(first + k * step) * NR; };
+      bool weighed = false;
+#pragma unroll 1
+      for (int i0 = 0; i0 < rows * (D / 4); i0 += C::kWarps * 32) {
+        const int i = i0 + tid_j, r = i / (D / 4), d = (i % (D / 4)) * 4;
+        const bool mine = r < rows;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-        for (int k = 0; k < n; ++k) {
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(
-              a.records + ((long long)slot_of(first + k * step) * NR + r) * D + d));
-          const float f = merge[k * NR + r];
-          o.x += f * v.x;
-          o.y += f * v.y;
-          o.z += f * v.z;
-          o.w += f * v.w;
+#pragma unroll 1
+        for (int k0 = 0; k0 < n; k0 += kAhead) {
+          float4 v[kAhead];
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k)
+            v[k] = mine && k0 + k < n
+                       ? __ldcg(reinterpret_cast<const float4*>(records + (long long)(record(k0 + k) + r) * D + d))
+                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (!weighed) {
+            weighed = true;
+#pragma unroll 1
+            for (int q = warp_j; q < rows; q += C::kWarps) {
+              float top = -INFINITY, sum = 0.0f, m2[2], l2[2];  // n is at most 48
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int k = lane_j + 32 * h;
+                m2[h] = k < n ? __ldcg(rec_m + record(k) + q) : -INFINITY;
+                l2[h] = k < n ? __ldcg(rec_l + record(k) + q) : 0.0f;
+                top = fmaxf(top, m2[h]);
+              }
+#pragma unroll
+              for (int e = 1; e < 32; e *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, e));
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float f = m2[h] == -INFINITY ? 1.0f : ex2_ftz(m2[h] - top);
+                if (lane_j + 32 * h < n) merge_j[(lane_j + 32 * h) * NR + q] = f;
+                sum += f * l2[h];
+              }
+#pragma unroll
+              for (int e = 1; e < 32; e *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, e);
+              if (lane_j == 0) {
+                l_j[q] = sum;
+                if (!whole) {
+                  m_j[q] = top;
+                } else if (a.lse) {
+                  a.lse[(long long)walk.row * a.n_heads + h0 + q] = (top + log2f(sum)) * kLn2;
+                }
+              }
+            }
+            sync();
+          }
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k)
+          {
+            const float f = mine && k0 + k < n ? merge_j[(k0 + k) * NR + r] : 0.0f;
+            o.x += f * v[k].x;
+            o.y += f * v[k].y;
+            o.z += f * v[k].z;
+            o.w += f * v[k].w;
+          }
         }
+        if (!mine) continue;
         if (!whole) {
-          *reinterpret_cast<float4*>(a.records + ((long long)slot_of(first) * NR + r) * D + d) = o;
+          *reinterpret_cast<float4*>(records + (long long)(record(0) + r) * D + d) = o;
           continue;
         }
-        const float sum = warp_l[r];
-        o.x /= sum;
-        o.y /= sum;
-        o.z /= sum;
-        o.w /= sum;
+        const float inv = 1.0f / l_j[r];
         const long long at = ((long long)walk.row * a.n_heads + h0 + r) * D + d;
         if (a.out_f32) {
-          *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = o;
+          *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) =
+              make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
         } else {
           uint2 w;
-          if constexpr (C::kF16) w = make_uint2(pack_half2(o.x, o.y), pack_half2(o.z, o.w));
-          else w = make_uint2(pack_bf162(o.x, o.y), pack_bf162(o.z, o.w));
+          if constexpr (C::kF16) w = make_uint2(pack_half2(o.x * inv, o.y * inv), pack_half2(o.z * inv, o.w * inv));
+          else w = make_uint2(pack_bf162(o.x * inv, o.y * inv), pack_bf162(o.z * inv, o.w * inv));
           *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = w;
         }
       }
-      if (tid < NR) {
-        if (!whole) {
-          rec_m[slot_of(first) * NR + tid] = warp_m[tid];
-          rec_l[slot_of(first) * NR + tid] = warp_l[tid];
-        } else if (a.lse && tid < rows) {
-          a.lse[(long long)walk.row * a.n_heads + h0 + tid] = (warp_m[tid] + log2f(warp_l[tid])) * kLn2;
-        }
+      if (whole) {
+        sync();  // the buffers are the next unit's
+        break;
       }
-      sync();
-    };
-    join(group * size, min(size, pieces - group * size), 1, groups == 1);
-    if (groups == 1) continue;
-    __threadfence();
-    sync();
-    if (tid == 0) group_s = atomicAdd(a.counters + n_slots + slot0, 1) == groups - 1;
-    sync();
-    if (!group_s) continue;
-    __threadfence();
-    if (tid == 0) a.counters[n_slots + slot0] = 0;
-    join(0, groups, size, true);
+      if (tid_j < rows) {
+        rec_m[record(0) + tid_j] = m_j[tid_j];
+        rec_l[record(0) + tid_j] = l_j[tid_j];
+      }
+      first = 0;
+      n = groups;
+      step = size;
+      whole = true;
+      counter = a.counters + n_slots + slot0;
+    }
   }
   // a wait that ran into its limit (about two seconds): the outputs are not valid
   if (tid == 0 && ld_shared_volatile(&abort_s) && a.status) atomicMax(a.status, 2);
