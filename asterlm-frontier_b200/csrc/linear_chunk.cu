@@ -52,8 +52,6 @@ constexpr int kRegsA = 96, kRegsS = 168, kRegsIssue = 80;
 static_assert(kRegsA + 2 * kRegsS + kRegsIssue <= 4 * 128, "the split draws on the block's registers at launch");
 constexpr int kBoxBytes = kChunk * 128;
 constexpr float kLog2e = 1.44269504088896340736f;
-// tensor memory columns
-constexpr uint32_t kColA = 0, kColO = 128, kColU = 256, kColK = 384;
 
 // A part of the first pass: some chunks of one (sequence, head), from a state of zeros.
 struct Part {
@@ -145,6 +143,13 @@ template <int kDk, int kDv, bool kStateOnly>
 struct Cfg {
   static constexpr int kMaxD = kDk > kDv ? kDk : kDv;
   static constexpr int kSlotBytes = kMaxD / 64 * kBoxBytes;
+  // Tensor memory columns: A, the output, U (what a chunk adds to the state), and the keys' smaller and larger
+  // parts.  Where there is room (the first pass has no outputs, and 64 value dims take half) the larger parts
+  // have a place of their own and need not wait for the smaller parts' products, and the first pass adds a
+  // chunk's U to the state while the next chunk's products run.
+  static constexpr bool kTwoKeys = kStateOnly || kDv == 64;
+  static constexpr uint32_t kColA = 0, kColO = 128, kColU = kStateOnly ? 0 : 128 + kDv, kColU1 = kStateOnly ? 128 : kColU,
+                            kColK = kTwoKeys ? 256 : 384, kColL = 384;
   static constexpr int kStateBytes = kStateOnly ? 0 : kDk * kDv * 2;  // one bf16 part
   // barriers
   static constexpr int kFull = 0, kEmpty = kSlots, kQk = 2 * kSlots, kQs = kQk + 1, kULo = kQk + 2, kU = kQk + 3,
@@ -460,9 +465,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (tc::elect()) {
           const uint32_t v_desc = tc::desc_mn_major(base + values_of(c).slot * C::kSlotBytes, kBoxBytes);
           over_tokens(last_steps, [&](int s) {
-            const uint32_t at = tmem + kColA + 16 * s;
-            tc::mma_ts(tmem + kColO, at, v_desc + s * 128, kVDesc, last_carried || s > 0);
-            tc::mma_ts(tmem + kColO, at + 8, v_desc + s * 128, kVDesc, true);
+            const uint32_t at = tmem + C::kColA + 16 * s;
+            tc::mma_ts(tmem + C::kColO, at, v_desc + s * 128, kVDesc, last_carried || s > 0);
+            tc::mma_ts(tmem + C::kColO, at + 8, v_desc + s * 128, kVDesc, true);
           });
           tc::commit(bar(C::kO));
           tc::commit(bar(C::kEmpty + values_of(c).slot));
@@ -474,12 +479,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int rows = min(kChunk, walk.seq.rows - (walk.k0 + j) * kChunk), steps = (rows + 15) / 16;
           const Place kp = keys_of(c), vp = values_of(c);
           const uint32_t v_desc = tc::desc_mn_major(base + vp.slot * C::kSlotBytes, kBoxBytes);
+          const uint32_t u = tmem + (c & 1 ? C::kColU1 : C::kColU);
           ok = wait(C::kFull + vp.slot, vp.use) && (kStateOnly || wait(C::kChecked + (c & 1), c / 2)) && wait(C::kKeys, c);
           if (!ok) break;
           tc::fence_after();
           if (tc::elect()) {
-            over_tokens(steps, [&](int s) { tc::mma_ts(tmem + kColU, tmem + kColK + 8 * s, v_desc + s * 128, kVDesc, s > 0); });
-            over_tokens(steps, [&](int s) { tc::mma_ts(tmem + kColU, tmem + kColK + 64 + 8 * s, v_desc + s * 128, kVDesc, true); });
+            over_tokens(steps, [&](int s) { tc::mma_ts(u, tmem + C::kColK + 8 * s, v_desc + s * 128, kVDesc, s > 0); });
+            over_tokens(steps, [&](int s) { tc::mma_ts(u, tmem + C::kColK + 64 + 8 * s, v_desc + s * 128, kVDesc, true); });
             tc::commit(bar(C::kULo));
           }
           if (!kStateOnly && c > 0) a_times_v(c - 1);
@@ -487,8 +493,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           tc::fence_after();
           if (tc::elect()) {
-            over_tokens(steps, [&](int s) { tc::mma_ts(tmem + kColU, tmem + kColK + 8 * s, v_desc + s * 128, kVDesc, true); });
-            over_tokens(steps, [&](int s) { tc::mma_ts(tmem + kColU, tmem + kColK + 64 + 8 * s, v_desc + s * 128, kVDesc, true); });
+            over_tokens(steps, [&](int s) { tc::mma_ts(u, tmem + C::kColL + 8 * s, v_desc + s * 128, kVDesc, true); });
+            over_tokens(steps, [&](int s) { tc::mma_ts(u, tmem + C::kColL + 64 + 8 * s, v_desc + s * 128, kVDesc, true); });
             tc::commit(bar(C::kU));
             if (kStateOnly) {
               tc::commit(bar(C::kEmpty + kp.slot));
@@ -505,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
               for (int s = 0; s < kDk / 16; ++s) {
                 const uint32_t at = ((s / 4) * kBoxBytes + (s % 4) * 32) >> 4;
-                tc::mma_ss(tmem + kColA, q_desc + at, k_desc + at, kQkDesc, s > 0);
+                tc::mma_ss(tmem + C::kColA, q_desc + at, k_desc + at, kQkDesc, s > 0);
               }
               tc::commit(bar(C::kQk));
               tc::commit(bar(C::kEmpty + kp.slot));
@@ -522,8 +528,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
                 for (int s = 0; s < kDk / 16; ++s) {
                   const uint32_t at = ((s / 4) * kBoxBytes + (s % 4) * 32) >> 4;
-                  tc::mma_ss(tmem + kColO, q_desc + at, hi_desc + s * 128, kVDesc, s > 0);
-                  tc::mma_ss(tmem + kColO, q_desc + at, lo_desc + s * 128, kVDesc, true);
+                  tc::mma_ss(tmem + C::kColO, q_desc + at, hi_desc + s * 128, kVDesc, s > 0);
+                  tc::mma_ss(tmem + C::kColO, q_desc + at, lo_desc + s * 128, kVDesc, true);
                 }
               }
               tc::commit(bar(C::kQs));
@@ -709,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           float sum = 0.0f;
 #pragma unroll 1
           for (int half = 1; half >= 0; --half) {
-            const uint32_t at = lanes + kColA + 32 * warp + 16 * half;
+            const uint32_t at = lanes + C::kColA + 32 * warp + 16 * half;
             const float4* next = reinterpret_cast<const float4*>(g + 32 * warp + 16 * half);
             const int left = lane - 16 * half;  // columns of this step before the row's own
             tc::ld16(x, at);
@@ -738,7 +744,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           float far = ex2_ftz(sum + first_s[(c & 1) * 4 + warp]) * a.scale;
 #pragma unroll 1
           for (int step = 2 * warp - 1; step >= 0; --step) {
-            tc::ld16(x, lanes + kColA + 16 * step);
+            tc::ld16(x, lanes + C::kColA + 16 * step);
             const float4* fg = reinterpret_cast<const float4*>(f + 16 * step);
             tc::wait_ld();
             uint32_t out[16];
@@ -752,13 +758,13 @@ __global__ void __launch_bounds__(kThreads, 1)
               out[2 * e + 1] = split_part(x2, x3);
               out[8 + 2 * e + 1] = last_part(x2, x3);
             }
-            tc::st16(lanes + kColA + 16 * step, out);
+            tc::st16(lanes + C::kColA + 16 * step, out);
             if (step % 2 == 0) far *= p32[step / 2];
           }
 #pragma unroll
           for (int e = 0; e < 16; ++e) x[e] = 0;
 #pragma unroll 1
-          for (int step = 2 * warp + 2; step < steps; ++step) tc::st16(lanes + kColA + 16 * step, x);
+          for (int step = 2 * warp + 2; step < steps; ++step) tc::st16(lanes + C::kColA + 16 * step, x);
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(C::kDecayFree + (c & 1)));
           ok = wait(C::kQs, c) && wait(C::kChecked + (c & 1), c / 2);
@@ -767,11 +773,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (carried) {
 #pragma unroll 1
             for (int d = 0; d < kDv; d += 32) {
-              tc::ld32(r, lanes + kColO + d);
+              tc::ld32(r, lanes + C::kColO + d);
               tc::wait_ld();
 #pragma unroll
               for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * far);
-              tc::st32(lanes + kColO + d, r);
+              tc::st32(lanes + C::kColO + d, r);
             }
           }
           tc::wait_st();
@@ -785,7 +791,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint16_t* dst = static_cast<uint16_t*>(a.out) + (row * a.n_heads + walk.head) * kDv;
 #pragma unroll 1
           for (int d = 0; d < kDv; d += 32) {
-            tc::ld32(r, lanes + kColO + d);
+            tc::ld32(r, lanes + C::kColO + d);
             tc::wait_ld();
             if (d + 32 == kDv) {
               tc::fence_before();
@@ -823,6 +829,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t k_row = ((warp & 3) / 2) * kBoxBytes + (part * 64 + (lane & 7)) * 128 +
                            (((((warp & 3) % 2) * 4 + (lane >> 3)) ^ (lane & 7)) << 4);
     float s[kCols];
+    // s <- f s + what chunk c has added
+    auto add = [&](int c, float f) {
+      tc::fence_after();
+      if (has) {
+#pragma unroll
+        for (int d = 0; d < kCols; d += 32) {
+          uint32_t r[32];
+          tc::ld32(r, lanes + (c & 1 ? C::kColU1 : C::kColU) + part * kCols + d);
+          tc::wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) s[d + e] = fmaf(f, s[d + e], __uint_as_float(r[e]));
+        }
+      }
+    };
+    float last_whole = 0.0f;
     int c = 0;
     while (ok && walk.next(a)) {
       const Seq q = walk.seq;
@@ -849,8 +870,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const Place kp = keys_of(c), vp = values_of(c);
         const uint32_t k_at = base + kp.slot * C::kSlotBytes + k_row;
         const uint32_t* weight = reinterpret_cast<const uint32_t*>(w_s) + part * 32 + (lane & 3);
-        ok = wait(C::kW, c) && wait(C::kFull + kp.slot, kp.use);
+        ok = wait(C::kW, c) && wait(C::kFull + kp.slot, kp.use) && (!C::kTwoKeys || c == 0 || wait(C::kULo, c - 1));
         if (!ok) break;
+        tc::fence_after();
         const float whole = *whole_s;
         // 32 tokens of the warp's 32 key dims: values 4 h + m are key dims 8 m .. of tokens 8 h ..
         auto put = [&](uint32_t to, const uint32_t (&p)[16]) {
@@ -886,8 +908,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 l[h * 4 + e] = tc::fma_bf162(k[e], w3, tc::fma_bf162(k[e], w2, tc::neg_bf162(m[h * 4 + e])));
               }
             }
-            put(lanes + kColK + part * 32 + u * 16, l);
-            put(lanes + kColK + 64 + part * 32 + u * 16, m);
+            put(lanes + C::kColK + part * 32 + u * 16, l);
+            put(lanes + C::kColK + 64 + part * 32 + u * 16, m);
           }
         }
         ok = wait(C::kFull + vp.slot, vp.use);
@@ -908,7 +930,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(C::kKeys));
-        ok = wait(C::kULo, c) && (kStateOnly || wait(C::kChecked + (c & 1), c / 2));
+        if (C::kTwoKeys) ok = !kStateOnly || c == 0 || wait(C::kU, c - 1);
+        else ok = wait(C::kULo, c);
+        ok = ok && (kStateOnly || wait(C::kChecked + (c & 1), c / 2));
         if (!ok) break;
         tc::fence_after();
         // the larger parts in their place
@@ -926,8 +950,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               p2[h * 4 + e] = tc::fma_bf162(k[e], w1, tc::neg_bf162(p1[h * 4 + e]));
             }
           }
-          put(lanes + kColK + part * 32 + u * 16, p2);
-          put(lanes + kColK + 64 + part * 32 + u * 16, p1);
+          put(lanes + C::kColL + part * 32 + u * 16, p2);
+          put(lanes + C::kColL + 64 + part * 32 + u * 16, p1);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(C::kWFree));
@@ -968,18 +992,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) mbar_arrive(bar(C::kS));
         }
 
+        if (kStateOnly) {
+          if (j > 0) add(c - 1, last_whole);
+          last_whole = whole;
+          if (j + 1 < walk.n) continue;
+        }
         ok = wait(C::kU, c);
         if (!ok) break;
-        tc::fence_after();
+        add(c, whole);
         if (has) {
-#pragma unroll
-          for (int d = 0; d < kCols; d += 32) {
-            uint32_t r[32];
-            tc::ld32(r, lanes + kColU + part * kCols + d);
-            tc::wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) s[d + e] = fmaf(whole, s[d + e], __uint_as_float(r[e]));
-          }
           if (!kStateOnly && bad_s[c & 3]) {
             const uint32_t* bad = work.bad + (me * 4 + (c & 3)) * kDv + part * kCols;
 #pragma unroll

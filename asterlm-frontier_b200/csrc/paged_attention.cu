@@ -19,11 +19,11 @@
 // the order of the shares, so results do not depend on which CTA came last; of many records groups are
 // joined first, each by the CTA that stores its last one.  No CTA waits for another.
 //
-// Measured (bf16, 128 dims, 8 kv heads, pages of 64): 64 sequences of 1k to 32k tokens 358 us, 6.7 TB/s of keys
-// and values.  One sequence of 8192 tokens of 4 kv heads takes 17 us, of which the bytes are 2.6: launch, table
-// lookups, the pipeline's filling and the join of 37 pieces a head are the rest.  256 sequences of at most 512
-// visible tokens, 16 kv heads of 64: 91 us against 25 of bytes, 4096 units of some 1.7 us of fixed cost each on
-// 296 teams.
+// Measured (bf16, 128 dims, 8 kv heads, pages of 64): 64 sequences of 1k to 32k tokens 360 us, 6.7 TB/s of keys
+// and values.  One sequence of 8192 tokens of 4 kv heads takes 12.8 us, of which the bytes are 2.6: launch, lengths,
+// table, first tiles (5 us), the warps' join (1.2), records and their count (1.5) and the join of 37 pieces a head
+// (3) are chains of latencies.  256 sequences of at most 512 visible tokens, 16 kv heads of 64: 89 us against
+// 25 of bytes, since a unit of six tiles keeps a team's warps busy for 1,400 cycles a tile and 1,700 more.
 #include <cuda.h>
 
 #include "asterq_internal.h"
@@ -70,7 +70,7 @@ struct Cfg {
   static constexpr int kSlice = NR == 16 ? 16 : 32, kPad = kSlice + 4;
   static constexpr int kBufFloats = kWarps * NR * kPad, kMergeFloats = 2 * kBufFloats;
   static_assert(D / kSlice % 2 == 0, "the two buffers alternate across units");
-  static_assert(kMergeFloats >= 24 * NR, "weights of the records that are joined at once");
+  static_assert(kMergeFloats >= 48 * NR, "weights of the records that are joined at once");
   // What a unit costs beside its tiles, in tiles: a unit by itself takes 1.5 us, two at a time, a tile's share of
   // the memory bandwidth 0.75 us.
   // kUnitCost: what a unit costs by itself, in tiles.  Measured with 0, 1 and 2: 64 rows of 1 to 2048 tokens,
@@ -640,7 +640,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
         if (!solo && k >= kOwn / 2) continue;
         const int i = me_in + k * threads, r = i / C::kSlice, d = i % C::kSlice, dim = part * C::kSlice + d;
         if (part == 0) {
-          // A row's weights, a warp_j's by each of kWarps lanes: every thread for itself took 850 cycles of a
+          // A row's weights, by kWarps lanes of its warp: every thread for itself took 850 cycles of a
           // unit's 3,000.
           const int w = lane_j % C::kWarps;
           const float mw = w < wn ? m_j[(wa + w) * NR + r] : -INFINITY;
@@ -692,8 +692,9 @@ __global__ void __launch_bounds__(C::kThreads, 1)
     const int pieces = w1 - w0 + 1;
     const int slot0 = 2 * w0 + (u0 > total * w0 / W ? 1 : 0);  // pieces after the first are at 2 w
     auto slot_of = [&](int i) { return i == 0 ? slot0 : 2 * (w0 + i); };
-    // beyond 24 records, groups of about their square root are joined first
-    const int size = pieces <= 24 ? pieces : pieces <= 64 ? 8 : pieces <= 160 ? 12 : 16;
+    // Beyond 24 records (48 of 8 rows), groups of about their square root are joined first.  37 records of 4 rows
+    // at once 12.8 us, in groups 13.8; of 8 rows 13.6 and 14.2 (one sequence of 8192 tokens, 4 kv heads of 128).
+    const int size = pieces <= 24 || (pieces <= 48 && NR == 8) ? pieces : pieces <= 64 ? 8 : pieces <= 160 ? 12 : 16;
     const int groups = (pieces + size - 1) / size, group = (me - w0) / size;
     float* rec_m = records + n_slots * NR * D;
     float* rec_l = rec_m + n_slots * NR;
@@ -714,7 +715,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
       }
       sync();
       if (!last_s) break;
-      constexpr int kAhead = 8;
+      constexpr int kAhead = 16;
       auto record = [&](int k) { return slot_of(first + k * step) * NR; };
       bool weighed = false;
 #pragma unroll 1
