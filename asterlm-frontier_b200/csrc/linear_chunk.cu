@@ -44,8 +44,6 @@ namespace lin {
 namespace {
 
 constexpr int kChunk = 128;
-constexpr int kSlots = 5;       // tiles of 128 tokens in shared memory: two of keys, two of values, one of queries
-constexpr int kQSlot = 4;
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kRegsA = 96, kRegsS = 168, kRegsIssue = 80;
@@ -141,6 +139,27 @@ struct WalkOf<true> {
 
 template <int kDk, int kDv, bool kStateOnly>
 struct Cfg {
+  // Tiles of 128 tokens in shared memory.  Main pass: keys, values and queries of all chunks, in this order, take
+  // five slots in turn.  Values, which are held longest (until A V of their chunk, during the next one) and have to
+  // be checked, then follow queries into a slot and are asked for a whole chunk ahead; with two slots of
+  // their own the products waited 2,000 of a chunk's 10,400 cycles for them.  First pass: three chunks' keys and values.
+  static constexpr int kSlots = kStateOnly ? 6 : 5;
+  // A chunk's tile: its slot, how many tiles that held before, and the barrier and phase of its arrival.  In the main
+  // pass barriers belong to a kind of tile and not to a slot: whoever waits for a tile has seen the one before it on
+  // the same barrier, and none has its barrier used again before all have seen it.
+  struct Place {
+    int slot, use, full, phase;
+  };
+  ASTERQ_DEVICE static Place keys_of(int c) {
+    if (kStateOnly) return {2 * (c % 3), c / 3, kFull + 2 * (c % 3), c / 3};
+    return {3 * c % 5, 3 * c / 5, kFull + (c & 1), c / 2};
+  }
+  ASTERQ_DEVICE static Place values_of(int c) {
+    if (kStateOnly) return {2 * (c % 3) + 1, c / 3, kFull + 2 * (c % 3) + 1, c / 3};
+    return {(3 * c + 1) % 5, (3 * c + 1) / 5, kFull + 2 + (c & 1), c / 2};
+  }
+  ASTERQ_DEVICE static Place queries_of(int c) { return {(3 * c + 2) % 5, (3 * c + 2) / 5, kFull + 4, c}; }
+  static constexpr int kWBufs = kStateOnly ? 2 : 1;  // chunks' weights held (the main pass has no room for two)
   static constexpr int kMaxD = kDk > kDv ? kDk : kDv;
   static constexpr int kSlotBytes = kMaxD / 64 * kBoxBytes;
   // Tensor memory columns: A, the output, U (what a chunk adds to the state), and the keys' smaller and larger
@@ -154,20 +173,13 @@ struct Cfg {
   // barriers
   static constexpr int kFull = 0, kEmpty = kSlots, kQk = 2 * kSlots, kQs = kQk + 1, kULo = kQk + 2, kU = kQk + 3,
                        kO = kQk + 4, kKeys = kQk + 5, kKeysHi = kQk + 6, kS = kQk + 7, kA = kQk + 8,
-                       kOFree = kQk + 9, kDrain = kQk + 10, kW = kQk + 11, kWFree = kQk + 12, kDecay = kQk + 13,
-                       kDecayFree = kQk + 15, kChecked = kQk + 17, kBars = kQk + 19;
-  static constexpr int kMiscBytes = 2 * (kChunk + 96) * 4 + 4 * 4 * 4 + 3 * kChunk * 2 + 16 + kBars * 8 + 28 * 4;
+                       kOFree = kQk + 9, kDrain = kQk + 10, kW = kQk + 11, kWFree = kQk + 13, kDecay = kQk + 15,
+                       kDecayFree = kQk + 17, kChecked = kQk + 19, kBars = kQk + 23;
+  static constexpr int kMiscBytes = 2 * (kChunk + 96) * 4 + 4 * 4 * 4 + kWBufs * 3 * kChunk * 2 + 16 + kBars * 8 + 28 * 4;
   static_assert(kWarps <= 16, "scan_s");
   static constexpr int kTableBytes = kStateOnly ? (4 * kThreads + 2) * 4 : 0;  // FirstWalk's arrays
   static constexpr int kSmem = kSlots * kSlotBytes + 2 * kStateBytes + kMiscBytes + kTableBytes;
 };
-
-// The slot of a chunk's keys or values, and how many tiles it held before.  (Queries: slot kQSlot, use c.)
-struct Place {
-  int slot, use;
-};
-ASTERQ_DEVICE Place keys_of(int c) { return {2 * (c & 1), c / 2}; }
-ASTERQ_DEVICE Place values_of(int c) { return {2 * (c & 1) + 1, c / 2}; }
 
 ASTERQ_DEVICE void tma_rows(uint32_t dst, const CUtensorMap* map, int x, int head, int row, uint32_t bar) {
   asm volatile(
@@ -241,14 +253,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   using C = Cfg<kDk, kDv, kStateOnly>;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
-  const uint32_t s_hi = base + kSlots * C::kSlotBytes, s_lo = s_hi + C::kStateBytes;
+  const uint32_t s_hi = base + C::kSlots * C::kSlotBytes, s_lo = s_hi + C::kStateBytes;
   // decays of a chunk (log2 of a token's, and what follows from them), by warp 14
-  float* g_s = reinterpret_cast<float*>(smem + kSlots * C::kSlotBytes + 2 * C::kStateBytes);  // [2][kChunk], of the token after
+  float* g_s = reinterpret_cast<float*>(smem + C::kSlots * C::kSlotBytes + 2 * C::kStateBytes);  // [2][kChunk], of the token after
   float* f_s = g_s + 2 * kChunk;  // [2][96]: 2^(from a token of the first three 32s to the end of its 32)
   float* p32_s = f_s + 2 * 96;    // [2][4]: 2^(each 32's decay)
   float* first_s = p32_s + 8;     // [2][4]: decays (log2) of each 32's first token
-  uint16_t* w_s = reinterpret_cast<uint16_t*>(first_s + 8);      // [3][kChunk]: bf16 parts of the weight to the chunk's end
-  float* whole_s = reinterpret_cast<float*>(w_s + 3 * kChunk);  // [4], one used: 2^(the chunk's decay)
+  uint16_t* w_s = reinterpret_cast<uint16_t*>(first_s + 8);      // [kWBufs][3][kChunk]: bf16 parts of the weight to the chunk's end
+  float* whole_s = reinterpret_cast<float*>(w_s + C::kWBufs * 3 * kChunk);  // [4], kWBufs used: 2^(the chunk's decay)
   uint64_t* bars_s = reinterpret_cast<uint64_t*>(whole_s + 4);
   int* scan_s = reinterpret_cast<int*>(bars_s + C::kBars);  // [16]
   int* start_s = scan_s + 16;                               // sequence, its first chunk
@@ -266,13 +278,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   bool ok = true;
 
   if (tid == 0) {
-    for (int i = 0; i < kSlots; ++i) {
+    for (int i = 0; i < C::kSlots; ++i) {
       mbar_init(bar(C::kFull + i), 1);
       mbar_init(bar(C::kEmpty + i), 1);
     }
-    for (int i : {C::kQk, C::kQs, C::kULo, C::kU, C::kO, C::kDrain, C::kDecay, C::kDecay + 1, C::kChecked, C::kChecked + 1, C::kW})
+    for (int i : {C::kQk, C::kQs, C::kULo, C::kU, C::kO, C::kDrain, C::kDecay, C::kDecay + 1, C::kW, C::kW + 1})
       mbar_init(bar(i), 1);
-    for (int i : {C::kKeys, C::kKeysHi, C::kS, C::kWFree}) mbar_init(bar(i), 8);
+    for (int i = 0; i < 4; ++i) mbar_init(bar(C::kChecked + i), 1);
+    for (int i : {C::kKeys, C::kKeysHi, C::kS, C::kWFree, C::kWFree + 1}) mbar_init(bar(i), 8);
     for (int i : {C::kA, C::kOFree}) mbar_init(bar(i), 4);
     for (int i : {C::kDecayFree, C::kDecayFree + 1}) mbar_init(bar(i), 4);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -419,19 +432,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                        : "memory");
         for (int j = 0; j < walk.n && ok; ++j, ++c) {
           const int row = walk.seq.row0 + (walk.k0 + j) * kChunk;
+          // values first: their slot is the first to be free (but the very first chunk starts with its keys)
 #pragma unroll 1
-          for (int tile = 0; tile < (kStateOnly ? 2 : 3); ++tile) {
-            const Place at = tile == 0 ? keys_of(c) : tile == 1 ? values_of(c) : Place{kQSlot, c};
+          for (int i = 0; i < (kStateOnly ? 2 : 3); ++i) {
+            const int tile = i == 2 ? 2 : (i + (c > 0 && !kStateOnly)) & 1;
+            const typename C::Place at = tile == 0 ? C::keys_of(c) : tile == 1 ? C::values_of(c) : C::queries_of(c);
             const CUtensorMap* map = tile == 0 ? &k_map : tile == 1 ? &v_map : &q_map;
             const int boxes = tile == 1 ? kDv / 64 : kDk / 64;
             if (at.use > 0) ok = wait(C::kEmpty + at.slot, at.use - 1);
             if (!ok) break;
             if (lane == 0) {
-              mbar_expect_tx(bar(C::kFull + at.slot), boxes * kBoxBytes);
+              mbar_expect_tx(bar(at.full), boxes * kBoxBytes);
 #pragma unroll 1
               for (int b = 0; b < boxes; ++b)
                 tma_rows(base + at.slot * C::kSlotBytes + b * kBoxBytes, map, b * 64, walk.head, row,
-                         bar(C::kFull + at.slot));
+                         bar(at.full));
             }
           }
         }
@@ -440,9 +455,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       // last uses: of the chunk before this one, whichever was reached)
       if (!ok) {
         for (int last = max(0, c - 2); last <= c; ++last) {
-          (void)mbar_wait(bar(C::kFull + keys_of(last).slot), keys_of(last).use & 1, never_s, 200000000);
-          (void)mbar_wait(bar(C::kFull + values_of(last).slot), values_of(last).use & 1, never_s, 200000000);
-          if (!kStateOnly) (void)mbar_wait(bar(C::kFull + kQSlot), last & 1, never_s, 200000000);
+          (void)mbar_wait(bar(C::keys_of(last).full), C::keys_of(last).phase & 1, never_s, 200000000);
+          (void)mbar_wait(bar(C::values_of(last).full), C::values_of(last).phase & 1, never_s, 200000000);
+          if (!kStateOnly)
+            (void)mbar_wait(bar(C::queries_of(last).full), C::queries_of(last).phase & 1, never_s, 200000000);
         }
       }
     } else if (warp == 13) {
@@ -463,24 +479,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) return;
         tc::fence_after();
         if (tc::elect()) {
-          const uint32_t v_desc = tc::desc_mn_major(base + values_of(c).slot * C::kSlotBytes, kBoxBytes);
+          const uint32_t v_desc = tc::desc_mn_major(base + C::values_of(c).slot * C::kSlotBytes, kBoxBytes);
           over_tokens(last_steps, [&](int s) {
             const uint32_t at = tmem + C::kColA + 16 * s;
             tc::mma_ts(tmem + C::kColO, at, v_desc + s * 128, kVDesc, last_carried || s > 0);
             tc::mma_ts(tmem + C::kColO, at + 8, v_desc + s * 128, kVDesc, true);
           });
           tc::commit(bar(C::kO));
-          tc::commit(bar(C::kEmpty + values_of(c).slot));
+          tc::commit(bar(C::kEmpty + C::values_of(c).slot));
         }
       };
       int c = 0;
       while (ok && walk.next(a))
         for (int j = 0; j < walk.n; ++j, ++c) {
           const int rows = min(kChunk, walk.seq.rows - (walk.k0 + j) * kChunk), steps = (rows + 15) / 16;
-          const Place kp = keys_of(c), vp = values_of(c);
+          const typename C::Place kp = C::keys_of(c), vp = C::values_of(c);
           const uint32_t v_desc = tc::desc_mn_major(base + vp.slot * C::kSlotBytes, kBoxBytes);
           const uint32_t u = tmem + (c & 1 ? C::kColU1 : C::kColU);
-          ok = wait(C::kFull + vp.slot, vp.use) && (kStateOnly || wait(C::kChecked + (c & 1), c / 2)) && wait(C::kKeys, c);
+          ok = wait(vp.full, vp.phase) && (kStateOnly || wait(C::kChecked + (c & 3), c / 4)) && wait(C::kKeys, c);
           if (!ok) break;
           tc::fence_after();
           if (tc::elect()) {
@@ -501,10 +517,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               tc::commit(bar(C::kEmpty + vp.slot));
             }
           }
-          const uint32_t q_desc = tc::desc_k_major(base + kQSlot * C::kSlotBytes);
+          const typename C::Place qp = C::queries_of(c);
+          const uint32_t q_desc = tc::desc_k_major(base + qp.slot * C::kSlotBytes);
           if constexpr (!kStateOnly) {
             // the columns that Q K^T goes to are free when the last chunk's A has been read
-            ok = wait(C::kFull + kp.slot, kp.use) && wait(C::kFull + kQSlot, c) && (c == 0 || wait(C::kO, c - 1));
+            ok = wait(kp.full, kp.phase) && wait(qp.full, qp.phase) && (c == 0 || wait(C::kO, c - 1));
             if (!ok) break;
             if (tc::elect()) {
               const uint32_t k_desc = tc::desc_k_major(base + kp.slot * C::kSlotBytes);
@@ -533,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
               }
               tc::commit(bar(C::kQs));
-              tc::commit(bar(C::kEmpty + kQSlot));
+              tc::commit(bar(C::kEmpty + qp.slot));
             }
             last_steps = steps;
             last_carried = carried;
@@ -608,18 +625,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           float w[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) w[e] = ex2_ftz(after[e] + later);
-          if (c >= 1) {
-            ok = wait(C::kWFree, c - 1);
+          const int wb = c % C::kWBufs;
+          if (c >= C::kWBufs) {
+            ok = wait(C::kWFree + wb, c / C::kWBufs - 1);
             if (!ok) break;
           }
 #pragma unroll
           for (int part = 0; part < 3; ++part) {
             const uint32_t w01 = split_part(w[0], w[1]), w23 = split_part(w[2], w[3]);
-            reinterpret_cast<uint2*>(w_s + part * kChunk)[lane] = make_uint2(w01, w23);
+            reinterpret_cast<uint2*>(w_s + (wb * 3 + part) * kChunk)[lane] = make_uint2(w01, w23);
           }
-          if (lane == 0) *whole_s = exp2_once(whole);
+          if (lane == 0) whole_s[wb] = exp2_once(whole);
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(C::kW));
+          if (lane == 0) mbar_arrive(bar(C::kW + wb));
         }
         if constexpr (kStateOnly) {
           if (lane == 0) {
@@ -653,9 +671,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       while (ok && walk.next(a))
         for (int j = 0; j < walk.n; ++j, ++c) {
           const int rows = min(kChunk, walk.seq.rows - (walk.k0 + j) * kChunk);
-          const Place vp = values_of(c);
+          const typename C::Place vp = C::values_of(c);
           uint8_t* tile = smem + vp.slot * C::kSlotBytes;
-          ok = wait(C::kFull + vp.slot, vp.use);
+          ok = wait(vp.full, vp.phase);
           if (!ok) break;
           uint32_t most = 0;
 #pragma unroll 1
@@ -688,7 +706,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (lane == 0) bad_s[c & 3] = any;
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(C::kChecked + (c & 1)));
+          if (lane == 0) mbar_arrive(bar(C::kChecked + (c & 3)));
         }
     }
   } else if (warp < 4) {
@@ -767,7 +785,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int step = 2 * warp + 2; step < steps; ++step) tc::st16(lanes + C::kColA + 16 * step, x);
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(C::kDecayFree + (c & 1)));
-          ok = wait(C::kQs, c) && wait(C::kChecked + (c & 1), c / 2);
+          ok = wait(C::kQs, c) && wait(C::kChecked + (c & 3), c / 4);
           if (!ok) break;
           tc::fence_after();
           if (carried) {
@@ -867,13 +885,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = 0; j < walk.n; ++j, ++c) {
         const int rows = min(kChunk, q.rows - (walk.k0 + j) * kChunk), steps = (rows + 15) / 16;
         // the keys, weighted and split: thread t has key dims t / 4 + 8 m and tokens 2 (t % 4), + 1 of each block
-        const Place kp = keys_of(c), vp = values_of(c);
+        const typename C::Place kp = C::keys_of(c), vp = C::values_of(c);
         const uint32_t k_at = base + kp.slot * C::kSlotBytes + k_row;
-        const uint32_t* weight = reinterpret_cast<const uint32_t*>(w_s) + part * 32 + (lane & 3);
-        ok = wait(C::kW, c) && wait(C::kFull + kp.slot, kp.use) && (!C::kTwoKeys || c == 0 || wait(C::kULo, c - 1));
+        const int wb = c % C::kWBufs;
+        const uint32_t* weight = reinterpret_cast<const uint32_t*>(w_s) + wb * 192 + part * 32 + (lane & 3);
+        ok = wait(C::kW + wb, c / C::kWBufs) && wait(kp.full, kp.phase) && (!C::kTwoKeys || c == 0 || wait(C::kULo, c - 1));
         if (!ok) break;
         tc::fence_after();
-        const float whole = *whole_s;
+        const float whole = whole_s[wb];
         // 32 tokens of the warp's 32 key dims: values 4 h + m are key dims 8 m .. of tokens 8 h ..
         auto put = [&](uint32_t to, const uint32_t (&p)[16]) {
           tc::st_16x128b_x4(to, p[0], p[1], p[4], p[5], p[8], p[9], p[12], p[13]);
@@ -912,7 +931,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             put(lanes + C::kColK + 64 + part * 32 + u * 16, m);
           }
         }
-        ok = wait(C::kFull + vp.slot, vp.use);
+        ok = wait(vp.full, vp.phase);
         if (!ok) break;
         if (rows < steps * 16) {
           // the last chunk's products run over whole steps of 16 tokens: values past the end are zeros
@@ -932,7 +951,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(bar(C::kKeys));
         if (C::kTwoKeys) ok = !kStateOnly || c == 0 || wait(C::kU, c - 1);
         else ok = wait(C::kULo, c);
-        ok = ok && (kStateOnly || wait(C::kChecked + (c & 1), c / 2));
+        ok = ok && (kStateOnly || wait(C::kChecked + (c & 3), c / 4));
         if (!ok) break;
         tc::fence_after();
         // the larger parts in their place
@@ -954,7 +973,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           put(lanes + C::kColL + 64 + part * 32 + u * 16, p1);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::kWFree));
+        if (lane == 0) mbar_arrive(bar(C::kWFree + wb));
         tc::wait_st();
         tc::fence_before();
         __syncwarp();
