@@ -8,11 +8,11 @@
 // once (128 KB a chunk and head).  At one head-chunk a CTA, an SM's share of the memory bandwidth
 // takes 5,700 cycles for them; the products below take 4,600 on the tensor core.
 //
-// Measured (128 x 128 dims): 32777 tokens of 12 sequences and 32 heads 440 us, 2.5 TB/s (the bytes alone: 170 us).
-// A CTA's 55 chunks take 6.2 us each: the chain of a chunk, from keys through weighted parts, tensor memory
-// and products to the state, hides only in part behind the next one's, with shared memory 60% busy.  8192
-// tokens of one sequence and 16 heads: 104 us, of which the first pass takes 41 and the chain of states 8.  One
-// chunk of 16 heads: 23 us, three launches and the latency of one chunk.
+// Measured (128 x 128 dims): 32777 tokens of 12 sequences and 32 heads 430 us, 2.6 TB/s (the bytes alone: 170 us).
+// A CTA's 56 chunks take some 9,400 cycles each: the warp that issues the products is busy for 5,500 of them and
+// goes from one role's barrier to the next for the rest, since a chunk's state, its outputs and the next
+// chunk's keys wait for one another.  8192 tokens of one sequence and 16 heads: 97 us, some 40 of them the first pass
+// and the chain of states.  One chunk of 16 heads: 23 us, three launches and the latency of one chunk.
 //
 // Rounding.  Products take bf16 operands and sum in fp32.  A and S enter as two bf16 parts (16 bits:
 // beside the output's own rounding they vanish).  The state is an fp32 output, so its update must not
@@ -32,7 +32,8 @@
 // Roles in a CTA (512 threads): warps 0-3 turn Q K^T into A (row i = thread i) and write the output;
 // warps 4-11 hold S in registers (thread = key dim, half of the value dims), scale and split the keys
 // and update S; warp 12 loads by TMA; warp 13 issues all products; warp 14 sums the decays, a chunk
-// ahead; warp 15 looks for values that are not finite.  Warps 4-11 take registers from the other groups (at
+// ahead; warp 15 looks for values that are not finite (2% of the time: an answer must not depend on what comes after
+// it).  Warps 4-11 take registers from the other groups (at
 // 128 a thread S would spill to local memory).
 #include <cuda.h>
 
@@ -165,7 +166,8 @@ struct Cfg {
   // Tensor memory columns: A, the output, U (what a chunk adds to the state), and the keys' smaller and larger
   // parts.  Where there is room (the first pass has no outputs, and 64 value dims take half) the larger parts
   // have a place of their own and need not wait for the smaller parts' products, and the first pass adds a
-  // chunk's U to the state while the next chunk's products run.
+  // chunk's U to the state while the next chunk's products run: 32768 tokens of 16 heads 276 -> 254 us, of 12 heads
+  // of 64 x 64 dims 168 -> 158.
   static constexpr bool kTwoKeys = kStateOnly || kDv == 64;
   static constexpr uint32_t kColA = 0, kColO = 128, kColU = kStateOnly ? 0 : 128 + kDv, kColU1 = kStateOnly ? 128 : kColU,
                             kColK = kTwoKeys ? 256 : 384, kColL = 384;
