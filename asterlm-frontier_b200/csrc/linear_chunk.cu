@@ -278,6 +278,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   // each warp leaves its work as a whole and waits (again with a limit) for what it has in flight.
   auto wait = [&](int i, int phase) { return wait_for(bar(i), phase & 1, abort_s); };
   bool ok = true;
+  // The chain's CTAs and then the main pass's are set up as SMs become free; they wait for what they read.
+  if constexpr (kStateOnly) asm volatile("griddepcontrol.launch_dependents;");
 
   if (tid == 0) {
     for (int i = 0; i < C::kSlots; ++i) {
@@ -345,6 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (long long i = tid; i < (long long)q.rows * a.n_heads * (kDv / 8); i += kThreads)
         dst[i] = make_uint4(0, 0, 0, 0);
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // every thread, also of a CTA without a share
     __syncthreads();
     if (walk.x >= walk.end) return;
     walk.s = start_s[0];
@@ -1065,6 +1068,8 @@ template <int kDk, int kDv>
 __global__ void __launch_bounds__(256) chain_kernel(const __grid_constant__ Args a, const __grid_constant__ Work work) {
   __shared__ Part parts[2 * kThreads];
   __shared__ int list[2 * kThreads], count;
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // all CTAs: the next grid takes this one's end for both
   const int first = work.first[blockIdx.x];
   if (first < 0) return;
   // the parts that may belong to it, then their order: a chain of loads from memory would take longer than
@@ -1160,8 +1165,22 @@ int launch(const Args& a, int workers, int device, void* workspace, cudaStream_t
   work.starts = work.borders + (long long)workers * kDk * kDv;
   work.bad = reinterpret_cast<uint32_t*>(work.starts + (long long)workers * kDk * kDv);
   chunk_kernel<kDk, kDv, true><<<workers, kThreads, First::kSmem, s>>>(q_map, k_map, v_map, a, work);
-  chain_kernel<kDk, kDv><<<dim3(workers, kDk * kDv / 1024), 256, 0, s>>>(a, work);
-  chunk_kernel<kDk, kDv, false><<<workers, kThreads, Main::kSmem, s>>>(q_map, k_map, v_map, a, work);
+  cudaLaunchAttribute early[1];
+  early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t chain = {}, main = {};
+  chain.gridDim = dim3(workers, kDk * kDv / 1024);
+  chain.blockDim = 256;
+  main.gridDim = workers;
+  main.blockDim = kThreads;
+  main.dynamicSmemBytes = Main::kSmem;
+  chain.stream = main.stream = s;
+  chain.attrs = main.attrs = early;
+  chain.numAttrs = main.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&chain, chain_kernel<kDk, kDv>, a, work);
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&main, chunk_kernel<kDk, kDv, false>, q_map, k_map, v_map, a, work);
+  if (e != cudaSuccess)
+    return set_error(ASTERQ_ERR_CUDA, "linear_attention: launch failed: %s", cudaGetErrorString(e));
   return check_launch("linear_attention");
 }
 
