@@ -153,10 +153,10 @@ static int sm_count(int* device) {
 }
 
 // The chunked form takes bf16 prompts of 24 tokens a sequence or more on average.  Measured at 128 x 128
-// dims, chunked against the scan: 24 tokens, 16 heads of one sequence 21 against 12.5 us, 128 (sequence, head)
-// pairs 22 against 23, 512 pairs 48 against 58, 4096 pairs 232 against 451; 128 tokens, 16 pairs 23 against 57,
-// 4096 pairs 296 against 2147.  At 64 x 64 dims: 24 tokens, 128 pairs 17 against 18 us, 4096 pairs 130 against
-// 155; 128 tokens, 18 against 87 and 135 against 753.
+// dims, chunked against the scan: one sequence of 16 heads, 24 tokens 14.2 against 12.5 us, 32 tokens 14.4
+// against 15.8, 128 tokens 16.5 against 57; 4 of 32 heads, 24 tokens 15.0 against 22.8; 64 of 64 heads, 24 tokens
+// 232 against 451, 128 tokens 296 against 2147.  At 64 x 64 dims: one sequence of 16 heads, 24 tokens 9.8
+// against 12.6; 64 of 64 heads, 24 tokens 130 against 155, 128 tokens 135 against 753.
 static bool in_chunks(const asterq_linear_params* p) {
   return p->dtype == ASTERQ_DTYPE_BF16 && p->row_offsets && p->n_rows >= 24ll * p->n_seqs;
 }
