@@ -71,13 +71,11 @@ struct Cfg {
   static constexpr int kBufFloats = kWarps * NR * kPad, kMergeFloats = 2 * kBufFloats;
   static_assert(D / kSlice % 2 == 0, "the two buffers alternate across units");
   static_assert(kMergeFloats >= 48 * NR, "weights of the records that are joined at once");
-  // What a unit costs beside its tiles, in tiles: a unit by itself takes 1.5 us, two at a time, a tile's share of
-  // the memory bandwidth 0.75 us.
-  // kUnitCost: what a unit costs by itself, in tiles.  Measured with 0, 1 and 2: 64 rows of 1 to 2048 tokens,
-  // 8 kv heads of 128, 40.5, 32.4 and 30.6 us; 256 rows of at most 512 visible tokens, 16 kv heads of 64, 99.9, 91.7
-  // and 101.5; 64 rows of 1k to 32k tokens 372, 367 and 365.
-  // kSoloTiles: units up to this long are taken by one team.  Measured with 0, 4 and 8: the same three 34.2, 32.4 and
-  // 33.5 us; 99.1, 91.7 and 91.4; 372, 367 and 367.  (64 rows of 1 to 512 tokens, 20.7, 22.3 and 24.1, would have all.)
+  // kUnitCost: what a unit costs beside its tiles, in tiles.  Measured with 0, 1 and 2: 64 rows of 1 to 2048 tokens,
+  // 8 kv heads of 128, 38.1, 29.5 and 27.3 us; of 1 to 512 tokens 20.7, 19.6 and 20.8; of 1k to 32k tokens 368, 366 and
+  // 368; 256 rows of at most 512 visible tokens, 16 kv heads of 64, 100, 90 and 99.
+  // kSoloTiles: units up to this long are taken by one team.  Measured with 0, 4 and 8: the same four 34.5, 29.5 and
+  // 29.4 us; 21.6, 19.6 and 21.2; 365, 366 and 366; 101, 90 and 90.
   static constexpr int kUnitCost = 1;
   static constexpr int kSoloTiles = 4;
   static constexpr int kSmem =
