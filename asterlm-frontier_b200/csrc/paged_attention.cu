@@ -69,7 +69,7 @@ struct Cfg {
   // dims joined at a time, in two buffers taken in turn; their count is even, so a unit ends with the second
   static constexpr int kSlice = NR == 16 ? 16 : 32, kPad = kSlice + 4;
   static constexpr int kBufFloats = kWarps * NR * kPad, kMergeFloats = 2 * kBufFloats;
-  static_assert(D / kSlice % 2 == 0, "the two buffers alternate across units");
+  static_assert(D / kSlice % 2 == 0, "the two buffers alternate across units that the same warps join");
   static_assert(kMergeFloats >= 48 * NR, "weights of the records that are joined at once");
   // kUnitCost: what a unit costs beside its tiles, in tiles.  Measured with 0, 1 and 2: 64 rows of 1 to 2048 tokens,
   // 8 kv heads of 128, 38.1, 29.5 and 27.3 us; of 1 to 512 tokens 20.7, 19.6 and 20.8; of 1k to 32k tokens 368, 366 and
@@ -389,12 +389,17 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   const long long n_slots = 2ll * gridDim.x;
   int it = 0;
   uint32_t phase = 0;  // of each stage's barrier of this team
+  bool all_joined = false;  // the unit before was joined by all warps
   for (int piece = 0; walk.next(a, units_per_row); ++piece) {
     const int head = walk.unit / a.row_blocks, block = walk.unit - head * a.row_blocks;
     const int rows = min(NR, a.group - block * NR);
     const long long h0 = (long long)head * a.group + block * NR;  // query head of the block's row 0
     const bool cut = walk.n < walk.span.tiles, solo = !cut && walk.n <= C::kSoloTiles;
     const int q_slot = piece % C::kQSlots;
+    // All warps' join ends with reads of one another's sums that nothing orders.  The first barrier of another such
+    // join does, a team's own does not: its second slice would overwrite what the other team may still read.
+    if (solo && all_joined) named_sync(3, 32 * C::kWarps);
+    all_joined = !solo;
     // Every warp follows the queries of every unit, so that none falls a phase behind.  (After a wait has run
     // out all go on to the end, waits returning at once, since they still meet at barriers.)
     (void)mbar_wait(q_full0 + 8 * q_slot, (piece / C::kQSlots) & 1, &abort_s);
