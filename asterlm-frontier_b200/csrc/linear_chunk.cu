@@ -404,6 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool starts = need > 0 && unit >= border(w - 1);
       work.first[w] = starts ? w + (int)(((long long)(ahead + 1) * W - 1) / all) : -1;
     }
+    fence_async_shared();  // the copy engine writes tiles over `strips`
     __syncthreads();
     walk.x = me < W ? (int)((long long)all * me / W) : all;
     walk.end = me < W ? (int)((long long)all * (me + 1) / W) : all;
@@ -915,6 +916,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                          "r"(0)
                          : "memory");
           }
+          fence_async_shared();  // the slot's next tile is written by the copy engine
           __syncwarp();
         }
         {
