@@ -80,11 +80,13 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const asterq_kv_append
   const int s = find_sequence(p.row_offsets, p.n_seqs, row);
   const int length = __ldg(p.lengths + s);
   if (length < 0) return;  // an empty slot
-  const long long pos = (long long)length + (row - __ldg(p.row_offsets + s));
+  const long long begin = __ldg(p.row_offsets + s), pos = (long long)length + (row - begin);
   const long long col = pos / p.page_tokens;
   const int at = (int)(pos - col * p.page_tokens);
   int page = -1;
-  if (col < p.max_pages) page = __ldg(p.page_table + (long long)s * p.max_pages + col);
+  // the search finds a sequence that the row is not of where offsets are out of order
+  if (row >= begin && row < (long long)__ldg(p.row_offsets + s + 1) && col < p.max_pages)
+    page = __ldg(p.page_table + (long long)s * p.max_pages + col);
   if (page < 0 || page >= p.n_pages || (turn && pos >= p.n_positions)) {
     if (p.status && (threadIdx.x & 31) == 0) atomicMax(p.status, 1);
     return;

@@ -397,6 +397,7 @@ int asterq_cp_combine_wait(const void* mailbox, int32_t world, int32_t n_blocks,
  * dims are copied.  `lengths` is not advanced (the layers of a model share it).  A row whose position
  * has no page in the table, a page id outside [0, n_pages) or (rotary_dim > 0) no row in cos / sin is
  * left out with its query and sets *status to 1; rows of an empty slot or of no sequence are left out.
+ * row_offsets do not decrease; rows that offsets out of order keep from their sequence are left out with *status 1.
  * q may be NULL (keys and values only).  q_out must not overlap the inputs.
  * head_dim: a multiple of 16 up to 512; rotary_dim: a multiple of 16 up to head_dim, 0 for no rotation.
  */
