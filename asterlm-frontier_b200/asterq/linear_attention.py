@@ -149,7 +149,7 @@ def linear_attention_prefill(
     starts from a state of zeros, whatever its slot holds), None: all continue; row_offsets int32
     [n_seqs + 1].  q, k [rows, n_heads, dk] and v [rows, n_heads, dv] of one type, with any row and head
     stride.  log_decay float32 [n_heads] or [rows, n_heads], not above 0.  scale: 1 / sqrt(dk) unless
-    given.  status int32 [1]: set to 1 when a slot or row offset was out of range.
+    given.  status int32 [1]: set to 1 when a slot or row offset was out of range, or offsets decreased.
 
     bf16 prompts run in chunks of 128 tokens on the tensor cores where ``out`` and ``state`` are 32-byte aligned
     and no stride is 0, other types and short prompts token by token.  A value of v that is not finite reaches its

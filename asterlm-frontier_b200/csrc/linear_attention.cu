@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(const __grid_constant__ 
     end = __ldg(a.row_offsets + seq + 1);
   }
   if (row < 0 || end > a.n_rows || row >= end) {
-    if (tid == 0 && (row < 0 || end > a.n_rows) && a.status) atomicMax(a.status, 1);
+    if (tid == 0 && (row < 0 || end > a.n_rows || row > end) && a.status) atomicMax(a.status, 1);
     return;
   }
   if (slot < 0 || slot >= a.n_slots) {

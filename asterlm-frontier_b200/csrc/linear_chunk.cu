@@ -300,8 +300,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   // this CTA's share: a prefix sum over the sequences' chunks, thread t summing a strip of them
   const int strip = (a.n_seqs + kThreads - 1) / kThreads;
   const int s0 = min(tid * strip, a.n_seqs), s1 = min(s0 + strip, a.n_seqs);
-  int sum = 0;
-  for (int s = s0; s < s1; ++s) sum += seq_of(a, s).chunks;
+  int sum = 0, disorder = 0;
+  for (int s = s0; s < s1; ++s) {
+    sum += seq_of(a, s).chunks;
+    disorder |= __ldg(a.row_offsets + s + 1) < __ldg(a.row_offsets + s);
+  }
   sum *= a.n_heads;
   int scan = sum;
 #pragma unroll
@@ -310,13 +313,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane >= d) scan += up;
   }
   if (lane == 31) scan_s[warp] = scan;
-  __syncthreads();
+  // Sequences that share rows could count up to any number of chunks: offsets out of order leave the call undone.
+  disorder = __syncthreads_or(disorder);
   int before = scan - sum, total = 0;
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) before += scan_s[w];
     total += scan_s[w];
   }
   const int me = blockIdx.x;
+  if (disorder) {
+    total = 0;
+    if (!kStateOnly && me == 0 && tid == 0 && a.status) atomicMax(a.status, 1);
+  }
   // As many shares as the longest needs: fewer cuts inside a (sequence, head).
   const int longest = max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x);
   const int W = max(1, (total + longest - 1) / longest);

@@ -493,8 +493,8 @@ int asterq_paged_attention(const asterq_paged_attention_params* p, void* stream)
  * (decay_row_stride 0: one constant for each head), not above 0.  lengths (may be NULL): sequences with
  * lengths[s] <= 0 start from a state of zeros, whatever their slot holds.  A slot below 0 is an empty
  * one: its rows are written as zeros; one at or above n_slots is taken the same way and sets *status
- * to 1, and so do row offsets outside [0, n_rows], whose sequence is left out.  Sequences of a call
- * have slots of their own.  A value of v that is not finite reaches its column of the state, and of the outputs
+ * to 1, and so do row offsets outside [0, n_rows], whose sequence is left out, and offsets that decrease,
+ * which leave out that sequence or the whole call.  Sequences of a call have slots of their own.  A value of v that is not finite reaches its column of the state, and of the outputs
  * from its row on (where an infinity may become NaN), and nothing else.
  * dk, dv: 64 or 128.  q, k, v, out of one type: bf16, f16 or f32.
  * workspace: asterq_linear_workspace_bytes bytes (0: none needed), not kept between calls; calls that

@@ -39,3 +39,39 @@ def test_append_leaves_out_rows_that_offsets_out_of_order_hide(cuda, offsets):
         want[found[0][0], 0, found[0][1]] = x[row, 0]
     assert int(status) == (hidden > 0)
     assert torch.equal(pools.k, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("offsets", [[0, 300, 100, 300], [0, 300, 0, 300, 0, 300], [200, 100], [0, 1, 0, 299, 300]])
+def test_prompts_say_that_offsets_are_out_of_order(cuda, dtype, offsets):
+    """Both forms (bf16 in chunks, f16 token by token) report it; slots of no sequence keep their states, and calls that
+    follow are right."""
+    from asterq.linear_attention import linear_attention_prefill
+
+    n, h = len(offsets) - 1, 2
+    q, k, v = (torch.randn(300, h, 64, device="cuda").to(dtype) for _ in range(3))
+    decay = torch.full((h,), -0.1, device="cuda")
+    state = torch.randn(n + 1, h, 64, 64, device="cuda")
+    last, status = state[n].clone(), _ints([0])
+    linear_attention_prefill(state, _ints(list(range(n))), None, _ints(offsets), q, k, v, decay, status=status)
+    assert int(status) == 1 and torch.equal(state[n], last)
+    if dtype == torch.bfloat16:
+        fresh = [torch.zeros(1, h, 64, 64, device="cuda") for _ in range(2)]
+        out = [linear_attention_prefill(s, _ints([0]), None, _ints([0, 300]), q, k, v, decay) for s in fresh]
+        assert torch.equal(*out) and torch.equal(*fresh) and bool(out[0].isfinite().all())
+
+
+def test_chunks_of_sequences_that_share_rows_would_not_fit_32_bits(cuda):
+    """Every other sequence holds all rows: 20833 times 7813 chunks of 16 heads would count up to 2.6e9."""
+    from asterq.linear_attention import linear_attention_prefill
+
+    rows, h = 1000000, 16
+    n = 2 * (rows // 48) - 1
+    offsets = torch.tensor([0, rows], dtype=torch.int32).repeat((n + 1) // 2).cuda()
+    x = torch.zeros(rows, h, 64, dtype=torch.bfloat16, device="cuda")
+    state = torch.ones(n, h, 64, 64, device="cuda")
+    status = _ints([0])
+    out = torch.zeros_like(x)
+    linear_attention_prefill(state, torch.arange(n, dtype=torch.int32, device="cuda"), None, offsets, x, x, x,
+                             torch.zeros(h, device="cuda"), out=out, status=status)
+    assert int(status) == 1 and bool((state == 1).all()) and bool((out == 0).all())
