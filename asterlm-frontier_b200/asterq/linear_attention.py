@@ -10,8 +10,8 @@ slot, float32 [n_slots, n_heads, dk, dv], updated in place:
 * ``linear_attention_step``: one new token a sequence.
 
 Both call ``asterq_linear_attention``; nothing waits for the GPU or reads from it, so calls can be
-recorded in a CUDA graph (the first prompt call on a stream allocates that stream's workspace: make it
-before the capture).
+recorded in a CUDA graph.  A first prompt call on a stream, or ``workspace``, gives that stream's prompts
+their workspace; a captured prompt without either has one in the graph's memory.
 """
 from __future__ import annotations
 
@@ -20,7 +20,7 @@ import math
 import torch
 
 from . import _lib
-from .paged_kv import _call, _check_int, _quick
+from .paged_kv import _call, _capturing, _check_int, _quick
 
 _PARAMS = _lib.packer(_lib.LinearParams)
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
@@ -59,7 +59,10 @@ def _workspace(device: torch.device, stream: int) -> LinearAttentionWorkspace:
     """The workspace that calls on this stream share when the caller brings none."""
     ws = _workspaces.get((device.index, stream))
     if ws is None:
-        ws = _workspaces[(device.index, stream)] = LinearAttentionWorkspace(device)
+        ws = LinearAttentionWorkspace(device)
+        if _capturing(device):
+            return ws  # of the graph's own memory
+        _workspaces[(device.index, stream)] = ws
         if _quick() is not None:
             _quick().workspace(1, device.index, stream, ws.buffer.data_ptr(), ws.nbytes)
     return ws

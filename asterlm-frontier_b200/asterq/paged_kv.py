@@ -11,8 +11,9 @@ the GPU:
 * ``PagedKVBatch``: the pools of a stack of layers with the page tables they share, for a server that
   admits, steps and removes sequences.
 
-Nothing here waits for the GPU or reads from it, so all of it can be recorded in a CUDA graph (the
-first call on a stream allocates that stream's workspace: make it before the capture).
+Nothing here waits for the GPU or reads from it, so all of it can be recorded in a CUDA graph.  A first
+call on a stream, or ``workspace``, gives that stream's calls their workspace; a captured ``paged_attention``
+without either has one of its own, zeroed at every replay (5 MB).
 """
 from __future__ import annotations
 
@@ -86,11 +87,19 @@ class PagedAttentionWorkspace:
 _workspaces: dict[tuple[int, int], PagedAttentionWorkspace] = {}
 
 
+def _capturing(device: torch.device) -> bool:
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _workspace(device: torch.device, stream: int) -> PagedAttentionWorkspace:
     """The workspace that calls on this stream share when the caller brings none."""
     ws = _workspaces.get((device.index, stream))
     if ws is None:
-        ws = _workspaces[(device.index, stream)] = PagedAttentionWorkspace(device)
+        ws = PagedAttentionWorkspace(device)
+        if _capturing(device):
+            return ws  # of the graph's own memory and zeroed when the graph runs: not for any call but this one
+        _workspaces[(device.index, stream)] = ws
         if _quick() is not None:
             _quick().workspace(0, device.index, stream, ws.buffer.data_ptr(), ws.nbytes)
     return ws
