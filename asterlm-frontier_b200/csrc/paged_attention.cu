@@ -506,6 +506,15 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             hi[t][0] = fmaxf(hi[t][0], __shfl_xor_sync(0xffffffffu, hi[t][0], d));
             hi[t][1] = fmaxf(hi[t][1], __shfl_xor_sync(0xffffffffu, hi[t][1], d));
           }
+        if constexpr (C::kF16) {
+          // Weights are up to 2^15 and not 1: below 2^-14 a 16-bit part of them would be subnormal, and of many small
+          // weights beside a large one (a sink's, say) little was left, up to all of an eighth of them.
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            hi[t][0] -= 15.0f;
+            hi[t][1] -= 15.0f;
+          }
+        }
         bool higher = false;
 #pragma unroll
         for (int t = 0; t < NT; ++t) higher = higher || hi[t][0] > m[t][0] || hi[t][1] > m[t][1];
