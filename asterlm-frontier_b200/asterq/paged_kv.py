@@ -247,7 +247,8 @@ def paged_attention(
     tokens, get zeros and a log-sum-exp of -inf.  ``window_size`` keeps the first ``sink_tokens`` and the
     newest ``window_size - sink_tokens`` tokens (the trim rule of the latent cache).  Scores are
     ``softmax_scale`` (1 / sqrt(head_dim)) q . k, softcapped to ``logit_softcap`` if given.  ``out``: the
-    queries' type or float32.  A sequence longer than its row of the table ends with it.  status int32 [1]: set
+    queries' type, or float32 good to some 2^-17 of the values (weights enter as two 16-bit parts).  Infinities
+    and NaN in visible values reach their dim as in the formula, in other places of the pages nothing.  A sequence longer than its row of the table ends with it.  status int32 [1]: set
     to 1 when a needed page id was outside the pool.
     """
     quick = _quick()

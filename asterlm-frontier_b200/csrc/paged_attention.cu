@@ -96,6 +96,16 @@ ASTERQ_DEVICE uint32_t transpose8(uint32_t x) {
   return d;
 }
 
+// Two 16-bit values: an infinity as the largest finite value, a NaN as any finite one.  With b positive, xorsign gives
+// min(|x|, |b|) the sign of x; of a number and a NaN it takes the number.
+template <bool kF16>
+ASTERQ_DEVICE uint32_t finite2(uint32_t x) {
+  uint32_t r;
+  if constexpr (kF16) asm("min.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x7bff7bffu));
+  else asm("min.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x7f7f7f7fu));
+  return r;
+}
+
 // The visible tiles of one sequence.  Tile k of its list is tokens [kTile j, kTile (j + 1)) with
 // j = k below sink_tiles and first + k - sink_tiles from there on.
 struct Span {
@@ -590,14 +600,19 @@ __global__ void __launch_bounds__(C::kThreads, 1)
               f[2] &= keep[u][1];
               f[3] &= keep[u][1];
             }
+            // The weights' smaller parts are zero or negative at times: an infinity times them is not what the
+            // formula has, and the larger parts bring it in.
+            uint32_t fl[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) fl[e] = finite2<C::kF16>(f[e]);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
               if constexpr (C::kF16) {
                 mma_f16(acc[i][t], f, ph[u][t][0], ph[u][t][1]);
-                mma_f16(acc[i][t], f, pl[u][t][0], pl[u][t][1]);
+                mma_f16(acc[i][t], fl, pl[u][t][0], pl[u][t][1]);
               } else {
                 mma_bf16(acc[i][t], f, ph[u][t][0], ph[u][t][1]);
-                mma_bf16(acc[i][t], f, pl[u][t][0], pl[u][t][1]);
+                mma_bf16(acc[i][t], fl, pl[u][t][0], pl[u][t][1]);
               }
             }
           }

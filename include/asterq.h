@@ -445,7 +445,9 @@ int asterq_kv_append(const asterq_kv_append_params* p, void* stream);
  * tokens (lengths[b] < 0, or L = 0) gets zeros and -inf.  Pages with no visible token may have any id;
  * where a needed id is outside [0, n_pages) the row's output is not valid and *status becomes 1.  A sequence
  * longer than its row of the table (max_pages * page_tokens) ends there.
- * Products of the weights are taken in two 16-bit parts, softmax statistics and sums in fp32.
+ * Products of the weights are taken in two 16-bit parts, softmax statistics and sums in fp32.  Infinities and NaN among
+ * the visible values reach their dim of the output as in the formula, a weight below 2^-39 (f16) or 2^-126 (bf16) of the
+ * largest counting as zero there; a score of +inf makes its row's output and log-sum NaN.
  * head_dim 64, 128 or 256; page_tokens a multiple of 16.
  *
  * workspace: asterq_paged_attention_workspace_bytes bytes, zeroed once before its first use; every
