@@ -48,7 +48,7 @@ struct Args {
   long long q_row_stride, q_head_stride, n_pages, capacity;  // capacity: tokens a row of the table can hold
   int n_rows, n_heads, n_kv_heads, group, row_blocks;
   int page_tokens, max_pages, box_rows, n_new, window, sink, out_f32;
-  float scale, softcap, cap_in;  // cap_in: 2 log2(e) scale / softcap
+  float scale, softcap, cap_in;  // cap_in: scale / softcap
 };
 
 // D: head dim.  NR: query rows of a block (the query heads of one kv head, in eights).
@@ -104,6 +104,18 @@ ASTERQ_DEVICE uint32_t finite2(uint32_t x) {
   if constexpr (kF16) asm("min.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x7bff7bffu));
   else asm("min.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x7f7f7f7fu));
   return r;
+}
+
+// tanh x to a few 2^-23 of itself (of 1 it is not enough: under a cap far above the scores that is the scores' whole size).
+// Below 0.9 Lambert's continued fraction x / (1 + x^2 / (3 + x^2 / (5 + x^2 / (7 + x^2 / 9)))) as a quotient, its error
+// x^10 / 9.8e6 < 2^-24; from there on (e^2x - 1) / (e^2x + 1), the exponent held within what 2^x and the quotient take.
+ASTERQ_DEVICE float tanh_of(float x) {
+  const float x2 = x * x;
+  const float e2x = ex2_ftz(fminf(fmaxf(x * (2.0f * kLog2e), -64.0f), 64.0f));
+  const bool large = fabsf(x) >= 0.9f;  // not of a NaN
+  const float num = large ? e2x - 1.0f : x * fmaf(x2, x2 + 105.0f, 945.0f);
+  const float den = large ? e2x + 1.0f : fmaf(x2, fmaf(x2, 15.0f, 420.0f), 945.0f);
+  return __fdividef(num, den);
 }
 
 // The visible tiles of one sequence.  Tile k of its list is tokens [kTile j, kTile (j + 1)) with
@@ -495,9 +507,7 @@ __global__ void __launch_bounds__(C::kThreads, 1)
             if (a.softcap > 0.0f) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                // cap tanh(x / cap) with tanh(y) = 1 - 2 / (1 + e^2y), good to a few 1e-7 of cap
-                const float e2y = ex2_ftz(sc[u][t][e] * a.cap_in);
-                sc[u][t][e] = a.softcap * kLog2e * (1.0f - __fdividef(2.0f, 1.0f + e2y));
+                sc[u][t][e] = a.softcap * kLog2e * tanh_of(sc[u][t][e] * a.cap_in);
               }
             } else {
 #pragma unroll
@@ -990,7 +1000,7 @@ extern "C" int asterq_paged_attention(const asterq_paged_attention_params* p, vo
   a.out_f32 = p->out_dtype == ASTERQ_DTYPE_F32;
   a.scale = p->softmax_scale;
   a.softcap = p->logit_softcap > 0.0f ? p->logit_softcap : 0.0f;
-  a.cap_in = a.softcap > 0.0f ? 2.0f * pat::kLog2e * a.scale / a.softcap : 0.0f;
+  a.cap_in = a.softcap > 0.0f ? a.scale / a.softcap : 0.0f;
   // a box of a tile lies in one page: the largest of the tile, its half, .. down to 16 tokens that divides the page
   a.box_rows = 8192 / p->head_dim;
   while (p->page_tokens % a.box_rows) a.box_rows /= 2;
