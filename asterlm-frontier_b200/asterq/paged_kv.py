@@ -303,8 +303,9 @@ class PagedKVBatch:
     Slot s is row s of ``page_table`` and ``lengths``, which live on the GPU beside a host mirror that
     hands out pages ahead of need.  A decode step is ``begin_step`` once, then for each layer ``append``
     and ``attend`` with one row a slot (rows of idle slots are ignored, their outputs are zeros), then
-    ``end_step``.  A prompt chunk is ``begin_rows`` with the tokens each slot gets, ``append`` for each
-    layer, ``end_step``; the prompt's own attention is the caller's.
+    ``end_step`` (or ``abandon_step``, where it failed on the way).  A prompt chunk is ``begin_rows`` with the tokens each slot gets, ``append`` for each
+    layer, ``end_step``; the prompt's own attention is the caller's.  A slot holds its pages until it is
+    removed, also those that a window has passed.
     """
 
     def __init__(self, n_layers: int, n_kv_heads: int, head_dim: int, *, max_seqs: int, max_tokens: int,
@@ -444,6 +445,13 @@ class PagedKVBatch:
             raise RuntimeError("no step is open")
         self.lengths.add_(self._new_dev)
         self._length += self._new
+        self._open = False
+
+    def abandon_step(self) -> None:
+        """Close the open step without advancing: the sequences stay as they were before it.  What it has appended is
+        never read, and the next step's tokens go in its place; pages that it was handed stay with their slots."""
+        if not self._open:
+            raise RuntimeError("no step is open")
         self._open = False
 
     def raise_if_failed(self) -> None:
