@@ -301,7 +301,7 @@ class PagedKVBatch:
     """The paged keys and values of a stack of attention layers that share sequence slots.
 
     Slot s is row s of ``page_table`` and ``lengths``, which live on the GPU beside a host mirror that
-    hands out pages ahead of need.  A decode step is ``begin_step`` once, then for each layer ``append``
+    hands out pages ahead of need (sequences added or removed reach the GPU with the next step).  A decode step is ``begin_step`` once, then for each layer ``append``
     and ``attend`` with one row a slot (rows of idle slots are ignored, their outputs are zeros), then
     ``end_step`` (or ``abandon_step``, where it failed on the way).  A prompt chunk is ``begin_rows`` with the tokens each slot gets, ``append`` for each
     layer, ``end_step``; the prompt's own attention is the caller's.  A slot holds its pages until it is

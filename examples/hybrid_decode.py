@@ -131,9 +131,9 @@ class Server:
 
     def step(self, x):
         """One token for every open slot: x [MAX_SEQS, WIDTH], row s for slot s (rows of free slots are ignored)."""
+        self.kv.begin_step()  # brings the lengths on the GPU up to date
         open_slots = self.kv.lengths >= 0
         slots = torch.where(open_slots, torch.arange(MAX_SEQS, dtype=torch.int32, device=self.device), -1).int()
-        self.kv.begin_step()
         at = {kind: 0 for kind in LAYERS}
         for kind, w_in, w_out in self.w.layers:
             i, at[kind] = at[kind], at[kind] + 1
