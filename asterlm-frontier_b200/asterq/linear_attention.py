@@ -63,8 +63,8 @@ def _workspace(device: torch.device, stream: int) -> LinearAttentionWorkspace:
         if _capturing(device):
             return ws  # of the graph's own memory
         _workspaces[(device.index, stream)] = ws
-        if _quick() is not None:
-            _quick().workspace(1, device.index, stream, ws.buffer.data_ptr(), ws.nbytes)
+    if _quick() is not None:  # whose calls come here until it knows the workspace
+        _quick().workspace(1, device.index, stream, ws.buffer.data_ptr(), ws.nbytes)
     return ws
 
 
