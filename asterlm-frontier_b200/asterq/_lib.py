@@ -286,13 +286,18 @@ _calls = None
 
 
 def quick_calls():
-    """The extension module ``_calls`` bound to the loaded library, or None where it is not built: the
-    callers' own checks then make every call."""
+    """The extension module ``_calls`` bound to the loaded library, or None where it is not built, or built
+    against another torch: the callers' own checks then make every call."""
     global _calls
     if _calls is None:
+        import torch
+
         try:
             from . import _calls as module
         except ImportError:
+            _calls = False
+            return None
+        if f"torch {torch.__version__};" not in getattr(module, "version", ""):
             _calls = False
             return None
         lib = load()

@@ -97,17 +97,20 @@ def build(verbose: bool = False, force: bool = False, ptxas_verbose: bool = Fals
 
 def build_calls(verbose: bool = False, force: bool = False) -> Path:
     """Compile ``asterq/_calls`` (the quick way from torch tensors to the library's calls, g++)."""
-    if not force and not _stale(CALLS_PATH, [CALLS_SRC, *sorted(INCLUDE.glob("*.h"))]):
-        return CALLS_PATH
     import torch
     from torch.utils import cpp_extension
 
+    # of one version of torch, whose name the module holds between these words
+    version = f"asterq._calls of torch {torch.__version__};"
+    if not force and not _stale(CALLS_PATH, [CALLS_SRC, *sorted(INCLUDE.glob("*.h"))]) and \
+            version.encode() in CALLS_PATH.read_bytes():
+        return CALLS_PATH
     tmp = CALLS_PATH.with_name(CALLS_PATH.name + ".tmp")
     libs = Path(torch.__file__).resolve().parent / "lib"
     cuda = Path(nvcc_path()).resolve().parent.parent
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *(f"-I{p}" for p in cpp_extension.include_paths()), f"-I{cuda / 'include'}",
+           f'-DASTERQ_CALLS_VERSION="{version}"', *(f"-I{p}" for p in cpp_extension.include_paths()), f"-I{cuda / 'include'}",
            f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}", str(CALLS_SRC), "-o", str(tmp), f"-L{libs}",
            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     if verbose:

@@ -362,4 +362,9 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, g_methods,
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__calls() { return PyModule_Create(&g_module); }
+// `version` names the torch that this was compiled against: with another one the module is not to be used
+PyMODINIT_FUNC PyInit__calls() {
+  PyObject* m = PyModule_Create(&g_module);
+  if (m && PyModule_AddStringConstant(m, "version", ASTERQ_CALLS_VERSION) != 0) Py_CLEAR(m);
+  return m;
+}
