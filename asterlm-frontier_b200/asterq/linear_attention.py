@@ -9,6 +9,7 @@ slot, float32 [n_slots, n_heads, dk, dv], updated in place:
 * ``linear_attention_prefill``: ragged prompt chunks, rows ``row_offsets[s]`` and on for sequence s;
 * ``linear_attention_step``: one new token a sequence.
 
+There is no backward pass: inputs that require a gradient are refused outside of ``torch.no_grad()``.
 Both call ``asterq_linear_attention``; nothing waits for the GPU or reads from it, so calls can be
 recorded in a CUDA graph.  A first prompt call on a stream, or ``workspace``, gives that stream's prompts
 their workspace; a captured prompt without either has one in the graph's memory.
@@ -20,7 +21,7 @@ import math
 import torch
 
 from . import _lib
-from .paged_kv import _call, _capturing, _check_int, _quick
+from .paged_kv import _call, _capturing, _check_int, _check_no_gradient, _quick
 
 _PARAMS = _lib.packer(_lib.LinearParams)
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
@@ -33,6 +34,7 @@ def _rows(x: torch.Tensor, name: str, q: torch.Tensor, dim: int) -> torch.Tensor
         raise TypeError(f"{name} is {x.dtype}, q is {q.dtype}")
     if x.device != q.device:
         raise RuntimeError(f"{name} is on {x.device}, q is on {q.device}")
+    _check_no_gradient(x, name)
     row, head, one = x.stride()
     if one != 1 or (row | head) % 8 or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
@@ -93,6 +95,8 @@ def _run(state, slots, lengths, row_offsets, q, k, v, log_decay, scale, out, wor
     if log_decay.dtype != torch.float32 or log_decay.device != q.device or log_decay.stride(-1) != 1 or (
             log_decay.shape != (heads,) and log_decay.shape != (rows, heads)):
         raise ValueError(f"log_decay must be float32 [{heads}] or [{rows}, {heads}] on q's device, its heads contiguous")
+    _check_no_gradient(log_decay, "log_decay")
+    _check_no_gradient(state, "state")
     if slots.dim() != 1:
         raise ValueError("slots must be [n_seqs]")
     n_seqs = slots.shape[0]

@@ -11,6 +11,7 @@ the GPU:
 * ``PagedKVBatch``: the pools of a stack of layers with the page tables they share, for a server that
   admits, steps and removes sequences.
 
+There is no backward pass: inputs that require a gradient are refused outside of ``torch.no_grad()``.
 Nothing here waits for the GPU or reads from it, so all of it can be recorded in a CUDA graph.  A first
 call on a stream, or ``workspace``, gives that stream's calls their workspace; a captured ``paged_attention``
 without either has one of its own, zeroed at every replay (5 MB).
@@ -105,6 +106,12 @@ def _workspace(device: torch.device, stream: int) -> PagedAttentionWorkspace:
     return ws
 
 
+def _check_no_gradient(x: torch.Tensor, name: str) -> None:
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires a gradient, and there is no backward pass: call under torch.no_grad(), or "
+                           "detach it")
+
+
 def _check_rows(x: torch.Tensor, name: str, like: torch.Tensor, heads: int | None, dim: int) -> torch.Tensor:
     """[rows, heads, dim] of the pools' type whose rows and heads the kernels can read in 16-byte loads; a
     copy where they cannot."""
@@ -114,6 +121,7 @@ def _check_rows(x: torch.Tensor, name: str, like: torch.Tensor, heads: int | Non
         raise TypeError(f"{name} is {x.dtype}, the pools are {like.dtype}")
     if x.device != like.device:
         raise RuntimeError(f"{name} is on {x.device}, the pools are on {like.device}")
+    _check_no_gradient(x, name)
     row, head, one = x.stride()
     if one != 1 or (row | head) % 8 or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)

@@ -8,6 +8,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -40,10 +41,13 @@ bool ints(const at::Tensor* t, int device, std::initializer_list<int64_t> shape)
   return on(t, device) && t->scalar_type() == at::kInt && t->sizes() == at::IntArrayRef(shape) && t->is_contiguous();
 }
 
+// what Python refuses: there is no backward pass
+bool wants_gradient(const at::Tensor* t) { return t->requires_grad() && at::GradMode::is_enabled(); }
+
 // [rows, heads, dim] that the kernels read in 16-byte loads
 bool rows(const at::Tensor* t, int device, at::ScalarType type, int64_t dim) {
   return on(t, device) && t->dim() == 3 && t->scalar_type() == type && t->size(2) == dim && t->stride(2) == 1 &&
-         ((t->stride(0) | t->stride(1)) & 7) == 0 && (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0;
+         ((t->stride(0) | t->stride(1)) & 7) == 0 && (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0 && !wants_gradient(t);
 }
 
 int type_code(at::ScalarType t) {
@@ -245,7 +249,7 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
       k->size(1) != heads || v->size(1) != heads || !ints(slots, device, {n_seqs}) || n_seqs > INT32_MAX ||
       heads > INT32_MAX || state->size(0) > INT32_MAX)
     return pass();
-  if (!on(g, device) || g->scalar_type() != at::kFloat || g->dim() < 1 || g->dim() > 2 || g->stride(-1) != 1 ||
+  if (!on(g, device) || wants_gradient(g) || wants_gradient(state) || g->scalar_type() != at::kFloat || g->dim() < 1 || g->dim() > 2 || g->stride(-1) != 1 ||
       g->size(-1) != heads || (g->dim() == 2 && g->size(0) != n_rows) || !PyFloat_CheckExact(args[8]))
     return pass();
   asterq_linear_params p = {};
