@@ -30,6 +30,7 @@ def test_the_extension_is_built_again_for_another_torch(monkeypatch):
         return types.SimpleNamespace(returncode=1, stdout="", stderr="")
 
     monkeypatch.setattr(build.subprocess, "run", run)
+    monkeypatch.setattr(build, "_stale", lambda target, deps: False)  # no source is newer
     build.build_calls()
     assert not runs
     monkeypatch.setattr(torch, "__version__", "0.0.1")
