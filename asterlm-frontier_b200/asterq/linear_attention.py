@@ -1,13 +1,15 @@
-"""Linear attention with a decay for each head: the recurrent layers beside the latent ones.
+"""Linear attention with a decay for each head: recurrent layers beside the latent ones.
 
-Three of four layers of a hybrid model keep a fixed-size state instead of a cache
-(``AsterCache.kda_states`` holds the reference's).  Here a layer's states are a pool by sequence
+Such a layer keeps a fixed-size state instead of a cache.  Here a layer's states are a pool by sequence
 slot, float32 [n_slots, n_heads, dk, dv], updated in place:
 
     S_t = exp(g_t) S_{t-1} + k_t v_t^T,   out_t = scale q_t S_t
 
 * ``linear_attention_prefill``: ragged prompt chunks, rows ``row_offsets[s]`` and on for sequence s;
 * ``linear_attention_step``: one new token a sequence.
+
+This is the plain recurrence.  The reference's KDA layers, whose states ``AsterCache.kda_states`` holds, update
+theirs by a gated delta rule (a correction by what the state has for the key already): not served here.
 
 There is no backward pass: inputs that require a gradient are refused outside of ``torch.no_grad()``.
 Both call ``asterq_linear_attention``; nothing waits for the GPU or reads from it, so calls can be
@@ -158,9 +160,14 @@ def linear_attention_prefill(
     stride.  log_decay float32 [n_heads] or [rows, n_heads], not above 0.  scale: 1 / sqrt(dk) unless
     given.  status int32 [1]: set to 1 when a slot or row offset was out of range, or offsets decreased.
 
-    bf16 prompts run in chunks of 128 tokens on the tensor cores where ``out`` and ``state`` are 32-byte aligned
-    and no stride is 0, other types and short prompts token by token.  A value of v that is not finite reaches its
-    column of the state and of the outputs from its row on, where an infinity may become NaN, and nothing else.
+    bf16 prompts run in chunks of 128 tokens on the tensor cores where ``out`` and ``state`` are 32-byte aligned,
+    no stride is 0 and there are 24 rows a slot or more on average, other types and shorter prompts token by token:
+    pass the slots that have rows, not idle ones beside them, and long prompts apart from single rows.
+
+    What is not finite reaches what the recurrence takes it to, and nothing else: a value of v its column of the state
+    and of the outputs from its row on; of k its row of the state and the outputs from its row on; of q its row's
+    outputs; of a state its column's outputs.  An infinity may become NaN on the way.  Rows of no sequence are not
+    written.
     """
     return _run(state, slots, lengths, row_offsets, q, k, v, log_decay, scale, out, workspace, status)
 

@@ -6,7 +6,7 @@
 // in pairs (x, y): x' = x c - y s, y' = y c + x s with c = cos[p][j], s = sin[p][j], computed in
 // fp32 and rounded once; pair j is dims (j, j + rotary_dim / 2), or (2j, 2j + 1) interleaved.
 //
-// Measured: 16411 prompt rows of 32 query and 2 x 8 kv heads of 128 dims in 73 us, 5.6 TB/s; 256 single tokens 4.0 us
+// Measured: 16411 prompt rows of 32 query and 2 x 8 kv heads of 128 dims in 72 us, 5.7 TB/s; 256 single tokens 3.9 us
 // and 8 of them 3.0, which is the latency of a launch and four dependent loads.
 #include "asterq_internal.h"
 #include "common.cuh"

@@ -156,7 +156,9 @@ static int sm_count(int* device) {
 // dims, chunked against the scan: one sequence of 16 heads, 24 tokens 14.2 against 12.5 us, 32 tokens 14.4
 // against 15.8, 128 tokens 16.5 against 57; 4 of 32 heads, 24 tokens 15.0 against 22.8; 64 of 64 heads, 24 tokens
 // 232 against 451, 128 tokens 296 against 2147.  At 64 x 64 dims: one sequence of 16 heads, 24 tokens 9.8
-// against 12.6; 64 of 64 heads, 24 tokens 130 against 155, 128 tokens 135 against 753.
+// against 12.6; 64 of 64 heads, 24 tokens 130 against 155, 128 tokens 135 against 753.  These are sequences of one
+// length, and the host sees no other: a long prompt among many idle slots or single rows has a small average and goes
+// token by token, where it would take a fraction of the time by itself.
 static bool in_chunks(const asterq_linear_params* p) {
   return p->dtype == ASTERQ_DTYPE_BF16 && p->row_offsets && p->n_rows >= 24ll * p->n_seqs;
 }

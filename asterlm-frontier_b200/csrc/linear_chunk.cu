@@ -8,10 +8,11 @@
 // once (128 KB a chunk and head).  At one head-chunk a CTA, an SM's share of the memory bandwidth
 // takes 5,700 cycles for them; the products below take 4,600 on the tensor core.
 //
-// Measured (128 x 128 dims): 32777 tokens of 12 sequences and 32 heads 430 us, 2.6 TB/s (the bytes alone: 170 us).
+// Measured (128 x 128 dims): 32777 tokens of 12 sequences and 32 heads 425 us, 2.6 TB/s (the bytes alone: 170 us); call
+// after call its power takes the clock from 1965 to some 1650 MHz, and the time, which is all cycles, goes to 480 us.
 // A CTA's 56 chunks take some 9,400 cycles each: the warp that issues the products is busy for 5,500 of them and
 // goes from one role's barrier to the next for the rest, since a chunk's state, its outputs and the next
-// chunk's keys wait for one another.  8192 tokens of one sequence and 16 heads: 93 us, some 35 of them the first pass
+// chunk's keys wait for one another.  8192 tokens of one sequence and 16 heads: 94 us, some 35 of them the first pass
 // and the chain of states.  One chunk of 16 heads: 15 us, a launch and the latency of one chunk.
 //
 // Rounding.  Products take bf16 operands and sum in fp32.  A and S enter as two bf16 parts (16 bits:

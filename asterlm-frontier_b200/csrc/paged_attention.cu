@@ -19,11 +19,11 @@
 // the order of the shares, so results do not depend on which CTA came last; of many records groups are
 // joined first, each by the CTA that stores its last one.  No CTA waits for another.
 //
-// Measured (bf16, 128 dims, 8 kv heads, pages of 64): 64 sequences of 1k to 32k tokens 360 us, 6.7 TB/s of keys
+// Measured (bf16, 128 dims, 8 kv heads, pages of 64): 64 sequences of 1k to 32k tokens 362 us, 6.6 TB/s of keys
 // and values.  One sequence of 8192 tokens of 4 kv heads takes 12.8 us, of which the bytes are 2.6: launch, lengths,
 // table, first tiles (5 us), the warps' join (1.2), records and their count (1.5) and the join of 37 pieces a head
-// (3) are chains of latencies.  256 sequences of at most 512 visible tokens, 16 kv heads of 64: 89 us against
-// 25 of bytes, since a unit of six tiles keeps a team's warps busy for 1,400 cycles a tile and 1,700 more.
+// (3) are chains of latencies.  256 sequences of at most 512 visible tokens, 16 kv heads of 64, with a softcap: 93 us
+// against 25 of bytes, since a unit of six tiles keeps a team's warps busy for some 1,450 cycles a tile and 1,700 more.
 #include <cuda.h>
 
 #include "asterq_internal.h"
@@ -72,10 +72,10 @@ struct Cfg {
   static_assert(D / kSlice % 2 == 0, "the two buffers alternate across units that the same warps join");
   static_assert(kMergeFloats >= 48 * NR, "weights of the records that are joined at once");
   // kUnitCost: what a unit costs beside its tiles, in tiles.  Measured with 0, 1 and 2: 64 rows of 1 to 2048 tokens,
-  // 8 kv heads of 128, 38.1, 29.5 and 27.3 us; of 1 to 512 tokens 20.7, 19.6 and 20.8; of 1k to 32k tokens 368, 366 and
-  // 368; 256 rows of at most 512 visible tokens, 16 kv heads of 64, 100, 90 and 99.
-  // kSoloTiles: units up to this long are taken by one team.  Measured with 0, 4 and 8: the same four 34.5, 29.5 and
-  // 29.4 us; 21.6, 19.6 and 21.2; 365, 366 and 366; 101, 90 and 90.
+  // 8 kv heads of 128, 39.2, 30.1 and 27.9 us; of 1 to 512 tokens 20.3, 19.9 and 20.7; of 1k to 32k tokens 366, 364 and
+  // 362; 256 rows of at most 512 visible tokens, 16 kv heads of 64, 111, 93 and 103.
+  // kSoloTiles: units up to this long are taken by one team.  Measured with 0, 4 and 8: the same four 34.7, 30.1 and
+  // 30.1 us; 21.0, 19.9 and 20.7; 364, 364 and 364; 108, 93 and 92.
   static constexpr int kUnitCost = 1;
   static constexpr int kSoloTiles = 4;
   static constexpr int kSmem =

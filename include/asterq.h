@@ -451,8 +451,9 @@ int asterq_kv_append(const asterq_kv_append_params* p, void* stream);
  * head_dim 64, 128 or 256; page_tokens a multiple of 16.
  *
  * workspace: asterq_paged_attention_workspace_bytes bytes, zeroed once before its first use; every
- * call leaves it ready for the next one on the same stream.  Calls that overlap on the GPU need a
- * workspace each.  A workspace serves calls of any shape that need no more bytes than it has.
+ * call leaves it ready for the next one on the same stream (but after *status 2, a wait that ran out,
+ * it has to be zeroed again).  Calls that overlap on the GPU need a workspace each.  A workspace serves
+ * calls of any shape that need no more bytes than it has.
  */
 typedef struct asterq_paged_attention_params {
   int32_t dtype;     /* of q and the pools: ASTERQ_DTYPE_BF16 or ASTERQ_DTYPE_F16 */
@@ -496,12 +497,13 @@ int asterq_paged_attention(const asterq_paged_attention_params* p, void* stream)
  * lengths[s] <= 0 start from a state of zeros, whatever their slot holds.  A slot below 0 is an empty
  * one: its rows are written as zeros; one at or above n_slots is taken the same way and sets *status
  * to 1, and so do row offsets outside [0, n_rows], whose sequence is left out, and offsets that decrease,
- * which leave out that sequence or the whole call.  Sequences of a call have slots of their own.  A value of v that is not finite reaches its column of the state, and of the outputs
- * from its row on (where an infinity may become NaN), and nothing else.
+ * which leave out that sequence or the whole call.  Sequences of a call have slots of their own.  What is not finite reaches what the recurrence takes it to and nothing else (an infinity may
+ * become NaN): of v its column of the state and of the outputs from its row on, of k its row of the state and the outputs
+ * from its row on, of q its row's outputs.
  * dk, dv: 64 or 128.  q, k, v, out of one type: bf16, f16 or f32.
  * workspace: asterq_linear_workspace_bytes bytes (0: none needed), not kept between calls; calls that
- * overlap on the GPU need one each.  bf16 prompts run in chunks where state, out and workspace are 32-byte aligned
- * and strides are positive, and token by token otherwise.
+ * overlap on the GPU need one each.  bf16 prompts of 24 rows a sequence or more on average run in chunks where state, out
+ * and workspace are 32-byte aligned and strides are positive, and token by token otherwise.
  */
 typedef struct asterq_linear_params {
   int32_t dtype;
