@@ -14,7 +14,8 @@ theirs by a gated delta rule (a correction by what the state has for the key alr
 There is no backward pass: inputs that require a gradient are refused outside of ``torch.no_grad()``.
 Both call ``asterq_linear_attention``; nothing waits for the GPU or reads from it, so calls can be
 recorded in a CUDA graph.  A first prompt call on a stream, or ``workspace``, gives that stream's prompts
-their workspace; a captured prompt without either has one in the graph's memory.
+their workspace; a captured prompt without either has one in the graph's memory.  Graphs that overlap each
+other, or other prompts of the stream that they were captured on, need a ``workspace`` each.
 """
 from __future__ import annotations
 

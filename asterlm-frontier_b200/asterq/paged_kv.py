@@ -14,7 +14,8 @@ the GPU:
 There is no backward pass: inputs that require a gradient are refused outside of ``torch.no_grad()``.
 Nothing here waits for the GPU or reads from it, so all of it can be recorded in a CUDA graph.  A first
 call on a stream, or ``workspace``, gives that stream's calls their workspace; a captured ``paged_attention``
-without either has one of its own, zeroed at every replay (5 MB).
+without either has one of its own, zeroed at every replay (5 MB).  A captured call keeps its workspace wherever
+its graph is replayed: graphs that overlap each other, or other calls of the stream, need one each.
 """
 from __future__ import annotations
 
