@@ -42,38 +42,38 @@ def _package():
 def listed():
     return [
         # the drafted tree of a few interactive requests: eight nodes each, where the launch is what counts
-        dict(name="append, 4 trees of 8", op="append", seqs=4, tokens=32, tree=True, context=1500, heads=16, kv_heads=4,
+        dict(name="append 4 trees of 8", op="append", seqs=4, tokens=32, tree=True, context=1500, heads=16, kv_heads=4,
              head_dim=128, rotary_dim=128, interleaved=False, dtype="bf16", page_tokens=64),
         # prompt chunks of a few requests admitted together, ragged, on top of what they have cached
-        dict(name="append, ragged prompts", op="append", seqs=11, tokens=16387, tree=False, context=2048, heads=32,
+        dict(name="append ragged prompts", op="append", seqs=11, tokens=16387, tree=False, context=2048, heads=32,
              kv_heads=8, head_dim=128, rotary_dim=64, interleaved=True, dtype="f16", page_tokens=64),
         # a short follow-up question in a chat: few rows over a cached conversation
-        dict(name="prompt, one of 150", op="prompt", seqs=1, tokens=150, min_context=1111, max_context=1111, heads=16,
+        dict(name="prompt one of 150", op="prompt", seqs=1, tokens=150, min_context=1111, max_context=1111, heads=16,
              kv_heads=4, head_dim=128, dtype="bf16", page_tokens=64, window=0, sink=0, softcap=0.0),
         # prompts admitted together, ragged, in a layer with a sliding window whose first tokens stay visible
-        dict(name="prompt, 9 ragged, window", op="prompt", seqs=9, tokens=16393, min_context=0, max_context=4096,
+        dict(name="prompt 9 ragged with window", op="prompt", seqs=9, tokens=16393, min_context=0, max_context=4096,
              heads=16, kv_heads=8, head_dim=64, dtype="f16", page_tokens=16, window=1024, sink=4, softcap=0.0),
         # a chunk of a long document over what is cached of it: the matrix products' case
-        dict(name="prompt, 8192 over 24576", op="prompt", seqs=1, tokens=8192, min_context=24576, max_context=24576,
+        dict(name="prompt 8192 over 24576", op="prompt", seqs=1, tokens=8192, min_context=24576, max_context=24576,
              heads=32, kv_heads=8, head_dim=128, dtype="bf16", page_tokens=512, window=0, sink=0, softcap=0.0),
         # the drafted tree of one interactive request: latency, the cache split over all SMs
-        dict(name="tree, one of 8", op="tree", seqs=1, nodes=8, min_context=2011, max_context=2011, heads=16, kv_heads=4,
+        dict(name="tree one of 8", op="tree", seqs=1, nodes=8, min_context=2011, max_context=2011, heads=16, kv_heads=4,
              head_dim=128, dtype="bf16", page_tokens=64, window=0, sink=0, softcap=0.0),
         # an ordinary batch with trees of 16 nodes
-        dict(name="tree, 32 of 16", op="tree", seqs=32, nodes=16, min_context=500, max_context=8192, heads=32,
+        dict(name="tree 32 of 16", op="tree", seqs=32, nodes=16, min_context=500, max_context=8192, heads=32,
              kv_heads=8, head_dim=128, dtype="bf16", page_tokens=64, window=0, sink=0, softcap=0.0),
         # wide trees over long contexts, sixteen query heads for each key/value head
-        dict(name="tree, 24 of 61, long", op="tree", seqs=24, nodes=61, min_context=2048, max_context=32768, heads=32,
+        dict(name="tree 24 of 61 long", op="tree", seqs=24, nodes=61, min_context=2048, max_context=32768, heads=32,
              kv_heads=2, head_dim=128, dtype="f16", page_tokens=128, window=0, sink=0, softcap=0.0),
         # a chain of drafted tokens of a few requests, drafted greedily (no probabilities of the drafts)
-        dict(name="verify, 4 chains of 6", op="verify", seqs=4, nodes=6, tree=False, vocab=32000, drafted=False),
+        dict(name="verify 4 chains of 6", op="verify", seqs=4, nodes=6, tree=False, vocab=32000, drafted=False),
         # a full batch of drafted trees with the draft's probabilities, a large vocabulary
-        dict(name="verify, 96 trees of 12", op="verify", seqs=96, nodes=12, tree=True, vocab=128256, drafted=True),
+        dict(name="verify 96 trees of 12", op="verify", seqs=96, nodes=12, tree=True, vocab=128256, drafted=True),
         # a batch's accepted paths closed up behind their contexts, in all layers
-        dict(name="pages, keep of 48 trees", op="pages", kind="keep", layers=16, seqs=48, nodes=32, context=300,
+        dict(name="pages keep of 48 trees", op="pages", kind="keep", layers=16, seqs=48, nodes=32, context=300,
              kv_heads=8, head_dim=128, dtype="bf16", page_tokens=64),
         # pages copied where forked sequences part, in all layers
-        dict(name="pages, copy of 60", op="pages", kind="copy", layers=24, pages=200, pairs=60, kv_heads=8, head_dim=128,
+        dict(name="pages copy of 60", op="pages", kind="copy", layers=24, pages=200, pairs=60, kv_heads=8, head_dim=128,
              dtype="f16", page_tokens=64),
     ]
 
