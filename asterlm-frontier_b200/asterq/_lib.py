@@ -75,6 +75,8 @@ EXPORTED_SYMBOLS = (
     "asterq_kv_append",
     "asterq_paged_attention_workspace_bytes",
     "asterq_paged_attention",
+    "asterq_rows_attention_workspace_bytes",
+    "asterq_rows_attention",
     "asterq_linear_workspace_bytes",
     "asterq_linear_attention",
 )
@@ -240,6 +242,41 @@ class PagedAttentionParams(ctypes.Structure):
     ]
 
 
+class RowsAttentionParams(ctypes.Structure):
+    """Mirror of ``asterq_rows_attention_params``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("n_seqs", ctypes.c_int32),
+        ("n_heads", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_tokens", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("sink", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float),
+        ("logit_softcap", ctypes.c_float),
+        ("n_rows", ctypes.c_int64),
+        ("n_pages", ctypes.c_int64),
+        ("q_row_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("q", ctypes.c_void_p),
+        ("k_pool", ctypes.c_void_p),
+        ("v_pool", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("row_offsets", ctypes.c_void_p),
+        ("parents", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("status", ctypes.c_void_p),
+    ]
+
+
 class LinearParams(ctypes.Structure):
     """Mirror of ``asterq_linear_params``."""
 
@@ -385,6 +422,10 @@ def load() -> ctypes.CDLL:
     lib.asterq_paged_attention_workspace_bytes.argtypes = [vp]
     lib.asterq_paged_attention.restype = ctypes.c_int
     lib.asterq_paged_attention.argtypes = [vp, vp]
+    lib.asterq_rows_attention_workspace_bytes.restype = i64
+    lib.asterq_rows_attention_workspace_bytes.argtypes = [vp]
+    lib.asterq_rows_attention.restype = ctypes.c_int
+    lib.asterq_rows_attention.argtypes = [vp, vp]
     lib.asterq_linear_workspace_bytes.restype = i64
     lib.asterq_linear_workspace_bytes.argtypes = [vp]
     lib.asterq_linear_attention.restype = ctypes.c_int

@@ -31,6 +31,7 @@ from .batch import _PagePool
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 _APPEND = _lib.packer(_lib.KvAppendParams)
 _ATTEND = _lib.packer(_lib.PagedAttentionParams)
+_ROWS = _lib.packer(_lib.RowsAttentionParams)
 ATTENTION_HEAD_DIMS = (64, 128, 256)
 
 
@@ -304,6 +305,149 @@ def paged_attention(
                        ws.buffer.data_ptr(), ws.nbytes, 0 if status is None else status.data_ptr()),
           device, stream)
     return (out, lse) if return_lse else out
+
+
+class RowsAttentionWorkspace:
+    """Device memory in which ``paged_prompt_attention`` and ``paged_tree_attention`` join the pieces of work that
+    several SMs share (some 40 MB); its contents are of one call.  One serves any sequence of calls on one stream;
+    calls that overlap on the GPU need one each."""
+
+    def __init__(self, device="cuda") -> None:
+        device = torch.device(device)
+        p = _lib.RowsAttentionParams()
+        p.dtype = p.out_dtype = _lib.DTYPE_BF16
+        p.n_heads, p.n_kv_heads, p.page_tokens = 1, 1, 16
+        with torch.cuda.device(device):
+            self.nbytes = 0
+            for p.head_dim in ATTENTION_HEAD_DIMS:
+                self.nbytes = max(self.nbytes, int(_lib.load().asterq_rows_attention_workspace_bytes(_lib.ctypes.byref(p))))
+            self.buffer = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
+
+
+_rows_workspaces: dict[tuple[int, int], RowsAttentionWorkspace] = {}
+
+
+def _rows_workspace(device: torch.device, stream: int) -> RowsAttentionWorkspace:
+    ws = _rows_workspaces.get((device.index, stream))
+    if ws is None:
+        ws = RowsAttentionWorkspace(device)
+        if not _capturing(device):  # in a capture it is of the graph's own memory, and not for any call but this one
+            _rows_workspaces[(device.index, stream)] = ws
+    return ws
+
+
+def _rows_attention(pools, page_table, lengths, row_offsets, parents, q, softmax_scale, logit_softcap, window_size,
+                    sink_tokens, out, return_lse, workspace, status):
+    if q.dim() != 3 or page_table.dim() != 2 or row_offsets.dim() != 1:
+        raise ValueError("q must be [rows, n_heads, head_dim], page_table [n_seqs, max_pages], row_offsets [n_seqs + 1]")
+    n_pages, n_kv, page, dim = pools.k.shape
+    q = _check_rows(q, "q", pools.k, None, dim)
+    if min(q.stride()) <= 0 and q.numel():
+        q = q.clone(memory_format=torch.contiguous_format)  # heads or rows that repeat
+    rows, heads, _ = q.shape
+    if heads == 0 or heads % n_kv:
+        raise ValueError(f"{heads} query heads over {n_kv} kv heads")
+    n_seqs, max_pages = page_table.shape
+    _check_int(page_table, "page_table", (n_seqs, max_pages), pools.k)
+    _check_int(lengths, "lengths", (n_seqs,), pools.k)
+    _check_int(row_offsets, "row_offsets", (n_seqs + 1,), pools.k)
+    if parents is not None:
+        _check_int(parents, "parents", (rows,), pools.k)
+    if status is not None:
+        _check_int(status, "status", (1,), pools.k)
+    if sink_tokens < 0:
+        raise ValueError("sink_tokens must not be negative")
+    if window_size is not None and window_size <= 0:
+        raise ValueError("window_size must be positive")
+    dtype = _DTYPES[q.dtype]
+    out_dtype = dtype
+    if out is None:
+        out = torch.empty((rows, heads, dim), dtype=q.dtype, device=q.device)
+    else:
+        if out.shape != q.shape or out.device != q.device or not out.is_contiguous():
+            raise ValueError("out must be a contiguous tensor of q's shape")
+        _check_no_gradient(out, "out")
+        out_dtype = _lib.DTYPE_F32 if out.dtype == torch.float32 else _DTYPES.get(out.dtype, -1)
+    lse = torch.empty((rows, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    device = q.device
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if rows and n_seqs:
+        ws = _rows_workspace(device, stream) if workspace is None else workspace
+        q_row, q_head, _ = q.stride()
+        _call(_lib.load().asterq_rows_attention,
+              _ROWS.pack(dtype, out_dtype, n_seqs, heads, n_kv, dim, page, max_pages, window_size or 0, sink_tokens,
+                         1.0 / math.sqrt(dim) if softmax_scale is None else softmax_scale, logit_softcap or 0.0, rows,
+                         n_pages, q_row, q_head, q.data_ptr(), pools.k.data_ptr(), pools.v.data_ptr(),
+                         page_table.data_ptr(), lengths.data_ptr(), row_offsets.data_ptr(),
+                         0 if parents is None else parents.data_ptr(), out.data_ptr(),
+                         0 if lse is None else lse.data_ptr(), ws.buffer.data_ptr(), ws.nbytes,
+                         0 if status is None else status.data_ptr()),
+              device, stream)
+    return (out, lse) if return_lse else out
+
+
+def paged_prompt_attention(
+    pools: PagedKVPools,
+    page_table: torch.Tensor,
+    lengths: torch.Tensor,
+    row_offsets: torch.Tensor,
+    q: torch.Tensor,
+    *,
+    softmax_scale: float | None = None,
+    logit_softcap: float | None = None,
+    window_size: int | None = None,
+    sink_tokens: int = 0,
+    out: torch.Tensor | None = None,
+    return_lse: bool = False,
+    workspace: RowsAttentionWorkspace | None = None,
+    status: torch.Tensor | None = None,
+):
+    """Attention of prompt chunks over their pages: out [rows, n_heads, head_dim], and with ``return_lse`` the scores'
+    log-sum-exp, float32 [rows, n_heads], beside it.
+
+    Rows ``row_offsets[s]`` .. ``row_offsets[s + 1]`` of q [rows, n_heads, head_dim] (any row and head stride) are
+    sequence s's new tokens, whose keys and values ``append_kv`` has written and ``lengths`` does not count yet: token i
+    has position ``lengths[s] + i`` and sees the positions up to its own.  With ``window_size`` it sees, of these, the
+    first ``sink_tokens`` and the newest ``window_size - sink_tokens``.  Other arguments, types and values that are not
+    finite as for ``paged_attention``, but weights enter their product rounded once to the pools' type, so that
+    outputs are good to that rounding of the values, also float32 ones.  Rows of empty slots get zeros and a log-sum-exp
+    of -inf; rows of no sequence are not written.  status int32 [1]: set to 1 when a needed page id was outside the pool,
+    a row's place behind the table (it gets zeros), or offsets are out of order (nothing is written then).
+    """
+    return _rows_attention(pools, page_table, lengths, row_offsets, None, q, softmax_scale, logit_softcap, window_size,
+                           sink_tokens, out, return_lse, workspace, status)
+
+
+def paged_tree_attention(
+    pools: PagedKVPools,
+    page_table: torch.Tensor,
+    lengths: torch.Tensor,
+    row_offsets: torch.Tensor,
+    parents: torch.Tensor,
+    q: torch.Tensor,
+    *,
+    softmax_scale: float | None = None,
+    logit_softcap: float | None = None,
+    window_size: int | None = None,
+    sink_tokens: int = 0,
+    out: torch.Tensor | None = None,
+    return_lse: bool = False,
+    workspace: RowsAttentionWorkspace | None = None,
+    status: torch.Tensor | None = None,
+):
+    """Attention of trees of drafted tokens over their pages, one tree a sequence of at most 128 nodes.
+
+    parents int32 [rows]: the parent of each row among its sequence's rows (0: the first), before it, or -1 for a
+    root.  A node sees the sequence's ``lengths[s]`` cached tokens, its ancestors and itself, and with a window of these
+    the ones that the window of its position ``lengths[s] + depth`` shows.  Node i's key and value are at place
+    ``lengths[s] + i`` of the pages (``append_kv`` with ``positions`` puts them there).  A parent out of range is taken as -1
+    and sets ``status``; a tree of more nodes leaves the call undone with ``status`` 1.  Other arguments as for
+    ``paged_prompt_attention``.
+    """
+    if parents is None:
+        raise ValueError("parents must be int32 [rows]")
+    return _rows_attention(pools, page_table, lengths, row_offsets, parents, q, softmax_scale, logit_softcap, window_size,
+                           sink_tokens, out, return_lse, workspace, status)
 
 
 class PagedKVBatch:

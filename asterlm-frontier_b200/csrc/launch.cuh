@@ -1,0 +1,47 @@
+// What the launches of the paged layers' kernels share on the host.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "asterq_internal.h"
+
+namespace asterq {
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// cuTensorMapEncodeTiled, without linking to the driver's library; null where it is not there
+inline EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+                   q == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<EncodeTiled>(ptr)
+               : nullptr;
+  }();
+  return fn;
+}
+
+// A map of 16-bit values in boxes of 64 of the first dim (128 bytes, swizzled); strides in bytes, of the dims from the
+// second on.
+inline bool map_of_16bit(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                         const cuuint32_t* box) {
+  const cuuint32_t step[5] = {1u, 1u, 1u, 1u, 1u};
+  const EncodeTiled fn = encode_tiled();
+  return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, rank, const_cast<void*>(base), dims, strides, box, step,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// SMs of the current device and its ordinal; 0 where there is none
+inline int current_sms(int* dev) {
+  int n = 0;
+  if (cudaGetDevice(dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, *dev) != cudaSuccess)
+    return 0;
+  return n;
+}
+
+}  // namespace asterq

@@ -488,6 +488,59 @@ int64_t asterq_paged_attention_workspace_bytes(const asterq_paged_attention_para
 int asterq_paged_attention(const asterq_paged_attention_params* p, void* stream);
 
 /*
+ * Attention of many new tokens a sequence over such a cache, whose keys and values asterq_kv_append has put in their pages
+ * (`lengths` not advanced yet): rows row_offsets[s] .. row_offsets[s + 1] - 1 of q and out are sequence s's tokens,
+ * row i of them at place lengths[s] + i of its pages.
+ *   out[i][h] = sum over visible j of softmax(score) v_j,  score = softmax_scale q[i][h] . k_j  (softcapped as above)
+ * parents NULL: prompts.  Token i has position p = lengths[s] + i and sees the keys j <= p with j < min(sink, window)
+ * or j > p - (window - min(sink, window)); all j <= p without a window.
+ * parents int32 [n_rows]: trees of drafted tokens.  parents[r] is the parent of row r among its sequence's rows (0 is the
+ * first), below the row's own number, or -1 for a root.  A node sees the cached tokens, its ancestors and
+ * itself; with a window by position, which is lengths[s] + depth for a node.  At most 128 nodes a sequence.  A parent out of
+ * this range is taken as -1 and sets *status to 1.
+ * Rows of an empty slot (lengths[s] < 0) get zeros and a log-sum of -inf, and so do rows whose place is behind the table's
+ * row (these with *status 1); rows of no sequence are not written.  Offsets that decrease or leave [0, n_rows], and trees of
+ * too many nodes, leave the whole call undone with *status 1.
+ * Weights enter their product rounded once to dtype, softmax statistics and sums are fp32.  Infinities and NaN in keys and
+ * values that a row does not see have no part in it; those it sees reach it as for asterq_paged_attention.
+ * head_dim 64, 128 or 256; at most 128 query heads a kv head; page_tokens a multiple of 16; positive strides of q.
+ * workspace: asterq_rows_attention_workspace_bytes bytes, of any content, used within the call; calls that overlap on the
+ * GPU need one each.
+ */
+typedef struct asterq_rows_attention_params {
+  int32_t dtype;     /* of q and the pools: ASTERQ_DTYPE_BF16 or ASTERQ_DTYPE_F16 */
+  int32_t out_dtype; /* the same or ASTERQ_DTYPE_F32 */
+  int32_t n_seqs;
+  int32_t n_heads;
+  int32_t n_kv_heads;
+  int32_t head_dim;
+  int32_t page_tokens;
+  int32_t max_pages;
+  int32_t window; /* 0: none */
+  int32_t sink;
+  float softmax_scale;
+  float logit_softcap; /* <= 0: off */
+  int64_t n_rows;
+  int64_t n_pages;
+  int64_t q_row_stride, q_head_stride; /* in elements, multiples of 8; a head's dims are contiguous */
+  const void* q;
+  const void* k_pool;
+  const void* v_pool;
+  const int32_t* page_table;
+  const int32_t* lengths;
+  const int32_t* row_offsets; /* [n_seqs + 1], not decreasing */
+  const int32_t* parents;     /* [n_rows] or NULL */
+  void* out;                  /* [n_rows][n_heads][head_dim] */
+  float* lse;                 /* [n_rows][n_heads] or NULL */
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* status; /* may be NULL */
+} asterq_rows_attention_params;
+
+int64_t asterq_rows_attention_workspace_bytes(const asterq_rows_attention_params* p);
+int asterq_rows_attention(const asterq_rows_attention_params* p, void* stream);
+
+/*
  * Linear attention with a decay for each head: the recurrent layers beside the latent ones.  Each
  * (slot, head) has a state S fp32 [dk][dv] in `state` [n_slots][n_heads][dk][dv], updated in place:
  *   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   out_t = scale q_t S_t
