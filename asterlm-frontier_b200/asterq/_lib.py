@@ -77,6 +77,10 @@ EXPORTED_SYMBOLS = (
     "asterq_paged_attention",
     "asterq_rows_attention_workspace_bytes",
     "asterq_rows_attention",
+    "asterq_kv_append_normed",
+    "asterq_kv_keep",
+    "asterq_kv_copy_pages",
+    "asterq_verify_drafts",
     "asterq_linear_workspace_bytes",
     "asterq_linear_attention",
 )
@@ -277,6 +281,117 @@ class RowsAttentionParams(ctypes.Structure):
     ]
 
 
+class KvAppendNormedParams(ctypes.Structure):
+    """Mirror of ``asterq_kv_append_normed_params``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("norm_dtype", ctypes.c_int32),
+        ("n_seqs", ctypes.c_int32),
+        ("n_heads", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("page_tokens", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("norm_eps", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("n_rows", ctypes.c_int64),
+        ("n_pages", ctypes.c_int64),
+        ("n_positions", ctypes.c_int64),
+        ("q_row_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("k_row_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("v_row_stride", ctypes.c_int64),
+        ("v_head_stride", ctypes.c_int64),
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("q_norm", ctypes.c_void_p),
+        ("k_norm", ctypes.c_void_p),
+        ("cos", ctypes.c_void_p),
+        ("sin", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("row_offsets", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("k_pool", ctypes.c_void_p),
+        ("v_pool", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class KvKeepParams(ctypes.Structure):
+    """Mirror of ``asterq_kv_keep_params``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("n_layers", ctypes.c_int32),
+        ("n_seqs", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_tokens", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("n_rows", ctypes.c_int64),
+        ("n_pages", ctypes.c_int64),
+        ("k_pools", ctypes.c_void_p),
+        ("v_pools", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("row_offsets", ctypes.c_void_p),
+        ("kept", ctypes.c_void_p),
+        ("n_kept", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class KvCopyParams(ctypes.Structure):
+    """Mirror of ``asterq_kv_copy_params``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("n_layers", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_tokens", ctypes.c_int32),
+        ("n_pairs", ctypes.c_int32),
+        ("n_pages", ctypes.c_int64),
+        ("k_pools", ctypes.c_void_p),
+        ("v_pools", ctypes.c_void_p),
+        ("pairs", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class VerifyParams(ctypes.Structure):
+    """Mirror of ``asterq_verify_params``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("n_seqs", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("n_rows", ctypes.c_int64),
+        ("target_stride", ctypes.c_int64),
+        ("draft_stride", ctypes.c_int64),
+        ("target", ctypes.c_void_p),
+        ("draft", ctypes.c_void_p),
+        ("tokens", ctypes.c_void_p),
+        ("parents", ctypes.c_void_p),
+        ("row_offsets", ctypes.c_void_p),
+        ("accept", ctypes.c_void_p),
+        ("sample", ctypes.c_void_p),
+        ("kept", ctypes.c_void_p),
+        ("n_kept", ctypes.c_void_p),
+        ("next_token", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
 class LinearParams(ctypes.Structure):
     """Mirror of ``asterq_linear_params``."""
 
@@ -426,6 +541,9 @@ def load() -> ctypes.CDLL:
     lib.asterq_rows_attention_workspace_bytes.argtypes = [vp]
     lib.asterq_rows_attention.restype = ctypes.c_int
     lib.asterq_rows_attention.argtypes = [vp, vp]
+    for name in ("asterq_kv_append_normed", "asterq_kv_keep", "asterq_kv_copy_pages", "asterq_verify_drafts"):
+        getattr(lib, name).restype = ctypes.c_int
+        getattr(lib, name).argtypes = [vp, vp]
     lib.asterq_linear_workspace_bytes.restype = i64
     lib.asterq_linear_workspace_bytes.argtypes = [vp]
     lib.asterq_linear_attention.restype = ctypes.c_int

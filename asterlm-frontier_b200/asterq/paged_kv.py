@@ -32,7 +32,11 @@ _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 _APPEND = _lib.packer(_lib.KvAppendParams)
 _ATTEND = _lib.packer(_lib.PagedAttentionParams)
 _ROWS = _lib.packer(_lib.RowsAttentionParams)
+_NORMED = _lib.packer(_lib.KvAppendNormedParams)
+_KEEP = _lib.packer(_lib.KvKeepParams)
+_COPY = _lib.packer(_lib.KvCopyParams)
 ATTENTION_HEAD_DIMS = (64, 128, 256)
+MAX_TREE_NODES = 128
 
 
 _quick_module = 0  # not looked for yet
@@ -159,6 +163,10 @@ def append_kv(
     sin: torch.Tensor | None = None,
     interleaved: bool = False,
     q_out: torch.Tensor | None = None,
+    q_norm: torch.Tensor | None = None,
+    k_norm: torch.Tensor | None = None,
+    norm_eps: float = 1e-6,
+    positions: torch.Tensor | None = None,
     status: torch.Tensor | None = None,
 ) -> torch.Tensor | None:
     """Write new keys and values behind each sequence's cached tokens; returns the rotated queries.
@@ -173,9 +181,13 @@ def append_kv(
     are copied as they are.  q [rows, n_heads, head_dim] comes back rotated as a contiguous tensor
     (``q_out``, not overlapping q, if given); rows left out leave it unwritten.  status int32 [1]: set to
     1 when a row had no page in the table or no row in cos / sin and was left out.
+
+    q_norm, k_norm [head_dim], float32 or the pools' type: each head x of q or k becomes x / sqrt(mean(x^2) + ``norm_eps``)
+    times the weight before it turns, in float32.  positions int32 [rows]: the rows of cos and sin, where a row's position
+    is not its place behind the cached tokens (a drafted node's is ``lengths[s]`` and its depth).
     """
     quick = _quick()
-    if quick is not None:
+    if quick is not None and q_norm is None and k_norm is None and positions is None:
         done = quick.append(pools.k, pools.v, page_table, lengths, row_offsets, k, v, q, cos, sin, interleaved, q_out, status)
         if done is not NotImplemented:
             return done
@@ -208,7 +220,7 @@ def append_kv(
         q_row, q_head, _ = q.stride()
     elif q_out is not None:
         raise ValueError("q_out without q")
-    rotary = positions = 0
+    rotary = positions_n = 0
     cos_ptr = sin_ptr = None
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together")
@@ -217,14 +229,44 @@ def append_kv(
             raise ValueError("cos and sin must be contiguous [positions, rotary_dim / 2]")
         if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.device != k.device or sin.device != k.device:
             raise TypeError("cos and sin must be float32 on the pools' device")
-        positions, rotary = cos.shape[0], 2 * cos.shape[1]
+        positions_n, rotary = cos.shape[0], 2 * cos.shape[1]
         cos_ptr, sin_ptr = cos.data_ptr(), sin.data_ptr()
     k_row, k_head, _ = k.stride()
     v_row, v_head, _ = v.stride()
     device = pools.k.device
+    if q_norm is not None or k_norm is not None or positions is not None:
+        norm_dtype = _DTYPES[k.dtype]
+        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+            if w is None:
+                continue
+            if w.shape != (dim,) or not w.is_contiguous() or w.device != device:
+                raise ValueError(f"{name} must be a contiguous tensor ({dim},) on {device}")
+            if w.dtype != torch.float32 and w.dtype != k.dtype:
+                raise TypeError(f"{name} is {w.dtype}: float32 or the pools' type")
+            _check_no_gradient(w, name)
+            norm_dtype = _lib.DTYPE_F32 if w.dtype == torch.float32 else norm_dtype
+        if q_norm is not None and k_norm is not None and q_norm.dtype != k_norm.dtype:
+            raise TypeError("q_norm and k_norm must be of one type")
+        if q_norm is not None and q is None:
+            raise ValueError("q_norm without q")
+        if not norm_eps >= 0:
+            raise ValueError("norm_eps must not be negative")
+        if positions is not None:
+            _check_int(positions, "positions", (rows,), pools.k)
+            if cos is None:
+                raise ValueError("positions without cos and sin")
+        _call(_lib.load().asterq_kv_append_normed,
+              _NORMED.pack(_DTYPES[k.dtype], norm_dtype, n_seqs, heads, n_kv, dim, rotary, 1 if interleaved else 0, page,
+                           max_pages, norm_eps, 0, rows, pools.k.shape[0], positions_n, q_row, q_head, k_row, k_head,
+                           v_row, v_head, q_ptr or 0, k.data_ptr(), v.data_ptr(), _lib.ptr(q_norm) or 0,
+                           _lib.ptr(k_norm) or 0, cos_ptr or 0, sin_ptr or 0, _lib.ptr(positions) or 0,
+                           page_table.data_ptr(), lengths.data_ptr(), row_offsets.data_ptr(), out_ptr or 0,
+                           pools.k.data_ptr(), pools.v.data_ptr(), 0 if status is None else status.data_ptr()),
+              device, torch.cuda.current_stream(device).cuda_stream)
+        return q_out
     _call(_lib.load().asterq_kv_append,
           _APPEND.pack(_DTYPES[k.dtype], n_seqs, heads, n_kv, dim, rotary, 1 if interleaved else 0, page, max_pages, 0,
-                       rows, pools.k.shape[0], positions, q_row, q_head, k_row, k_head, v_row, v_head, q_ptr or 0,
+                       rows, pools.k.shape[0], positions_n, q_row, q_head, k_row, k_head, v_row, v_head, q_ptr or 0,
                        k.data_ptr(), v.data_ptr(), cos_ptr or 0, sin_ptr or 0, page_table.data_ptr(),
                        lengths.data_ptr(), row_offsets.data_ptr(), out_ptr or 0, pools.k.data_ptr(),
                        pools.v.data_ptr(), 0 if status is None else status.data_ptr()),
@@ -450,15 +492,105 @@ def paged_tree_attention(
                            sink_tokens, out, return_lse, workspace, status)
 
 
+class PagedKVStack:
+    """The pools of a stack of layers that share page tables: one geometry, type and device, no pool twice.  It holds
+    the pools' addresses for ``keep_kv_rows`` and ``copy_kv_pages``, which work on all layers at once."""
+
+    __slots__ = ("layers", "_k", "_v")
+
+    def __init__(self, layers: Sequence[PagedKVPools]) -> None:
+        self.layers = tuple(layers)
+        if not self.layers:
+            raise ValueError("a stack without layers")
+        first = self.layers[0].k
+        for pools in self.layers:
+            if pools.k.shape != first.shape or pools.k.dtype != first.dtype or pools.k.device != first.device:
+                raise ValueError(f"layers of {tuple(first.shape)} {first.dtype} on {first.device} and "
+                                 f"{tuple(pools.k.shape)} {pools.k.dtype} on {pools.k.device}")
+        address = [pools.k.data_ptr() for pools in self.layers] + [pools.v.data_ptr() for pools in self.layers]
+        if first.numel() and len(set(address)) < len(address):
+            raise ValueError("a pool is in the stack twice")
+        n = len(self.layers)
+        self._k = (_lib.ctypes.c_void_p * n)(*address[:n])
+        self._v = (_lib.ctypes.c_void_p * n)(*address[n:])
+
+    @property
+    def like(self) -> torch.Tensor:
+        return self.layers[0].k
+
+
+def keep_kv_rows(
+    stack: PagedKVStack,
+    page_table: torch.Tensor,
+    lengths: torch.Tensor,
+    row_offsets: torch.Tensor,
+    kept: torch.Tensor,
+    n_kept: torch.Tensor,
+    *,
+    status: torch.Tensor | None = None,
+) -> None:
+    """Close the accepted rows of drafts up behind the cached tokens, in all layers of a stack (one launch).
+
+    kept int32 [rows] and n_kept int32 [n_seqs] as ``speculative.verify_drafts`` gives them: the keys and values at place
+    ``lengths[s] + kept[row_offsets[s] + i]`` go to place ``lengths[s] + i``, for i < ``n_kept[s]``.  kept ascends within a
+    sequence.  ``lengths`` is not advanced; empty slots are left out.  Sequences must not share a page that rows are moved
+    in.  status int32 [1]: set to 1 when a sequence's kept does not ascend or leaves its rows, its offsets are out of order
+    (the sequence is left as it is), or a place has no page (the row is left out).
+    """
+    if page_table.dim() != 2 or row_offsets.dim() != 1 or kept.dim() != 1:
+        raise ValueError("page_table must be [n_seqs, max_pages], row_offsets [n_seqs + 1] and kept [rows]")
+    n_seqs, max_pages = page_table.shape
+    like = stack.like
+    n_pages, n_kv, page, dim = like.shape
+    _check_int(page_table, "page_table", (n_seqs, max_pages), like)
+    _check_int(lengths, "lengths", (n_seqs,), like)
+    _check_int(row_offsets, "row_offsets", (n_seqs + 1,), like)
+    _check_int(kept, "kept", (kept.shape[0],), like)
+    _check_int(n_kept, "n_kept", (n_seqs,), like)
+    if status is not None:
+        _check_int(status, "status", (1,), like)
+    _call(_lib.load().asterq_kv_keep,
+          _KEEP.pack(_DTYPES[like.dtype], len(stack.layers), n_seqs, n_kv, dim, page, max_pages, 0, kept.shape[0], n_pages,
+                     _lib.ctypes.addressof(stack._k), _lib.ctypes.addressof(stack._v), page_table.data_ptr(),
+                     lengths.data_ptr(), row_offsets.data_ptr(), kept.data_ptr(), n_kept.data_ptr(),
+                     0 if status is None else status.data_ptr()),
+          like.device, torch.cuda.current_stream(like.device).cuda_stream)
+
+
+def copy_kv_pages(stack: PagedKVStack, pairs: torch.Tensor, *, status: torch.Tensor | None = None) -> None:
+    """Copy pages in all layers of a stack (one launch): pairs int32 [n, 2], page ``pairs[i, 1]`` becomes a copy of page
+    ``pairs[i, 0]``.  A pair with a negative entry is left out.  So is, with status int32 [1] set to 1, one with a page
+    outside the pools, and every pair whose destination another pair names too or whose source another pair writes."""
+    like = stack.like
+    n_pages, n_kv, page, dim = like.shape
+    if pairs.dim() != 2:
+        raise ValueError("pairs must be [n, 2]")
+    _check_int(pairs, "pairs", (pairs.shape[0], 2), like)
+    if pairs.data_ptr() % 8:
+        pairs = pairs.clone()
+    if status is not None:
+        _check_int(status, "status", (1,), like)
+    _call(_lib.load().asterq_kv_copy_pages,
+          _COPY.pack(_DTYPES[like.dtype], len(stack.layers), n_kv, dim, page, pairs.shape[0], n_pages,
+                     _lib.ctypes.addressof(stack._k), _lib.ctypes.addressof(stack._v), pairs.data_ptr(),
+                     0 if status is None else status.data_ptr()),
+          like.device, torch.cuda.current_stream(like.device).cuda_stream)
+
+
 class PagedKVBatch:
     """The paged keys and values of a stack of attention layers that share sequence slots.
 
     Slot s is row s of ``page_table`` and ``lengths``, which live on the GPU beside a host mirror that
     hands out pages ahead of need (sequences added or removed reach the GPU with the next step).  A decode step is ``begin_step`` once, then for each layer ``append``
     and ``attend`` with one row a slot (rows of idle slots are ignored, their outputs are zeros), then
-    ``end_step`` (or ``abandon_step``, where it failed on the way).  A prompt chunk is ``begin_rows`` with the tokens each slot gets, ``append`` for each
-    layer, ``end_step``; the prompt's own attention is the caller's.  A slot holds its pages until it is
-    removed, also those that a window has passed.
+    ``end_step`` (or ``abandon_step``, where it failed on the way).  A prompt chunk is ``begin_rows`` with the tokens each slot gets, ``append`` and
+    ``attend_rows`` for each layer, ``end_step``.  A step of drafted tokens is ``begin_tree`` with the slots' trees,
+    ``append`` and ``attend_rows`` for each layer, ``speculative.verify_drafts`` with the batch's ``row_offsets`` and ``parents``, and
+    ``accept`` with what it kept.
+
+    ``fork_sequence`` gives a slot that shares another's pages; a page that both hold is copied when one of them is about
+    to write into it.  A slot holds its pages until it is removed or truncated, or ``release_behind_window`` gives up those that a
+    window has passed.  ``compact_pages`` moves the pages in use to the front of the pools.
     """
 
     def __init__(self, n_layers: int, n_kv_heads: int, head_dim: int, *, max_seqs: int, max_tokens: int,
@@ -479,8 +611,11 @@ class PagedKVBatch:
                        for _ in range(n_layers)]
         self.cos, self.sin, self.interleaved = cos, sin, interleaved
         self.window_size, self.sink_tokens = window_size, sink_tokens
+        self.stack = PagedKVStack(self.layers)
         self._free = _PagePool(pool_pages)
-        self._held = [0] * max_seqs  # pages of each slot
+        self._users = np.zeros(pool_pages, np.int32)  # slots that hold each page
+        self._held = [0] * max_seqs  # entries of each slot's row of the table
+        self._passed = [0] * max_seqs  # tokens before this may have no page any more, but for the sink's
         self._length = np.full(max_seqs, -1, np.int32)
         self._table = np.full((max_seqs, self.max_pages), -1, np.int32)
         i32 = dict(dtype=torch.int32, device=self.device)
@@ -491,6 +626,8 @@ class PagedKVBatch:
         self._new = np.zeros(max_seqs, np.int32)
         self._new_dev = torch.zeros(max_seqs, **i32)
         self._open = False
+        self._tree = False
+        self.parents = self.positions = None  # of an open step's drafted trees
         self._dirty = False
         self.status = torch.zeros(1, **i32)
 
@@ -523,6 +660,7 @@ class PagedKVBatch:
         elif not 0 <= slot < self.max_seqs or self._length[slot] >= 0:
             raise ValueError(f"slot {slot} is not free")
         self._length[slot] = 0
+        self._passed[slot] = 0
         self._dirty = True
         return slot
 
@@ -531,12 +669,97 @@ class PagedKVBatch:
             raise RuntimeError("a step is open: end_step first")
         if not 0 <= slot < self.max_seqs or self._length[slot] < 0:
             raise ValueError(f"slot {slot} holds no sequence")
-        n = self._held[slot]
-        self._free.release(self._table[slot, :n].tolist())
-        self._table[slot] = -1
-        self._held[slot] = 0
+        self._drop(slot, 0)
         self._length[slot] = -1
+        self._passed[slot] = 0
+
+    def _drop(self, slot: int, first: int) -> None:
+        """The slot's pages from entry ``first`` on are not held by it any more."""
+        pages = self._table[slot, first : self._held[slot]]
+        pages = pages[pages >= 0]
+        self._users[pages] -= 1  # a slot holds a page once
+        self._free.release(pages[self._users[pages] == 0].tolist())
+        self._table[slot, first : self._held[slot]] = -1
+        self._held[slot] = first
         self._dirty = True
+
+    def fork_sequence(self, slot: int, into: int | None = None) -> int:
+        """Open a sequence that has the tokens of ``slot``, in a free slot (the given one, or the lowest), by sharing its
+        pages: nothing is copied until one of the two writes into a page that both hold."""
+        if not 0 <= slot < self.max_seqs or self._length[slot] < 0:
+            raise ValueError(f"slot {slot} holds no sequence")
+        new = self.add_sequence(into)
+        n = -(-int(self._length[slot]) // self.page_tokens)
+        self._table[new, :n] = self._table[slot, :n]
+        pages = self._table[new, :n]
+        self._users[pages[pages >= 0]] += 1
+        self._held[new] = n
+        self._length[new] = self._length[slot]
+        self._passed[new] = self._passed[slot]
+        return new
+
+    def truncate_sequence(self, slot: int, tokens: int) -> None:
+        """Keep the first ``tokens`` tokens of a sequence; pages behind them are given up."""
+        if self._open:
+            raise RuntimeError("a step is open: end_step first")
+        if not 0 <= slot < self.max_seqs or self._length[slot] < 0:
+            raise ValueError(f"slot {slot} holds no sequence")
+        if not 0 <= tokens <= self._length[slot]:
+            raise ValueError(f"slot {slot} has {self._length[slot]} tokens, not {tokens}")
+        if self._passed[slot] and tokens - self._reach() + 1 < self._passed[slot]:
+            raise ValueError(f"slot {slot}: a window behind {tokens} tokens needs pages that were given up")
+        self._drop(slot, min(self._held[slot], -(-tokens // self.page_tokens)))
+        self._length[slot] = tokens
+
+    def _reach(self) -> int:
+        return self.window_size - min(self.sink_tokens, self.window_size)
+
+    def release_behind_window(self) -> int:
+        """Give up the pages between the sink and what the window still shows; returns how many entries were."""
+        if self._open:
+            raise RuntimeError("a step is open: end_step first")
+        if self.window_size is None:
+            return 0
+        released = 0
+        sink, page = min(self.sink_tokens, self.window_size), self.page_tokens
+        for s in self.active():
+            first = -(-sink // page)
+            last = min(max(0, int(self._length[s]) - self._reach() + 1) // page, self._held[s])  # tokens below it are passed
+            if last <= first:
+                continue
+            pages = self._table[s, first:last]
+            pages = pages[pages >= 0]
+            if pages.size:
+                self._users[pages] -= 1
+                self._free.release(pages[self._users[pages] == 0].tolist())
+                self._table[s, first:last] = -1
+                released += int(pages.size)
+                self._dirty = True
+            self._passed[s] = max(self._passed[s], last * page)
+        return released
+
+    def compact_pages(self) -> int:
+        """Move the pages in use to the front of the pools (one launch); returns their number."""
+        if self._open:
+            raise RuntimeError("a step is open: end_step first")
+        used = np.nonzero(self._users > 0)[0]
+        n = int(used.size)
+        source = used[used >= n]
+        if source.size:
+            target = np.nonzero(self._users[:n] == 0)[0]
+            self._copy(np.stack((source, target), 1))
+            to = np.arange(self._users.size, dtype=np.int32)
+            to[source] = target
+            self._table = np.where(self._table >= 0, to[self._table], -1).astype(np.int32)
+            self._users[target] = self._users[source]
+            self._users[source] = 0
+            self._free.free = list(range(self._users.size - 1, n - 1, -1))
+            self._dirty = True
+        return n
+
+    def _copy(self, pairs: np.ndarray) -> None:
+        pairs = torch.from_numpy(np.ascontiguousarray(pairs, np.int32)).pin_memory().to(self.device, non_blocking=True)
+        copy_kv_pages(self.stack, pairs, status=self.status)
 
     def _begin(self, new: np.ndarray, one_row: bool) -> None:
         if self._open:
@@ -544,15 +767,33 @@ class PagedKVBatch:
         want = np.where(new > 0, self._length + new, 0)
         if (want > self.max_tokens).any():
             raise ValueError(f"a sequence would pass {self.max_tokens} tokens")
-        need = -(-want // self.page_tokens) - np.asarray(self._held)
-        short = np.nonzero(need > 0)[0]
-        pages = self._free.alloc(int(need[short].sum())) if short.size else []
-        for s in short:
+        need = np.maximum(-(-want // self.page_tokens) - np.asarray(self._held), 0)
+        # entries that a slot is about to write into and that others hold too: the last of its holders keeps the page
+        shared, users = [], {}
+        for s in np.nonzero(new > 0)[0]:
+            for at in range(int(self._length[s]) // self.page_tokens, min(self._held[s], -(-int(want[s]) // self.page_tokens))):
+                page = int(self._table[s, at])
+                left = users.get(page, int(self._users[page]))
+                if left > 1:
+                    users[page] = left - 1
+                    shared.append((int(s), at, page))
+        pages = self._free.alloc(int(need.sum()) + len(shared)) if need.any() or shared else []
+        self._users[pages] = 1
+        pairs = []
+        for s, at, page in shared:
+            self._users[page] -= 1
+            self._table[s, at] = pages.pop()
+            if at * self.page_tokens < self._length[s]:
+                pairs.append((page, self._table[s, at]))
+            self._dirty = True
+        for s in np.nonzero(need > 0)[0]:
             at, n = self._held[s], int(need[s])
             self._table[s, at : at + n] = pages[:n]
             pages = pages[n:]
             self._held[s] = at + n
             self._dirty = True
+        if pairs:
+            self._copy(np.asarray(pairs, np.int32))
         self._upload()
         if one_row:
             self.row_offsets = self._one_row
@@ -578,12 +819,68 @@ class PagedKVBatch:
             new[s] = n
         self._begin(new, False)
 
-    def append(self, layer: int, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor | None:
-        """The open step's keys and values into layer ``layer``'s pages; returns the rotated queries."""
+    def begin_tree(self, slots: Sequence[int], parents: Sequence[Sequence[int]]) -> None:
+        """Open a step of drafted tokens: for slot ``slots[i]`` a tree whose node j's parent is ``parents[i][j]``, below j
+        (-1 for node 0, the root: the token after the cached ones).  The rows are the slots' nodes in the order of the slots;
+        ``parents`` and ``positions`` hold their parents and positions on the GPU."""
+        new = np.zeros(self.max_seqs, np.int32)
+        trees = {}
+        for s, tree in zip(slots, parents, strict=True):
+            if not 0 <= s < self.max_seqs or self._length[s] < 0 or s in trees or not 0 < len(tree) <= MAX_TREE_NODES:
+                raise ValueError(f"slot {s}: a tree of {len(tree)} nodes (1 to {MAX_TREE_NODES})")
+            if tree[0] != -1 or any(not 0 <= p < j for j, p in enumerate(tree) if j):
+                raise ValueError(f"slot {s}: the first node is the root (-1), others have a parent before them")
+            depth = []
+            for p in tree:
+                depth.append(0 if p < 0 else depth[p] + 1)
+            trees[s] = (list(tree), depth)
+            new[s] = len(tree)
+        order = sorted(trees)
+        flat = [p for s in order for p in trees[s][0]]
+        at = [int(self._length[s]) + d for s in order for d in trees[s][1]]
+        self._begin(new, False)
+        both = torch.tensor([flat, at], dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
+        self.parents, self.positions = both[0], both[1]
+        self._tree = True
+
+    def append(self, layer: int, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, *,
+               q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,
+               norm_eps: float = 1e-6) -> torch.Tensor | None:
+        """The open step's keys and values into layer ``layer``'s pages; returns the rotated queries (of normed heads where
+        weights are given)."""
         if not self._open:
             raise RuntimeError("no step is open: begin_step or begin_rows first")
         return append_kv(self.layers[layer], self.page_table, self.lengths, self.row_offsets, k, v, q=q, cos=self.cos,
-                         sin=self.sin, interleaved=self.interleaved, status=self.status)
+                         sin=self.sin, interleaved=self.interleaved, q_norm=q_norm, k_norm=k_norm, norm_eps=norm_eps,
+                         positions=self.positions if self._tree and self.cos is not None else None, status=self.status)
+
+    def attend_rows(self, layer: int, q: torch.Tensor, **kw):
+        """Attention of the open prompt chunk's or drafted trees' rotated queries over layer ``layer`` with their own tokens."""
+        if not self._open or self.row_offsets is self._one_row:
+            raise RuntimeError("no rows are open: begin_rows or begin_tree first")
+        kw = dict(window_size=self.window_size, sink_tokens=self.sink_tokens, status=self.status, **kw)
+        if self._tree:
+            return paged_tree_attention(self.layers[layer], self.page_table, self.lengths, self.row_offsets, self.parents, q, **kw)
+        return paged_prompt_attention(self.layers[layer], self.page_table, self.lengths, self.row_offsets, q, **kw)
+
+    def accept(self, kept: torch.Tensor, n_kept: torch.Tensor) -> list[int]:
+        """Close the open step of drafted tokens with what ``speculative.verify_drafts`` kept of it: the accepted rows are
+        closed up behind the cached tokens in all layers and the sequences advance by them.  Returns the slots' numbers of
+        accepted rows; waits for the GPU, since pages are handed out on the host."""
+        if not self._open or self.row_offsets is self._one_row:
+            raise RuntimeError("no drafted rows are open: begin_tree or begin_rows first")
+        keep_kv_rows(self.stack, self.page_table, self.lengths, self.row_offsets, kept, n_kept, status=self.status)
+        counts = n_kept.cpu().numpy()
+        if (counts < 0).any() or (counts > self._new).any():
+            raise ValueError("more rows kept than were drafted")
+        self.lengths.add_(n_kept)
+        self._length += counts
+        self._close()
+        return counts.tolist()
+
+    def _close(self) -> None:
+        self._open = self._tree = False
+        self.parents = self.positions = None
 
     def attend(self, layer: int, q: torch.Tensor, **kw):
         """Attention of the open decode step's rotated queries over layer ``layer`` with its new token."""
@@ -596,16 +893,18 @@ class PagedKVBatch:
         """Advance the sequences by the open step's tokens (one small launch; nothing is copied)."""
         if not self._open:
             raise RuntimeError("no step is open")
+        if self._tree:
+            raise RuntimeError("drafted tokens are open: accept or abandon_step")
         self.lengths.add_(self._new_dev)
         self._length += self._new
-        self._open = False
+        self._close()
 
     def abandon_step(self) -> None:
         """Close the open step without advancing: the sequences stay as they were before it.  What it has appended is
         never read, and the next step's tokens go in its place; pages that it was handed stay with their slots."""
         if not self._open:
             raise RuntimeError("no step is open")
-        self._open = False
+        self._close()
 
     def raise_if_failed(self) -> None:
         """Synchronize; raise if a row was left out or an attention did not finish."""

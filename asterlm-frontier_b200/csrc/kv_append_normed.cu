@@ -1,0 +1,240 @@
+// Append of new keys and values to a paged grouped-query cache with the norms of queries and keys: each head is
+// divided by its root mean square and weighted, then rotated by its position, in one pass from a projection's rows to
+// the pages (csrc/kv_append.cu is the append without norms).
+//
+//   y = x / sqrt(mean(x^2) + eps) w  for each head of q and of k (where weights are given), fp32;
+//   the first rotary_dim dims of y turn in pairs by cos[p][j], sin[p][j]; one rounding at the end.
+// p is the row's place behind the sequence's cached tokens, or positions[row] (a drafted node's place in the
+// pages goes by its number, its position by its depth).
+//
+// Bound by memory: 2 bytes in and 2 out a value, and some ten operations.  A head is held by the lanes of one
+// group, 16 dims each (two 16-byte vectors whose pairs share eight cos and sin values), so its sum of squares
+// is a few shuffles; a group walks over heads, and CTAs over rows with the weights in registers.
+#include "asterq_internal.h"
+#include "common.cuh"
+#include "launch.cuh"
+
+namespace asterq {
+namespace kvn {
+
+constexpr int kThreads = 256;
+
+template <bool kF16>
+ASTERQ_DEVICE float2 unpack2(uint32_t w) {
+  return kF16 ? unpack_half2(w) : unpack_bf162(w);
+}
+template <bool kF16>
+ASTERQ_DEVICE uint32_t pack2(float lo, float hi) {
+  return kF16 ? pack_half2(lo, hi) : pack_bf162(lo, hi);
+}
+
+// The last s in [0, n) with off[s] <= row (off[0] <= row), by all lanes of a warp.
+ASTERQ_DEVICE int find_sequence(const int* __restrict__ off, int n, long long row) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, len = n;
+  while (len > 1) {
+    const int step = (len + 31) / 32;
+    const bool below = lane * step < len && (long long)__ldg(off + lo + lane * step) <= row;
+    const int skip = (max(__popc(__ballot_sync(0xffffffffu, below)), 1) - 1) * step;
+    lo += skip;
+    len = min(step, len - skip);
+  }
+  return lo;
+}
+
+template <bool kF16>
+ASTERQ_DEVICE void weights_of(float (&w)[16], const void* from, bool f32, int d0, int d1) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (f32) {
+      w[i] = __ldg(static_cast<const float*>(from) + d0 + i);
+      w[8 + i] = __ldg(static_cast<const float*>(from) + d1 + i);
+    } else {
+      const uint16_t a = __ldg(static_cast<const uint16_t*>(from) + d0 + i), b = __ldg(static_cast<const uint16_t*>(from) + d1 + i);
+      w[i] = unpack2<kF16>(a).x;
+      w[8 + i] = unpack2<kF16>(b).x;
+    }
+  }
+}
+
+template <bool kF16>
+__global__ void __launch_bounds__(kThreads) append_kernel(const asterq_kv_append_normed_params p, int rows_per_block, int lanes) {
+  const int D = p.head_dim, units = D / 16, turn = p.rotary_dim / 16;
+  const int per_row = kThreads / rows_per_block;  // threads of one row: whole warps
+  const int sub = threadIdx.x / per_row, r = threadIdx.x % per_row;
+  const int u = r % lanes, g = r / lanes, groups = per_row / lanes;  // a head's lanes: a power of two
+  const bool works = u < units;
+  const int n_q = p.q ? p.n_heads : 0, n_all = n_q + 2 * p.n_kv_heads;
+  const bool half = !p.interleaved && u < turn;
+  const int d0 = !works ? 0 : half ? 8 * u : 16 * u, d1 = !works ? 8 : half ? p.rotary_dim / 2 + 8 * u : 16 * u + 8;
+  float wq[16], wk[16];
+  const bool f32 = p.norm_dtype == ASTERQ_DTYPE_F32;
+  if (p.q_norm) weights_of<kF16>(wq, p.q_norm, f32, d0, d1);
+  if (p.k_norm) weights_of<kF16>(wk, p.k_norm, f32, d0, d1);
+
+  for (long long row = (long long)blockIdx.x * rows_per_block + sub; row < p.n_rows; row += (long long)gridDim.x * rows_per_block) {
+    auto source = [&](int h) -> const uint16_t* {
+      if (h < n_q) return (const uint16_t*)p.q + row * p.q_row_stride + (long long)h * p.q_head_stride;
+      h -= n_q;
+      if (h < p.n_kv_heads) return (const uint16_t*)p.k + row * p.k_row_stride + (long long)h * p.k_head_stride;
+      return (const uint16_t*)p.v + row * p.v_row_stride + (long long)(h - p.n_kv_heads) * p.v_head_stride;
+    };
+    uint4 a = make_uint4(0, 0, 0, 0), b = a;
+    if (works && g < n_all) {
+      const uint16_t* src = source(g);
+      a = ldg_nc_v4(src + d0);
+      b = ldg_nc_v4(src + d1);
+    }
+    // where the row belongs; every warp looks it up for itself
+    if ((long long)__ldg(p.row_offsets) > row || row >= (long long)__ldg(p.row_offsets + p.n_seqs)) continue;
+    const int s = find_sequence(p.row_offsets, p.n_seqs, row);
+    const int length = __ldg(p.lengths + s);
+    if (length < 0) continue;  // an empty slot
+    const long long begin = __ldg(p.row_offsets + s), place = (long long)length + (row - begin);
+    const long long col = place / p.page_tokens;
+    const int at = (int)(place - col * p.page_tokens);
+    const long long pos = p.positions ? (long long)__ldg(p.positions + row) : place;
+    int page = -1;
+    // the search finds a sequence that the row is not of where offsets are out of order
+    if (row >= begin && row < (long long)__ldg(p.row_offsets + s + 1) && col < p.max_pages)
+      page = __ldg(p.page_table + (long long)s * p.max_pages + col);
+    if (page < 0 || page >= p.n_pages || (turn && (pos < 0 || pos >= p.n_positions))) {
+      if (p.status && (threadIdx.x & 31) == 0) atomicMax(p.status, 1);
+      continue;
+    }
+    float c[8], sn[8];
+    if (works && u < turn) {
+      const float4* cp = reinterpret_cast<const float4*>(p.cos + pos * (p.rotary_dim / 2) + 8 * u);
+      const float4* sp = reinterpret_cast<const float4*>(p.sin + pos * (p.rotary_dim / 2) + 8 * u);
+      *reinterpret_cast<float4*>(c) = __ldg(cp);
+      *reinterpret_cast<float4*>(c + 4) = __ldg(cp + 1);
+      *reinterpret_cast<float4*>(sn) = __ldg(sp);
+      *reinterpret_cast<float4*>(sn + 4) = __ldg(sp + 1);
+    }
+    const long long page0 = (long long)page * p.n_kv_heads;
+    for (int h0 = 0; h0 < n_all; h0 += groups) {  // every lane all rounds: a head's lanes meet in shuffles
+      const int h = h0 + g;
+      uint4 na = a, nb = b;
+      if (works && h + groups < n_all) {
+        const uint16_t* src = source(h + groups);
+        na = ldg_nc_v4(src + d0);
+        nb = ldg_nc_v4(src + d1);
+      }
+      const bool is_q = h < n_q, is_k = !is_q && h < n_q + p.n_kv_heads;
+      const bool normed = (is_q && p.q_norm) || (is_k && p.k_norm);
+      float x[8], y[8];
+      const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 xf = unpack2<kF16>(aw[i]), yf = unpack2<kF16>(bw[i]);
+        x[2 * i] = xf.x;
+        x[2 * i + 1] = xf.y;
+        y[2 * i] = yf.x;
+        y[2 * i + 1] = yf.y;
+        sum = fmaf(xf.x, xf.x, fmaf(xf.y, xf.y, fmaf(yf.x, yf.x, fmaf(yf.y, yf.y, sum))));
+      }
+      if (!works) sum = 0.0f;
+      for (int d = 1; d < lanes; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (normed) {
+        const float scale = rsqrtf(sum / (float)D + p.norm_eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[i] = x[i] * scale * (is_q ? wq[i] : wk[i]);
+          y[i] = y[i] * scale * (is_q ? wq[8 + i] : wk[8 + i]);
+        }
+      }
+      if (works && h < n_all) {
+        if (u < turn && (is_q || is_k)) {
+          if (half) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float t = x[i];
+              x[i] = t * c[i] - y[i] * sn[i];
+              y[i] = y[i] * c[i] + t * sn[i];
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float t = x[2 * i], v = y[2 * i];
+              x[2 * i] = t * c[i] - x[2 * i + 1] * sn[i];
+              x[2 * i + 1] = x[2 * i + 1] * c[i] + t * sn[i];
+              y[2 * i] = v * c[4 + i] - y[2 * i + 1] * sn[4 + i];
+              y[2 * i + 1] = y[2 * i + 1] * c[4 + i] + v * sn[4 + i];
+            }
+          }
+        }
+        if (is_q || is_k) {  // values go as they came
+          a = make_uint4(pack2<kF16>(x[0], x[1]), pack2<kF16>(x[2], x[3]), pack2<kF16>(x[4], x[5]), pack2<kF16>(x[6], x[7]));
+          b = make_uint4(pack2<kF16>(y[0], y[1]), pack2<kF16>(y[2], y[3]), pack2<kF16>(y[4], y[5]), pack2<kF16>(y[6], y[7]));
+        }
+        uint16_t* dst;
+        if (is_q) {
+          dst = (uint16_t*)p.q_out + (row * n_q + h) * D;
+        } else {
+          const int kv = h - n_q, hk = is_k ? kv : kv - p.n_kv_heads;
+          dst = (uint16_t*)(is_k ? p.k_pool : p.v_pool) + ((page0 + hk) * p.page_tokens + at) * D;
+        }
+        *reinterpret_cast<uint4*>(dst + d0) = a;
+        *reinterpret_cast<uint4*>(dst + d1) = b;
+      }
+      a = na;
+      b = nb;
+    }
+  }
+}
+
+}  // namespace kvn
+}  // namespace asterq
+
+using namespace asterq;
+
+extern "C" int asterq_kv_append_normed(const asterq_kv_append_normed_params* p, void* stream) {
+  clear_error();
+  if (!p) return set_error(ASTERQ_ERR_INVALID_ARGUMENT, "kv_append_normed: null parameters");
+  if (p->n_seqs < 0 || p->n_rows < 0 || p->n_pages < 0 || p->max_pages < 0 || p->n_kv_heads <= 0 || p->n_heads < 0 ||
+      p->n_positions < 0 || p->page_tokens <= 0)
+    return set_error(ASTERQ_ERR_INVALID_ARGUMENT, "kv_append_normed: bad sizes");
+  if (p->dtype != ASTERQ_DTYPE_BF16 && p->dtype != ASTERQ_DTYPE_F16)
+    return set_error(ASTERQ_ERR_UNSUPPORTED, "kv_append_normed: dtype %d: bf16 or f16", p->dtype);
+  if ((p->q_norm || p->k_norm) && p->norm_dtype != p->dtype && p->norm_dtype != ASTERQ_DTYPE_F32)
+    return set_error(ASTERQ_ERR_UNSUPPORTED, "kv_append_normed: weights are of the rows' type or f32");
+  if (p->head_dim <= 0 || p->head_dim % 16 || p->head_dim > 512)
+    return set_error(ASTERQ_ERR_UNSUPPORTED, "kv_append_normed: head_dim %d must be a multiple of 16 up to 512", p->head_dim);
+  if (p->rotary_dim < 0 || p->rotary_dim > p->head_dim || p->rotary_dim % 16)
+    return set_error(ASTERQ_ERR_UNSUPPORTED, "kv_append_normed: rotary_dim %d must be a multiple of 16 up to head_dim",
+                     p->rotary_dim);
+  if (!(p->norm_eps >= 0.0f)) return set_error(ASTERQ_ERR_INVALID_ARGUMENT, "kv_append_normed: negative norm_eps");
+  if (p->n_rows == 0 || p->n_seqs == 0) return ASTERQ_OK;
+  if (p->n_rows > 0x7fffffffLL) return set_error(ASTERQ_ERR_INVALID_ARGUMENT, "kv_append_normed: more than 2^31 - 1 rows");
+  if (!p->k || !p->v || !p->k_pool || !p->v_pool || !p->lengths || !p->row_offsets ||
+      (p->max_pages > 0 && !p->page_table) || (p->q && (!p->q_out || p->n_heads <= 0)) ||
+      (p->rotary_dim > 0 && (!p->cos || !p->sin)))
+    return set_error(ASTERQ_ERR_INVALID_ARGUMENT, "kv_append_normed: null pointer");
+  const void* vec[] = {p->q, p->k, p->v, p->cos, p->sin, p->q_out, p->k_pool, p->v_pool};
+  for (const void* ptr : vec)
+    if (reinterpret_cast<uintptr_t>(ptr) & 15)
+      return set_error(ASTERQ_ERR_MISALIGNED, "kv_append_normed: arrays must be 16-byte aligned");
+  const int64_t strides[] = {p->q ? p->q_row_stride : 0, p->q ? p->q_head_stride : 0, p->k_row_stride,
+                             p->k_head_stride, p->v_row_stride, p->v_head_stride};
+  for (int64_t st : strides)
+    if (st % 8) return set_error(ASTERQ_ERR_MISALIGNED, "kv_append_normed: row and head strides must be multiples of 8");
+  int dev = 0;
+  const int sms = current_sms(&dev);
+  if (sms <= 0) return set_error(ASTERQ_ERR_CUDA, "kv_append_normed: no CUDA device");
+  int lanes = 1;
+  while (lanes < p->head_dim / 16) lanes *= 2;
+  // threads of a row: for all its heads at once while rows are few, 64 for many
+  const int64_t items = (int64_t)lanes * ((p->q ? p->n_heads : 0) + 2 * p->n_kv_heads);
+  int per_row = kvn::kThreads;
+  while (per_row > 64 && (per_row / 2 >= items || p->n_rows >= 600)) per_row /= 2;
+  const int rows_per_block = kvn::kThreads / per_row;
+  const int64_t blocks = (p->n_rows + rows_per_block - 1) / rows_per_block, most = (int64_t)sms * 8;
+  const unsigned grid = (unsigned)(blocks < most ? blocks : most);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (p->dtype == ASTERQ_DTYPE_F16)
+    kvn::append_kernel<true><<<grid, kvn::kThreads, 0, s>>>(*p, rows_per_block, lanes);
+  else
+    kvn::append_kernel<false><<<grid, kvn::kThreads, 0, s>>>(*p, rows_per_block, lanes);
+  return check_launch("kv_append_normed");
+}

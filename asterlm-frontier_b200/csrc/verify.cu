@@ -1,0 +1,350 @@
+// Verification of drafted tokens against the target's probabilities, by given random numbers.
+//
+// A sequence's drafted tokens are the nodes of a tree (or a chain); node 0 is the root, its token is accepted
+// already.  target[i] is the target's distribution behind node i, draft[i] the one that i's children were drawn from.
+// The walk is at cur = 0 with r = target[cur], m = 1.  Nodes i = 1, 2, ..: where parent(i) = cur, x its token,
+//   accepted if accept[i] draft[cur][x] m < r(x): cur = i, r = target[i], m = 1;
+//   rejected: r = max(r - m draft[cur], 0), m = sum r; if nothing is left (m = 0), r = target[cur], m = 1 again.
+// At the end the next token is the least t with r(0) + .. + r(t) > sample sum r.  This draws from the target's
+// distribution whatever the draft's was.  Without draft probabilities drafts are taken as certain: accepted if
+// accept[i] m < r(x), rejected r(x) = 0 and m = m - r(x).
+//
+// What bounds it: one row of the target's probabilities a sequence, and one of the draft's, are read for each
+// rejection behind which something follows, and to draw; the nodes' own values are gathered at once.  A cluster of CTAs shares a
+// sequence's vocabulary while sequences are few.  Sums are in 64 bits: a border between two tokens among 10^5 is hit
+// by the rounding of a 32-bit sum once in some hundred draws.
+#include <cooperative_groups.h>
+
+#include "asterq_internal.h"
+#include "common.cuh"
+#include "launch.cuh"
+
+namespace asterq {
+namespace ver {
+
+namespace cg = cooperative_groups;
+
+constexpr int kThreads = 512, kWarps = 16, kMaxNodes = 1024, kMaxCluster = 8;
+
+struct Args {
+  const void* target;
+  const void* draft;
+  const int* tokens;
+  const int* parents;
+  const int* row_offsets;
+  const float* accept;
+  const float* sample;
+  int* kept;
+  int* n_kept;
+  int* next_token;
+  int* status;
+  long long target_stride, draft_stride, n_rows;
+  int vocab;
+};
+
+template <int kType>
+ASTERQ_DEVICE double value_at(const void* x, long long i) {
+  if constexpr (kType == ASTERQ_DTYPE_F32) return (double)__ldg(static_cast<const float*>(x) + i);
+  const uint32_t w = __ldg(static_cast<const uint16_t*>(x) + i);
+  return (double)(kType == ASTERQ_DTYPE_F16 ? unpack_half2(w).x : unpack_bf162(w).x);
+}
+
+ASTERQ_DEVICE double warp_sum(double x) {
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) x += __shfl_xor_sync(0xffffffffu, x, d);
+  return x;
+}
+
+template <int kType>
+__global__ void __launch_bounds__(kThreads) verify_kernel(const Args a) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), s = blockIdx.x / ranks;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  __shared__ int parent_s[kMaxNodes], token_s[kMaxNodes];
+  __shared__ double p_s[kMaxNodes], q_s[kMaxNodes];
+  __shared__ float u_s[kMaxNodes];
+  __shared__ double mass_s[kMaxNodes];     // m before each rejection at cur
+  __shared__ int gone_s[kMaxNodes];        // tokens rejected at cur, of drafts without probabilities
+  __shared__ double warp_sums[kWarps], rank_sums[2][kMaxCluster];
+  __shared__ double found_rest;
+  __shared__ int found_part;
+  const long long begin = __ldg(a.row_offsets + s), end = __ldg(a.row_offsets + s + 1);
+  const bool bad = begin < 0 || end < begin || end > a.n_rows || end - begin > kMaxNodes;
+  const int n = bad ? 0 : (int)(end - begin);
+  if (n == 0) {  // the whole cluster
+    if (rank == 0 && tid == 0) {
+      a.n_kept[s] = 0;
+      a.next_token[s] = -1;
+      if (bad && a.status) atomicMax(a.status, 1);
+    }
+    return;
+  }
+  bool odd = false;
+  for (int i = tid; i < n; i += kThreads) {
+    int up = a.parents ? __ldg(a.parents + begin + i) : i - 1;
+    const bool root = i == 0;
+    if (root ? up != -1 : (up < -1 || up >= i)) {
+      odd = true;
+      up = -1;
+    }
+    if (root) up = -1;
+    const int x = __ldg(a.tokens + begin + i);
+    const bool in = x >= 0 && x < a.vocab;
+    odd = odd || (!root && !in);
+    const bool use = !root && up >= 0 && in;
+    parent_s[i] = up;
+    token_s[i] = in ? x : -1;
+    u_s[i] = __ldg(a.accept + begin + i);
+    p_s[i] = use ? value_at<kType>(a.target, (begin + up) * a.target_stride + x) : 0.0;
+    q_s[i] = use && a.draft ? value_at<kType>(a.draft, (begin + up) * a.draft_stride + x) : use ? 1.0 : 0.0;
+  }
+  if (odd && rank == 0 && a.status) atomicMax(a.status, 1);
+  __syncthreads();
+
+  // this CTA's part of the vocabulary, and its warps' parts
+  const int chunk = (a.vocab + ranks - 1) / ranks;
+  const int v0 = min(rank * chunk, a.vocab), v1 = min(v0 + chunk, a.vocab);
+  int cur = 0, rejected = 0, count = 1, round = 0;
+  double m = 1.0;
+  // what is left of the target at t after the rejections so far
+  auto left_at = [&](int t) {
+    double r = value_at<kType>(a.target, (begin + cur) * a.target_stride + t);
+    if (a.draft) {
+      if (rejected > 0) {
+        const double q = value_at<kType>(a.draft, (begin + cur) * a.draft_stride + t);
+        for (int k = 0; k < rejected; ++k) r = fmax(__dsub_rn(r, __dmul_rn(mass_s[k], q)), 0.0);
+      }
+    } else {
+      for (int k = 0; k < rejected; ++k) r = gone_s[k] == t ? 0.0 : r;
+    }
+    return r;
+  };
+  // The sum of what is left over [from, to) by this warp, lanes side by side.
+  auto sum_of = [&](int from, int to) {
+    double sum = 0.0;
+    constexpr int kAhead = 8;
+    for (int t = from + lane; t < to; t += 32 * kAhead) {
+      double r[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) r[k] = t + 32 * k < to ? left_at(t + 32 * k) : 0.0;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) sum += r[k];
+    }
+    return warp_sum(sum);
+  };
+  auto part_of = [](int from, int to, int w, int& a0, int& a1) {
+    const int each = ((to - from + kWarps - 1) / kWarps + 31) / 32 * 32;
+    a0 = min(from + w * each, to);
+    a1 = min(a0 + each, to);
+  };
+  // the sum over the vocabulary, the same in every thread of the cluster; warps' and CTAs' sums stay in shared memory
+  auto total_left = [&]() {
+    int a0, a1;
+    part_of(v0, v1, warp, a0, a1);
+    const double mine = sum_of(a0, a1);
+    __syncthreads();
+    if (lane == 0) warp_sums[warp] = mine;
+    __syncthreads();
+    double* sums = rank_sums[round & 1];
+    ++round;
+    if (tid < ranks) {
+      double sum = 0.0;
+      for (int w = 0; w < kWarps; ++w) sum += warp_sums[w];
+      *cluster.map_shared_rank(sums + rank, tid) = sum;
+    }
+    if (ranks > 1) cluster.sync();
+    else __syncthreads();
+    double all = 0.0;
+    for (int k = 0; k < ranks; ++k) all += sums[k];
+    return all;
+  };
+  if (rank == 0 && tid == 0) a.kept[begin] = 0;
+  int at = 0;  // every warp walks for itself: no barrier until sums are needed
+  double total = -1.0;  // of what is left, once known
+  while (true) {
+    // the next node whose parent is cur
+    int next = n;
+    for (int base = (at + 1) & ~31; base < n && next == n; base += 32) {
+      const int i = base + lane;
+      const uint32_t hit = __ballot_sync(0xffffffffu, i > at && i < n && parent_s[i] == cur);
+      if (hit) next = base + __ffs(hit) - 1;
+    }
+    if (next == n) break;
+    at = next;
+    const int x = token_s[next];
+    double r = p_s[next];
+    if (a.draft) {
+      for (int k = 0; k < rejected; ++k) r = fmax(__dsub_rn(r, __dmul_rn(mass_s[k], q_s[next])), 0.0);
+    } else {
+      for (int k = 0; k < rejected; ++k) r = gone_s[k] == x ? 0.0 : r;
+    }
+    if (__dmul_rn(__dmul_rn((double)u_s[next], q_s[next]), m) < r) {
+      cur = next;
+      if (rank == 0 && tid == 0) a.kept[begin + count] = next;
+      ++count;
+      rejected = 0;
+      m = 1.0;
+      total = -1.0;
+      continue;
+    }
+    __syncthreads();  // no warp still reads the lists
+    if (tid == 0) {
+      mass_s[rejected] = m;
+      gone_s[rejected] = x;
+    }
+    __syncthreads();
+    ++rejected;
+    if (a.draft) {
+      total = total_left();
+      m = total;
+      if (total == 0.0) {
+        rejected = 0;
+        m = 1.0;
+        total = -1.0;
+      }
+    } else {
+      m = __dsub_rn(m, r);
+    }
+  }
+  __syncthreads();
+  if (total < 0.0) total = total_left();
+  if (total == 0.0 && rejected > 0) {
+    rejected = 0;
+    total = total_left();
+  }
+  for (int i = count + rank * kThreads + tid; i < n; i += ranks * kThreads) a.kept[begin + i] = -1;
+  if (rank == 0 && tid == 0) {
+    a.n_kept[s] = count;
+    if (!(total > 0.0)) {  // no distribution
+      a.next_token[s] = -1;
+      if (a.status) atomicMax(a.status, 1);
+    }
+  }
+  if (total > 0.0) {
+    // The CTA, then the warp's part, then parts of it, in which the running sum passes `rest`.
+    const double* sums = rank_sums[(round - 1) & 1];
+    double rest = __dmul_rn((double)__ldg(a.sample + s), total);
+    if (rest < 0.0) rest = 0.0;
+    int owner = -1, last = 0;
+    for (int k = 0; k < ranks; ++k) {
+      if (sums[k] > 0.0) last = k;
+      if (owner < 0) {
+        if (rest < sums[k]) owner = k;
+        else rest -= sums[k];
+      }
+    }
+    bool over = owner < 0;  // by rounding, or a random number of 1: the last token that has a probability
+    if (over) owner = last;
+    if (rank == owner) {
+      int from = v0, to = v1;
+      bool known = true;  // this CTA's warps' sums
+      while (to - from > 32) {
+        int a0, a1;
+        part_of(from, to, warp, a0, a1);
+        if (!known) {
+          const double mine = sum_of(a0, a1);
+          if (lane == 0) warp_sums[warp] = mine;
+          __syncthreads();
+        }
+        known = false;
+        int pick = -1, final = 0;
+        double left = rest;
+        for (int w = 0; w < kWarps; ++w) {
+          if (warp_sums[w] > 0.0) final = w;
+          if (pick < 0 && !over) {
+            if (left < warp_sums[w]) pick = w;
+            else left -= warp_sums[w];
+          }
+        }
+        if (pick < 0) {
+          over = true;
+          pick = final;
+        } else {
+          rest = left;
+        }
+        __syncthreads();
+        part_of(from, to, pick, a0, a1);
+        from = a0;
+        to = a1;
+      }
+      if (warp == 0) {
+        const double r = from + lane < to ? left_at(from + lane) : 0.0;
+        double scan = r;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+          const double up = __shfl_up_sync(0xffffffffu, scan, d);
+          if (lane >= d) scan += up;
+        }
+        const uint32_t above = __ballot_sync(0xffffffffu, scan > rest && r > 0.0), some = __ballot_sync(0xffffffffu, r > 0.0);
+        const int hit = !over && above ? __ffs(above) - 1 : 31 - __clz(some);
+        if (lane == 0) a.next_token[s] = from + hit;
+      }
+    }
+  }
+  if (ranks > 1) cluster.sync();  // no CTA leaves while another may still write into it
+}
+
+template <int kType>
+static cudaError_t launch(const Args& a, int n_seqs, int ranks, cudaStream_t s) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3(n_seqs * ranks);
+  c.blockDim = kThreads;
+  c.stream = s;
+  c.attrs = attr;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, verify_kernel<kType>, a);
+}
+
+}  // namespace ver
+}  // namespace asterq
+
+using namespace asterq;
+
+extern "C" int asterq_verify_drafts(const asterq_verify_params* p, void* stream) {
+  clear_error();
+  if (!p) return set_error(ASTERQ_ERR_INVALID_ARGUMENT, "verify_drafts: null parameters");
+  if (p->n_seqs < 0 || p->n_rows < 0 || p->vocab <= 0)
+    return set_error(ASTERQ_ERR_INVALID_ARGUMENT, "verify_drafts: bad sizes");
+  if (p->dtype != ASTERQ_DTYPE_F32 && p->dtype != ASTERQ_DTYPE_BF16 && p->dtype != ASTERQ_DTYPE_F16)
+    return set_error(ASTERQ_ERR_UNSUPPORTED, "verify_drafts: dtype %d: f32, bf16 or f16", p->dtype);
+  if (p->vocab > 0x7fff0000 || p->n_seqs > (1 << 27))
+    return set_error(ASTERQ_ERR_UNSUPPORTED, "verify_drafts: more than 2^31 tokens or 2^27 sequences");
+  if (p->n_seqs == 0) return ASTERQ_OK;
+  if (!p->row_offsets || !p->n_kept || !p->next_token || !p->sample ||
+      (p->n_rows > 0 && (!p->target || !p->tokens || !p->accept || !p->kept)))
+    return set_error(ASTERQ_ERR_INVALID_ARGUMENT, "verify_drafts: null pointer");
+  if (p->target_stride < 0 || p->draft_stride < 0)
+    return set_error(ASTERQ_ERR_INVALID_ARGUMENT, "verify_drafts: negative strides");
+  int dev = 0;
+  const int sms = current_sms(&dev);
+  if (sms <= 0) return set_error(ASTERQ_ERR_CUDA, "verify_drafts: no CUDA device");
+  ver::Args a;
+  a.target = p->target;
+  a.draft = p->draft;
+  a.tokens = p->tokens;
+  a.parents = p->parents;
+  a.row_offsets = p->row_offsets;
+  a.accept = p->accept;
+  a.sample = p->sample;
+  a.kept = p->kept;
+  a.n_kept = p->n_kept;
+  a.next_token = p->next_token;
+  a.status = p->status;
+  a.target_stride = p->target_stride;
+  a.draft_stride = p->draft_stride;
+  a.n_rows = p->n_rows;
+  a.vocab = p->vocab;
+  // CTAs of a sequence: as many as keep a part of 2048 tokens or more and fill the SMs some twice
+  int ranks = 1;
+  while (ranks < ver::kMaxCluster && (int64_t)p->n_seqs * ranks * 2 <= 4 * sms && p->vocab / (ranks * 2) >= 2048) ranks *= 2;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const cudaError_t e = p->dtype == ASTERQ_DTYPE_F32    ? ver::launch<ASTERQ_DTYPE_F32>(a, p->n_seqs, ranks, s)
+                        : p->dtype == ASTERQ_DTYPE_BF16 ? ver::launch<ASTERQ_DTYPE_BF16>(a, p->n_seqs, ranks, s)
+                                                        : ver::launch<ASTERQ_DTYPE_F16>(a, p->n_seqs, ranks, s);
+  if (e != cudaSuccess) return set_error(ASTERQ_ERR_CUDA, "verify_drafts: launch failed: %s", cudaGetErrorString(e));
+  return check_launch("verify_drafts");
+}

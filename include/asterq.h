@@ -435,6 +435,142 @@ typedef struct asterq_kv_append_params {
 int asterq_kv_append(const asterq_kv_append_params* p, void* stream);
 
 /*
+ * The append with norms of queries and keys for each head in the same pass, and with positions of their own for the
+ * rotation: where q_norm (k_norm) is given, each head x of q (k) becomes
+ *   x / sqrt(mean(x^2) + norm_eps) * weight,  weight [head_dim] of norm_dtype (dtype or ASTERQ_DTYPE_F32),
+ * in fp32 and not rounded before it is rotated.  positions int32 [n_rows] (or NULL: the row's place, as above): the row of
+ * cos and sin; a place in the pages stays lengths[s] + r - row_offsets[s].  A row whose position has no row in cos / sin is left
+ * out with *status 1.  All else as for asterq_kv_append.
+ */
+typedef struct asterq_kv_append_normed_params {
+  int32_t dtype; /* ASTERQ_DTYPE_BF16 or ASTERQ_DTYPE_F16, of q, k, v and the pools */
+  int32_t norm_dtype;
+  int32_t n_seqs;
+  int32_t n_heads;
+  int32_t n_kv_heads;
+  int32_t head_dim;
+  int32_t rotary_dim;
+  int32_t interleaved;
+  int32_t page_tokens;
+  int32_t max_pages; /* row stride of page_table */
+  float norm_eps;
+  int32_t reserved;
+  int64_t n_rows;      /* rows of q, k and v */
+  int64_t n_pages;     /* pages of the pools */
+  int64_t n_positions; /* rows of cos and sin */
+  int64_t q_row_stride, q_head_stride; /* in elements, multiples of 8; a head's dims are contiguous */
+  int64_t k_row_stride, k_head_stride;
+  int64_t v_row_stride, v_head_stride;
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* q_norm; /* may be NULL */
+  const void* k_norm; /* may be NULL */
+  const float* cos; /* [n_positions][rotary_dim / 2] */
+  const float* sin;
+  const int32_t* positions; /* may be NULL */
+  const int32_t* page_table;
+  const int32_t* lengths;
+  const int32_t* row_offsets; /* [n_seqs + 1], not decreasing */
+  void* q_out;                /* [n_rows][n_heads][head_dim] */
+  void* k_pool;
+  void* v_pool;
+  int32_t* status; /* may be NULL */
+} asterq_kv_append_normed_params;
+
+int asterq_kv_append_normed(const asterq_kv_append_normed_params* p, void* stream);
+
+/*
+ * Accepted rows of a draft closed up behind the cached tokens, in all layers of a stack (k_pools and v_pools: host
+ * arrays of n_layers device pointers, pools as above, sharing page_table and lengths): for sequence s the keys
+ * and values at place lengths[s] + kept[row_offsets[s] + i] go to place lengths[s] + i, for i < n_kept[s].  kept ascends
+ * within a sequence and is below its rows, row_offsets[s + 1] - row_offsets[s]; a sequence whose kept does not, or whose offsets are
+ * out of order, is left as it is with *status 1, and so is a row whose place has no page.  Empty slots (lengths[s] < 0)
+ * are left out.  No two sequences may share a page that rows are moved in.
+ */
+typedef struct asterq_kv_keep_params {
+  int32_t dtype;
+  int32_t n_layers;
+  int32_t n_seqs;
+  int32_t n_kv_heads;
+  int32_t head_dim; /* a multiple of 8 */
+  int32_t page_tokens;
+  int32_t max_pages;
+  int32_t reserved;
+  int64_t n_rows; /* of kept */
+  int64_t n_pages;
+  void* const* k_pools;
+  void* const* v_pools;
+  const int32_t* page_table;
+  const int32_t* lengths;
+  const int32_t* row_offsets; /* [n_seqs + 1] */
+  const int32_t* kept;        /* [n_rows] */
+  const int32_t* n_kept;      /* [n_seqs] */
+  int32_t* status;            /* may be NULL */
+} asterq_kv_keep_params;
+
+int asterq_kv_keep(const asterq_kv_keep_params* p, void* stream);
+
+/*
+ * Pages copied in all layers of a stack: page pairs[i][1] becomes a copy of pages pairs[i][0].  A pair with a negative
+ * entry is left out; so is, with *status 1, one with a page outside the pools, and every pair whose destination another
+ * pair names too or whose source another pair writes (what they leave would depend on the order).
+ */
+typedef struct asterq_kv_copy_params {
+  int32_t dtype;
+  int32_t n_layers;
+  int32_t n_kv_heads;
+  int32_t head_dim; /* a multiple of 8 */
+  int32_t page_tokens;
+  int32_t n_pairs;
+  int64_t n_pages;
+  void* const* k_pools;
+  void* const* v_pools;
+  const int32_t* pairs; /* [n_pairs][2], 8-byte aligned */
+  int32_t* status;      /* may be NULL */
+} asterq_kv_copy_params;
+
+int asterq_kv_copy_pages(const asterq_kv_copy_params* p, void* stream);
+
+/*
+ * Verification of drafted tokens.  Sequence s has the nodes row_offsets[s] <= r < row_offsets[s + 1] (at most 1024), node
+ * i at row row_offsets[s] + i; node 0 is the root, whose token is accepted already.  parents[r]: the parent's number
+ * among the sequence's nodes, below the node's own (-1 for the root); NULL: a chain.  target [n_rows][vocab]: the
+ * target's probabilities behind each node, rows that sum to 1; draft (or NULL) [n_rows][vocab]: those that a node's children
+ * were drawn from.  accept [n_rows] and sample [n_seqs]: random numbers in [0, 1).
+ * The walk starts at cur = 0 with r = target[cur] and m = 1 and goes through the nodes i = 1, 2, .. in their order.  Node i
+ * with parent cur and token x is accepted if accept[i] draft[cur][x] m < r(x) (draft[cur][x] = 1 without draft), and cur
+ * becomes i with r = target[i], m = 1.  Otherwise it is rejected: r = max(r - m draft[cur], 0) and m = sum of r, or, where that is 0,
+ * r = target[cur] and m = 1 again; without draft r(x) = 0 and m = m - r(x).  At the end the next token is the least t
+ * with r(0) + .. + r(t) > sample[s] (sum of r); where nothing is left of r it is drawn from target[cur].  In 64 bits.
+ * kept [n_rows]: the accepted nodes of each sequence from its first row on, the root first, then -1; n_kept [n_seqs]
+ * their number, next_token [n_seqs].  A sequence without nodes has 0 and -1.  A token outside the vocabulary is never accepted,
+ * a node whose parent is out of range is never reached, offsets out of order or too many nodes leave a sequence with 0
+ * and -1, a row without a positive sum gives the next token -1: all with *status 1.
+ */
+typedef struct asterq_verify_params {
+  int32_t dtype; /* of target and draft: ASTERQ_DTYPE_F32, _BF16 or _F16 */
+  int32_t n_seqs;
+  int32_t vocab;
+  int32_t reserved;
+  int64_t n_rows;
+  int64_t target_stride, draft_stride; /* from row to row, in elements */
+  const void* target;
+  const void* draft; /* may be NULL */
+  const int32_t* tokens;
+  const int32_t* parents; /* may be NULL */
+  const int32_t* row_offsets;
+  const float* accept;
+  const float* sample;
+  int32_t* kept;
+  int32_t* n_kept;
+  int32_t* next_token;
+  int32_t* status; /* may be NULL */
+} asterq_verify_params;
+
+int asterq_verify_drafts(const asterq_verify_params* p, void* stream);
+
+/*
  * Attention of one new token a sequence over such a cache:
  *   out[b][h] = sum over visible t of softmax(score) v_t,  score = softmax_scale q[b][h] . k_t
  *   (softcapped to logit_softcap tanh(score / logit_softcap) when logit_softcap > 0),
