@@ -13,10 +13,12 @@
 //
 // Rows.  The g = n_heads / n_kv_heads query heads of one kv head share its keys, so a tile of 128 rows is 128 / g
 // tokens times g heads.  A unit of work is two such tiles of one (sequence, kv head), which share the tiles of keys
-// and values that TMA brings; two warpgroups take a tile each, thread t row t, so that maxima and sums need no
-// shuffles, and one's exponentials run under the other's products.  A unit of at most 128 rows has both warpgroups on
-// the same rows and alternate tiles of keys; they join at its end, through tensor memory.
-// S = Q K^T (128 x 128) lies in tensor memory, its weights as 16-bit values over it, O beside it.
+// and values that TMA brings; a warpgroup takes each, thread t row t, so that maxima and sums need no shuffles, and one's
+// exponentials run under the other's products.  A unit of at most 128 rows has both warpgroups on the same rows and alternate
+// tiles of keys; they join at its end, through tensor memory.
+// S = Q K^T (128 x 128, fp32) lies in tensor memory, its weights as 16-bit values over it, O beside it.  The chain of a tile
+// (softmax, then product and next scores, 1,024 cycles of the tensor cores, and two waits of some 300 until one side sees
+// the other) is what sets the pace; the weights are handed over in halves to shorten it.
 //
 // Split.  The key tiles of all units laid end to end (with kUnitCost in front of each) are cut into equal contiguous
 // shares, one for each CTA, by sums over lengths and offsets that every CTA does for itself: no planning launch, no
@@ -31,7 +33,9 @@ namespace asterq {
 namespace rat {
 
 constexpr int kMaxWorkers = 256;
-constexpr int kThreads = 384, kWarps = 12;
+// Warps 0 to 7: softmax, a warpgroup a row tile; then loads, products, and two that look values over.  (With eight warps beside
+// the softmax the waiting ones alone slow the others: a wait reads shared memory, which the products keep busy.)
+constexpr int kThreads = 384, kWarps = 12, kLoads = 8, kProducts = 9, kLook = 10;
 constexpr int kRowsTile = 128;
 constexpr int kMaxNodes = 128;
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -62,22 +66,32 @@ struct Args {
   int n_seqs, n_heads, n_kv_heads, group, tile_tokens, unit_tokens;
   int page_tokens, max_pages, box_rows;
   int window, sink, reach;  // reach: newest tokens that a window shows, window - sink
-  int out_f32, premultiply;
+  int out_f32;
   float scale, scale2, softcap, cap_in;
 };
 
-template <bool kF16_, int D_>
+// kPre: scores are changed before their maximum is taken (a softcap, or a scale that is not positive)
+template <bool kF16_, int D_, bool kPre_>
 struct Cfg {
-  static constexpr bool kF16 = kF16_;
+  static constexpr bool kF16 = kF16_, kPre = kPre_;
   static constexpr int D = D_;
   static constexpr int kTiles = D == 256 ? 1 : 2;  // row tiles of a unit: two accumulators of 256 dims leave no room for scores
-  static constexpr int kKeys = D == 256 ? 64 : 128;
-  static constexpr int kRows = kTiles * kRowsTile;
-  static constexpr int kQBytes = kRowsTile * D * 2, kSlotBytes = kKeys * D * 2;
+  static constexpr int kRows = kTiles * kRowsTile, kKeys = D == 256 ? 64 : 128;
+  static constexpr int kQBytes = kRowsTile * D * 2, kSlotBytes = kKeys * D * 2;  // a slot holds a tile of keys or of values
   static constexpr int kSlots = D == 64 ? 12 : 5;
-  static constexpr int kColS = 0, kColO = 256, kStepS = 128, kStepO = D;
-  static constexpr int kSmall = 2048;  // barriers, work entries, parents, the sums of a joined pair
-  static constexpr int kSmem = 1024 + kTiles * kQBytes + kSlots * kSlotBytes + kSmall;
+  // columns of tensor memory: two places for scores and the weights over them (one for each row tile, or for every other
+  // tile of keys), then the accumulators
+  static constexpr int kColO = 2 * kKeys, kStepO = D;
+  static_assert(kColO + kTiles * D <= 512, "tensor memory");
+  // barriers: full, empty and looked over of each slot, the others by name; of scores one for each place, of weights for
+  // each place and half, so that whoever waits sees all phases of one
+  static constexpr int kEmpty = kSlots, kClean = 2 * kSlots, kQFull = 3 * kSlots, kQEmpty = kQFull + 1, kWFull = kQEmpty + 1,
+                       kWEmpty = kWFull + 2, kSFull = kWEmpty + 2, kPReady = kSFull + 2, kDone = kPReady + 4,
+                       kDrain = kDone + 2, kBars = kDrain + 1;
+  // behind the slots: barriers, two work entries, what threads exchange
+  static constexpr int kAtWork = (kBars * 8 + 15) / 16 * 16, kAtFlags = kAtWork + 160, kAtUp = kAtFlags + 16,
+                       kAtSwap = kAtUp + 2 * kMaxNodes, kSmall = kAtSwap + 2 * kRowsTile * 4;
+  static constexpr int kSmem = kTiles * kQBytes + kSlots * kSlotBytes + kSmall;
   static_assert(kSmem <= 232448, "more shared memory than a CTA has");
 };
 
@@ -105,6 +119,10 @@ ASTERQ_DEVICE bool named_all(int id, int count, bool pred) {
       : "memory");
   return r != 0;
 }
+
+// a value that all lanes have, known as such to the compiler: what comes of it stays in uniform registers, where the
+// tensor cores' instructions have their operands (otherwise each takes some 110 cycles to issue instead of 64)
+ASTERQ_DEVICE int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 
 constexpr uint32_t idesc(bool f16, int n, bool b_mn_major) {
   return (1u << 4) | ((f16 ? 0u : 1u) << 7) | ((f16 ? 0u : 1u) << 10) | ((b_mn_major ? 1u : 0u) << 16) |
@@ -195,9 +213,13 @@ struct View {
 };
 
 struct Start {
-  long long x;
   int s, head, block, at;
 };
+
+// a b / d; in 32 bits where that holds it, since a 64-bit division takes some hundred cycles
+ASTERQ_DEVICE long long share_of(long long a, int b, long long d) {
+  return a < (1 << 22) && d < (1ll << 31) ? (long long)((uint32_t)a * (uint32_t)b / (uint32_t)d) : a * b / d;
+}
 
 // tanh x to a few 2^-23 of itself: below 0.9 Lambert's continued fraction x / (1 + x^2 / (3 + x^2 / (5 + x^2 / (7 + x^2 / 9))))
 // as a quotient, its error x^10 / 9.8e6 < 2^-24; from there on (e^2x - 1) / (e^2x + 1).
@@ -221,54 +243,91 @@ ASTERQ_DEVICE uint32_t not_finite2(uint32_t w) {
   return ((w & e) == e ? 0xffffu : 0u) | ((w & (e << 16)) == (e << 16) ? 0xffff0000u : 0u);
 }
 
+template <bool kF16>
+ASTERQ_DEVICE bool all_finite(uint4 x) {
+  uint32_t s;
+  if constexpr (kF16) s = hfma2_u32(x.w, 0u, hfma2_u32(x.z, 0u, hfma2_u32(x.y, 0u, hmul2_u32(x.x, 0u))));
+  else s = tc::fma_bf162(x.w, 0u, tc::fma_bf162(x.z, 0u, tc::fma_bf162(x.y, 0u, tc::mul_bf162(x.x, 0u))));
+  return (s & 0x7fff7fffu) == 0;  // zeros of either sign
+}
+ASTERQ_DEVICE float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// the end of loads from tensor memory whose values are in r: nothing reads r before it
+ASTERQ_DEVICE void wait_ld32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                 "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+// A wait of a whole warp in few instructions, since the roles' loops together have to fit the instruction cache.  A round
+// suspends for up to 20 us, so the limit is some seconds.
+ASTERQ_DEVICE void wait_quietly(uint32_t bar, uint32_t parity, volatile int* abort_flag, int rounds = 1 << 18) {
+  if (mbar_try(bar, parity)) return;
+#pragma unroll 1
+  while (mbar_try_sleep(bar, parity, 20000u) == 0) {
+    if (--rounds < 0) *abort_flag = 1;
+    if (ld_shared_volatile(abort_flag)) break;
+  }
+}
+// false where a wait has run out
+ASTERQ_DEVICE bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort_flag, int rounds = 1 << 18) {
+  uint32_t done = mbar_try(bar, parity);
+#pragma unroll 1
+  while (done == 0 && (done = mbar_try_sleep(bar, parity, 20000u)) == 0) {
+    if (--rounds < 0) *abort_flag = 1;
+    if (ld_shared_volatile(abort_flag)) break;
+  }
+  return __all_sync(0xffffffffu, (int)done) != 0;
+}
+
 template <class C>
 __global__ void __launch_bounds__(kThreads, 1)
     rows_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                 const __grid_constant__ CUtensorMap v_map, const __grid_constant__ Args a) {
   constexpr int D = C::D, kKeys = C::kKeys;
   constexpr bool kF16 = C::kF16;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t q_base = smem_u32(smem), ring = q_base + C::kTiles * C::kQBytes;
   uint8_t* small = smem + C::kTiles * C::kQBytes + C::kSlots * C::kSlotBytes;
-  // barriers: full and empty of each slot, the others by name, and at the end whether a slot's values were looked over
   const uint32_t bars = smem_u32(small);
-  constexpr int kEmpty = C::kSlots, kQFull = 2 * C::kSlots, kQEmpty = kQFull + 1, kWFull = kQEmpty + 1, kWEmpty = kWFull + 2,
-                kSFull = kWEmpty + 2, kPReady = kSFull + 2, kOFull = kPReady + 2, kClean = kOFull + 2, kDrain = kClean + C::kSlots,
-                kBars = kDrain + 1;
-  static_assert(kBars * 8 <= 448, "barriers");
   auto bar = [&](int i) { return bars + 8 * i; };
-  Work* work = reinterpret_cast<Work*>(small + 448);                   // [2]
-  int8_t* up_s = reinterpret_cast<int8_t*>(small + 448 + 160);      // [2][kMaxNodes]
-  float* pair_s = reinterpret_cast<float*>(small + 448 + 160 + 256);   // [2][kRowsTile]: m and l of the second warpgroup
-  long long* scan_s = reinterpret_cast<long long*>(small + 448 + 160 + 256 + 1024);  // [kWarps]
-  Start* start_s = reinterpret_cast<Start*>(small + 448 + 160 + 256 + 1024 + 96);
-  uint32_t* tmem_s = reinterpret_cast<uint32_t*>(small + 448 + 160 + 256 + 1024 + 96 + 32);
+  Work* work = reinterpret_cast<Work*>(small + C::kAtWork);  // [2]
+  uint32_t* tmem_s = reinterpret_cast<uint32_t*>(small + C::kAtFlags);
   volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_s + 1);
   volatile int* never_s = reinterpret_cast<volatile int*>(tmem_s + 2);
-  static_assert(sizeof(Work) == 80 && sizeof(Start) <= 32 && 448 + 160 + 256 + 1024 + 96 + 32 + 12 <= C::kSmall, "small");
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, me = blockIdx.x;
+  int8_t* up_s = reinterpret_cast<int8_t*>(small + C::kAtUp);     // [2][kMaxNodes]: parents, for each row tile
+  float* swap_s = reinterpret_cast<float*>(small + C::kAtSwap);   // [2][kRowsTile]: m and l of a joined unit's second warpgroup
+  long long* scan_s = reinterpret_cast<long long*>(swap_s);       // [kWarps], and the share's start, before all that
+  Start* start_s = reinterpret_cast<Start*>(swap_s + kRowsTile);
+  static_assert(sizeof(Work) == 80 && sizeof(Start) <= kRowsTile * 4 && kWarps * 8 <= kRowsTile * 4, "small");
+  const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31, me = blockIdx.x;
 
   asm volatile("griddepcontrol.launch_dependents;");
   if (tid == 0) {
-    for (int i = 0; i < C::kSlots; ++i) {
-      mbar_init(bar(i), 1);
-      mbar_init(bar(kEmpty + i), 3);  // the products', and two warps that look values over
-      mbar_init(bar(kClean + i), 2);
+    for (int i = 0; i < C::kBars; ++i) {
+      int count = 1;
+      if (i >= C::kEmpty && i < C::kClean) count = 3;  // the products', and two warps that look values over
+      else if (i >= C::kClean && i < C::kQFull) count = 2;
+      else if (i >= C::kWEmpty && i < C::kSFull) count = 11;
+      else if (i >= C::kPReady && i < C::kDone) count = 4;  // a warp each
+      mbar_init(bar(i), count);
     }
-    mbar_init(bar(kQFull), 1);
-    mbar_init(bar(kQEmpty), 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(kWFull + i), 1);
-      mbar_init(bar(kWEmpty + i), 11);
-      mbar_init(bar(kSFull + i), 1);
-      mbar_init(bar(kPReady + i), 4);
-      mbar_init(bar(kOFull + i), 1);
-    }
-    mbar_init(bar(kDrain), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    *abort_s = 0;
+    // boxes lie in patterns of 1024 bytes
+    *abort_s = (q_base & 1023) != 0;
     *never_s = 0;
+  }
+  if (warp == kProducts) tc::alloc512(smem_u32(tmem_s));
+  if (warp == kLoads && lane < 3) {
+    const CUtensorMap* map = lane == 0 ? &q_map : lane == 1 ? &k_map : &v_map;
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
   }
 
   // ---------------------------------------------------------------------------------- the share
@@ -285,9 +344,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     any_bad = any_bad || bad;
     const int blocks = (q.n + a.unit_tokens - 1) / a.unit_tokens;
     long long cost = 0;
-    if (blocks <= 4)
-      for (int b = 0; b < blocks; ++b) cost += span_of<kKeys>(a, q, b).tiles + kUnitCost;
-    uint32_t many = __ballot_sync(0xffffffffu, blocks > 4);
+    if (blocks == 1) cost = span_of<kKeys>(a, q, 0).tiles + kUnitCost;
+    uint32_t many = __ballot_sync(0xffffffffu, blocks > 1);
+#pragma unroll 1
     while (many) {
       const int from = __ffs(many) - 1;
       many &= many - 1;
@@ -295,24 +354,31 @@ __global__ void __launch_bounds__(kThreads, 1)
       o.n = __shfl_sync(0xffffffffu, q.n, from);
       o.length = __shfl_sync(0xffffffffu, q.length, from);
       const int n = __shfl_sync(0xffffffffu, blocks, from);
-      long long sum = 0;
-      for (int b = lane; b < n; b += 32) sum += span_of<kKeys>(a, o, b).tiles + kUnitCost;
+      long long all = 0;
+#pragma unroll 1
+      for (int b = lane; b < n; b += 32) all += span_of<kKeys>(a, o, b).tiles + kUnitCost;
 #pragma unroll
-      for (int d = 1; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      if (lane == from) cost = sum;
+      for (int d = 1; d < 32; d *= 2) all += __shfl_xor_sync(0xffffffffu, all, d);
+      if (lane == from) cost = all;
     }
     return cost * a.n_kv_heads;
   };
-  long long sum = 0;
+  long long sum = 0, cost = 0;
+  Seq q;
+  q.n = 0;
+#pragma unroll 1
   for (int base = s_begin; base < s_end; base += 32) {
-    Seq q;
-    sum += costs_of(base, q);
+    cost = costs_of(base, q);
+    sum += cost;
   }
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   if (lane == 0) scan_s[warp] = sum;
   // offsets out of order or out of range: which rows are whose is not known, and the call is left undone
+  tc::fence_before();
   if (__syncthreads_or(any_bad)) {
+    tc::fence_after();
+    if (warp == kProducts) tc::dealloc512(*tmem_s);
     if (tid == 0) {
       a.desc[me].pieces = 0;
       if (a.status) atomicMax(a.status, 1);
@@ -320,18 +386,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
   long long before = 0, total = 0;
+#pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += scan_s[w];
-    total += scan_s[w];
+    const long long x = scan_s[w];
+    before += w < warp ? x : 0;
+    total += x;
   }
   // CTAs that take part: each has kMinShare tiles or more
   const int W = (int)max(1ll, min((long long)gridDim.x, total / kMinShare));
-  const long long x0 = total * min(me, W) / W, x1 = total * min(me + 1, W) / W;
+  const long long x0 = share_of(total, min(me, W), W), x1 = share_of(total, min(me + 1, W), W);
   if (x0 < x1 && before <= x0 && x0 < before + sum) {
     long long at = before;
+#pragma unroll 1
     for (int base = s_begin; base < s_end; base += 32) {
-      Seq q;
-      const long long cost = costs_of(base, q);
+      if (strip > 32) cost = costs_of(base, q);
       long long scan = cost;
 #pragma unroll
       for (int d = 1; d < 32; d *= 2) {
@@ -345,15 +413,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const int here = __ffs(beyond) - 1;
       at += __shfl_sync(0xffffffffu, scan - cost, here);
-      const long long head_cost = __shfl_sync(0xffffffffu, cost, here) / a.n_kv_heads;
+      const long long head_cost = share_of(__shfl_sync(0xffffffffu, cost, here), 1, a.n_kv_heads);
       Seq o;
       o.n = __shfl_sync(0xffffffffu, q.n, here);
       o.length = __shfl_sync(0xffffffffu, q.length, here);
-      const int head = (int)((x0 - at) / head_cost);
+      const int head = (int)share_of(x0 - at, 1, head_cost);
       long long rest = x0 - at - head * head_cost;
       const int blocks = (o.n + a.unit_tokens - 1) / a.unit_tokens;
+#pragma unroll 1
       for (int b0 = 0; b0 < blocks; b0 += 32) {
-        long long c = b0 + lane < blocks ? span_of<kKeys>(a, o, b0 + lane).tiles + kUnitCost : 0, up_to = c;
+        const int c = b0 + lane < blocks ? span_of<kKeys>(a, o, b0 + lane).tiles + kUnitCost : 0;
+        long long up_to = c;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
           const long long up = __shfl_up_sync(0xffffffffu, up_to, d);
@@ -364,96 +434,142 @@ __global__ void __launch_bounds__(kThreads, 1)
           rest -= __shfl_sync(0xffffffffu, up_to, 31);
           continue;
         }
-        const int l = __ffs(in) - 1;
-        if (lane == l) {
-          start_s->s = base + here;
-          start_s->head = head;
-          start_s->block = b0 + l;
-          start_s->at = (int)(rest - (up_to - c));
-        }
+        if (lane == __ffs(in) - 1) *start_s = {base + here, head, b0 + lane, (int)(rest - (up_to - c))};
         break;
       }
       break;
     }
   }
-  // rows that are not answered: zeros, and a log-sum of -inf
-  for (int base = (me * kWarps + warp) * 32; base < a.n_seqs; base += gridDim.x * kWarps * 32) {
-    bool bad = false;
-    int dead = 0;
-    Seq q;
-    q.n = 0;
-    if (base + lane < a.n_seqs) q = seq_of(a, base + lane, bad, dead);
-    if (dead > 0 && q.length >= 0 && a.status) atomicMax(a.status, 1);
-    uint32_t some = __ballot_sync(0xffffffffu, dead > 0);
-    while (some) {
-      const int from = __ffs(some) - 1;
-      some &= some - 1;
-      const long long row = __shfl_sync(0xffffffffu, q.row0 + q.n, from), rows = __shfl_sync(0xffffffffu, dead, from);
-      const long long w0 = row * a.n_heads * D, n = rows * a.n_heads * D;
-      for (long long i = lane * 8; i < n; i += 256) {
-        if (a.out_f32) {
-          float4* o = reinterpret_cast<float4*>(static_cast<float*>(a.out) + w0 + i);
-          o[0] = o[1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        } else {
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + w0 + i) = make_uint4(0, 0, 0, 0);
-        }
-      }
-      if (a.lse)
-        for (long long i = lane; i < rows * a.n_heads; i += 32) a.lse[row * a.n_heads + i] = -INFINITY;
-    }
-  }
-  __syncthreads();
-  if (x0 >= x1) {
-    if (tid == 0) a.desc[me].pieces = 0;
-    return;
-  }
-  if (warp == 9) tc::alloc512(smem_u32(tmem_s));
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  const uint32_t tmem = *tmem_s;
+  const uint32_t tmem = uniform(*tmem_s);
+  if (warp >= kLook) {
+    // rows that are not answered: zeros, and a log-sum of -inf
+#pragma unroll 1
+    for (int base = (me * 2 + warp - kLook) * 32; base < a.n_seqs; base += gridDim.x * 64) {
+      bool bad = false;
+      int dead = 0;
+      Seq o;
+      o.n = 0;
+      if (base + lane < a.n_seqs) o = seq_of(a, base + lane, bad, dead);
+      if (dead > 0 && o.length >= 0 && a.status) atomicMax(a.status, 1);
+      uint32_t some = __ballot_sync(0xffffffffu, dead > 0);
+#pragma unroll 1
+      while (some) {
+        const int from = __ffs(some) - 1;
+        some &= some - 1;
+        const long long row = __shfl_sync(0xffffffffu, o.row0 + o.n, from);
+        const long long n = (long long)__shfl_sync(0xffffffffu, dead, from) * a.n_heads;
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<char*>(a.out) + row * a.n_heads * D * (a.out_f32 ? 4 : 2));
+#pragma unroll 1
+        for (long long i = lane; i < n * (a.out_f32 ? D / 4 : D / 8); i += 32) dst[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+        for (long long i = lane; a.lse && i < n; i += 32) a.lse[row * a.n_heads + i] = -INFINITY;
+      }
+    }
+  }
+  if (x0 >= x1 || *abort_s) {
+    if (tid == 0) {
+      a.desc[me].pieces = 0;
+      if (*abort_s && a.status) atomicMax(a.status, 2);
+    }
+    if (warp == kProducts) tc::dealloc512(tmem);
+    return;
+  }
 
-  // tiles that some row of the unit does not see all of
-  auto partial = [&](const Work& u, int c) {
-    const bool seen = c + kKeys <= (a.parents ? u.length : u.length + u.tok0 + 1);
-    if (!seen) return true;
-    if (a.window == 0 || c + kKeys <= a.sink) return false;
-    const long long newest = (long long)u.length + (a.parents ? u.nodes : u.tok0 + u.tokens) - 1;
-    return c <= newest - a.reach;
+  // the keys that all rows of a unit see: below hi, and from lo on or in the sink
+  struct Seen {
+    int hi, lo;
+    ASTERQ_DEVICE bool all(int key, int sink) const { return key < hi && (key >= lo || key < sink); }
+    ASTERQ_DEVICE bool all_of_tile(int c, int sink) const { return c + kKeys <= hi && (c >= lo || c + kKeys <= sink); }
   };
-  // where a piece's tiles lie in the ring: K0 K1 V0 K2 V1 .., behind `base` uses of it
-  auto place_k = [](int j) { return j == 0 ? 0 : 2 * j - 1; };
-  auto place_v = [](int j, int n) { return j + 1 < n ? 2 * j + 2 : 2 * n - 1; };
-
-  if (warp >= 8) {
+  auto seen_of = [&](const Work& u) {
+    Seen s;
+    s.hi = a.parents ? u.length : u.length + u.tok0 + 1;
+    const long long newest = (long long)u.length + (a.parents ? u.nodes : u.tok0 + u.tokens) - 1;
+    s.lo = a.window == 0 ? 0 : (int)max(0ll, newest - a.reach + 1);
+    return s;
+  };
+  if (warp >= kLoads) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsHelp));
-    if (warp == 8) {
+    bool ok = true;
+    // each role follows the ring by itself
+    int slot = 0, phase = 0;
+    auto step = [&]() {
+      if (++slot == C::kSlots) {
+        slot = 0;
+        phase ^= 1;
+      }
+    };
+    if (warp == kLoads) {
       // ------------------------------------------------------------------------------ loads
       Desc desc;
       desc.pieces = 0;
-      bool ok = true;
       int s = start_s->s, head = start_s->head, block = start_s->block, at = start_s->at;
       long long x = x0;
       bool bad;
       int dead;
       Seq q = seq_of(a, s, bad, dead);
       Span span = span_of<kKeys>(a, q, block);
-      uint32_t base = 0;  // uses of the ring's slots
-      uint32_t q_bytes = 0;
       int pieces = 0;
-      const int boxes = kKeys / a.box_rows, halves = D / 64;
+      bool round = false;  // the slots have been used before
+      // one lane a box: box_rows keys (a divisor of the page and of the tile) of 64 dims
+      constexpr int halves = D / 64;
+      const int my_key = lane / halves * a.box_rows, my_half = lane % halves;
+      const bool works = my_key < kKeys;
       const uint32_t box_bytes = a.box_rows * 128;
-      const int my_box = lane / halves, my_half = lane % halves;  // one lane a box
+      const uint32_t box_at = ring + my_half * (kKeys * 128) + my_key * 128;
+      const int columns = kKeys / a.page_tokens, rest = kKeys - columns * a.page_tokens;  // from a tile to the next
+#pragma unroll 1
       while (ok && x < x1) {
         const int cost = (int)min((long long)(span.tiles + kUnitCost - at), x1 - x);
         const int k0 = max(at - kUnitCost, 0), n = max(at + cost - kUnitCost, 0) - k0;
         if (n > 0) {
+          // A tile's pages are looked up two tiles before it is wanted.
+          struct Box {
+            int page, offset;
+            bool want;
+          };
+          int k_at = k0, key = 0, column = 0, offset = 0;
+          const int* table = a.page_table + (long long)s * a.max_pages;
+          auto look_up = [&]() {
+            Box box = {0, 0, false};
+            if (k_at < k0 + n) {
+              if (k_at == k0 || k_at == span.sink_tiles) {
+                key = (k_at < span.sink_tiles ? k_at : span.first + (k_at - span.sink_tiles)) * kKeys + my_key;
+                column = key / a.page_tokens;
+                offset = key - column * a.page_tokens;
+              }
+              box.offset = offset;
+              box.want = works && key < span.end && (key < a.sink || key + a.box_rows > span.from);
+              if (box.want) box.page = __ldg(table + column);
+              key += kKeys;
+              column += columns;
+              offset += rest;
+              if (offset >= a.page_tokens) {
+                offset -= a.page_tokens;
+                ++column;
+              }
+              ++k_at;
+            }
+            return box;
+          };
+          Box now = look_up(), ahead = look_up();
+          // queries
+          if (pieces > 0 && !(ok = wait_for(bar(C::kQEmpty), (pieces - 1) & 1, abort_s))) break;
+          const int q_tiles = span.tokens > a.tile_tokens ? 2 : 1;
+          if (lane == 0) mbar_expect_tx(bar(C::kQFull), q_tiles * halves * a.tile_tokens * a.group * 128);
+          __syncwarp();
+          if (lane < q_tiles * halves) {
+            const int t = lane / halves, h = lane % halves;
+            tma_q(q_base + t * C::kQBytes + h * (kRowsTile * 128), &q_map, h * 64, head * a.group,
+                  q.row0 + span.tok0 + t * a.tile_tokens, bar(C::kQFull));
+          }
           const int e = pieces & 1;
-          if (pieces >= 2) ok = mbar_wait(bar(kWEmpty + e), ((pieces >> 1) - 1) & 1, abort_s);
-          ok = __all_sync(0xffffffffu, (int)ok) != 0;
-          if (!ok) break;
-          const bool cut = n < span.tiles;
+          if (pieces >= 2 && !(ok = wait_for(bar(C::kWEmpty + e), ((pieces >> 1) - 1) & 1, abort_s))) break;
           if (lane == 0) {
+            const bool cut = n < span.tiles;
             Work u;
             u.n = n;
             u.k0 = k0;
@@ -466,70 +582,50 @@ __global__ void __launch_bounds__(kThreads, 1)
             u.tok0 = span.tok0;
             u.from = span.from;
             u.seq_row0 = q.row0;
-            u.seq = s;
             u.nodes = span.tok0 + span.tokens;
+            u.seq = s;
             u.pair = C::kTiles == 2 && span.tokens <= a.tile_tokens;
             u.cut = cut;
             u.slot = 2 * me + (k0 == 0);
             u.poison = 0;
             work[e] = u;
-            mbar_arrive(bar(kWFull + e));
+            mbar_arrive(bar(C::kWFull + e));
             if (cut && k0 == 0) {
               // the pieces after this one are in the next CTAs' first slots
               const long long u1 = x - at + kUnitCost + span.tiles;
-              desc.pieces = (int)((u1 * W - 1) / total) - me + 1;
+              desc.pieces = (int)(u1 < (1 << 22) ? (uint32_t)(u1 * W - 1) / (uint32_t)total : (u1 * W - 1) / total) - me + 1;
               desc.row0 = u.row0;
               desc.tokens = u.tokens;
               desc.head = head;
             }
           }
           __syncwarp();
-          // queries
-          if (pieces > 0) ok = mbar_wait(bar(kQEmpty), (pieces - 1) & 1, abort_s);
-          ok = __all_sync(0xffffffffu, (int)ok) != 0;
-          if (!ok) break;
-          const int q_tiles = span.tokens > a.tile_tokens ? 2 : 1;
-          q_bytes = q_tiles * halves * a.tile_tokens * a.group * 128;
-          if (lane == 0) mbar_expect_tx(bar(kQFull), q_bytes);
-          __syncwarp();
-          if (lane < q_tiles * halves) {
-            const int t = lane / halves, h = lane % halves;
-            tma_q(q_base + t * C::kQBytes + h * (kRowsTile * 128), &q_map, h * 64, head * a.group,
-                  q.row0 + span.tok0 + t * a.tile_tokens, bar(kQFull));
-          }
           ++pieces;
           // keys and values
-          for (int i = 0; i < 2 * n && ok; ++i) {
-            // position i of K0 K1 V0 K2 V1 .. K(n-1) V(n-2) V(n-1)
-            const bool is_v = i == 2 * n - 1 || (i > 0 && (i & 1) == 0);
-            const int j = i == 2 * n - 1 ? n - 1 : i == 0 ? 0 : is_v ? i / 2 - 1 : (i + 1) / 2;
-            const uint32_t use = base + i, slot = use % C::kSlots, round = use / C::kSlots;
-            const int k = k0 + j, tile = k < span.sink_tiles ? k : span.first + (k - span.sink_tiles);
-            const int token = tile * kKeys + my_box * a.box_rows;
-            const bool want = lane < boxes * halves && token < span.end &&
-                              (token < a.sink || token + a.box_rows > span.from);
-            int page = 0, column = 0;
-            if (want) {
-              column = token / a.page_tokens;
-              page = __ldg(a.page_table + (long long)s * a.max_pages + column);
+#pragma unroll 1
+          for (int i = 0; i < n; ++i) {
+            const Box later = look_up();
+            const uint32_t wanted = __ballot_sync(0xffffffffu, now.want);
+            int page = now.page;
+            if (now.want && (page < 0 || page >= a.n_pages)) {
+              if (a.status) atomicMax(a.status, 1);
+              page = 0;
             }
-            if (round > 0) ok = mbar_wait(bar(kEmpty + slot), (round - 1) & 1, abort_s);
-            ok = __all_sync(0xffffffffu, (int)ok) != 0;
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+              if (round && !(ok = wait_for(bar(C::kEmpty + slot), phase ^ 1, abort_s))) break;
+              if (lane == 0) mbar_expect_tx(bar(slot), __popc(wanted) * box_bytes);
+              __syncwarp();
+              if (now.want)
+                tma_kv(box_at + slot * C::kSlotBytes, v ? &v_map : &k_map, now.offset, my_half, page * a.n_kv_heads + head, bar(slot));
+              step();
+              if (slot == 0) round = true;
+            }
             if (!ok) break;
-            const uint32_t wanted = __ballot_sync(0xffffffffu, want);
-            if (lane == 0) mbar_expect_tx(bar(slot), __popc(wanted) * box_bytes);
-            __syncwarp();
-            if (want) {
-              if (page < 0 || page >= a.n_pages) {
-                if (a.status) atomicMax(a.status, 1);
-                page = 0;
-              }
-              tma_kv(ring + slot * C::kSlotBytes + my_half * (kKeys * 128) + my_box * box_bytes, is_v ? &v_map : &k_map,
-                     token - column * a.page_tokens, my_half, page * a.n_kv_heads + head, bar(slot));
-            }
+            now = ahead;
+            ahead = later;
           }
           if (!ok) break;
-          base += 2 * n;
         }
         x += cost;
         at += cost;
@@ -540,6 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             block = 0;
             if (++head == a.n_kv_heads) {
               head = 0;
+#pragma unroll 1
               do q = seq_of(a, ++s, bad, dead);
               while (q.n == 0);
             }
@@ -549,372 +646,415 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (ok) {
         const int e = pieces & 1;
-        if (pieces >= 2) ok = mbar_wait(bar(kWEmpty + e), ((pieces >> 1) - 1) & 1, abort_s);
-        ok = __all_sync(0xffffffffu, (int)ok) != 0;
+        if (pieces >= 2) ok = wait_for(bar(C::kWEmpty + e), ((pieces >> 1) - 1) & 1, abort_s);
         if (ok && lane == 0) {
           work[e].n = 0;
-          mbar_arrive(bar(kWFull + e));
+          mbar_arrive(bar(C::kWFull + e));
         }
       }
       if (!ok) {
-        // the last copies have landed before the exit, also when nobody waits for them any more: each slot's barrier
-        // ends a phase that it is in within the limit, or has ended the ones begun
-        __syncwarp();
-        for (int i = 0; i <= kQFull; i = i + 1 == C::kSlots ? kQFull : i + 1)
-          for (int parity = 0; parity < 2; ++parity) (void)mbar_wait(bar(i), parity, never_s, 50000000);
+        // the last copies have landed before the exit, also when nobody waits for them any more: each barrier
+        // ends the phase that it is in within the limit, or has ended the ones begun
+#pragma unroll 1
+        for (int i = 0; i < 2 * (C::kSlots + 1); ++i)
+          (void)wait_for(bar(i / 2 == C::kSlots ? C::kQFull : i / 2), i & 1, never_s, 1000);
       }
       if (lane == 0) a.desc[me] = desc;
-    } else if (warp == 9) {
+    } else if (warp == kProducts) {
       // ------------------------------------------------------------------------------ products
+      // Job i of a unit: a row tile's scores with a tile of keys, and its weights' product.  The scores of job i + 2, which take
+      // the place of job i's weights, are asked for right behind that product.
       constexpr uint32_t kQk = idesc(kF16, kKeys, false), kPv = idesc(kF16, D, true);
-      bool ok = true;
-      uint32_t base = 0, s_ready[2] = {0, 0};
-      for (int piece = 0; ok; ++piece) {
-        const int e = piece & 1;
-        ok = mbar_wait(bar(kWFull + e), (piece >> 1) & 1, abort_s);
-        ok = __all_sync(0xffffffffu, (int)ok) != 0;
-        if (!ok) break;
-        const Work u = work[e];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(kWEmpty + e));
-        if (u.n == 0) break;
-        ok = mbar_wait(bar(kQFull), piece & 1, abort_s);
-        auto slot_of = [&](int place) { return (base + place) % C::kSlots; };
-        auto wait_slot = [&](int place) {
-          const uint32_t use = base + place;
-          ok = ok && mbar_wait(bar(use % C::kSlots), (use / C::kSlots) & 1, abort_s);
-        };
-        auto qk = [&](int stream, int row_tile, int j) {
-          const uint32_t q0 = tc::desc_k_major(q_base + row_tile * C::kQBytes);
-          const uint32_t k0 = tc::desc_k_major(ring + slot_of(place_k(j)) * C::kSlotBytes);
-          if (tc::elect()) {
-#pragma unroll
-            for (int s = 0; s < D / 16; ++s)
-              tc::mma_ss(tmem + C::kColS + stream * C::kStepS, q0 + s / 4 * (kRowsTile * 8) + s % 4 * 2,
-                         k0 + s / 4 * (kKeys * 8) + s % 4 * 2, kQk, s > 0);
-            tc::commit(bar(kSFull + stream));
-          }
-          __syncwarp();
-        };
-        auto pv = [&](int stream, int j, bool first) {
-          const uint32_t v0 = tc::desc_mn_major(ring + slot_of(place_v(j, u.n)) * C::kSlotBytes, kKeys * 128);
-          ok = ok && mbar_wait(bar(kPReady + stream), s_ready[stream] & 1, abort_s);
-          ++s_ready[stream];
-          ok = __all_sync(0xffffffffu, (int)ok) != 0;
-          if (!ok) return;
-          tc::fence_after();
-          if (tc::elect()) {
-#pragma unroll
-            for (int s = 0; s < kKeys / 16; ++s)
-              tc::mma_ts(tmem + C::kColO + stream * C::kStepO, tmem + C::kColS + stream * C::kStepS + 8 * s, v0 + s * 128,
-                         kPv, !first || s > 0);
-          }
-          __syncwarp();
-        };
-        auto wait_values = [&](int j) {
-          wait_slot(place_v(j, u.n));
-          if (partial(u, u.tile(u.k0 + j) * kKeys)) {
-            const uint32_t use = base + place_v(j, u.n);
-            ok = ok && mbar_wait(bar(kClean + use % C::kSlots), (use / C::kSlots) & 1, abort_s);
-          }
-        };
-        auto signal = [&](int b) {
-          if (tc::elect()) tc::commit(bar(b));
-          __syncwarp();
-        };
-        const int streams = C::kTiles == 2 ? 2 : 1;
-        wait_slot(place_k(0));
-        ok = __all_sync(0xffffffffu, (int)ok) != 0;
-        if (!ok) break;
-        if (u.pair) {
-          qk(0, 0, 0);
-          signal(kEmpty + slot_of(place_k(0)));
-          if (u.n > 1) {
-            wait_slot(place_k(1));
-            ok = __all_sync(0xffffffffu, (int)ok) != 0;
-            if (!ok) break;
-            qk(1, 0, 1);
-            signal(kEmpty + slot_of(place_k(1)));
-          }
-          if (u.n <= 2) signal(kQEmpty);
-          for (int j = 0; j < u.n && ok; ++j) {
-            wait_values(j);
-            pv(j & 1, j, j < 2);
-            if (!ok) break;
-            signal(kEmpty + slot_of(place_v(j, u.n)));
-            if (j + 2 < u.n) {
-              wait_slot(place_k(j + 2));
-              ok = __all_sync(0xffffffffu, (int)ok) != 0;
-              if (!ok) break;
-              qk(j & 1, 0, j + 2);
-              signal(kEmpty + slot_of(place_k(j + 2)));
-              if (j + 3 == u.n) signal(kQEmpty);
-            }
-          }
-          if (!ok) break;
-          signal(kOFull);
-          signal(kOFull + 1);
-        } else {
-          for (int t = 0; t < streams; ++t) qk(t, t, 0);
-          signal(kEmpty + slot_of(place_k(0)));
-          if (u.n == 1) signal(kQEmpty);
-          for (int j = 0; j < u.n && ok; ++j) {
-            wait_values(j);
-            for (int t = 0; t < streams && ok; ++t) {
-              pv(t, j, j == 0);
-              if (!ok) break;
-              if (t + 1 == streams) signal(kEmpty + slot_of(place_v(j, u.n)));
-              if (j + 1 == u.n) signal(kOFull + t);
-              if (j + 1 < u.n) {
-                if (t == 0) wait_slot(place_k(j + 1));
-                ok = __all_sync(0xffffffffu, (int)ok) != 0;
-                if (!ok) break;
-                qk(t, t, j + 1);
-                if (t + 1 == streams) {
-                  signal(kEmpty + slot_of(place_k(j + 1)));
-                  if (j + 2 == u.n) signal(kQEmpty);
-                }
-              }
-            }
-          }
-          if (!ok) break;
+      uint32_t weights = 0;            // phases of kPReady, a bit a place
+      int v_slot = 0, v_phase = 0;     // of the next values; slot and phase: of the next keys
+      auto next_tile = [&](int& s, int& ph) {  // keys and values take the slots in turn
+        s += 2;
+        if (s >= C::kSlots) {
+          s -= C::kSlots;
+          ph ^= 1;
         }
-        base += 2 * u.n;
+      };
+      v_slot = 1;
+#pragma unroll 1
+      for (int piece = 0;; ++piece) {
+        const int e = piece & 1;
+        if (!(ok = wait_for(bar(C::kWFull + e), (piece >> 1) & 1, abort_s))) break;
+        const int n = uniform(work[e].n), pair = uniform(work[e].pair);
+        const int k0 = uniform(work[e].k0), sink_tiles = uniform(work[e].sink_tiles), first = uniform(work[e].first);
+        Seen seen_all = seen_of(work[e]);
+        seen_all.hi = uniform(seen_all.hi);
+        seen_all.lo = uniform(seen_all.lo);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::kWEmpty + e));
+        if (n == 0) break;
+        if (!(ok = wait_for(bar(C::kQFull), piece & 1, abort_s))) break;
+        const bool both = C::kTiles == 2 && !pair;  // two row tiles to each tile of keys
+        const int jobs = both ? 2 * n : n;
+        int j = 0;  // tile of keys of job i
+#pragma unroll 1
+        for (int i = -2; i < jobs; ++i) {
+          const int b = i & 1;
+          const bool last = !both || b == 1;  // the last job of its tile of keys
+          const uint32_t s_at = uniform(tmem + b * kKeys);
+          if (i >= 0) {
+            if (!both || b == 0) {
+              const int k = k0 + j, c = (k < sink_tiles ? k : first + (k - sink_tiles)) * kKeys;
+              if (!(ok = wait_for(bar((seen_all.all_of_tile(c, a.sink) ? 0 : C::kClean) + v_slot), v_phase, abort_s))) break;
+            }
+            const uint32_t v0 = uniform(tc::desc_mn_major(ring + v_slot * C::kSlotBytes, kKeys * 128));
+            const uint32_t d = tmem + C::kColO + (C::kTiles == 2 ? b : 0) * C::kStepO;
+            const bool add = i >= C::kTiles;
+            if (!(ok = wait_for(bar(C::kPReady + 2 * b), weights >> b & 1, abort_s))) break;
+            tc::fence_after();
+            if (tc::elect()) {
+#pragma unroll
+              for (int s = 0; s < kKeys / 32; ++s) tc::mma_ts(d, s_at + 8 * s, v0 + s * 128, kPv, add || s > 0);
+            }
+            __syncwarp();
+            if (i + 2 < jobs && (!both || b == 0) && !(ok = wait_for(bar(slot), phase, abort_s))) break;
+            if (!(ok = wait_for(bar(C::kPReady + 2 * b + 1), weights >> b & 1, abort_s))) break;
+            weights ^= 1u << b;
+            tc::fence_after();
+            if (tc::elect()) {
+#pragma unroll
+              for (int s = kKeys / 32; s < kKeys / 16; ++s) tc::mma_ts(d, s_at + 8 * s, v0 + s * 128, kPv, true);
+              if (last) tc::commit(bar(C::kEmpty + v_slot));
+              if (i + C::kTiles >= jobs) tc::commit(bar(C::kDone + (C::kTiles == 2 ? b : 0)));
+              if (C::kTiles == 1) tc::commit(bar(C::kDone + 1));  // of each job
+            }
+            __syncwarp();
+            if (last) {
+              next_tile(v_slot, v_phase);
+              ++j;
+            }
+          } else if (i + 2 < jobs && (!both || b == 0) && !(ok = wait_for(bar(slot), phase, abort_s))) {
+            break;
+          }
+          if (i + 2 < jobs) {
+            const uint32_t q0 = uniform(tc::desc_k_major(q_base + (both ? b : 0) * C::kQBytes));
+            const uint32_t kd = uniform(tc::desc_k_major(ring + slot * C::kSlotBytes));
+            if (tc::elect()) {
+#pragma unroll
+              for (int s = 0; s < D / 16; ++s)
+                tc::mma_ss(s_at, q0 + s / 4 * (kRowsTile * 8) + s % 4 * 2, kd + s / 4 * (kKeys * 8) + s % 4 * 2, kQk, s > 0);
+              tc::commit(bar(C::kSFull + b));
+              if (last) tc::commit(bar(C::kEmpty + slot));
+              if (i + 3 == jobs) tc::commit(bar(C::kQEmpty));
+            }
+            __syncwarp();
+            if (last) next_tile(slot, phase);
+          }
+        }
+        if (!ok) break;
       }
       if (!ok) {  // products under way end before tensor memory goes
+        if (tc::elect()) tc::commit(bar(C::kDrain));
         __syncwarp();
-        if (tc::elect()) tc::commit(bar(kDrain));
-        __syncwarp();
-        (void)mbar_wait(bar(kDrain), 0, never_s, 200000000);
+        (void)wait_for(bar(C::kDrain), 0, never_s, 10000);
       }
     } else {
       // ------------------------------------------------------------------------------ values looked over
       // In a tile that not every row sees all of, a weight of zero meets values that the row does not see, and zero
       // times an infinity or NaN is not zero.  Values that no row sees become zeros; of the others those that are not
       // finite do, and the rows' threads add them where they are seen (poison).
-      bool ok = true;
-      uint32_t base = 0;
-      const int part = warp - 10;
-      for (int piece = 0; ok; ++piece) {
-        const int e = piece & 1;
-        ok = mbar_wait(bar(kWFull + e), (piece >> 1) & 1, abort_s);
-        ok = __all_sync(0xffffffffu, (int)ok) != 0;
-        if (!ok) break;
-        const Work u = work[e];
-        const int end = u.length + u.nodes;
-        if (u.n > 0) {
-          for (int i = 0; i < 2 * u.n && ok; ++i) {
-            const bool is_v = i == 2 * u.n - 1 || (i > 0 && (i & 1) == 0);
-            const int j = i == 2 * u.n - 1 ? u.n - 1 : i / 2 - 1;
-            const uint32_t use = base + i, slot = use % C::kSlots;
-            ok = mbar_wait(bar(slot), (use / C::kSlots) & 1, abort_s);
-            ok = __all_sync(0xffffffffu, (int)ok) != 0;
-            if (!ok) break;
-            const int c = is_v ? u.tile(u.k0 + j) * kKeys : 0;
-            if (is_v && partial(u, c)) {
-              uint4* v = reinterpret_cast<uint4*>(smem + C::kTiles * C::kQBytes + slot * C::kSlotBytes);
-              bool found = false;
-              constexpr int kAll = C::kSlotBytes / 16, kEach = kAll / 64, kBatch = 8;
+      const int part = warp - kLook;
 #pragma unroll 1
-              for (int r = 0; r < kEach; r += kBatch) {
-                uint4 w[kBatch];
-#pragma unroll
-                for (int b = 0; b < kBatch; ++b) w[b] = v[(r + b) * 64 + part * 32 + lane];
-#pragma unroll
-                for (int b = 0; b < kBatch; ++b) {
-                  const int at = (r + b) * 64 + part * 32 + lane, token = c + (at / 8) % kKeys;
-                  const bool seen = token < end && (token >= u.from || token < a.sink);
-                  uint4 mask;
-                  mask.x = not_finite2<kF16>(w[b].x);
-                  mask.y = not_finite2<kF16>(w[b].y);
-                  mask.z = not_finite2<kF16>(w[b].z);
-                  mask.w = not_finite2<kF16>(w[b].w);
-                  const bool odd = (mask.x | mask.y | mask.z | mask.w) != 0;
-                  if (!seen || odd) {
-                    found = found || seen;
-                    v[at] = seen ? make_uint4(w[b].x & ~mask.x, w[b].y & ~mask.y, w[b].z & ~mask.z, w[b].w & ~mask.w)
-                                 : make_uint4(0, 0, 0, 0);
-                  }
-                }
-              }
-              if (found) *reinterpret_cast<volatile int*>(&work[e].poison) = 1;
-              fence_async_shared();
-            }
-            __syncwarp();
-            if (lane == 0) {  // for every use, so that no phase is left out
-              mbar_arrive(bar(kClean + slot));
-              mbar_arrive(bar(kEmpty + slot));
-            }
+      for (int piece = 0;; ++piece) {
+        const int e = piece & 1;
+        if (!(ok = wait_for(bar(C::kWFull + e), (piece >> 1) & 1, abort_s))) break;
+        const int n = work[e].n, k0 = work[e].k0, sink_tiles = work[e].sink_tiles, first = work[e].first;
+        const int end = work[e].length + work[e].nodes, from = work[e].from;
+        const Seen seen_all = seen_of(work[e]);
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+          if (!(ok = wait_for(bar(slot), phase, abort_s))) break;
+          if (lane == 0) {  // keys
+            mbar_arrive(bar(C::kClean + slot));
+            mbar_arrive(bar(C::kEmpty + slot));
           }
+          step();
+          if (!(ok = wait_for(bar(slot), phase, abort_s))) break;
+          const int k = k0 + i, c = (k < sink_tiles ? k : first + (k - sink_tiles)) * kKeys;
+          if (!seen_all.all_of_tile(c, a.sink)) {
+            uint4* v = reinterpret_cast<uint4*>(smem + C::kTiles * C::kQBytes + slot * C::kSlotBytes);
+            constexpr int kAll = C::kSlotBytes / 16 / 64;  // vectors a lane
+            uint4* mine = v + part * 32 + lane;
+            if (c + kKeys > end || (c < from && c + kKeys > a.sink)) {
+#pragma unroll 1
+              for (int x = 0; x < kAll; ++x) {
+                const int key = c + (x * 8 + part * 4 + lane / 8) % kKeys;
+                if (key >= end || (key < from && key >= a.sink)) mine[64 * x] = make_uint4(0, 0, 0, 0);
+              }
+            }
+            // A sum of zero times each value is zero, or a NaN where one of them is not finite.
+            bool found = false;
+            constexpr int kBatch = 8;
+#pragma unroll 1
+            for (int x0 = 0; x0 < kAll; x0 += kBatch) {
+              uint4 w[kBatch];
+#pragma unroll
+              for (int x = 0; x < kBatch; ++x) w[x] = mine[64 * (x0 + x)];
+              bool fine = true;
+#pragma unroll
+              for (int x = 0; x < kBatch; ++x) fine = all_finite<kF16>(w[x]) && fine;
+              if (__all_sync(0xffffffffu, fine)) continue;
+#pragma unroll 1
+              for (int x = x0; x < x0 + kBatch; ++x) {
+                uint4 o = mine[64 * x];
+                if (all_finite<kF16>(o)) continue;
+                o.x &= ~not_finite2<kF16>(o.x);
+                o.y &= ~not_finite2<kF16>(o.y);
+                o.z &= ~not_finite2<kF16>(o.z);
+                o.w &= ~not_finite2<kF16>(o.w);
+                mine[64 * x] = o;
+                found = true;
+              }
+            }
+            if (found) *reinterpret_cast<volatile int*>(&work[e].poison) = 1;
+            fence_async_shared();
+          }
+          __syncwarp();
+          if (lane == 0) {  // for every use, so that no phase is left out
+            mbar_arrive(bar(C::kClean + slot));
+            mbar_arrive(bar(C::kEmpty + slot));
+          }
+          step();
         }
+        if (!ok) break;
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(kWEmpty + e));
-        if (u.n == 0) break;
-        base += 2 * u.n;
+        if (lane == 0) mbar_arrive(bar(C::kWEmpty + e));
+        if (n == 0) break;
       }
     }
   } else {
     // -------------------------------------------------------------------------------- softmax, one row a thread
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-    const int stream = warp >> 2, r = tid & 127, wg = stream;
+    const int tile = warp >> 2, r = tid & 127;
     const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
-    const uint32_t col_s = lanes + C::kColS + stream * C::kStepS, col_o = lanes + C::kColO + stream * C::kStepO;
+    const uint32_t col_o = lanes + C::kColO + tile * C::kStepO;
     const int token_in = r / a.group, head_in = r - token_in * a.group;
     const bool in_tile = token_in < a.tile_tokens;
-    const float scale2 = a.premultiply ? 1.0f : a.scale2;
-    uint32_t tiles_done = 0, units_done = 0;
+    const float scale2 = C::kPre ? 1.0f : a.scale2;
+    uint32_t full = 0, done = 0, rests = 0;  // phases: of kSFull (a bit a place) and kDone; jobs so far
+    View view;
+    int view_row = -1, view_tok0 = 0;
+    bool view_pair = false;
+#pragma unroll 1
     for (int piece = 0;; ++piece) {
       const int e = piece & 1;
-      bool got = mbar_wait(bar(kWFull + e), (piece >> 1) & 1, abort_s);
+      const bool got = wait_for(bar(C::kWFull + e), (piece >> 1) & 1, abort_s);
       // all warps go on or none does: they meet at barriers (after a wait has run out, waits return at once)
       if (!named_all(1, 256, got)) break;
       const Work* u = work + e;
       const int n = u->n, k0 = u->k0;
       if (n == 0) break;
-      if (C::kTiles == 1 && stream == 1) {  // one row tile: the second warpgroup has nothing to do
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(kWEmpty + e));
+      if (C::kTiles == 1 && tile == 1) {  // one row tile: these have nothing to do
+        if (lane == 0) mbar_arrive(bar(C::kWEmpty + e));
         continue;
       }
       const bool pair = u->pair;
-      const int token = token_in + (pair ? 0 : stream * a.tile_tokens);  // of the unit
+      const int token = token_in + (pair ? 0 : tile * a.tile_tokens);  // of the unit
       const bool valid = in_tile && token < u->tokens;
-      View view;
-      view.length = u->length;
-      {
+      // heads of one tree's rows in turn: what they see is the same
+      if (!(a.parents && view_row == u->seq_row0 && view_tok0 == u->tok0 && view_pair == pair)) {
+        view_row = u->seq_row0;
+        view_tok0 = u->tok0;
+        view_pair = pair;
+        view.length = u->length;
         int position = u->length + u->tok0 + token;
+        view.hi = position + 1;
         if (a.parents) {
           // the sequence's nodes up to the unit's end, then a walk up from the row's own
-          const int nodes = u->nodes;
-          int8_t* up = up_s + wg * kMaxNodes;
+          int8_t* up = up_s + tile * kMaxNodes;
           const int me_in = tid & 127;
-          if (me_in < nodes) {
+          if (me_in < u->nodes) {
             const int p = __ldg(a.parents + u->seq_row0 + me_in);
             const bool fine = p >= -1 && p < me_in;
             if (!fine && a.status) atomicMax(a.status, 1);
             up[me_in] = (int8_t)(fine ? p : -1);
           }
-          named_sync(2 + wg, 128);
+          named_sync(2 + tile, 128);
           const int own = u->tok0 + token;
-          int depth = 0;
 #pragma unroll
           for (int i = 0; i < kMaxNodes / 32; ++i) view.node[i] = 0;
           if (valid) {
-            for (int i = up[own]; i >= 0; i = up[i]) ++depth;
-            position = u->length + depth;
+            position = u->length;
+#pragma unroll 1
+            for (int i = up[own]; i >= 0; i = up[i]) ++position;
             int at = position;
+#pragma unroll 1
             for (int i = own; i >= 0; i = up[i], --at) {
               const bool seen = a.window == 0 || at > position - a.reach || at < a.sink;
 #pragma unroll
               for (int k = 0; k < kMaxNodes / 32; ++k) view.node[k] |= seen && (i >> 5) == k ? 1u << (i & 31) : 0u;
             }
           }
-          named_sync(2 + wg, 128);
+          named_sync(2 + tile, 128);
           view.hi = u->length;
-        } else {
-          view.hi = position + 1;
         }
         view.lo = a.window == 0 ? 0 : max(0, position - a.reach + 1);
         view.sink = a.window == 0 ? 0 : min(a.sink, view.hi);
       }
       float m = -INFINITY, l = 0.0f;  // m: what exponents are taken from (log2 units), at most 8 below the maximum
-      const int step = pair ? 2 : 1, mine = pair ? (n - stream + 1) / 2 : n;
-      for (int i = 0; i < mine; ++i) {
-        const int c = u->tile(k0 + (pair ? stream + step * i : i)) * kKeys;
-        (void)mbar_wait(bar(kSFull + stream), tiles_done & 1, abort_s);
-        ++tiles_done;
+      const bool rows_here = __any_sync(0xffffffffu, valid);
+      const Seen seen_all = seen_of(*u);
+      const int sink_tiles = u->sink_tiles, gap = (u->first - sink_tiles) * kKeys;
+      const int jobs = C::kTiles == 2 && !pair ? 2 * n : n;
+#pragma unroll 1
+      for (int i = C::kTiles == 2 ? tile : 0; i < jobs; i += C::kTiles) {
+        const int k_at = k0 + (C::kTiles == 2 && !pair ? i >> 1 : i), c = k_at * kKeys + (k_at < sink_tiles ? 0 : gap);
+        const int b = i & 1;
+        const uint32_t s_at = lanes + b * kKeys, p_ready = bar(C::kPReady + 2 * b);
+        wait_quietly(bar(C::kSFull + b), full >> b & 1, abort_s);
+        full ^= 1u << b;
         __syncwarp();
         tc::fence_after();
-        uint32_t raw[kKeys / 32][32];
-#pragma unroll
-        for (int k = 0; k < kKeys / 32; ++k) tc::ld32(raw[k], col_s + 32 * k);
-        tc::wait_ld();
-        float s[kKeys];
-#pragma unroll
-        for (int k = 0; k < kKeys; ++k) s[k] = __uint_as_float(raw[k / 32][k % 32]);
-        if (a.premultiply) {
-          if (a.softcap > 0.0f) {
-#pragma unroll
-            for (int k = 0; k < kKeys; ++k) s[k] = a.softcap * kLog2e * tanh_of(s[k] * a.cap_in);
-          } else {
-#pragma unroll
-            for (int k = 0; k < kKeys; ++k) s[k] *= a.scale2;
-          }
-        }
-        if (partial(*u, c)) {
-#pragma unroll
-          for (int k = 0; k < kKeys / 32; ++k) {
-            const uint32_t w = a.parents ? view.bits<true>(c + 32 * k) : view.bits<false>(c + 32 * k);
-#pragma unroll
-            for (int b = 0; b < 32; ++b) s[32 * k + b] = w >> b & 1u ? s[32 * k + b] : -INFINITY;
-          }
-        }
-        float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int k = 4; k < kKeys; k += 4) {
-          top[0] = fmaxf(top[0], s[k]);
-          top[1] = fmaxf(top[1], s[k + 1]);
-          top[2] = fmaxf(top[2], s[k + 2]);
-          top[3] = fmaxf(top[3], s[k + 3]);
-        }
-        // Weights are up to 2^7 in f16 (and, with the eight below, 2^15): under 2^-14 a 16-bit weight would be subnormal.
-        const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2 - (kF16 ? 7.0f : 0.0f);
-        // O keeps its scale while maxima go up by less than 2^8: l and O stay exact multiples, far from overflow
-        const bool higher = high > m + 8.0f || (m == -INFINITY && high > m);
-        if (__any_sync(0xffffffffu, higher)) {
-          const float now = fmaxf(m, high);
-          const float turn = now == -INFINITY ? 1.0f : ex2_ftz(m - now);
-          m = now;
-          l *= turn;
-          if (i > 0) {
+        auto ready = [&](int half) {
+          tc::wait_st();
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_ready + 8 * half);
+        };
+        // A row's new maximum (in log2 units): O keeps its scale while maxima go up by less than 2^8, l and O stay exact
+        // multiples, far from overflow.  A row's own maximum alone decides for it, so that it does not depend on the rows
+        // beside it.  Weights are up to 2^7 in f16 (and, with the eight, 2^15): under 2^-14 a 16-bit weight would be
+        // subnormal.  O is at rest: these scores were asked for behind the product before.
+        auto raise = [&](float top) {
+          const float high = top * scale2 - (kF16 ? 7.0f : 0.0f);
+          const bool higher = high > m + 8.0f || (m == -INFINITY && high > m);
+          if (__any_sync(0xffffffffu, higher)) {
+            const float turn = higher ? ex2_ftz(m - high) : 1.0f;
+            m = higher ? high : m;
+            l *= turn;
+            if (i >= C::kTiles) {
+              if (C::kTiles == 1) {  // of the other place: its product may still be under way
+                wait_quietly(bar(C::kDone + 1), (rests - 1) & 1, abort_s);
+                __syncwarp();
+                tc::fence_after();
+              }
 #pragma unroll 1
-            for (int d = 0; d < D; d += 32) {
-              uint32_t o[32];
-              tc::ld32(o, col_o + d);
-              tc::wait_ld();
+              for (int d = 0; d < D; d += 32) {
+                uint32_t o[32];
+                tc::ld32(o, col_o + d);
+                wait_ld32(o);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * turn);
-              tc::st32(col_o + d, o);
+                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * turn);
+                tc::st32(col_o + d, o);
+              }
             }
-            tc::wait_st();
           }
-        }
-        const float minus = m == -INFINITY ? 0.0f : -m;  // a row that has seen nothing keeps weights of exp2(-inf) = 0
-        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        };
+        constexpr int kParts = kKeys / 32;
+        const bool whole = seen_all.all_of_tile(c, a.sink);
+        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        auto weigh = [&](uint32_t (&p)[16], const uint32_t (&s)[32], float2 scale_2, float2 minus_2) {
 #pragma unroll
-        for (int k = 0; k < kKeys / 64; ++k) {
-          uint32_t p[32];
-#pragma unroll
-          for (int b = 0; b < 32; ++b) {
-            const float e0 = ex2_ftz(fmaf(s[64 * k + 2 * b], scale2, minus));
-            const float e1 = ex2_ftz(fmaf(s[64 * k + 2 * b + 1], scale2, minus));
-            part[b & 1] += e0;
-            part[2 + (b & 1)] += e1;
-            p[b] = pack2<kF16>(e0, e1);
+          for (int x = 0; x < 16; ++x) {
+            float2 y = fma2(make_float2(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1])), scale_2, minus_2);
+            y.x = ex2_ftz(y.x);
+            y.y = ex2_ftz(y.y);
+            sum[x & 1] = add2(sum[x & 1], y);
+            p[x] = pack2<kF16>(y.x, y.y);
           }
-          tc::st32(col_s + 32 * k, p);
+        };
+        if (!rows_here) {  // what is in these rows' weights and sums, nobody reads
+          if (lane == 0) {
+            mbar_arrive(p_ready);
+            mbar_arrive(p_ready + 8);
+          }
+        } else if (!C::kPre && whole) {
+          uint32_t s[kParts][32];
+#pragma unroll
+          for (int k = 0; k < kParts; ++k) tc::ld32(s[k], s_at + 32 * k);
+#pragma unroll
+          for (int k = 0; k < kParts; ++k) wait_ld32(s[k]);
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int k = 0; k < kParts; ++k)
+#pragma unroll
+            for (int x = 0; x < 32; x += 8)
+#pragma unroll
+              for (int y = 0; y < 4; ++y)
+                top[y] = max3(top[y], __uint_as_float(s[k][x + 2 * y]), __uint_as_float(s[k][x + 2 * y + 1]));
+          raise(fmaxf(max3(top[0], top[1], top[2]), top[3]));
+          const float minus = m == -INFINITY ? 0.0f : -m;  // a row that has seen nothing keeps weights of exp2(-inf) = 0
+          const float2 scale_2 = make_float2(scale2, scale2), minus_2 = make_float2(minus, minus);
+#pragma unroll
+          for (int k = 0; k < kParts; ++k) {
+            uint32_t p[16];
+            weigh(p, s[k], scale_2, minus_2);
+            tc::st16(s_at + 16 * k, p);
+            if (k == kParts / 2 - 1) ready(0);
+          }
+          ready(1);
+        } else {
+          // Tiles that some row does not see all of, and scores that are changed: 32 keys at a time, the scores as they are meant
+          // put back by a first round.  Keys that none of the warp's rows sees cost nothing more.
+          uint32_t live = 0;
+          float top = -INFINITY;
+#pragma unroll 1
+          for (int k = 0; k < kParts; ++k) {
+            uint32_t w = 0xffffffffu;
+            if (!whole) w = a.parents ? view.template bits<true>(c + 32 * k) : view.template bits<false>(c + 32 * k);
+            if (!__any_sync(0xffffffffu, valid && w != 0)) continue;
+            live |= 1u << k;
+            uint32_t s[32];
+            tc::ld32(s, s_at + 32 * k);
+            wait_ld32(s);
+#pragma unroll
+            for (int x = 0; x < 32; ++x) {
+              float y = __uint_as_float(s[x]);
+              if constexpr (C::kPre) y = a.softcap > 0.0f ? a.softcap * kLog2e * tanh_of(y * a.cap_in) : y * a.scale2;
+              y = w >> x & 1u ? y : -INFINITY;
+              top = fmaxf(top, y);
+              s[x] = __float_as_uint(y);
+            }
+            tc::st32(s_at + 32 * k, s);
+          }
+          tc::wait_st();
+          raise(top);
+          const float minus = m == -INFINITY ? 0.0f : -m;
+          const float2 scale_2 = make_float2(scale2, scale2), minus_2 = make_float2(minus, minus);
+#pragma unroll 1
+          for (int k = 0; k < kParts; ++k) {
+            uint32_t p[16];
+            if (live >> k & 1u) {
+              uint32_t s[32];
+              tc::ld32(s, s_at + 32 * k);
+              wait_ld32(s);
+              weigh(p, s, scale_2, minus_2);
+            } else {
+#pragma unroll
+              for (int x = 0; x < 16; ++x) p[x] = 0;
+            }
+            tc::st16(s_at + 16 * k, p);  // over scores that have been read
+            if (k == kParts / 2 - 1) ready(0);
+          }
+          ready(1);
         }
-        l += (part[0] + part[1]) + (part[2] + part[3]);
-        tc::wait_st();
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(kPReady + stream));
+        sum[0] = add2(sum[0], sum[1]);
+        l += sum[0].x + sum[0].y;
+        ++rests;
       }
 
       // ------------------------------------------------------------------------------ the unit's rows
-      (void)mbar_wait(bar(kOFull + stream), units_done & 1, abort_s);
-      ++units_done;
-      __syncwarp();
+      if (jobs > (C::kTiles == 2 ? tile : 0)) {
+        wait_quietly(bar(C::kDone + tile), done, abort_s);
+        done ^= 1;
+        __syncwarp();
+      }
       tc::fence_after();
-      const bool poison = *reinterpret_cast<volatile const int*>(&u->poison) != 0;
       // Values that were taken out of tiles come back, to the rows that see them (32 dims from d on of this row): rare,
       // and one by one.
       auto put_back = [&](uint32_t (&o)[32], int d) {
+#pragma unroll 1
         for (int i = 0; i < n; ++i) {
           const int c = u->tile(k0 + i) * kKeys;
-          if (!partial(*u, c)) continue;
+          if (seen_all.all_of_tile(c, a.sink)) continue;
+#pragma unroll 1
           for (int k = 0; k < kKeys; k += 32) {
-            uint32_t w = valid ? (a.parents ? view.bits<true>(c + k) : view.bits<false>(c + k)) : 0u;
+            uint32_t w = valid ? (a.parents ? view.template bits<true>(c + k) : view.template bits<false>(c + k)) : 0u;
+#pragma unroll 1
             while (w) {
               const int key = c + k + __ffs(w) - 1;
               w &= w - 1;
@@ -935,37 +1075,39 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       float f0 = 1.0f, f1 = 0.0f;
-      bool second = false;  // this thread's row has a part in the other warpgroup's accumulator
+      const bool second = pair && n > 1;  // the other accumulator has a part
       if (pair) {
-        if (stream == 1) {
-          pair_s[r] = m;
-          pair_s[kRowsTile + r] = l;
+        if (tile == 1) {
+          swap_s[r] = m;
+          swap_s[kRowsTile + r] = l;
         }
         tc::fence_before();
         named_sync(1, 256);
         tc::fence_after();
-        if (stream == 0) {
-          const float m1 = pair_s[r], l1 = pair_s[kRowsTile + r];
-          second = n > 1;
-          const float now = fmaxf(m, m1);
+        if (second && tile == 0) {
+          const float m1 = swap_s[r], l1 = swap_s[kRowsTile + r], now = fmaxf(m, m1);
           f0 = now == -INFINITY ? 1.0f : ex2_ftz(m - now);
           f1 = now == -INFINITY ? 1.0f : ex2_ftz(m1 - now);
-          l = second ? l * f0 + l1 * f1 : l;
-          if (!second) f0 = 1.0f;
-          else m = now;
+          l = l * f0 + l1 * f1;
+          m = now;
         }
       }
-      if (!pair || stream == 0) {
-        const int row_in = (pair ? 0 : stream * kRowsTile) + r;
+      // behind the barrier: the other row tile's last values may be looked over after this one's products are done
+      const bool poison = *reinterpret_cast<volatile const int*>(&u->poison) != 0;
+      if (rows_here && (!pair || tile == 0)) {
+        const int row_in = (pair ? 0 : tile * kRowsTile) + r;
         const long long row = u->row0 + token, at_head = row * a.n_heads + (long long)u->head * a.group + head_in;
         const float inverse = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // nothing seen: zeros
         const long long n_slots = 2ll * gridDim.x;
-        if (u->cut && valid) {
-          float* rm = a.records + n_slots * C::kRows * D + (long long)u->slot * C::kRows + row_in;
-          rm[0] = m;
-          rm[n_slots * C::kRows] = l;
-        } else if (a.lse && valid) {  // not cut
-          a.lse[at_head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+        const bool cut = u->cut;
+        if (valid) {
+          if (cut) {
+            float* rm = a.records + n_slots * C::kRows * D + (long long)u->slot * C::kRows + row_in;
+            rm[0] = m;
+            rm[n_slots * C::kRows] = l;
+          } else if (a.lse) {
+            a.lse[at_head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+          }
         }
 #pragma unroll 1
         for (int d = 0; d < D; d += 32) {
@@ -973,17 +1115,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::ld32(o, col_o + d);
           if (second) {
             uint32_t o1[32];
-            tc::ld32(o1, lanes + C::kColO + C::kStepO + d);
-            tc::wait_ld();
+            tc::ld32(o1, col_o + C::kStepO + d);
+            wait_ld32(o1);
+            wait_ld32(o);
 #pragma unroll
-            for (int k = 0; k < 32; ++k)
-              o[k] = __float_as_uint(__uint_as_float(o[k]) * f0 + __uint_as_float(o1[k]) * f1);
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f0 + __uint_as_float(o1[k]) * f1);
           } else {
-            tc::wait_ld();
+            wait_ld32(o);
           }
           if (poison) put_back(o, d);
-          if (u->cut) {
-            if (!valid) continue;
+          if (cut && valid) {
             float4* rec = reinterpret_cast<float4*>(a.records) + ((long long)u->slot * (D / 4) + d / 4) * C::kRows + row_in;
 #pragma unroll
             for (int k = 0; k < 8; ++k)
@@ -1008,72 +1149,148 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           }
+          __syncwarp();
         }
         tc::fence_before();
       }
-      if (pair) named_sync(1, 256);  // the second accumulator and its sums have been read
+      // the sums, and the second accumulator, have been read
+      if (pair) named_sync(1, 256);
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kWEmpty + e));
+      if (lane == 0) mbar_arrive(bar(C::kWEmpty + e));
     }
   }
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  if (warp == 9) tc::dealloc512(tmem);
-  // a wait that ran into its limit (about two seconds): the outputs are not valid
+  if (warp == kProducts) tc::dealloc512(tmem);
+  // a wait that ran into its limit (some seconds): the outputs are not valid
   if (tid == 0 && *abort_s && a.status) atomicMax(a.status, 2);
 }
 
-// The records of a cut unit become its rows: thread by thread a row's four dims, rows side by side, so that loads and
-// the records' layout agree.  blockIdx.x: the CTA that has the unit's first piece; blockIdx.y takes a part of the rows and dims.
-constexpr int kJoinParts = 8;
+// The records of the cut units become their rows.  A place is four dims of a row; rows lie side by side, as the records have
+// them.  A CTA lists the units (one descriptor a thread) and takes every gridDim.x-th strip of places: 256 with a
+// thread each, or 64 of a unit of many pieces, whose pieces four threads take in turn and join in shared memory.  What it takes
+// is latency: two rounds of loads for up to eight pieces, and enough CTAs beside one another.  (Strips of 64 throughout, 2.4
+// times fewer CTAs: 55 us for 148 units of two pieces, 256 rows and 128 dims; so 7.)
+constexpr int kJoinThreads = 256, kJoinFew = 8, kJoinLoads = 4, kJoinCtas = 5;
 template <class C>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kJoinThreads, kJoinCtas) join_kernel(const __grid_constant__ Args a, int workers) {
   constexpr int D = C::D;
+  __shared__ Desc desc_s[kMaxWorkers];
+  __shared__ int first_s[kMaxWorkers + 1], sums_s[kJoinThreads / 32];
+  __shared__ float part_s[3][6][kJoinThreads / 4];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const Desc u = a.desc[blockIdx.x];
-  if (u.pieces == 0) return;
-  const long long n_slots = 2ll * gridDim.x;
+  Desc mine;
+  mine.pieces = 0;
+  if (tid < workers) mine = a.desc[tid];
+  const int wide = mine.pieces > kJoinFew ? kJoinThreads / 4 : kJoinThreads;  // places of a strip
+  const int strips = mine.pieces > 0 ? (mine.tokens * a.group * (D / 4) + wide - 1) / wide : 0;
+  int scan = strips;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int up = __shfl_up_sync(0xffffffffu, scan, d);
+    if (lane >= d) scan += up;
+  }
+  if (lane == 31) sums_s[warp] = scan;
+  __syncthreads();
+  int total = 0;
+  for (int w = 0; w < kJoinThreads / 32; ++w) {
+    if (w < warp) scan += sums_s[w];
+    total += sums_s[w];
+  }
+  desc_s[tid] = mine;
+  first_s[tid] = scan - strips;
+  __syncthreads();
+  const long long n_slots = 2ll * workers;
   const float4* o = reinterpret_cast<const float4*>(a.records);
   const float* rm = a.records + n_slots * C::kRows * D;
   const float* rl = rm + n_slots * C::kRows;
-  auto slot_of = [&](int k) { return k == 0 ? 2ll * blockIdx.x + 1 : 2ll * (blockIdx.x + k); };
-  for (int i = blockIdx.y * 256 + threadIdx.x; i < C::kRows * (D / 4); i += kJoinParts * 256) {
-    const int row_in = i % C::kRows, d4 = i / C::kRows, r = row_in % kRowsTile;
-    const int token_in = r / a.group, token = row_in / kRowsTile * a.tile_tokens + token_in;
-    if (token_in >= a.tile_tokens || token >= u.tokens) continue;
-    float m = -INFINITY;
-#pragma unroll 4
-    for (int k = 0; k < u.pieces; ++k) m = fmaxf(m, __ldcg(rm + slot_of(k) * C::kRows + row_in));
+#pragma unroll 1
+  for (int strip = blockIdx.x; strip < total; strip += gridDim.x) {
+    int lo = 0, hi = kJoinThreads - 1;  // the last unit that starts at the strip or before
+#pragma unroll 1
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (first_s[mid] <= strip) lo = mid;
+      else hi = mid - 1;
+    }
+    const Desc u = desc_s[lo];
+    const bool many = u.pieces > kJoinFew;
+    const int ways = many ? 4 : 1, way = many ? tid / (kJoinThreads / 4) : 0, at_strip = many ? tid % (kJoinThreads / 4) : tid;
+    const int rows = u.tokens * a.group, place = (strip - first_s[lo]) * (kJoinThreads / ways) + at_strip;
+    const int d4 = place / rows, r = place - d4 * rows, token = r / a.group;
+    const int tile = token / a.tile_tokens, row_in = tile * kRowsTile + r - tile * a.tile_tokens * a.group;
+    const bool real = d4 < D / 4;
+    float m = -INFINITY, l = 0.0f;
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float l = 0.0f;
-#pragma unroll 4
-    for (int k = 0; k < u.pieces; ++k) {
-      const long long slot = slot_of(k);
-      const float mk = __ldcg(rm + slot * C::kRows + row_in), lk = __ldcg(rl + slot * C::kRows + row_in);
-      const float4 v = __ldcg(o + (slot * (D / 4) + d4) * C::kRows + row_in);
-      const bool none = lk == 0.0f;  // nothing seen in this piece, and nothing to be taken from it
-      const float f = mk == m ? 1.0f : ex2_ftz(mk - m);
-      if (!none) {
-        l += f * lk;
-        sum.x += f * v.x;
-        sum.y += f * v.y;
-        sum.z += f * v.z;
-        sum.w += f * v.w;
+    // another part with maximum mk and sum lk: of none nothing is taken
+    auto join = [&](float mk, float lk, float4 v) {
+      if (lk == 0.0f) return;
+      const float top = fmaxf(m, mk), f0 = m == top ? 1.0f : ex2_ftz(m - top), f1 = mk == top ? 1.0f : ex2_ftz(mk - top);
+      m = top;
+      l = l * f0 + lk * f1;
+      sum.x = sum.x * f0 + v.x * f1;
+      sum.y = sum.y * f0 + v.y * f1;
+      sum.z = sum.z * f0 + v.z * f1;
+      sum.w = sum.w * f0 + v.w * f1;
+    };
+    if (real) {
+#pragma unroll 1
+      for (int k0 = way; k0 < u.pieces; k0 += ways * kJoinLoads) {
+        float mk[kJoinLoads], lk[kJoinLoads];
+        float4 v[kJoinLoads];
+#pragma unroll
+        for (int i = 0; i < kJoinLoads; ++i) {
+          const int k = k0 + ways * i;
+          mk[i] = lk[i] = 0.0f;
+          v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (k < u.pieces) {
+            const long long slot = k == 0 ? 2ll * lo + 1 : 2ll * (lo + k);  // the CTA's of the first piece, then the next ones'
+            mk[i] = __ldcg(rm + slot * C::kRows + row_in);
+            lk[i] = __ldcg(rl + slot * C::kRows + row_in);
+            v[i] = __ldcg(o + (slot * (D / 4) + d4) * C::kRows + row_in);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kJoinLoads; ++i) join(mk[i], lk[i], v[i]);
       }
     }
-    const float inverse = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    if (inverse == 0.0f) sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const long long at_head = (long long)(u.row0 + token) * a.n_heads + (long long)u.head * a.group + r - token_in * a.group;
-    const long long at = at_head * D + 4 * d4;
-    if (a.out_f32) {
-      *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) =
-          make_float4(sum.x * inverse, sum.y * inverse, sum.z * inverse, sum.w * inverse);
-    } else {
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) =
-          make_uint2(pack2<C::kF16>(sum.x * inverse, sum.y * inverse), pack2<C::kF16>(sum.z * inverse, sum.w * inverse));
+    if (many) {
+      if (way > 0) {
+        float* p = &part_s[way - 1][0][at_strip];
+        p[0] = m;
+        p[kJoinThreads / 4] = l;
+        p[2 * kJoinThreads / 4] = sum.x;
+        p[3 * kJoinThreads / 4] = sum.y;
+        p[4 * kJoinThreads / 4] = sum.z;
+        p[5 * kJoinThreads / 4] = sum.w;
+      }
+      __syncthreads();
+      if (way == 0) {
+#pragma unroll 1
+        for (int i = 0; i < 3; ++i) {
+          const float* p = &part_s[i][0][at_strip];
+          join(p[0], p[kJoinThreads / 4], make_float4(p[2 * kJoinThreads / 4], p[3 * kJoinThreads / 4], p[4 * kJoinThreads / 4],
+                                                      p[5 * kJoinThreads / 4]));
+        }
+      }
     }
-    if (a.lse && d4 == 0) a.lse[at_head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+    if (way == 0 && real) {
+      const float inverse = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+      if (inverse == 0.0f) sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const long long at_head = (long long)(u.row0 + token) * a.n_heads + (long long)u.head * a.group + r - token * a.group;
+      const long long at = at_head * D + 4 * d4;
+      if (a.out_f32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) =
+            make_float4(sum.x * inverse, sum.y * inverse, sum.z * inverse, sum.w * inverse);
+      } else {
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) =
+            make_uint2(pack2<C::kF16>(sum.x * inverse, sum.y * inverse), pack2<C::kF16>(sum.z * inverse, sum.w * inverse));
+      }
+      if (a.lse && d4 == 0) a.lse[at_head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+    }
+    if (many) __syncthreads();
   }
 }
 
@@ -1119,14 +1336,19 @@ static int launch(const asterq_rows_attention_params* p, Args& a, int workers, i
   early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t join = {};
-  join.gridDim = dim3(workers, kJoinParts);
-  join.blockDim = 256;
+  join.gridDim = kJoinCtas * workers;
+  join.blockDim = kJoinThreads;
   join.stream = s;
   join.attrs = early;
   join.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&join, join_kernel<C>, a);
+  const cudaError_t e = cudaLaunchKernelEx(&join, join_kernel<C>, a, workers);
   if (e != cudaSuccess) return set_error(ASTERQ_ERR_CUDA, "rows_attention: launch failed: %s", cudaGetErrorString(e));
   return check_launch("rows_attention");
+}
+
+template <bool kF16, int D>
+static int by_scale(const asterq_rows_attention_params* p, Args& a, bool pre, int workers, int dev, cudaStream_t s) {
+  return pre ? launch<Cfg<kF16, D, true>>(p, a, workers, dev, s) : launch<Cfg<kF16, D, false>>(p, a, workers, dev, s);
 }
 
 static int check(const asterq_rows_attention_params* p) {
@@ -1217,15 +1439,14 @@ extern "C" int asterq_rows_attention(const asterq_rows_attention_params* p, void
   a.softcap = p->logit_softcap > 0.0f ? p->logit_softcap : 0.0f;
   a.cap_in = a.softcap > 0.0f ? a.scale / a.softcap : 0.0f;
   // the maximum is taken of what the tensor cores give, before the scale, where that keeps the order
-  a.premultiply = a.softcap > 0.0f || !(a.scale > 0.0f);
+  const bool pre = a.softcap > 0.0f || !(a.scale > 0.0f);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const bool f16 = p->dtype == ASTERQ_DTYPE_F16;
   switch (p->head_dim) {
-    case 64: return f16 ? rat::launch<rat::Cfg<true, 64>>(p, a, workers, dev, s)
-                        : rat::launch<rat::Cfg<false, 64>>(p, a, workers, dev, s);
-    case 128: return f16 ? rat::launch<rat::Cfg<true, 128>>(p, a, workers, dev, s)
-                         : rat::launch<rat::Cfg<false, 128>>(p, a, workers, dev, s);
-    default: return f16 ? rat::launch<rat::Cfg<true, 256>>(p, a, workers, dev, s)
-                        : rat::launch<rat::Cfg<false, 256>>(p, a, workers, dev, s);
+    case 64: return f16 ? rat::by_scale<true, 64>(p, a, pre, workers, dev, s) : rat::by_scale<false, 64>(p, a, pre, workers, dev, s);
+    case 128: return f16 ? rat::by_scale<true, 128>(p, a, pre, workers, dev, s)
+                         : rat::by_scale<false, 128>(p, a, pre, workers, dev, s);
+    default: return f16 ? rat::by_scale<true, 256>(p, a, pre, workers, dev, s)
+                        : rat::by_scale<false, 256>(p, a, pre, workers, dev, s);
   }
 }
