@@ -43,21 +43,6 @@ ASTERQ_DEVICE int find_sequence(const int* __restrict__ off, int n, long long ro
 }
 
 template <bool kF16>
-ASTERQ_DEVICE void weights_of(float (&w)[16], const void* from, bool f32, int d0, int d1) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (f32) {
-      w[i] = __ldg(static_cast<const float*>(from) + d0 + i);
-      w[8 + i] = __ldg(static_cast<const float*>(from) + d1 + i);
-    } else {
-      const uint16_t a = __ldg(static_cast<const uint16_t*>(from) + d0 + i), b = __ldg(static_cast<const uint16_t*>(from) + d1 + i);
-      w[i] = unpack2<kF16>(a).x;
-      w[8 + i] = unpack2<kF16>(b).x;
-    }
-  }
-}
-
-template <bool kF16>
 __global__ void __launch_bounds__(kThreads) append_kernel(const asterq_kv_append_normed_params p, int rows_per_block, int lanes) {
   const int D = p.head_dim, units = D / 16, turn = p.rotary_dim / 16;
   const int per_row = kThreads / rows_per_block;  // threads of one row: whole warps
@@ -66,11 +51,18 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const asterq_kv_append
   const bool works = u < units;
   const int n_q = p.q ? p.n_heads : 0, n_all = n_q + 2 * p.n_kv_heads;
   const bool half = !p.interleaved && u < turn;
+  const float per_dim = 1.0f / (float)D;
   const int d0 = !works ? 0 : half ? 8 * u : 16 * u, d1 = !works ? 8 : half ? p.rotary_dim / 2 + 8 * u : 16 * u + 8;
-  float wq[16], wk[16];
-  const bool f32 = p.norm_dtype == ASTERQ_DTYPE_F32;
-  if (p.q_norm) weights_of<kF16>(wq, p.q_norm, f32, d0, d1);
-  if (p.k_norm) weights_of<kF16>(wk, p.k_norm, f32, d0, d1);
+  // the weights in shared memory: 32 registers of them cost half of the CTAs that an SM holds
+  __shared__ __align__(16) float weight_s[2][512];
+  for (int i = threadIdx.x; i < 2 * D; i += kThreads) {
+    const int of = i >= D, d = i - of * D;
+    const void* w = of ? p.k_norm : p.q_norm;
+    if (w)
+      weight_s[of][d] = p.norm_dtype == ASTERQ_DTYPE_F32 ? __ldg(static_cast<const float*>(w) + d)
+                                                         : unpack2<kF16>(__ldg(static_cast<const uint16_t*>(w) + d)).x;
+  }
+  __syncthreads();
 
   for (long long row = (long long)blockIdx.x * rows_per_block + sub; row < p.n_rows; row += (long long)gridDim.x * rows_per_block) {
     auto source = [&](int h) -> const uint16_t* {
@@ -92,7 +84,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const asterq_kv_append
     if (length < 0) continue;  // an empty slot
     const long long begin = __ldg(p.row_offsets + s), place = (long long)length + (row - begin);
     const long long col = place / p.page_tokens;
-    const int at = (int)(place - col * p.page_tokens);
+    const int inside = (int)(place - col * p.page_tokens);
     const long long pos = p.positions ? (long long)__ldg(p.positions + row) : place;
     int page = -1;
     // the search finds a sequence that the row is not of where offsets are out of order
@@ -122,58 +114,52 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const asterq_kv_append
       }
       const bool is_q = h < n_q, is_k = !is_q && h < n_q + p.n_kv_heads;
       const bool normed = (is_q && p.q_norm) || (is_k && p.k_norm);
-      float x[8], y[8];
-      const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
-      float sum = 0.0f;
+      uint32_t* x = reinterpret_cast<uint32_t*>(&a);
+      uint32_t* y = reinterpret_cast<uint32_t*>(&b);
+      float scale = 1.0f;
+      if (__any_sync(0xffffffffu, normed)) {
+        float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 xf = unpack2<kF16>(aw[i]), yf = unpack2<kF16>(bw[i]);
-        x[2 * i] = xf.x;
-        x[2 * i + 1] = xf.y;
-        y[2 * i] = yf.x;
-        y[2 * i + 1] = yf.y;
-        sum = fmaf(xf.x, xf.x, fmaf(xf.y, xf.y, fmaf(yf.x, yf.x, fmaf(yf.y, yf.y, sum))));
-      }
-      if (!works) sum = 0.0f;
-      for (int d = 1; d < lanes; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      if (normed) {
-        const float scale = rsqrtf(sum / (float)D + p.norm_eps);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[i] = x[i] * scale * (is_q ? wq[i] : wk[i]);
-          y[i] = y[i] * scale * (is_q ? wq[8 + i] : wk[8 + i]);
+        for (int i = 0; i < 4; ++i) {
+          const float2 xf = unpack2<kF16>(x[i]), yf = unpack2<kF16>(y[i]);
+          sum = fmaf(xf.x, xf.x, fmaf(xf.y, xf.y, fmaf(yf.x, yf.x, fmaf(yf.y, yf.y, sum))));
         }
+        if (!works) sum = 0.0f;
+        for (int d = 1; d < lanes; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        scale = rsqrtf(sum * per_dim + p.norm_eps);
       }
       if (works && h < n_all) {
-        if (u < turn && (is_q || is_k)) {
-          if (half) {
+        const bool turns = u < turn && (is_q || is_k);
+        if (normed || turns) {  // values go as they came
+          const float2* wx = reinterpret_cast<const float2*>(weight_s[is_q ? 0 : 1] + d0);
+          const float2* wy = reinterpret_cast<const float2*>(weight_s[is_q ? 0 : 1] + d1);
+          // two pairs at a time, so that few are held in 32 bits
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float t = x[i];
-              x[i] = t * c[i] - y[i] * sn[i];
-              y[i] = y[i] * c[i] + t * sn[i];
+          for (int i = 0; i < 4; ++i) {
+            float2 xf = unpack2<kF16>(x[i]), yf = unpack2<kF16>(y[i]);
+            if (normed) {
+              const float2 wa = wx[i], wb = wy[i];
+              xf = make_float2(xf.x * scale * wa.x, xf.y * scale * wa.y);
+              yf = make_float2(yf.x * scale * wb.x, yf.y * scale * wb.y);
             }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float t = x[2 * i], v = y[2 * i];
-              x[2 * i] = t * c[i] - x[2 * i + 1] * sn[i];
-              x[2 * i + 1] = x[2 * i + 1] * c[i] + t * sn[i];
-              y[2 * i] = v * c[4 + i] - y[2 * i + 1] * sn[4 + i];
-              y[2 * i + 1] = y[2 * i + 1] * c[4 + i] + v * sn[4 + i];
+            if (turns && half) {
+              x[i] = pack2<kF16>(xf.x * c[2 * i] - yf.x * sn[2 * i], xf.y * c[2 * i + 1] - yf.y * sn[2 * i + 1]);
+              y[i] = pack2<kF16>(yf.x * c[2 * i] + xf.x * sn[2 * i], yf.y * c[2 * i + 1] + xf.y * sn[2 * i + 1]);
+            } else if (turns) {
+              x[i] = pack2<kF16>(xf.x * c[i] - xf.y * sn[i], xf.y * c[i] + xf.x * sn[i]);
+              y[i] = pack2<kF16>(yf.x * c[4 + i] - yf.y * sn[4 + i], yf.y * c[4 + i] + yf.x * sn[4 + i]);
+            } else {
+              x[i] = pack2<kF16>(xf.x, xf.y);
+              y[i] = pack2<kF16>(yf.x, yf.y);
             }
           }
-        }
-        if (is_q || is_k) {  // values go as they came
-          a = make_uint4(pack2<kF16>(x[0], x[1]), pack2<kF16>(x[2], x[3]), pack2<kF16>(x[4], x[5]), pack2<kF16>(x[6], x[7]));
-          b = make_uint4(pack2<kF16>(y[0], y[1]), pack2<kF16>(y[2], y[3]), pack2<kF16>(y[4], y[5]), pack2<kF16>(y[6], y[7]));
         }
         uint16_t* dst;
         if (is_q) {
           dst = (uint16_t*)p.q_out + (row * n_q + h) * D;
         } else {
           const int kv = h - n_q, hk = is_k ? kv : kv - p.n_kv_heads;
-          dst = (uint16_t*)(is_k ? p.k_pool : p.v_pool) + ((page0 + hk) * p.page_tokens + at) * D;
+          dst = (uint16_t*)(is_k ? p.k_pool : p.v_pool) + ((page0 + hk) * p.page_tokens + inside) * D;
         }
         *reinterpret_cast<uint4*>(dst + d0) = a;
         *reinterpret_cast<uint4*>(dst + d1) = b;
@@ -229,7 +215,7 @@ extern "C" int asterq_kv_append_normed(const asterq_kv_append_normed_params* p, 
   int per_row = kvn::kThreads;
   while (per_row > 64 && (per_row / 2 >= items || p->n_rows >= 600)) per_row /= 2;
   const int rows_per_block = kvn::kThreads / per_row;
-  const int64_t blocks = (p->n_rows + rows_per_block - 1) / rows_per_block, most = (int64_t)sms * 8;
+  const int64_t blocks = (p->n_rows + rows_per_block - 1) / rows_per_block, most = (int64_t)sms * 4;
   const unsigned grid = (unsigned)(blocks < most ? blocks : most);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (p->dtype == ASTERQ_DTYPE_F16)

@@ -43,10 +43,10 @@ struct Args {
 };
 
 template <int kType>
-ASTERQ_DEVICE double value_at(const void* x, long long i) {
-  if constexpr (kType == ASTERQ_DTYPE_F32) return (double)__ldg(static_cast<const float*>(x) + i);
+ASTERQ_DEVICE float value_at(const void* x, long long i) {
+  if constexpr (kType == ASTERQ_DTYPE_F32) return __ldg(static_cast<const float*>(x) + i);
   const uint32_t w = __ldg(static_cast<const uint16_t*>(x) + i);
-  return (double)(kType == ASTERQ_DTYPE_F16 ? unpack_half2(w).x : unpack_bf162(w).x);
+  return kType == ASTERQ_DTYPE_F16 ? unpack_half2(w).x : unpack_bf162(w).x;
 }
 
 ASTERQ_DEVICE double warp_sum(double x) {
@@ -56,7 +56,7 @@ ASTERQ_DEVICE double warp_sum(double x) {
 }
 
 template <int kType>
-__global__ void __launch_bounds__(kThreads) verify_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const Args a) {
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), s = blockIdx.x / ranks;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -66,8 +66,6 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Args a) {
   __shared__ double mass_s[kMaxNodes];     // m before each rejection at cur
   __shared__ int gone_s[kMaxNodes];        // tokens rejected at cur, of drafts without probabilities
   __shared__ double warp_sums[kWarps], rank_sums[2][kMaxCluster];
-  __shared__ double found_rest;
-  __shared__ int found_part;
   const long long begin = __ldg(a.row_offsets + s), end = __ldg(a.row_offsets + s + 1);
   const bool bad = begin < 0 || end < begin || end > a.n_rows || end - begin > kMaxNodes;
   const int n = bad ? 0 : (int)(end - begin);
@@ -108,25 +106,56 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Args a) {
   double m = 1.0;
   // what is left of the target at t after the rejections so far
   auto left_at = [&](int t) {
-    double r = value_at<kType>(a.target, (begin + cur) * a.target_stride + t);
-    if (a.draft) {
-      if (rejected > 0) {
-        const double q = value_at<kType>(a.draft, (begin + cur) * a.draft_stride + t);
-        for (int k = 0; k < rejected; ++k) r = fmax(__dsub_rn(r, __dmul_rn(mass_s[k], q)), 0.0);
+    double r = (double)value_at<kType>(a.target, (begin + cur) * a.target_stride + t);
+    const double q = a.draft && rejected > 0 ? (double)value_at<kType>(a.draft, (begin + cur) * a.draft_stride + t) : 0.0;
+#pragma unroll 1
+    for (int j = 0; j < rejected; ++j) {
+      if (a.draft) {
+        const double d = __dsub_rn(r, __dmul_rn(mass_s[j], q));
+        r = d > 0.0 ? d : 0.0;
+      } else {
+        r = gone_s[j] == t ? 0.0 : r;
       }
-    } else {
-      for (int k = 0; k < rejected; ++k) r = gone_s[k] == t ? 0.0 : r;
     }
     return r;
   };
-  // The sum of what is left over [from, to) by this warp, lanes side by side.
+  // The sum of what is left over [from, to) by this warp, lanes side by side: the loads of kAhead rounds are under way before
+  // the first is used.
   auto sum_of = [&](int from, int to) {
     double sum = 0.0;
-    constexpr int kAhead = 8;
+    constexpr int kAhead = 6;
+    const long long p0 = (begin + cur) * a.target_stride, q0 = (begin + cur) * a.draft_stride;
+    const bool drafted = a.draft && rejected > 0;
+#pragma unroll 1
     for (int t = from + lane; t < to; t += 32 * kAhead) {
+      float p[kAhead], q[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) p[k] = t + 32 * k < to ? value_at<kType>(a.target, p0 + t + 32 * k) : 0.0f;
+      if (drafted) {
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) q[k] = t + 32 * k < to ? value_at<kType>(a.draft, q0 + t + 32 * k) : 0.0f;
+      }
       double r[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) r[k] = t + 32 * k < to ? left_at(t + 32 * k) : 0.0;
+      for (int k = 0; k < kAhead; ++k) r[k] = (double)p[k];
+      if (drafted) {
+#pragma unroll 1
+        for (int j = 0; j < rejected; ++j) {
+          const double mj = mass_s[j];
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) {
+            const double d = __dsub_rn(r[k], __dmul_rn(mj, (double)q[k]));
+            r[k] = d > 0.0 ? d : 0.0;
+          }
+        }
+      } else if (!a.draft) {
+#pragma unroll 1
+        for (int j = 0; j < rejected; ++j) {
+          const int gone = gone_s[j] - t;
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) r[k] = gone == 32 * k ? 0.0 : r[k];
+        }
+      }
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) sum += r[k];
     }
@@ -174,7 +203,10 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Args a) {
     const int x = token_s[next];
     double r = p_s[next];
     if (a.draft) {
-      for (int k = 0; k < rejected; ++k) r = fmax(__dsub_rn(r, __dmul_rn(mass_s[k], q_s[next])), 0.0);
+      for (int k = 0; k < rejected; ++k) {
+        const double d = __dsub_rn(r, __dmul_rn(mass_s[k], q_s[next]));
+        r = d > 0.0 ? d : 0.0;
+      }
     } else {
       for (int k = 0; k < rejected; ++k) r = gone_s[k] == x ? 0.0 : r;
     }
