@@ -454,7 +454,9 @@ def quick_calls():
             return None
         lib = load()
         module.bind(*(ctypes.cast(f, ctypes.c_void_p).value
-                      for f in (lib.asterq_kv_append, lib.asterq_paged_attention, lib.asterq_linear_attention)))
+                      for f in (lib.asterq_kv_append, lib.asterq_paged_attention, lib.asterq_linear_attention,
+                                lib.asterq_kv_append_normed, lib.asterq_rows_attention, lib.asterq_kv_keep,
+                                lib.asterq_verify_drafts)))
         _calls = module
     return _calls or None
 

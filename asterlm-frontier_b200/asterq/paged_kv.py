@@ -187,8 +187,9 @@ def append_kv(
     is not its place behind the cached tokens (a drafted node's is ``lengths[s]`` and its depth).
     """
     quick = _quick()
-    if quick is not None and q_norm is None and k_norm is None and positions is None:
-        done = quick.append(pools.k, pools.v, page_table, lengths, row_offsets, k, v, q, cos, sin, interleaved, q_out, status)
+    if quick is not None:
+        done = quick.append(pools.k, pools.v, page_table, lengths, row_offsets, k, v, q, cos, sin, interleaved, q_out, status,
+                            q_norm, k_norm, norm_eps, positions)
         if done is not NotImplemented:
             return done
     n_kv, page, dim = pools.k.shape[1:]
@@ -370,16 +371,25 @@ _rows_workspaces: dict[tuple[int, int], RowsAttentionWorkspace] = {}
 
 
 def _rows_workspace(device: torch.device, stream: int) -> RowsAttentionWorkspace:
+    if _capturing(device):
+        return RowsAttentionWorkspace(device)  # of the graph's own memory: graphs may run beside each other and other calls
     ws = _rows_workspaces.get((device.index, stream))
     if ws is None:
-        ws = RowsAttentionWorkspace(device)
-        if not _capturing(device):  # in a capture it is of the graph's own memory, and not for any call but this one
-            _rows_workspaces[(device.index, stream)] = ws
+        ws = _rows_workspaces[(device.index, stream)] = RowsAttentionWorkspace(device)
+    if _quick() is not None:  # whose calls come here until it knows the workspace
+        _quick().workspace(2, device.index, stream, ws.buffer.data_ptr(), ws.nbytes)
     return ws
 
 
 def _rows_attention(pools, page_table, lengths, row_offsets, parents, q, softmax_scale, logit_softcap, window_size,
                     sink_tokens, out, return_lse, workspace, status):
+    quick = _quick()
+    if quick is not None and workspace is None and window_size != 0:
+        done = quick.rows(pools.k, pools.v, page_table, lengths, row_offsets, parents, q,
+                          1.0 / math.sqrt(pools.k.shape[3]) if softmax_scale is None else softmax_scale, logit_softcap or 0.0,
+                          window_size or 0, sink_tokens, out, return_lse, status)
+        if done is not NotImplemented:
+            return done
     if q.dim() != 3 or page_table.dim() != 2 or row_offsets.dim() != 1:
         raise ValueError("q must be [rows, n_heads, head_dim], page_table [n_seqs, max_pages], row_offsets [n_seqs + 1]")
     n_pages, n_kv, page, dim = pools.k.shape
@@ -496,7 +506,7 @@ class PagedKVStack:
     """The pools of a stack of layers that share page tables: one geometry, type and device, no pool twice.  It holds
     the pools' addresses for ``keep_kv_rows`` and ``copy_kv_pages``, which work on all layers at once."""
 
-    __slots__ = ("layers", "_k", "_v")
+    __slots__ = ("layers", "like", "_k", "_v", "_k_address", "_v_address")
 
     def __init__(self, layers: Sequence[PagedKVPools]) -> None:
         self.layers = tuple(layers)
@@ -513,10 +523,8 @@ class PagedKVStack:
         n = len(self.layers)
         self._k = (_lib.ctypes.c_void_p * n)(*address[:n])
         self._v = (_lib.ctypes.c_void_p * n)(*address[n:])
-
-    @property
-    def like(self) -> torch.Tensor:
-        return self.layers[0].k
+        self._k_address, self._v_address = _lib.ctypes.addressof(self._k), _lib.ctypes.addressof(self._v)
+        self.like = first
 
 
 def keep_kv_rows(
@@ -537,6 +545,12 @@ def keep_kv_rows(
     in.  status int32 [1]: set to 1 when a sequence's kept does not ascend or leaves its rows, its offsets are out of order
     (the sequence is left as it is), or a place has no page (the row is left out).
     """
+    quick = _quick()
+    if quick is not None:
+        done = quick.keep(stack.like, len(stack.layers), stack._k_address, stack._v_address, page_table, lengths, row_offsets,
+                          kept, n_kept, status)
+        if done is not NotImplemented:
+            return
     if page_table.dim() != 2 or row_offsets.dim() != 1 or kept.dim() != 1:
         raise ValueError("page_table must be [n_seqs, max_pages], row_offsets [n_seqs + 1] and kept [rows]")
     n_seqs, max_pages = page_table.shape
@@ -551,7 +565,7 @@ def keep_kv_rows(
         _check_int(status, "status", (1,), like)
     _call(_lib.load().asterq_kv_keep,
           _KEEP.pack(_DTYPES[like.dtype], len(stack.layers), n_seqs, n_kv, dim, page, max_pages, 0, kept.shape[0], n_pages,
-                     _lib.ctypes.addressof(stack._k), _lib.ctypes.addressof(stack._v), page_table.data_ptr(),
+                     stack._k_address, stack._v_address, page_table.data_ptr(),
                      lengths.data_ptr(), row_offsets.data_ptr(), kept.data_ptr(), n_kept.data_ptr(),
                      0 if status is None else status.data_ptr()),
           like.device, torch.cuda.current_stream(like.device).cuda_stream)
@@ -572,7 +586,7 @@ def copy_kv_pages(stack: PagedKVStack, pairs: torch.Tensor, *, status: torch.Ten
         _check_int(status, "status", (1,), like)
     _call(_lib.load().asterq_kv_copy_pages,
           _COPY.pack(_DTYPES[like.dtype], len(stack.layers), n_kv, dim, page, pairs.shape[0], n_pages,
-                     _lib.ctypes.addressof(stack._k), _lib.ctypes.addressof(stack._v), pairs.data_ptr(),
+                     stack._k_address, stack._v_address, pairs.data_ptr(),
                      0 if status is None else status.data_ptr()),
           like.device, torch.cuda.current_stream(like.device).cuda_stream)
 

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _lib
+from . import _lib, paged_kv
 from .paged_kv import _call, _check_int, _check_no_gradient
 
 _PARAMS = _lib.packer(_lib.VerifyParams)
@@ -63,6 +63,11 @@ def verify_drafts(
     vocabulary (never accepted), a parent out of range (never reached), a distribution without a positive sum (next token
     -1), offsets out of order or too many nodes (nothing is kept, next token -1).
     """
+    quick = paged_kv._quick()
+    if quick is not None:
+        done = quick.verify(target_probs, tokens, row_offsets, parents, accept_uniforms, sample_uniforms, draft_probs, status)
+        if done is not NotImplemented:
+            return done
     if target_probs.dim() != 2 or row_offsets.dim() != 1 or row_offsets.shape[0] < 1:
         raise ValueError("target_probs must be [rows, vocab] and row_offsets [n_seqs + 1]")
     if target_probs.dtype not in _DTYPES:

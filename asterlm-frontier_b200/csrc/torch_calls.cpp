@@ -1,5 +1,5 @@
-// The shortest way from torch tensors to three entry points of the C library: a decode step calls them
-// for every layer, and at a few microseconds of GPU work the checks of a call in Python (some 15 us)
+// The shortest way from torch tensors to the entry points of the C library that a step calls for every
+// layer, or once for its drafts: and at a few microseconds of GPU work the checks of a call in Python (some 15 us)
 // are what the step waits for.
 //
 // A function here takes well-formed calls only.  Whatever else it is given (a wrong type, shape or device,
@@ -10,6 +10,7 @@
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -23,13 +24,14 @@
 namespace {
 
 using Entry = int (*)(const void*, void*);
-Entry g_append = nullptr, g_attend = nullptr, g_linear = nullptr;
+Entry g_append = nullptr, g_attend = nullptr, g_linear = nullptr, g_normed = nullptr, g_rows = nullptr, g_keep = nullptr,
+      g_verify = nullptr;
 
 struct Workspace {
   void* ptr;
   int64_t bytes;
 };
-std::map<std::pair<int, intptr_t>, Workspace> g_workspaces[2];  // of paged attention, of linear attention
+std::map<std::pair<int, intptr_t>, Workspace> g_workspaces[3];  // of paged attention, of linear attention, of the attention of prompts and trees
 
 PyObject* pass() { Py_RETURN_NOTIMPLEMENTED; }
 
@@ -76,9 +78,22 @@ PyObject* check_pools(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_RETURN_FALSE;
 }
 
-// append(k_pool, v_pool, page_table, lengths, row_offsets, k, v, q, cos, sin, interleaved, q_out, status)
+// What a vector of weights [dim] is to a call: absent, of a type code, or not for here
+bool weights(PyObject* o, int device, int64_t dim, int rows_type, const void*& ptr, int& type) {
+  if (o == Py_None) return true;
+  const at::Tensor* w = tensor(o);
+  if (!on(w, device) || w->sizes() != at::IntArrayRef({dim}) || !w->is_contiguous() || wants_gradient(w)) return false;
+  const int code = type_code(w->scalar_type());
+  if ((code != ASTERQ_DTYPE_F32 && code != rows_type) || (type >= 0 && type != code)) return false;
+  ptr = w->data_ptr();
+  type = code;
+  return true;
+}
+
+// append(k_pool, v_pool, page_table, lengths, row_offsets, k, v, q, cos, sin, interleaved, q_out, status,
+//        q_norm, k_norm, norm_eps, positions)
 PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 13 || !g_append) return pass();
+  if (n != 17 || !g_append || !g_normed) return pass();
   const at::Tensor *kp = tensor(args[0]), *vp = tensor(args[1]), *table = tensor(args[2]), *lengths = tensor(args[3]),
                    *offsets = tensor(args[4]), *k = tensor(args[5]), *v = tensor(args[6]);
   if (!pools_ok(kp, vp) || !table || table->dim() != 2) return pass();
@@ -126,28 +141,63 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return pass();
   }
   if (has_q && !given) out = at::empty({k->size(0), p.n_heads, dim}, k->options());
-  p.dtype = type_code(type);
-  p.n_seqs = (int32_t)n_seqs;
-  p.n_kv_heads = (int32_t)n_kv;
-  p.head_dim = (int32_t)dim;
-  p.interleaved = interleaved;
-  p.page_tokens = (int32_t)page;
-  p.max_pages = (int32_t)max_pages;
-  p.n_rows = k->size(0);
-  p.n_pages = kp->size(0);
-  p.k_row_stride = k->stride(0);
-  p.k_head_stride = k->stride(1);
-  p.v_row_stride = v->stride(0);
-  p.v_head_stride = v->stride(1);
-  p.k = k->data_ptr();
-  p.v = v->data_ptr();
-  p.page_table = static_cast<const int32_t*>(table->data_ptr());
-  p.lengths = static_cast<const int32_t*>(lengths->data_ptr());
-  p.row_offsets = static_cast<const int32_t*>(offsets->data_ptr());
-  p.q_out = has_q ? out.data_ptr() : nullptr;
-  p.k_pool = kp->data_ptr();
-  p.v_pool = vp->data_ptr();
-  if (g_append(&p, reinterpret_cast<void*>(stream_of(device))) != ASTERQ_OK) return pass();
+  const bool normed = args[13] != Py_None || args[14] != Py_None || args[16] != Py_None;
+  asterq_kv_append_normed_params w = {};
+  if (normed) {
+    int norm_type = -1;
+    if ((args[13] != Py_None && !has_q) || !PyFloat_CheckExact(args[15]) || !(PyFloat_AS_DOUBLE(args[15]) >= 0) ||
+        !weights(args[13], device, dim, type_code(type), w.q_norm, norm_type) ||
+        !weights(args[14], device, dim, type_code(type), w.k_norm, norm_type))
+      return pass();
+    w.norm_dtype = norm_type < 0 ? type_code(type) : norm_type;
+    w.norm_eps = (float)PyFloat_AS_DOUBLE(args[15]);
+    if (args[16] != Py_None) {
+      const at::Tensor* at = tensor(args[16]);
+      if (!p.cos || !ints(at, device, {k->size(0)})) return pass();
+      w.positions = static_cast<const int32_t*>(at->data_ptr());
+    }
+  }
+  const auto fill = [&](auto& p) {
+    p.dtype = type_code(type);
+    p.n_seqs = (int32_t)n_seqs;
+    p.n_kv_heads = (int32_t)n_kv;
+    p.head_dim = (int32_t)dim;
+    p.interleaved = interleaved;
+    p.page_tokens = (int32_t)page;
+    p.max_pages = (int32_t)max_pages;
+    p.n_rows = k->size(0);
+    p.n_pages = kp->size(0);
+    p.k_row_stride = k->stride(0);
+    p.k_head_stride = k->stride(1);
+    p.v_row_stride = v->stride(0);
+    p.v_head_stride = v->stride(1);
+    p.k = k->data_ptr();
+    p.v = v->data_ptr();
+    p.page_table = static_cast<const int32_t*>(table->data_ptr());
+    p.lengths = static_cast<const int32_t*>(lengths->data_ptr());
+    p.row_offsets = static_cast<const int32_t*>(offsets->data_ptr());
+    p.q_out = has_q ? out.data_ptr() : nullptr;
+    p.k_pool = kp->data_ptr();
+    p.v_pool = vp->data_ptr();
+  };
+  int status;
+  if (normed) {
+    w.n_heads = p.n_heads;
+    w.rotary_dim = p.rotary_dim;
+    w.n_positions = p.n_positions;
+    w.q_row_stride = p.q_row_stride;
+    w.q_head_stride = p.q_head_stride;
+    w.q = p.q;
+    w.cos = p.cos;
+    w.sin = p.sin;
+    w.status = p.status;
+    fill(w);
+    status = g_normed(&w, reinterpret_cast<void*>(stream_of(device)));
+  } else {
+    fill(p);
+    status = g_append(&p, reinterpret_cast<void*>(stream_of(device)));
+  }
+  if (status != ASTERQ_OK) return pass();
   if (!has_q) Py_RETURN_NONE;
   if (given) {
     Py_INCREF(args[11]);
@@ -313,14 +363,200 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return THPVariable_Wrap(out);
 }
 
-// bind(append, attend, linear): addresses of the library's entry points
+// rows(k_pool, v_pool, page_table, lengths, row_offsets, parents, q, scale, softcap, window, sink, out, want_lse, status)
+//   -> out, or (out, lse)
+PyObject* rows_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 14 || !g_rows) return pass();
+  const at::Tensor *kp = tensor(args[0]), *vp = tensor(args[1]), *table = tensor(args[2]), *lengths = tensor(args[3]),
+                   *offsets = tensor(args[4]), *q = tensor(args[6]);
+  if (!pools_ok(kp, vp) || !table || table->dim() != 2) return pass();
+  const int device = kp->get_device();
+  const at::ScalarType type = kp->scalar_type();
+  const int64_t n_seqs = table->size(0), max_pages = table->size(1), n_kv = kp->size(1), dim = kp->size(3);
+  if (device != c10::cuda::current_device() || !rows(q, device, type, dim) || n_kv == 0 || q->size(1) == 0 ||
+      q->size(1) % n_kv || q->size(0) == 0 || n_seqs == 0 || q->stride(0) <= 0 || q->stride(1) <= 0 ||
+      !ints(table, device, {n_seqs, max_pages}) || !ints(lengths, device, {n_seqs}) || !ints(offsets, device, {n_seqs + 1}) ||
+      n_seqs > INT32_MAX || max_pages > INT32_MAX)
+    return pass();
+  if (!PyFloat_CheckExact(args[7]) || !PyFloat_CheckExact(args[8]) || !PyLong_CheckExact(args[9]) || !PyLong_CheckExact(args[10]))
+    return pass();
+  const long window = PyLong_AsLong(args[9]), sink = PyLong_AsLong(args[10]);
+  const int want_lse = PyObject_IsTrue(args[12]);
+  if (PyErr_Occurred() || window < 0 || sink < 0 || window > INT32_MAX || sink > INT32_MAX) {
+    PyErr_Clear();
+    return pass();
+  }
+  // a graph's calls take a workspace of the graph's own memory
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return pass();
+  const intptr_t stream = stream_of(device);
+  const auto ws = g_workspaces[2].find({device, stream});
+  if (ws == g_workspaces[2].end()) return pass();
+  asterq_rows_attention_params p = {};
+  bool ok = true;
+  p.status = static_cast<int32_t*>(status_of(args[13], device, ok));
+  if (!ok) return pass();
+  if (args[5] != Py_None) {
+    const at::Tensor* parents = tensor(args[5]);
+    if (!ints(parents, device, {q->size(0)})) return pass();
+    p.parents = static_cast<const int32_t*>(parents->data_ptr());
+  }
+  at::Tensor out, lse;
+  const bool given = args[11] != Py_None;
+  if (given) {
+    const at::Tensor* o = tensor(args[11]);
+    if (!on(o, device) || o->sizes() != q->sizes() || !o->is_contiguous() || wants_gradient(o)) return pass();
+    out = *o;
+  } else {
+    out = at::empty(q->sizes(), q->options());
+  }
+  if (want_lse) lse = at::empty({q->size(0), q->size(1)}, q->options().dtype(at::kFloat));
+  p.dtype = type_code(type);
+  p.out_dtype = type_code(out.scalar_type());
+  p.n_seqs = (int32_t)n_seqs;
+  p.n_heads = (int32_t)q->size(1);
+  p.n_kv_heads = (int32_t)n_kv;
+  p.head_dim = (int32_t)dim;
+  p.page_tokens = (int32_t)kp->size(2);
+  p.max_pages = (int32_t)max_pages;
+  p.window = (int32_t)window;
+  p.sink = (int32_t)sink;
+  p.softmax_scale = (float)PyFloat_AS_DOUBLE(args[7]);
+  p.logit_softcap = (float)PyFloat_AS_DOUBLE(args[8]);
+  p.n_rows = q->size(0);
+  p.n_pages = kp->size(0);
+  p.q_row_stride = q->stride(0);
+  p.q_head_stride = q->stride(1);
+  p.q = q->data_ptr();
+  p.k_pool = kp->data_ptr();
+  p.v_pool = vp->data_ptr();
+  p.page_table = static_cast<const int32_t*>(table->data_ptr());
+  p.lengths = static_cast<const int32_t*>(lengths->data_ptr());
+  p.row_offsets = static_cast<const int32_t*>(offsets->data_ptr());
+  p.out = out.data_ptr();
+  p.lse = want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr;
+  p.workspace = ws->second.ptr;
+  p.workspace_bytes = ws->second.bytes;
+  if (g_rows(&p, reinterpret_cast<void*>(stream)) != ASTERQ_OK) return pass();
+  PyObject* o = args[11];
+  if (given) Py_INCREF(o);
+  else o = THPVariable_Wrap(out);
+  if (!want_lse) return o;
+  PyObject* l = THPVariable_Wrap(lse);
+  PyObject* both = o && l ? PyTuple_Pack(2, o, l) : nullptr;
+  Py_XDECREF(o);
+  Py_XDECREF(l);
+  return both;
+}
+
+// keep(k_pool of layer 0, n_layers, address of the k pools' addresses, of the v pools', page_table, lengths, row_offsets,
+//      kept, n_kept, status)
+PyObject* keep(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 10 || !g_keep) return pass();
+  const at::Tensor *kp = tensor(args[0]), *table = tensor(args[4]), *lengths = tensor(args[5]), *offsets = tensor(args[6]),
+                   *kept = tensor(args[7]), *n_kept = tensor(args[8]);
+  if (!pools_ok(kp, kp) || !table || table->dim() != 2 || !kept || kept->dim() != 1) return pass();
+  const int device = kp->get_device();
+  const int64_t n_seqs = table->size(0), max_pages = table->size(1);
+  if (device != c10::cuda::current_device() || !ints(table, device, {n_seqs, max_pages}) || !ints(lengths, device, {n_seqs}) ||
+      !ints(offsets, device, {n_seqs + 1}) || !ints(kept, device, {kept->size(0)}) || !ints(n_kept, device, {n_seqs}) ||
+      n_seqs > INT32_MAX || max_pages > INT32_MAX)
+    return pass();
+  asterq_kv_keep_params p = {};
+  bool ok = true;
+  p.status = static_cast<int32_t*>(status_of(args[9], device, ok));
+  const long layers = PyLong_AsLong(args[1]);
+  p.k_pools = reinterpret_cast<void* const*>(PyLong_AsSize_t(args[2]));
+  p.v_pools = reinterpret_cast<void* const*>(PyLong_AsSize_t(args[3]));
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return pass();
+  }
+  if (!ok || layers > INT32_MAX) return pass();
+  p.dtype = type_code(kp->scalar_type());
+  p.n_layers = (int32_t)layers;
+  p.n_seqs = (int32_t)n_seqs;
+  p.n_kv_heads = (int32_t)kp->size(1);
+  p.head_dim = (int32_t)kp->size(3);
+  p.page_tokens = (int32_t)kp->size(2);
+  p.max_pages = (int32_t)max_pages;
+  p.n_rows = kept->size(0);
+  p.n_pages = kp->size(0);
+  p.page_table = static_cast<const int32_t*>(table->data_ptr());
+  p.lengths = static_cast<const int32_t*>(lengths->data_ptr());
+  p.row_offsets = static_cast<const int32_t*>(offsets->data_ptr());
+  p.kept = static_cast<const int32_t*>(kept->data_ptr());
+  p.n_kept = static_cast<const int32_t*>(n_kept->data_ptr());
+  if (g_keep(&p, reinterpret_cast<void*>(stream_of(device))) != ASTERQ_OK) return pass();
+  Py_RETURN_NONE;
+}
+
+// verify(target_probs, tokens, row_offsets, parents, accept_uniforms, sample_uniforms, draft_probs, status)
+//   -> (kept, n_kept, next_token)
+PyObject* verify(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 8 || !g_verify) return pass();
+  const at::Tensor *target = tensor(args[0]), *tokens = tensor(args[1]), *offsets = tensor(args[2]), *accept = tensor(args[4]),
+                   *sample = tensor(args[5]);
+  if (!target || !target->is_cuda() || target->dim() != 2 || !offsets || offsets->dim() != 1 || offsets->size(0) < 2) return pass();
+  const int device = target->get_device();
+  const int64_t n_rows = target->size(0), vocab = target->size(1), n_seqs = offsets->size(0) - 1;
+  const auto probs = [&](const at::Tensor* t) {
+    return on(t, device) && t->sizes() == target->sizes() && t->scalar_type() == target->scalar_type() && t->stride(1) == 1 &&
+           !wants_gradient(t);
+  };
+  const auto uniforms = [&](const at::Tensor* t, int64_t count) {
+    return on(t, device) && t->scalar_type() == at::kFloat && t->sizes() == at::IntArrayRef({count}) && t->is_contiguous();
+  };
+  if (device != c10::cuda::current_device() || type_code(target->scalar_type()) < 0 || vocab == 0 || vocab > INT32_MAX ||
+      n_seqs > INT32_MAX || !probs(target) || !ints(tokens, device, {n_rows}) || !ints(offsets, device, {n_seqs + 1}) ||
+      !uniforms(accept, n_rows) || !uniforms(sample, n_seqs))
+    return pass();
+  asterq_verify_params p = {};
+  bool ok = true;
+  p.status = static_cast<int32_t*>(status_of(args[7], device, ok));
+  if (!ok) return pass();
+  if (args[3] != Py_None) {
+    const at::Tensor* parents = tensor(args[3]);
+    if (!ints(parents, device, {n_rows})) return pass();
+    p.parents = static_cast<const int32_t*>(parents->data_ptr());
+  }
+  if (args[6] != Py_None) {
+    const at::Tensor* draft = tensor(args[6]);
+    if (!probs(draft)) return pass();
+    p.draft = draft->data_ptr();
+    p.draft_stride = draft->stride(0);
+  }
+  const auto kind = tokens->options();
+  at::Tensor kept = at::empty({n_rows}, kind), n_kept = at::empty({n_seqs}, kind), next = at::empty({n_seqs}, kind);
+  p.dtype = type_code(target->scalar_type());
+  p.n_seqs = (int32_t)n_seqs;
+  p.vocab = (int32_t)vocab;
+  p.n_rows = n_rows;
+  p.target_stride = target->stride(0);
+  p.target = target->data_ptr();
+  p.tokens = static_cast<const int32_t*>(tokens->data_ptr());
+  p.row_offsets = static_cast<const int32_t*>(offsets->data_ptr());
+  p.accept = static_cast<const float*>(accept->data_ptr());
+  p.sample = static_cast<const float*>(sample->data_ptr());
+  p.kept = static_cast<int32_t*>(kept.data_ptr());
+  p.n_kept = static_cast<int32_t*>(n_kept.data_ptr());
+  p.next_token = static_cast<int32_t*>(next.data_ptr());
+  if (g_verify(&p, reinterpret_cast<void*>(stream_of(device))) != ASTERQ_OK) return pass();
+  PyObject *a = THPVariable_Wrap(kept), *b = THPVariable_Wrap(n_kept), *c = THPVariable_Wrap(next);
+  PyObject* all = a && b && c ? PyTuple_Pack(3, a, b, c) : nullptr;
+  Py_XDECREF(a);
+  Py_XDECREF(b);
+  Py_XDECREF(c);
+  return all;
+}
+
+// bind(append, attend, linear, normed append, rows, keep, verify): addresses of the library's entry points
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 3) {
-    PyErr_SetString(PyExc_TypeError, "bind takes three addresses");
+  Entry* to[] = {&g_append, &g_attend, &g_linear, &g_normed, &g_rows, &g_keep, &g_verify};
+  if (n != 7) {
+    PyErr_SetString(PyExc_TypeError, "bind takes seven addresses");
     return nullptr;
   }
-  Entry* to[] = {&g_append, &g_attend, &g_linear};
-  for (int i = 0; i < 3; ++i) *to[i] = reinterpret_cast<Entry>(PyLong_AsSize_t(args[i]));
+  for (int i = 0; i < 7; ++i) *to[i] = reinterpret_cast<Entry>(PyLong_AsSize_t(args[i]));
   if (PyErr_Occurred()) return nullptr;
   Py_RETURN_NONE;
 }
@@ -335,8 +571,8 @@ PyObject* workspace(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const size_t stream = PyLong_AsSize_t(args[2]), ptr = PyLong_AsSize_t(args[3]);
   const long long bytes = PyLong_AsLongLong(args[4]);
   if (PyErr_Occurred()) return nullptr;
-  if (kind < 0 || kind > 1) {
-    PyErr_SetString(PyExc_ValueError, "kind is 0 or 1");
+  if (kind < 0 || kind > 2) {
+    PyErr_SetString(PyExc_ValueError, "kind is 0, 1 or 2");
     return nullptr;
   }
   g_workspaces[kind][{(int)device, (intptr_t)stream}] = {reinterpret_cast<void*>(ptr), bytes};
@@ -361,6 +597,7 @@ PyMethodDef method(const char* name) {
 
 PyMethodDef g_methods[] = {method<check_pools>("check_pools"), method<append>("append"), method<attend>("attend"),
                            method<linear>("linear"),           method<bind>("bind"),     method<workspace>("workspace"),
+                           method<rows_attention>("rows"),     method<keep>("keep"),     method<verify>("verify"),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
