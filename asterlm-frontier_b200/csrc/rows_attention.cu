@@ -87,7 +87,7 @@ struct Cfg {
   // each place and half, so that whoever waits sees all phases of one
   static constexpr int kEmpty = kSlots, kClean = 2 * kSlots, kQFull = 3 * kSlots, kQEmpty = kQFull + 1, kWFull = kQEmpty + 1,
                        kWEmpty = kWFull + 2, kSFull = kWEmpty + 2, kPReady = kSFull + 2, kDone = kPReady + 4,
-                       kDrain = kDone + 2, kBars = kDrain + 1;
+                       kDrain = kDone + 2, kMeet = kDrain + 1, kBars = kMeet + 1;
   // behind the slots: barriers, two work entries, what threads exchange
   static constexpr int kAtWork = (kBars * 8 + 15) / 16 * 16, kAtFlags = kAtWork + 160, kAtUp = kAtFlags + 16,
                        kAtSwap = kAtUp + 2 * kMaxNodes, kSmall = kAtSwap + 2 * kRowsTile * 4;
@@ -310,16 +310,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31, me = blockIdx.x;
 
   asm volatile("griddepcontrol.launch_dependents;");
-  if (tid == 0) {
-    for (int i = 0; i < C::kBars; ++i) {
-      int count = 1;
-      if (i >= C::kEmpty && i < C::kClean) count = 3;  // the products', and two warps that look values over
-      else if (i >= C::kClean && i < C::kQFull) count = 2;
-      else if (i >= C::kWEmpty && i < C::kSFull) count = 11;
-      else if (i >= C::kPReady && i < C::kDone) count = 4;  // a warp each
-      mbar_init(bar(i), count);
-    }
+  if (tid < C::kBars) {
+    const int i = tid;
+    int count = 1;
+    if (i >= C::kEmpty && i < C::kClean) count = 3;  // the products', and two warps that look values over
+    else if (i >= C::kClean && i < C::kQFull) count = 2;
+    else if (i >= C::kWEmpty && i < C::kSFull) count = 11;
+    else if (i >= C::kPReady && i < C::kDone) count = 4;  // a warp each
+    else if (i == C::kMeet) count = 8;
+    mbar_init(bar(i), count);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (tid == 0) {
     // boxes lie in patterns of 1024 bytes
     *abort_s = (q_base & 1023) != 0;
     *never_s = 0;
@@ -835,7 +837,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int token_in = r / a.group, head_in = r - token_in * a.group;
     const bool in_tile = token_in < a.tile_tokens;
     const float scale2 = C::kPre ? 1.0f : a.scale2;
-    uint32_t full = 0, done = 0, rests = 0;  // phases: of kSFull (a bit a place) and kDone; jobs so far
+    uint32_t full = 0, done = 0, met = 0, rests = 0;  // phases: of kSFull (a bit a place), kDone and kMeet; jobs so far
+    // Both warpgroups of a unit that they share.  With others each goes its own way, and one's outputs are written under the
+    // other's products.
+    auto meet = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(C::kMeet));
+      wait_quietly(bar(C::kMeet), met, abort_s);
+      met ^= 1;
+      __syncwarp();
+    };
     View view;
     int view_row = -1, view_tok0 = 0;
     bool view_pair = false;
@@ -843,8 +854,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int piece = 0;; ++piece) {
       const int e = piece & 1;
       const bool got = wait_for(bar(C::kWFull + e), (piece >> 1) & 1, abort_s);
-      // all warps go on or none does: they meet at barriers (after a wait has run out, waits return at once)
-      if (!named_all(1, 256, got)) break;
+      // a warpgroup goes on or does not: its warps meet at barriers (after a wait has run out, waits return at once)
+      if (!named_all(2 + tile, 128, got)) break;
       const Work* u = work + e;
       const int n = u->n, k0 = u->k0;
       if (n == 0) break;
@@ -962,12 +973,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_arrive(p_ready);
             mbar_arrive(p_ready + 8);
           }
-        } else if (!C::kPre && whole) {
+        } else if (!C::kPre && (whole || !a.parents)) {
           uint32_t s[kParts][32];
 #pragma unroll
           for (int k = 0; k < kParts; ++k) tc::ld32(s[k], s_at + 32 * k);
 #pragma unroll
           for (int k = 0; k < kParts; ++k) wait_ld32(s[k]);
+          if (!whole) {
+            uint32_t w[kParts];
+#pragma unroll
+            for (int k = 0; k < kParts; ++k) w[k] = view.template bits<false>(c + 32 * k);
+#pragma unroll
+            for (int k = 0; k < kParts; ++k) {
+              if (__all_sync(0xffffffffu, w[k] == 0xffffffffu)) continue;
+#pragma unroll
+              for (int x = 0; x < 32; ++x) s[k][x] = w[k] >> x & 1u ? s[k][x] : 0xff800000u;
+            }
+          }
           float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int k = 0; k < kParts; ++k)
@@ -988,8 +1010,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           ready(1);
         } else {
-          // Tiles that some row does not see all of, and scores that are changed: 32 keys at a time, the scores as they are meant
-          // put back by a first round.  Keys that none of the warp's rows sees cost nothing more.
+          // Trees' tiles that some row does not see all of, and scores that are changed: 32 keys at a time, the scores as they
+          // are meant put back by a first round.  Keys that none of the warp's rows sees cost nothing more.  (Prompts of 16,393
+          // tokens with a window of 1,024, four tiles of ten: 170 us so, 161 by masks in registers as above.  For trees, with
+          // one such tile or two, it makes no difference.)
           uint32_t live = 0;
           float top = -INFINITY;
 #pragma unroll 1
@@ -1082,7 +1106,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           swap_s[kRowsTile + r] = l;
         }
         tc::fence_before();
-        named_sync(1, 256);
+        meet();
         tc::fence_after();
         if (second && tile == 0) {
           const float m1 = swap_s[r], l1 = swap_s[kRowsTile + r], now = fmaxf(m, m1);
@@ -1123,7 +1147,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
             wait_ld32(o);
           }
-          if (poison) put_back(o, d);
+          if (__builtin_expect(poison, 0)) put_back(o, d);
           if (cut && valid) {
             float4* rec = reinterpret_cast<float4*>(a.records) + ((long long)u->slot * (D / 4) + d / 4) * C::kRows + row_in;
 #pragma unroll
@@ -1154,7 +1178,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::fence_before();
       }
       // the sums, and the second accumulator, have been read
-      if (pair) named_sync(1, 256);
+      if (pair) meet();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(C::kWEmpty + e));
     }
