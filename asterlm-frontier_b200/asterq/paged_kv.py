@@ -5,17 +5,24 @@ Their keys and values live in page pools (``PagedKVPools``) with int32 page tabl
 the GPU:
 
 * ``append_kv``: a step's or a prompt chunk's new keys and values at the end of each sequence,
-  rotated by position on the way, with the rotated queries beside them (``asterq_kv_append``);
+  rotated by position on the way, with the rotated queries beside them (``asterq_kv_append``), their heads
+  normed first and their positions given where asked (``asterq_kv_append_normed``);
 * ``paged_attention``: one new token a sequence over its pages, the work split evenly over all SMs
   and joined in the same launch (``asterq_paged_attention``);
+* ``paged_prompt_attention``, ``paged_tree_attention``: many new tokens a sequence, causal among themselves or
+  nodes of a tree of drafted tokens (``asterq_rows_attention``);
+* ``keep_kv_rows``, ``copy_kv_pages``: accepted rows closed up, pages copied, in all layers of a
+  ``PagedKVStack`` (``asterq_kv_keep``, ``asterq_kv_copy_pages``);
 * ``PagedKVBatch``: the pools of a stack of layers with the page tables they share, for a server that
-  admits, steps and removes sequences.
+  admits, steps, forks and removes sequences.
 
 There is no backward pass: inputs that require a gradient are refused outside of ``torch.no_grad()``.
-Nothing here waits for the GPU or reads from it, so all of it can be recorded in a CUDA graph.  A first
+But for ``PagedKVBatch.accept`` nothing here waits for the GPU or reads from it, so all of it can be recorded in a CUDA graph.  A first
 call on a stream, or ``workspace``, gives that stream's calls their workspace; a captured ``paged_attention``
 without either has one of its own, zeroed at every replay (5 MB).  A captured call keeps its workspace wherever
-its graph is replayed: graphs that overlap each other, or other calls of the stream, need one each.
+its graph is replayed: graphs that overlap each other, or other calls of the stream, need one each.  A captured
+``paged_prompt_attention`` or ``paged_tree_attention`` has one of its graph's own memory unless one is given (40 MB, shared by a
+graph's calls one after the other).
 """
 from __future__ import annotations
 

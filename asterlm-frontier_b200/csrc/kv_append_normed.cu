@@ -9,7 +9,10 @@
 //
 // Bound by memory: 2 bytes in and 2 out a value, and some ten operations.  A head is held by the lanes of one
 // group, 16 dims each (two 16-byte vectors whose pairs share eight cos and sin values), so its sum of squares
-// is a few shuffles; a group walks over heads, and CTAs over rows with the weights in registers.
+// is a few shuffles; a group walks over heads, and CTAs over rows with the weights in shared memory (in registers, 112
+// of them a thread, 16,387 rows took 107 us instead of 84).
+// Measured: 16,387 rows of 32 + 8 + 8 heads of 128 dims, 407 MB in and out: 84 us, 4.84 TB/s (0.74 of the measured copy
+// bandwidth); 32 rows 6.2 us, a launch.
 #include "asterq_internal.h"
 #include "common.cuh"
 #include "launch.cuh"
@@ -210,10 +213,12 @@ extern "C" int asterq_kv_append_normed(const asterq_kv_append_normed_params* p, 
   if (sms <= 0) return set_error(ASTERQ_ERR_CUDA, "kv_append_normed: no CUDA device");
   int lanes = 1;
   while (lanes < p->head_dim / 16) lanes *= 2;
-  // threads of a row: for all its heads at once while rows are few, 64 for many
+  // Threads of a row: for all its heads at once while rows are few, 64 for many.  With 32 + 8 + 8 heads of 128 dims, at
+  // once and by 64: 300 rows 6.2 and 8.3 us, 600 8.4 and 10.3, 1200 12.4 and 10.3, 4800 33 and 26.
+  // CTAs an SM: 4 84.3 us, 8 86.0, 16 88.1 (16,387 rows); one for each four rows 90.5.
   const int64_t items = (int64_t)lanes * ((p->q ? p->n_heads : 0) + 2 * p->n_kv_heads);
   int per_row = kvn::kThreads;
-  while (per_row > 64 && (per_row / 2 >= items || p->n_rows >= 600)) per_row /= 2;
+  while (per_row > 64 && (per_row / 2 >= items || p->n_rows >= 1000)) per_row /= 2;
   const int rows_per_block = kvn::kThreads / per_row;
   const int64_t blocks = (p->n_rows + rows_per_block - 1) / rows_per_block, most = (int64_t)sms * 4;
   const unsigned grid = (unsigned)(blocks < most ? blocks : most);

@@ -2,6 +2,8 @@
 //   keep   accepted rows of a draft closed up behind the cached tokens: place length + kept[i] to length + i
 //   copy   whole pages to others (a forked sequence's last page, pages moved together)
 // Bytes in and bytes out are all there is to it: both move 16-byte vectors, several loads of a thread under way.
+// Measured: 60 pages of 64 tokens, 8 heads of 128 f16 dims and 24 layers, 755 MB in and out: 113 us, 6.6 TB/s, the measured copy
+// bandwidth; 48 trees' accepted rows in 16 layers, 25 MB: 8.3 us.
 #include "asterq_internal.h"
 #include "common.cuh"
 

@@ -18,7 +18,14 @@
 // tiles of keys; they join at its end, through tensor memory.
 // S = Q K^T (128 x 128, fp32) lies in tensor memory, its weights as 16-bit values over it, O beside it.  The chain of a tile
 // (softmax, then product and next scores, 1,024 cycles of the tensor cores, and two waits of some 300 until one side sees
-// the other) is what sets the pace; the weights are handed over in halves to shorten it.
+// the other) is what sets the pace; the weights are handed over in halves to shorten it.  (Tried and slower: a third place for
+// scores of 64 dims, tiles of 64 keys, sixteen softmax warps, a warp of products for each row tile, and a quarter of the
+// exponentials by a polynomial: 5 to 8 % longer, although the softmax alone is 8 % faster so.)
+// Measured, one sequence of 8,192 rows over 24,576 cached, 32 over 8 heads of 128 dims, bf16: 3.1 to 3.4 ms, 1.13 to 1.22 PFLOP/s by
+// the clock that the power limit leaves, 0.67 to 0.73 of the measured burst of matrix products.  9 prompts of 16,393 rows with a
+// window of 1,024 (16 over 8 heads of 64 dims, f16): 161 us, whose 268 million exponentials in whole tiles are 74.  32
+// trees of 16 nodes: 93 us, 4.0 TB/s.  One tree of 8 nodes 19 us, a prompt of 150 tokens 25: one pass through code that no SM has
+// run before, some 5,000 cycles of it until the first copies.
 //
 // Split.  The key tiles of all units laid end to end (with kUnitCost in front of each) are cut into equal contiguous
 // shares, one for each CTA, by sums over lengths and offsets that every CTA does for itself: no planning launch, no
@@ -43,6 +50,9 @@ constexpr float kLn2 = 0.693147180559945309417f;
 // registers of a thread: 256 x 216 + 128 x 72 = 384 x 168 of the launch
 constexpr int kRegsLaunch = 168, kRegsSoftmax = 216, kRegsHelp = 72;
 static_assert(256 * kRegsSoftmax + 128 * kRegsHelp <= kThreads * kRegsLaunch, "more registers than launched with");
+// What a unit costs beside its tiles, and the least that a CTA takes, in tiles.  (kUnitCost, kMinShare): a prompt of 150 tokens,
+// 9 windowed prompts, one tree of 8, 32 of 16, 24 of 61 in us.  (1, 2): 26.8, 171, 18.8, 93, 294; (3, 2): 26.8, 174, 19.1, 95, 287;
+// (1, 6): 32.9, 171, 24.9, 93, 294; (1, 3): 24.9, 171, 23.6, 93, 293.
 constexpr int kUnitCost = 1;
 constexpr int kMinShare = 2;
 
@@ -1194,8 +1204,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 // The records of the cut units become their rows.  A place is four dims of a row; rows lie side by side, as the records have
 // them.  A CTA lists the units (one descriptor a thread) and takes every gridDim.x-th strip of places: 256 with a
 // thread each, or 64 of a unit of many pieces, whose pieces four threads take in turn and join in shared memory.  What it takes
-// is latency: two rounds of loads for up to eight pieces, and enough CTAs beside one another.  (Strips of 64 throughout, 2.4
-// times fewer CTAs: 55 us for 148 units of two pieces, 256 rows and 128 dims; so 7.)
+// is latency: two rounds of loads for up to eight pieces, and enough CTAs beside one another.  (Strips of 64 throughout and
+// 2.4 times fewer CTAs: 50 to 150 us a call.  So, on a cold cache: 8 us for one tree of 8, 16 for the cut units of 9 windowed
+// prompts of 64 dims, 26 for those of 24 trees of 61 nodes and 128 dims.)
 constexpr int kJoinThreads = 256, kJoinFew = 8, kJoinLoads = 4, kJoinCtas = 5;
 template <class C>
 __global__ void __launch_bounds__(kJoinThreads, kJoinCtas) join_kernel(const __grid_constant__ Args a, int workers) {
