@@ -79,6 +79,8 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const Args a) {
     }
     return;
   }
+  // a CTA's shared memory may be written by others once it has begun: arrived at here, waited for before the first sum
+  if (ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;");
   bool odd = false;
   for (int i = tid; i < n; i += kThreads) {
     int up = a.parents ? __ldg(a.parents + begin + i) : i - 1;
@@ -176,6 +178,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const Args a) {
     __syncthreads();
     if (lane == 0) warp_sums[warp] = mine;
     __syncthreads();
+    if (round == 0 && ranks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     double* sums = rank_sums[round & 1];
     ++round;
     if (tid < ranks) {
