@@ -581,7 +581,8 @@ def keep_kv_rows(
 def copy_kv_pages(stack: PagedKVStack, pairs: torch.Tensor, *, status: torch.Tensor | None = None) -> None:
     """Copy pages in all layers of a stack (one launch): pairs int32 [n, 2], page ``pairs[i, 1]`` becomes a copy of page
     ``pairs[i, 0]``.  A pair with a negative entry is left out.  So is, with status int32 [1] set to 1, one with a page
-    outside the pools, and every pair whose destination another pair names too or whose source another pair writes."""
+    outside the pools, and every pair whose destination another pair names too or whose source another pair writes.
+    Each pair is held against all others of the call for that, so thousands of pairs are better given in parts."""
     like = stack.like
     n_pages, n_kv, page, dim = like.shape
     if pairs.dim() != 2:
@@ -779,8 +780,10 @@ class PagedKVBatch:
         return n
 
     def _copy(self, pairs: np.ndarray) -> None:
+        # no page is written by one pair and named by another, so they can go in parts
         pairs = torch.from_numpy(np.ascontiguousarray(pairs, np.int32)).pin_memory().to(self.device, non_blocking=True)
-        copy_kv_pages(self.stack, pairs, status=self.status)
+        for part in pairs.split(2048):
+            copy_kv_pages(self.stack, part, status=self.status)
 
     def _begin(self, new: np.ndarray, one_row: bool) -> None:
         if self._open:

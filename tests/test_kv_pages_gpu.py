@@ -322,3 +322,30 @@ def test_a_pool_that_runs_out_leaves_the_batch_as_it_was(cuda):
     batch.remove_sequence(a)
     _write(batch, [b], [2], 2)
     _consistent(batch)
+
+
+def test_thousands_of_pages_move(cuda):
+    from asterq.paged_kv import PagedKVBatch
+
+    pages = 2700
+    batch = PagedKVBatch(2, 1, 64, max_seqs=2, max_tokens=16 * pages + 16, page_tokens=16)
+    for _ in range(2):
+        batch.begin_rows([batch.add_sequence()], [16 * pages])
+        batch.end_step()
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for pools in batch.layers:
+        pools.k.copy_(torch.randn(pools.k.shape, device="cuda", generator=g))
+        pools.v.copy_(torch.randn(pools.v.shape, device="cuda", generator=g))
+    first = batch.page_table[0, 0].item() < batch.page_table[1, 0].item()
+    batch.remove_sequence(0 if first else 1)  # the one in front
+    kept = 1 if first else 0
+    at = batch.page_table[kept, :pages].long()
+    want = [t[at].clone() for pools in batch.layers for t in (pools.k, pools.v)]
+    assert at.min().item() >= pages and batch.compact_pages() == pages
+    batch.begin_step()
+    batch.abandon_step()
+    now = batch.page_table[kept, :pages].long()
+    assert sorted(now.tolist()) == list(range(pages))
+    for x, y in zip(want, [t[now] for pools in batch.layers for t in (pools.k, pools.v)], strict=True):
+        assert torch.equal(x, y)
+    batch.raise_if_failed()
