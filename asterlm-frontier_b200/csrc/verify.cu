@@ -375,11 +375,14 @@ extern "C" int asterq_verify_drafts(const asterq_verify_params* p, void* stream)
   a.draft_stride = p->draft_stride;
   a.n_rows = p->n_rows;
   a.vocab = p->vocab;
-  // CTAs of a sequence: as many as keep a part of 2048 tokens or more and fill the SMs some twice.  Of 96 trees over 128,256
-  // tokens, at most 2, 4 and 8 CTAs for two SMs: 87, 64 and 74 us.  Parts from 512 or from 8192 tokens on make no difference above
-  // 2 us for vocabularies of 2,048 to 32,768.
+  // CTAs of a sequence: 8, where that leaves two a SM to each; more sequences have 4, as the passes of one wait for one another
+  // and the others' fill the SMs, and from twice the SMs on 2; each has a part of 2048 tokens or more.  Trees of 12 over 128,256
+  // tokens, 1, 2, 4 and 8 CTAs: 16 sequences 153, 86, 52, 37 us; 74: 157, 89, 63, 59; 96: 161, 89, 64, 75; 160: 242, 133,
+  // 95, 118; 240: 263, 152, 130, 173; 320: 227, 157, 162, 218; 480: 282, 228, 234, 321.  Parts from 512 or from 8192 tokens on make no
+  // difference above 2 us for vocabularies of 2,048 to 32,768.
+  const int most = p->n_seqs <= sms / 2 ? ver::kMaxCluster : p->n_seqs <= 2 * sms ? 4 : 2;
   int ranks = 1;
-  while (ranks < ver::kMaxCluster && (int64_t)p->n_seqs * ranks * 2 <= 4 * sms && p->vocab / (ranks * 2) >= 2048) ranks *= 2;
+  while (ranks < most && p->vocab / (ranks * 2) >= 2048) ranks *= 2;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const cudaError_t e = p->dtype == ASTERQ_DTYPE_F32    ? ver::launch<ASTERQ_DTYPE_F32>(a, p->n_seqs, ranks, s)
                         : p->dtype == ASTERQ_DTYPE_BF16 ? ver::launch<ASTERQ_DTYPE_BF16>(a, p->n_seqs, ranks, s)
