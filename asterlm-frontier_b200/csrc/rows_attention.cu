@@ -24,7 +24,7 @@
 // Measured, one sequence of 8,192 rows over 24,576 cached, 32 over 8 heads of 128 dims, bf16: 3.1 to 3.4 ms, 1.13 to 1.22 PFLOP/s by
 // the clock that the power limit leaves, 0.67 to 0.73 of the measured burst of matrix products.  9 prompts of 16,393 rows with a
 // window of 1,024 (16 over 8 heads of 64 dims, f16): 161 us, whose 268 million exponentials in whole tiles are 74.  32
-// trees of 16 nodes: 93 us, 4.0 TB/s.  One tree of 8 nodes 19 us, a prompt of 150 tokens 25: one pass through code that no SM has
+// trees of 16 nodes: 90 us, 4.1 TB/s.  One tree of 8 nodes 19 us, a prompt of 150 tokens 25: one pass through code that no SM has
 // run before, some 5,000 cycles of it until the first copies.
 //
 // Split.  The key tiles of all units laid end to end (with kUnitCost in front of each) are cut into equal contiguous
@@ -81,14 +81,15 @@ struct Args {
 };
 
 // kPre: scores are changed before their maximum is taken (a softcap, or a scale that is not positive)
-template <bool kF16_, int D_, bool kPre_>
+// kOne: no unit has more than one row tile, and the second one's queries leave their room to keys and values
+template <bool kF16_, int D_, bool kPre_, bool kOne_>
 struct Cfg {
-  static constexpr bool kF16 = kF16_, kPre = kPre_;
+  static constexpr bool kF16 = kF16_, kPre = kPre_, kOne = kOne_;
   static constexpr int D = D_;
   static constexpr int kTiles = D == 256 ? 1 : 2;  // row tiles of a unit: two accumulators of 256 dims leave no room for scores
   static constexpr int kRows = kTiles * kRowsTile, kKeys = D == 256 ? 64 : 128;
   static constexpr int kQBytes = kRowsTile * D * 2, kSlotBytes = kKeys * D * 2;  // a slot holds a tile of keys or of values
-  static constexpr int kSlots = D == 64 ? 12 : 5;
+  static constexpr int kQTiles = kOne ? 1 : kTiles, kSlots = D == 64 ? (kOne ? 13 : 12) : D == 128 && kOne ? 6 : 5;
   // columns of tensor memory: two places for scores and the weights over them (one for each row tile, or for every other
   // tile of keys), then the accumulators
   static constexpr int kColO = 2 * kKeys, kStepO = D;
@@ -101,7 +102,7 @@ struct Cfg {
   // behind the slots: barriers, two work entries, what threads exchange
   static constexpr int kAtWork = (kBars * 8 + 15) / 16 * 16, kAtFlags = kAtWork + 160, kAtUp = kAtFlags + 16,
                        kAtSwap = kAtUp + 2 * kMaxNodes, kSmall = kAtSwap + 2 * kRowsTile * 4;
-  static constexpr int kSmem = kTiles * kQBytes + kSlots * kSlotBytes + kSmall;
+  static constexpr int kSmem = kQTiles * kQBytes + kSlots * kSlotBytes + kSmall;
   static_assert(kSmem <= 232448, "more shared memory than a CTA has");
 };
 
@@ -304,8 +305,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int D = C::D, kKeys = C::kKeys;
   constexpr bool kF16 = C::kF16;
   extern __shared__ __align__(1024) uint8_t smem[];
-  const uint32_t q_base = smem_u32(smem), ring = q_base + C::kTiles * C::kQBytes;
-  uint8_t* small = smem + C::kTiles * C::kQBytes + C::kSlots * C::kSlotBytes;
+  const uint32_t q_base = smem_u32(smem), ring = q_base + C::kQTiles * C::kQBytes;
+  uint8_t* small = smem + C::kQTiles * C::kQBytes + C::kSlots * C::kSlotBytes;
   const uint32_t bars = smem_u32(small);
   auto bar = [&](int i) { return bars + 8 * i; };
   Work* work = reinterpret_cast<Work*>(small + C::kAtWork);  // [2]
@@ -700,7 +701,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(bar(C::kWEmpty + e));
         if (n == 0) break;
         if (!(ok = wait_for(bar(C::kQFull), piece & 1, abort_s))) break;
-        const bool both = C::kTiles == 2 && !pair;  // two row tiles to each tile of keys
+        const bool both = C::kQTiles == 2 && !pair;  // two row tiles to each tile of keys
         const int jobs = both ? 2 * n : n;
         int j = 0;  // tile of keys of job i
 #pragma unroll 1
@@ -788,7 +789,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!(ok = wait_for(bar(slot), phase, abort_s))) break;
           const int k = k0 + i, c = (k < sink_tiles ? k : first + (k - sink_tiles)) * kKeys;
           if (!seen_all.all_of_tile(c, a.sink)) {
-            uint4* v = reinterpret_cast<uint4*>(smem + C::kTiles * C::kQBytes + slot * C::kSlotBytes);
+            uint4* v = reinterpret_cast<uint4*>(smem + C::kQTiles * C::kQBytes + slot * C::kSlotBytes);
             constexpr int kAll = C::kSlotBytes / 16 / 64;  // vectors a lane
             uint4* mine = v + part * 32 + lane;
             if (c + kKeys > end || (c < from && c + kKeys > a.sink)) {
@@ -1341,7 +1342,7 @@ static int launch(const asterq_rows_attention_params* p, Args& a, int workers, i
   a.box_rows = C::kKeys;
   while (a.page_tokens % a.box_rows) a.box_rows /= 2;
   a.tile_tokens = kRowsTile / a.group;
-  a.unit_tokens = C::kTiles * a.tile_tokens;
+  a.unit_tokens = C::kQTiles * a.tile_tokens;
   CUtensorMap q_map, k_map, v_map;
   const cuuint64_t q_dims[3] = {(cuuint64_t)C::D, (cuuint64_t)a.n_heads, (cuuint64_t)a.n_rows};
   const cuuint64_t q_strides[2] = {(cuuint64_t)p->q_head_stride * 2, (cuuint64_t)p->q_row_stride * 2};
@@ -1381,9 +1382,21 @@ static int launch(const asterq_rows_attention_params* p, Args& a, int workers, i
   return check_launch("rows_attention");
 }
 
+// Units of one row tile where sequences have no more rows than that on average, and where there are units enough to be bound by
+// memory.  32 trees of 16 nodes of 4 heads (64 rows) of 8 kv heads: 93 us with two, 90 with one, whose sixth slot of 32 KB has more
+// loads under way; one tree of 8 of 4 kv heads 19.0 and 19.8.  24 trees of 61 nodes of 16 heads (976 rows): 295 with two, 357 with
+// one, as each tile of keys and values is then read by twice as many units.
+template <bool kF16, int D, bool kPre>
+static int by_rows(const asterq_rows_attention_params* p, Args& a, int workers, int dev, cudaStream_t s) {
+  if constexpr (D != 256) {
+    if ((int64_t)p->n_seqs * p->n_kv_heads >= workers && p->n_rows <= (int64_t)p->n_seqs * (kRowsTile / a.group))
+      return launch<Cfg<kF16, D, kPre, true>>(p, a, workers, dev, s);
+  }
+  return launch<Cfg<kF16, D, kPre, false>>(p, a, workers, dev, s);
+}
 template <bool kF16, int D>
 static int by_scale(const asterq_rows_attention_params* p, Args& a, bool pre, int workers, int dev, cudaStream_t s) {
-  return pre ? launch<Cfg<kF16, D, true>>(p, a, workers, dev, s) : launch<Cfg<kF16, D, false>>(p, a, workers, dev, s);
+  return pre ? by_rows<kF16, D, true>(p, a, workers, dev, s) : by_rows<kF16, D, false>(p, a, workers, dev, s);
 }
 
 static int check(const asterq_rows_attention_params* p) {
