@@ -746,7 +746,8 @@ class PagedKVBatch:
         sink, page = min(self.sink_tokens, self.window_size), self.page_tokens
         for s in self.active():
             first = -(-sink // page)
-            last = min(max(0, int(self._length[s]) - self._reach() + 1) // page, self._held[s])  # tokens below it are passed
+            # tokens below it are passed; the next token's own page is not, also where a window shows nothing but the sink
+            last = min(max(0, int(self._length[s]) - max(self._reach(), 1) + 1) // page, self._held[s])
             if last <= first:
                 continue
             pages = self._table[s, first:last]
@@ -792,17 +793,25 @@ class PagedKVBatch:
         if (want > self.max_tokens).any():
             raise ValueError(f"a sequence would pass {self.max_tokens} tokens")
         need = np.maximum(-(-want // self.page_tokens) - np.asarray(self._held), 0)
-        # entries that a slot is about to write into and that others hold too: the last of its holders keeps the page
-        shared, users = [], {}
+        # entries that a slot is about to write into: those that others hold too (the last of its holders keeps the page), and
+        # those without a page
+        shared, bare, users = [], [], {}
         for s in np.nonzero(new > 0)[0]:
             for at in range(int(self._length[s]) // self.page_tokens, min(self._held[s], -(-int(want[s]) // self.page_tokens))):
                 page = int(self._table[s, at])
+                if page < 0:
+                    bare.append((int(s), at))
+                    continue
                 left = users.get(page, int(self._users[page]))
                 if left > 1:
                     users[page] = left - 1
                     shared.append((int(s), at, page))
-        pages = self._free.alloc(int(need.sum()) + len(shared)) if need.any() or shared else []
+        wanted = int(need.sum()) + len(shared) + len(bare)
+        pages = self._free.alloc(wanted) if wanted else []
         self._users[pages] = 1
+        for s, at in bare:
+            self._table[s, at] = pages.pop()
+            self._dirty = True
         pairs = []
         for s, at, page in shared:
             self._users[page] -= 1

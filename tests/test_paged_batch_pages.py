@@ -1,0 +1,88 @@
+"""The pages that ``PagedKVBatch`` hands out, shares and gives up, by its host-side lists alone (no GPU needed): the device's
+tensors are stand-ins on the CPU, and a slot's tokens are where its table says."""
+from __future__ import annotations
+
+from types import SimpleNamespace
+
+import numpy as np
+import pytest
+import torch
+
+from asterq import paged_kv
+
+PAGE = 16
+
+
+@pytest.fixture
+def batch_of(monkeypatch):
+    def empty(n_pages, n_kv_heads, page_tokens, head_dim, *, dtype, device):
+        return SimpleNamespace(k=torch.empty(n_pages, n_kv_heads, page_tokens, head_dim, dtype=dtype),
+                               v=torch.empty(n_pages, n_kv_heads, page_tokens, head_dim, dtype=dtype))
+
+    monkeypatch.setattr(paged_kv.PagedKVPools, "empty", staticmethod(empty))
+    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda self: self)
+    copied = []
+    monkeypatch.setattr(paged_kv, "copy_kv_pages", lambda stack, pairs, status=None: copied.extend(pairs.tolist()))
+
+    def make(**kw):
+        kw = dict(max_seqs=3, max_tokens=200, page_tokens=PAGE, pool_pages=8) | kw
+        batch = paged_kv.PagedKVBatch(1, 1, 64, device="cpu", **kw)
+        batch.copied = copied
+        return batch
+
+    return make
+
+
+def _consistent(batch):
+    users = np.zeros(batch._users.size, int)
+    for s in range(batch.max_seqs):
+        pages = batch._table[s, : batch._held[s]]
+        assert (batch._table[s, batch._held[s] :] == -1).all()
+        pages = pages[pages >= 0]
+        assert len(set(pages.tolist())) == pages.size
+        users[pages] += 1
+    assert np.array_equal(users, batch._users)
+    assert sorted(batch._free.free) == np.nonzero(users == 0)[0].tolist()
+
+
+def _more(batch, slot, n):
+    """n more tokens of a slot; each of their places has a page that no other slot holds."""
+    at = batch.length(slot)
+    batch.begin_rows([slot], [n])
+    pages = batch._table[slot, at // PAGE : -(-(at + n) // PAGE)]
+    assert (pages >= 0).all(), f"places {at} to {at + n - 1} are in pages {pages}"
+    assert (batch._users[pages] == 1).all()
+    assert torch.equal(batch.page_table[slot], torch.from_numpy(batch._table[slot]))
+    batch.end_step()
+    _consistent(batch)
+
+
+@pytest.mark.parametrize("window,sink", [(4, 4), (16, 16), (3, 7), (1, 0), (2, 1), (5, 4)])
+@pytest.mark.parametrize("tokens", [15, 16, 17, 31, 32, 47, 63])
+def test_the_page_of_the_next_token_is_kept(batch_of, window, sink, tokens):
+    batch = batch_of(window_size=window, sink_tokens=sink)
+    a = batch.add_sequence()
+    _more(batch, a, tokens)
+    batch.release_behind_window()
+    _consistent(batch)
+    for n in (1, 1, 20):
+        _more(batch, a, n)
+        batch.release_behind_window()
+        _consistent(batch)
+
+
+def test_a_page_that_a_fork_holds_is_counted_for_its_holders_alone(batch_of):
+    batch = batch_of(window_size=4, sink_tokens=4, pool_pages=4)
+    a, c = batch.add_sequence(), batch.add_sequence()
+    _more(batch, a, 47)
+    _more(batch, c, 10)
+    d = batch.fork_sequence(c)
+    shared = int(batch._table[c, 0])
+    assert batch._users[shared] == 2 and shared == int(batch._table[d, 0])
+    batch.release_behind_window()
+    _more(batch, a, 1)
+    batch.remove_sequence(c)
+    _consistent(batch)
+    assert batch._users[shared] == 1 and shared not in batch._free.free
+
+
