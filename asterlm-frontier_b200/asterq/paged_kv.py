@@ -637,7 +637,6 @@ class PagedKVBatch:
         self._free = _PagePool(pool_pages)
         self._users = np.zeros(pool_pages, np.int32)  # slots that hold each page
         self._held = [0] * max_seqs  # entries of each slot's row of the table
-        self._passed = [0] * max_seqs  # tokens before this may have no page any more, but for the sink's
         self._length = np.full(max_seqs, -1, np.int32)
         self._table = np.full((max_seqs, self.max_pages), -1, np.int32)
         i32 = dict(dtype=torch.int32, device=self.device)
@@ -682,7 +681,6 @@ class PagedKVBatch:
         elif not 0 <= slot < self.max_seqs or self._length[slot] >= 0:
             raise ValueError(f"slot {slot} is not free")
         self._length[slot] = 0
-        self._passed[slot] = 0
         self._dirty = True
         return slot
 
@@ -693,7 +691,6 @@ class PagedKVBatch:
             raise ValueError(f"slot {slot} holds no sequence")
         self._drop(slot, 0)
         self._length[slot] = -1
-        self._passed[slot] = 0
 
     def _drop(self, slot: int, first: int) -> None:
         """The slot's pages from entry ``first`` on are not held by it any more."""
@@ -717,7 +714,6 @@ class PagedKVBatch:
         self._users[pages[pages >= 0]] += 1
         self._held[new] = n
         self._length[new] = self._length[slot]
-        self._passed[new] = self._passed[slot]
         return new
 
     def truncate_sequence(self, slot: int, tokens: int) -> None:
@@ -728,8 +724,10 @@ class PagedKVBatch:
             raise ValueError(f"slot {slot} holds no sequence")
         if not 0 <= tokens <= self._length[slot]:
             raise ValueError(f"slot {slot} has {self._length[slot]} tokens, not {tokens}")
-        if self._passed[slot] and tokens - self._reach() + 1 < self._passed[slot]:
-            raise ValueError(f"slot {slot}: a window behind {tokens} tokens needs pages that were given up")
+        if self.window_size is not None and self._reach() > 1:  # else nothing of the window is among them
+            first = max(0, tokens - self._reach() + 1)
+            if (self._table[slot, first // self.page_tokens : -(-tokens // self.page_tokens)] < 0).any():
+                raise ValueError(f"slot {slot}: a window behind {tokens} tokens needs pages that were given up")
         self._drop(slot, min(self._held[slot], -(-tokens // self.page_tokens)))
         self._length[slot] = tokens
 
@@ -758,7 +756,6 @@ class PagedKVBatch:
                 self._table[s, first:last] = -1
                 released += int(pages.size)
                 self._dirty = True
-            self._passed[s] = max(self._passed[s], last * page)
         return released
 
     def compact_pages(self) -> int:

@@ -86,3 +86,50 @@ def test_a_page_that_a_fork_holds_is_counted_for_its_holders_alone(batch_of):
     assert batch._users[shared] == 1 and shared not in batch._free.free
 
 
+@pytest.mark.parametrize("window,sink,tokens,to,fine", [
+    (40, 4, 120, 0, True),  # nothing is left that a window could show
+    (40, 4, 120, 16, True),  # all of it in the sink's page
+    (40, 4, 120, 17, False),  # token 16 has no page any more
+    (40, 4, 120, 114, False),  # its window begins at 79
+    (40, 4, 120, 115, True),
+    (40, 20, 120, 32, True),
+    (40, 20, 120, 33, False),
+    (4, 4, 63, 40, True),  # the sink alone is seen
+    (4, 4, 63, 0, True),
+    (1, 0, 63, 40, True),  # a token sees itself alone
+])
+def test_truncation_needs_what_the_window_shows(batch_of, window, sink, tokens, to, fine):
+    batch = batch_of(window_size=window, sink_tokens=sink, pool_pages=16)
+    a = batch.add_sequence()
+    _more(batch, a, tokens)
+    assert batch.release_behind_window() > 0
+    if not fine:
+        before = batch._table.copy()
+        with pytest.raises(ValueError):
+            batch.truncate_sequence(a, to)
+        assert batch.length(a) == tokens and np.array_equal(before, batch._table)
+        return
+    batch.truncate_sequence(a, to)
+    _consistent(batch)
+    assert batch.length(a) == to
+    _more(batch, a, 1)
+    _more(batch, a, 50)  # and on from there
+    batch.truncate_sequence(a, to + 51)
+    _consistent(batch)
+
+
+def test_truncation_behind_a_truncation(batch_of):
+    """What was given up before a truncation does not stand in the way of one behind it."""
+    batch = batch_of(window_size=40, sink_tokens=4, pool_pages=16)
+    a = batch.add_sequence()
+    _more(batch, a, 120)
+    batch.release_behind_window()
+    b = batch.fork_sequence(a)
+    batch.truncate_sequence(a, 16)
+    _more(batch, a, 60)
+    batch.truncate_sequence(a, 40)  # all of its pages are there
+    _consistent(batch)
+    with pytest.raises(ValueError):
+        batch.truncate_sequence(b, 40)
+    batch.truncate_sequence(b, 8)
+    _consistent(batch)
