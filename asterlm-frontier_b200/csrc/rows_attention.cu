@@ -157,7 +157,8 @@ ASTERQ_DEVICE Seq seq_of(const Args& a, int s, bool& bad, int& dead) {
 }
 
 // The key tiles of a unit: tile k of its list is keys [kKeys j, kKeys (j + 1)) with j = k below sink_tiles and
-// first + k - sink_tiles from there on.
+// first + k - sink_tiles from there on.  A node's key is at its number's place while it is seen by its position: where a window is
+// all sink, nodes at positions in the sink may have theirs behind its last tile.
 struct Span {
   int tok0, tokens, from, end, sink_tiles, first, tiles;
 };
@@ -172,11 +173,11 @@ ASTERQ_DEVICE Span span_of(const Args& a, const Seq& q, int block) {
   s.sink_tiles = 0;
   s.first = 0;
   if (a.window > 0) {
-    const int from = q.length + (a.parents ? 0 : s.tok0) - a.reach + 1;
+    const int from = q.length + (a.parents ? min(1 - a.reach, 0) : s.tok0 - a.reach + 1);
     if (from > 0) {
       s.from = from;
       s.sink_tiles = min((a.sink + kKeys - 1) / kKeys, last);
-      s.first = a.reach == 0 ? last : max(from / kKeys, s.sink_tiles);
+      s.first = a.reach == 0 && (!a.parents || q.length >= a.sink) ? last : max(from / kKeys, s.sink_tiles);
     }
   }
   s.tiles = s.sink_tiles + last - s.first;
