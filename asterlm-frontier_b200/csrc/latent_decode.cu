@@ -49,6 +49,7 @@
 
 #include "common.cuh"
 #include "asterq_internal.h"
+#include "launch.cuh"
 
 namespace asterq {
 namespace dec {
@@ -1958,22 +1959,6 @@ int validate(const asterq_decode_params* p) {
   return ASTERQ_OK;
 }
 
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  if (!fn) {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(ptr);
-  }
-  return fn;
-}
-
 // 2-D byte tensor [rows][row_bytes] read in boxes of [box_rows][128 B] with the
 // 128-byte swizzle.  With blocks > 1 the rows are blocks x 128 B and the map is 3-D
 // (128 B, rows, blocks): one box [blocks][box_rows][128 B] lands block-major, the layout
@@ -1982,7 +1967,7 @@ EncodeTiledFn encode_fn() {
 // that kind fail validation).
 int make_map(CUtensorMap* map, const void* base, int64_t rows, int row_bytes, int box_rows, const void* dummy,
              int dummy_row_bytes, int blocks = 1) {
-  EncodeTiledFn fn = encode_fn();
+  const EncodeTiled fn = encode_tiled();
   if (!fn) return set_error(ASTERQ_ERR_CUDA, "decode: cuTensorMapEncodeTiled unavailable");
   if (!base || rows <= 0) {
     base = dummy;

@@ -1,4 +1,4 @@
-// What the launches of the paged layers' kernels share on the host.
+// What the launches of kernels share on the host.
 #pragma once
 
 #include <cuda.h>
@@ -12,8 +12,12 @@ using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// cuTensorMapEncodeTiled, without linking to the driver's library; null where it is not there
+// cuTensorMapEncodeTiled, without linking to the driver's library; null where it is not there.  It needs a current context,
+// which a host thread has from its first call of the runtime that works on the device: this one, where the thread has made none.
 inline EncodeTiled encode_tiled() {
+  static thread_local bool bound = false;
+  int dev = 0;
+  if (!bound) bound = cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
   static const EncodeTiled fn = [] {
     void* ptr = nullptr;
     cudaDriverEntryPointQueryResult q;

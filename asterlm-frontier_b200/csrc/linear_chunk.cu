@@ -38,6 +38,7 @@
 // 128 a thread S would spill to local memory).
 #include <cuda.h>
 
+#include "launch.cuh"
 #include "linear.cuh"
 #include "tcgen05.cuh"
 
@@ -1114,25 +1115,9 @@ __global__ void __launch_bounds__(256) chain_kernel(const __grid_constant__ Args
   }
 }
 
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  if (!fn) {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(ptr);
-  }
-  return fn;
-}
-
 // rows of bf16 heads [n_rows][n_heads][dim] with any strides, read in boxes of 128 rows x 64 dims
 bool make_map(CUtensorMap* map, const void* base, const Args& a, int dim, long long row_stride, long long head_stride) {
-  EncodeTiledFn fn = encode_fn();
+  const EncodeTiled fn = encode_tiled();
   // outputs and states are read and written 32 bytes at a time
   if ((reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.state)) & 31) return false;
   if ((a.n_rows / kChunk + a.n_seqs) * a.n_heads > 0x7fffffff) return false;  // Walk counts in 32 bits

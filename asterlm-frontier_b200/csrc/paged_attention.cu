@@ -28,6 +28,7 @@
 
 #include "asterq_internal.h"
 #include "common.cuh"
+#include "launch.cuh"
 
 namespace asterq {
 namespace pat {
@@ -847,26 +848,10 @@ __global__ void __launch_bounds__(C::kThreads, 1)
   if (tid == 0 && ld_shared_volatile(&abort_s) && a.status) atomicMax(a.status, 2);
 }
 
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  if (!fn) {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(ptr);
-  }
-  return fn;
-}
-
 // [n_pages * n_kv_heads][page_tokens][D] 16-bit values, read in boxes of [D / 64][box_rows][64 dims] with the
 // 128-byte swizzle
 static int make_map(CUtensorMap* map, const void* base, const asterq_paged_attention_params* p, int box_rows) {
-  EncodeTiledFn fn = encode_fn();
+  const EncodeTiled fn = encode_tiled();
   if (!fn) return set_error(ASTERQ_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled unavailable");
   const cuuint64_t dims[4] = {64u, (cuuint64_t)p->page_tokens, (cuuint64_t)p->head_dim / 64,
                               (cuuint64_t)(p->n_pages > 0 ? p->n_pages * p->n_kv_heads : 1)};
