@@ -4,6 +4,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <mutex>
+
 #include "asterq_internal.h"
 
 namespace asterq {
@@ -38,6 +40,13 @@ inline bool map_of_16bit(CUtensorMap* map, const void* base, int rank, const cuu
   return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, rank, const_cast<void*>(base), dims, strides, box, step,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Held while a call makes launches that hand records to each other in its workspace: host threads that share a stream, and with it
+// a workspace, would otherwise put a launch of one call between those of another, which then joins the wrong records.
+inline std::mutex& launch_lock() {
+  static std::mutex lock;
+  return lock;
 }
 
 // SMs of the current device and its ordinal; 0 where there is none

@@ -1357,6 +1357,7 @@ static int launch(const asterq_rows_attention_params* p, Args& a, int workers, i
       !map_of_16bit(&k_map, pools ? p->k_pool : p->workspace, 4, dims, strides, box) ||
       !map_of_16bit(&v_map, pools ? p->v_pool : p->workspace, 4, dims, strides, box))
     return set_error(ASTERQ_ERR_CUDA, "rows_attention: tensor map encoding failed");
+  const std::lock_guard<std::mutex> guard(launch_lock());
   static unsigned long long configured = 0;  // one bit per device ordinal
   if (dev >= 64 || !(configured & (1ull << dev))) {
     cudaFuncAttributes f;
