@@ -1142,6 +1142,7 @@ int launch(const Args& a, int workers, int device, void* workspace, cudaStream_t
   if (!make_map(&q_map, a.q, a, kDk, a.q_row, a.q_head) || !make_map(&k_map, a.k, a, kDk, a.k_row, a.k_head) ||
       !make_map(&v_map, a.v, a, kDv, a.v_row, a.v_head) || (reinterpret_cast<uintptr_t>(workspace) & 31))
     return ASTERQ_ERR_UNSUPPORTED;
+  const std::lock_guard<std::mutex> guard(launch_lock());
   static unsigned long long configured = 0;  // one bit per device ordinal
   if (device >= 64 || !(configured & (1ull << device))) {
     cudaError_t e = cudaFuncSetAttribute(chunk_kernel<kDk, kDv, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
