@@ -34,6 +34,7 @@
 #include "asterq_internal.h"
 #include "common.cuh"
 #include "launch.cuh"
+#include "shares.h"
 #include "tcgen05.cuh"
 
 namespace asterq {
@@ -227,11 +228,6 @@ struct View {
 struct Start {
   int s, head, block, at;
 };
-
-// a b / d; in 32 bits where that holds it, since a 64-bit division takes some hundred cycles
-ASTERQ_DEVICE long long share_of(long long a, int b, long long d) {
-  return a < (1 << 22) && d < (1ll << 31) ? (long long)((uint32_t)a * (uint32_t)b / (uint32_t)d) : a * b / d;
-}
 
 // tanh x to a few 2^-23 of itself: below 0.9 Lambert's continued fraction x / (1 + x^2 / (3 + x^2 / (5 + x^2 / (7 + x^2 / 9))))
 // as a quotient, its error x^10 / 9.8e6 < 2^-24; from there on (e^2x - 1) / (e^2x + 1).
@@ -606,8 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_arrive(bar(C::kWFull + e));
             if (cut && k0 == 0) {
               // the pieces after this one are in the next CTAs' first slots
-              const long long u1 = x - at + kUnitCost + span.tiles;
-              desc.pieces = (int)(u1 < (1 << 22) ? (uint32_t)(u1 * W - 1) / (uint32_t)total : (u1 * W - 1) / total) - me + 1;
+              desc.pieces = shares_up_to(x - at + kUnitCost + span.tiles, W, total, me);
               desc.row0 = u.row0;
               desc.tokens = u.tokens;
               desc.head = head;
