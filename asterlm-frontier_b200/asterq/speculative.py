@@ -61,7 +61,7 @@ def verify_drafts(
     Returns kept int32 [rows] (a sequence's accepted nodes from its first row on, the root first, -1 behind them), n_kept int32
     [n_seqs] (the root counted) and next_token int32 [n_seqs].  status int32 [1]: set to 1 by a token outside the
     vocabulary (never accepted), a parent out of range (never reached), a distribution without a positive sum (next token
-    -1), offsets out of order or too many nodes (nothing is kept, next token -1).
+    -1), offsets out of order or too many nodes (nothing is kept, next token -1).  kept of rows of no sequence is not written.
     """
     quick = paged_kv._quick()
     if quick is not None:

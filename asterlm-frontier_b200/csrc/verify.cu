@@ -57,6 +57,51 @@ ASTERQ_DEVICE double warp_sum(double x) {
   return x;
 }
 
+// The offsets name no nodes that can be walked: out of order, out of range, or too many.
+ASTERQ_DEVICE bool refused(long long begin, long long end, long long n_rows) {
+  return begin < 0 || end < begin || end > n_rows || end - begin > kMaxNodes;
+}
+
+// Rows between the least and the greatest offset that no walked sequence has become -1, by the CTA of the first refused sequence;
+// the others' rows are written by their own CTAs, so none is written twice.  Taken = a bit a row of a window of 32 n_words rows.
+__device__ __noinline__ void clear_refused(const int* row_offsets, int* kept, long long n_rows, int s, int n_seqs, uint32_t* taken,
+                                           int n_words) {
+  const int tid = threadIdx.x;
+  bool later = false;
+  int least = 0x7fffffff, most = -0x7fffffff;
+  for (int t = tid; t < n_seqs; t += kThreads) {
+    const int begin = __ldg(row_offsets + t), end = __ldg(row_offsets + t + 1);
+    later = later || (t < s && refused(begin, end, n_rows));
+    least = min(least, min(begin, end));
+    most = max(most, max(begin, end));
+  }
+  if (__syncthreads_or(later)) return;
+  int* range = reinterpret_cast<int*>(taken);
+  if (tid == 0) {
+    range[0] = 0x7fffffff;
+    range[1] = -0x7fffffff;
+  }
+  __syncthreads();
+  atomicMin(range, least);
+  atomicMax(range + 1, most);
+  __syncthreads();
+  const long long from = max(0, range[0]), to = min(n_rows, (long long)range[1]);
+  for (long long w0 = from; w0 < to; w0 += 32ll * n_words) {
+    const long long w1 = min(to, w0 + 32ll * n_words);
+    __syncthreads();
+    for (int i = tid; i < n_words; i += kThreads) taken[i] = 0;
+    __syncthreads();
+    for (int t = tid; t < n_seqs; t += kThreads) {
+      const long long begin = __ldg(row_offsets + t), end = __ldg(row_offsets + t + 1);
+      if (refused(begin, end, n_rows)) continue;
+      for (long long r = max(begin, w0); r < min(end, w1); ++r) atomicOr(taken + (r - w0) / 32, 1u << ((r - w0) & 31));
+    }
+    __syncthreads();
+    for (long long r = w0 + tid; r < w1; r += kThreads)
+      if (!(taken[(r - w0) / 32] >> ((r - w0) & 31) & 1u)) kept[r] = -1;
+  }
+}
+
 template <int kType>
 __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const Args a) {
   cg::cluster_group cluster = cg::this_cluster();
@@ -69,7 +114,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const Args a) {
   __shared__ int gone_s[kMaxNodes];        // tokens rejected at cur, of drafts without probabilities
   __shared__ double warp_sums[kWarps], rank_sums[2][kMaxCluster];
   const long long begin = __ldg(a.row_offsets + s), end = __ldg(a.row_offsets + s + 1);
-  const bool bad = begin < 0 || end < begin || end > a.n_rows || end - begin > kMaxNodes;
+  const bool bad = refused(begin, end, a.n_rows);
   const int n = bad ? 0 : (int)(end - begin);
   if (n == 0) {  // the whole cluster
     if (rank == 0 && tid == 0) {
@@ -77,6 +122,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const Args a) {
       a.next_token[s] = -1;
       if (bad && a.status) atomicMax(a.status, 1);
     }
+    if (bad && rank == 0) clear_refused(a.row_offsets, a.kept, a.n_rows, s, gridDim.x / ranks, reinterpret_cast<uint32_t*>(mass_s), 2 * kMaxNodes);
     return;
   }
   // a CTA's shared memory may be written by others once it has begun: arrived at here, waited for before the first sum

@@ -546,7 +546,8 @@ int asterq_kv_copy_pages(const asterq_kv_copy_params* p, void* stream);
  * kept [n_rows]: the accepted nodes of each sequence from its first row on, the root first, then -1; n_kept [n_seqs]
  * their number, next_token [n_seqs].  A sequence without nodes has 0 and -1.  A token outside the vocabulary is never accepted,
  * a node whose parent is out of range is never reached, offsets out of order or too many nodes leave a sequence with 0
- * and -1, a row without a positive sum gives the next token -1: all with *status 1.
+ * and -1 (and -1 in those of its rows that no other sequence has), a row without a positive sum gives the next token -1: all
+ * with *status 1.  kept of rows of no sequence is not written.
  */
 typedef struct asterq_verify_params {
   int32_t dtype; /* of target and draft: ASTERQ_DTYPE_F32, _BF16 or _F16 */
