@@ -278,6 +278,8 @@ class RowsAttentionParams(ctypes.Structure):
         ("workspace", ctypes.c_void_p),
         ("workspace_bytes", ctypes.c_int64),
         ("status", ctypes.c_void_p),
+        ("n_active", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
     ]
 
 

@@ -389,12 +389,12 @@ def _rows_workspace(device: torch.device, stream: int) -> RowsAttentionWorkspace
 
 
 def _rows_attention(pools, page_table, lengths, row_offsets, parents, q, softmax_scale, logit_softcap, window_size,
-                    sink_tokens, out, return_lse, workspace, status):
+                    sink_tokens, out, return_lse, workspace, status, active_seqs):
     quick = _quick()
     if quick is not None and workspace is None and window_size != 0:
         done = quick.rows(pools.k, pools.v, page_table, lengths, row_offsets, parents, q,
                           1.0 / math.sqrt(pools.k.shape[3]) if softmax_scale is None else softmax_scale, logit_softcap or 0.0,
-                          window_size or 0, sink_tokens, out, return_lse, status)
+                          window_size or 0, sink_tokens, out, return_lse, status, active_seqs or 0)
         if done is not NotImplemented:
             return done
     if q.dim() != 3 or page_table.dim() != 2 or row_offsets.dim() != 1:
@@ -418,6 +418,8 @@ def _rows_attention(pools, page_table, lengths, row_offsets, parents, q, softmax
         raise ValueError("sink_tokens must not be negative")
     if window_size is not None and window_size <= 0:
         raise ValueError("window_size must be positive")
+    if active_seqs is not None and active_seqs < 0:
+        raise ValueError("active_seqs must not be negative")
     dtype = _DTYPES[q.dtype]
     out_dtype = dtype
     if out is None:
@@ -440,7 +442,7 @@ def _rows_attention(pools, page_table, lengths, row_offsets, parents, q, softmax
                          page_table.data_ptr(), lengths.data_ptr(), row_offsets.data_ptr(),
                          0 if parents is None else parents.data_ptr(), out.data_ptr(),
                          0 if lse is None else lse.data_ptr(), ws.buffer.data_ptr(), ws.nbytes,
-                         0 if status is None else status.data_ptr()),
+                         0 if status is None else status.data_ptr(), active_seqs or 0, 0),
               device, stream)
     return (out, lse) if return_lse else out
 
@@ -460,6 +462,7 @@ def paged_prompt_attention(
     return_lse: bool = False,
     workspace: RowsAttentionWorkspace | None = None,
     status: torch.Tensor | None = None,
+    active_seqs: int | None = None,
 ):
     """Attention of prompt chunks over their pages: out [rows, n_heads, head_dim], and with ``return_lse`` the scores'
     log-sum-exp, float32 [rows, n_heads], beside it.
@@ -472,9 +475,13 @@ def paged_prompt_attention(
     outputs are good to that rounding of the values, also float32 ones.  Rows of empty slots get zeros and a log-sum-exp
     of -inf; rows of no sequence are not written.  status int32 [1]: set to 1 when a needed page id was outside the pool,
     a row's place behind the table (it gets zeros), or offsets are out of order (nothing is written then).
+
+    ``active_seqs``: how many sequences have rows, where that is known.  It is for speed alone: the work is cut by
+    the average of rows a sequence, and idle slots beside a long prompt make that small.  Outputs of different cuts differ by the
+    rounding of float32 sums.
     """
     return _rows_attention(pools, page_table, lengths, row_offsets, None, q, softmax_scale, logit_softcap, window_size,
-                           sink_tokens, out, return_lse, workspace, status)
+                           sink_tokens, out, return_lse, workspace, status, active_seqs)
 
 
 def paged_tree_attention(
@@ -493,6 +500,7 @@ def paged_tree_attention(
     return_lse: bool = False,
     workspace: RowsAttentionWorkspace | None = None,
     status: torch.Tensor | None = None,
+    active_seqs: int | None = None,
 ):
     """Attention of trees of drafted tokens over their pages, one tree a sequence of at most 128 nodes.
 
@@ -506,7 +514,7 @@ def paged_tree_attention(
     if parents is None:
         raise ValueError("parents must be int32 [rows]")
     return _rows_attention(pools, page_table, lengths, row_offsets, parents, q, softmax_scale, logit_softcap, window_size,
-                           sink_tokens, out, return_lse, workspace, status)
+                           sink_tokens, out, return_lse, workspace, status, active_seqs)
 
 
 class PagedKVStack:
@@ -645,6 +653,7 @@ class PagedKVBatch:
         self._one_row = torch.arange(max_seqs + 1, **i32)  # a decode step's rows: row s is slot s
         self.row_offsets = self._one_row
         self._new = np.zeros(max_seqs, np.int32)
+        self._active_rows = 0  # slots that have rows in the open step
         self._new_dev = torch.zeros(max_seqs, **i32)
         self._open = False
         self._tree = False
@@ -832,6 +841,7 @@ class PagedKVBatch:
             self.row_offsets = torch.from_numpy(offsets).pin_memory().to(self.device, non_blocking=True)
         if not np.array_equal(new, self._new):
             self._new = new
+            self._active_rows = int(np.count_nonzero(new))
             self._new_dev.copy_(torch.from_numpy(new).pin_memory(), non_blocking=True)
         self._open = True
 
@@ -888,7 +898,8 @@ class PagedKVBatch:
         """Attention of the open prompt chunk's or drafted trees' rotated queries over layer ``layer`` with their own tokens."""
         if not self._open or self.row_offsets is self._one_row:
             raise RuntimeError("no rows are open: begin_rows or begin_tree first")
-        kw = dict(window_size=self.window_size, sink_tokens=self.sink_tokens, status=self.status, **kw)
+        kw = dict(window_size=self.window_size, sink_tokens=self.sink_tokens, status=self.status,
+                  active_seqs=self._active_rows, **kw)
         if self._tree:
             return paged_tree_attention(self.layers[layer], self.page_table, self.lengths, self.row_offsets, self.parents, q, **kw)
         return paged_prompt_attention(self.layers[layer], self.page_table, self.lengths, self.row_offsets, q, **kw)

@@ -1379,14 +1379,20 @@ static int launch(const asterq_rows_attention_params* p, Args& a, int workers, i
   return check_launch("rows_attention");
 }
 
-// Units of one row tile where sequences have no more rows than that on average, and where there are units enough to be bound by
-// memory.  32 trees of 16 nodes of 4 heads (64 rows) of 8 kv heads: 93 us with two, 90 with one, whose sixth slot of 32 KB has more
-// loads under way; one tree of 8 of 4 kv heads 19.0 and 19.8.  24 trees of 61 nodes of 16 heads (976 rows): 295 with two, 357 with
-// one, as each tile of keys and values is then read by twice as many units.
+// Units of one row tile where sequences have no more rows than that on average, and where there are units enough to be bound
+// by memory; the sixth slot of 32 KB has more loads under way then.  One and two row tiles a unit, 32 heads of 128 dims over 8 kv heads:
+// 32 trees of 16 nodes 123 and 130 us, 512 of them 636 and 718, 64 decode rows over 16,384 cached tokens 669 and 777, a chunk of
+// 1,900 tokens beside 63 decode rows over 4,096 each 329 and 430, 2,000 beside 255 860 and 1,263.  The average misses long rows among many
+// short ones over little cache (7,900 tokens beside 255 rows over 500: 895 and 711), as each tile of keys and values of the long one is then
+// read by twice as many units.
+// Idle sequences are left out of the average from four row tiles an SM on: one prompt beside 255 of them 43 and 47 us for 1,000
+// tokens, 83 and 82 for 2,000, 211 and 186 for 4,000, 642 and 551 for 8,000.
 template <bool kF16, int D, bool kPre>
 static int by_rows(const asterq_rows_attention_params* p, Args& a, int workers, int dev, cudaStream_t s) {
   if constexpr (D != 256) {
-    if ((int64_t)p->n_seqs * p->n_kv_heads >= workers && p->n_rows <= (int64_t)p->n_seqs * (kRowsTile / a.group))
+    const bool many = p->n_rows * p->n_heads > (int64_t)workers * 4 * kRowsTile;
+    const int64_t seqs = many && p->n_active > 0 && p->n_active < p->n_seqs ? p->n_active : p->n_seqs;
+    if (seqs * p->n_kv_heads >= workers && p->n_rows <= seqs * (kRowsTile / a.group))
       return launch<Cfg<kF16, D, kPre, true>>(p, a, workers, dev, s);
   }
   return launch<Cfg<kF16, D, kPre, false>>(p, a, workers, dev, s);
@@ -1399,7 +1405,7 @@ static int by_scale(const asterq_rows_attention_params* p, Args& a, bool pre, in
 static int check(const asterq_rows_attention_params* p) {
   if (!p) return set_error(ASTERQ_ERR_INVALID_ARGUMENT, "rows_attention: null parameters");
   if (p->n_seqs < 0 || p->n_rows < 0 || p->n_heads <= 0 || p->n_kv_heads <= 0 || p->n_heads % p->n_kv_heads ||
-      p->page_tokens <= 0 || p->max_pages < 0 || p->n_pages < 0 || p->window < 0 || p->sink < 0)
+      p->page_tokens <= 0 || p->max_pages < 0 || p->n_pages < 0 || p->window < 0 || p->sink < 0 || p->n_active < 0)
     return set_error(ASTERQ_ERR_INVALID_ARGUMENT, "rows_attention: bad sizes");
   if (p->dtype != ASTERQ_DTYPE_BF16 && p->dtype != ASTERQ_DTYPE_F16)
     return set_error(ASTERQ_ERR_UNSUPPORTED, "rows_attention: dtype %d: bf16 or f16", p->dtype);

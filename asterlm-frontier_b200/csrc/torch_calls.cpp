@@ -363,10 +363,11 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return THPVariable_Wrap(out);
 }
 
-// rows(k_pool, v_pool, page_table, lengths, row_offsets, parents, q, scale, softcap, window, sink, out, want_lse, status)
+// rows(k_pool, v_pool, page_table, lengths, row_offsets, parents, q, scale, softcap, window, sink, out, want_lse, status,
+//      active sequences)
 //   -> out, or (out, lse)
 PyObject* rows_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 14 || !g_rows) return pass();
+  if (n != 15 || !g_rows) return pass();
   const at::Tensor *kp = tensor(args[0]), *vp = tensor(args[1]), *table = tensor(args[2]), *lengths = tensor(args[3]),
                    *offsets = tensor(args[4]), *q = tensor(args[6]);
   if (!pools_ok(kp, vp) || !table || table->dim() != 2) return pass();
@@ -378,11 +379,12 @@ PyObject* rows_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       !ints(table, device, {n_seqs, max_pages}) || !ints(lengths, device, {n_seqs}) || !ints(offsets, device, {n_seqs + 1}) ||
       n_seqs > INT32_MAX || max_pages > INT32_MAX)
     return pass();
-  if (!PyFloat_CheckExact(args[7]) || !PyFloat_CheckExact(args[8]) || !PyLong_CheckExact(args[9]) || !PyLong_CheckExact(args[10]))
+  if (!PyFloat_CheckExact(args[7]) || !PyFloat_CheckExact(args[8]) || !PyLong_CheckExact(args[9]) || !PyLong_CheckExact(args[10]) ||
+      !PyLong_CheckExact(args[14]))
     return pass();
-  const long window = PyLong_AsLong(args[9]), sink = PyLong_AsLong(args[10]);
+  const long window = PyLong_AsLong(args[9]), sink = PyLong_AsLong(args[10]), active = PyLong_AsLong(args[14]);
   const int want_lse = PyObject_IsTrue(args[12]);
-  if (PyErr_Occurred() || window < 0 || sink < 0 || window > INT32_MAX || sink > INT32_MAX) {
+  if (PyErr_Occurred() || window < 0 || sink < 0 || window > INT32_MAX || sink > INT32_MAX || active < 0 || active > INT32_MAX) {
     PyErr_Clear();
     return pass();
   }
@@ -434,6 +436,7 @@ PyObject* rows_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   p.row_offsets = static_cast<const int32_t*>(offsets->data_ptr());
   p.out = out.data_ptr();
   p.lse = want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr;
+  p.n_active = (int32_t)active;
   p.workspace = ws->second.ptr;
   p.workspace_bytes = ws->second.bytes;
   if (g_rows(&p, reinterpret_cast<void*>(stream)) != ASTERQ_OK) return pass();

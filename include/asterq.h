@@ -641,6 +641,8 @@ int asterq_paged_attention(const asterq_paged_attention_params* p, void* stream)
  * Weights enter their product rounded once to dtype, softmax statistics and sums are fp32.  Infinities and NaN in keys and
  * values that a row does not see have no part in it; those it sees reach it as for asterq_paged_attention.
  * head_dim 64, 128 or 256; at most 128 query heads a kv head; page_tokens a multiple of 16; positive strides of q.
+ * n_active is for speed alone: how the work is cut goes by the average of rows a sequence, which idle slots make small beside
+ * a long prompt.  Outputs of different cuts differ by the rounding of fp32 sums.
  * workspace: asterq_rows_attention_workspace_bytes bytes, of any content, used within the call; calls that overlap on the
  * GPU need one each.
  */
@@ -672,6 +674,8 @@ typedef struct asterq_rows_attention_params {
   void* workspace;
   int64_t workspace_bytes;
   int32_t* status; /* may be NULL */
+  int32_t n_active; /* sequences that have rows, where the caller knows it (0: all may) */
+  int32_t reserved;
 } asterq_rows_attention_params;
 
 int64_t asterq_rows_attention_workspace_bytes(const asterq_rows_attention_params* p);

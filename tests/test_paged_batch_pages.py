@@ -133,3 +133,24 @@ def test_truncation_behind_a_truncation(batch_of):
         batch.truncate_sequence(b, 40)
     batch.truncate_sequence(b, 8)
     _consistent(batch)
+
+
+def test_attention_is_told_how_many_slots_have_rows(batch_of, monkeypatch):
+    """A long prompt beside idle slots is not to be cut as many short ones would be."""
+    told = []
+    monkeypatch.setattr(paged_kv, "paged_prompt_attention", lambda *args, **kw: told.append(kw["active_seqs"]))
+    monkeypatch.setattr(paged_kv, "paged_tree_attention", lambda *args, **kw: told.append(kw["active_seqs"]))
+    batch = batch_of(max_seqs=5, pool_pages=30)
+    slots = [batch.add_sequence() for _ in range(4)]
+    for rows in ([30], [30, 1, 1], [30, 0, 1], [30]):
+        batch.begin_rows(slots[: len(rows)], rows)
+        batch.attend_rows(0, torch.zeros(sum(rows), 1, 64))
+        batch.end_step()
+    batch.begin_tree(slots[1:3], [[-1, 0], [-1, 0, 0]])
+    batch.attend_rows(0, torch.zeros(5, 1, 64))
+    batch.abandon_step()
+    batch.begin_step()
+    batch.abandon_step()
+    batch.begin_rows(slots[:1], [7])
+    batch.attend_rows(0, torch.zeros(7, 1, 64))
+    assert told == [1, 3, 2, 1, 2, 1]
