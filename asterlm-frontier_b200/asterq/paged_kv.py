@@ -471,8 +471,8 @@ def paged_prompt_attention(
     sequence s's new tokens, whose keys and values ``append_kv`` has written and ``lengths`` does not count yet: token i
     has position ``lengths[s] + i`` and sees the positions up to its own.  With ``window_size`` it sees, of these, the
     first ``sink_tokens`` and the newest ``window_size - sink_tokens``.  Other arguments, types and values that are not
-    finite as for ``paged_attention``, but weights enter their product rounded once to the pools' type, so that
-    outputs are good to that rounding of the values, also float32 ones.  Rows of empty slots get zeros and a log-sum-exp
+    finite as for ``paged_attention``, but weights enter their product rounded once to the pools' type (float16: to zero below
+    2^-32 of the largest), so that outputs are good to that rounding of the values, also float32 ones.  Rows of empty slots get zeros and a log-sum-exp
     of -inf; rows of no sequence are not written.  status int32 [1]: set to 1 when a needed page id was outside the pool,
     a row's place behind the table (it gets zeros), or offsets are out of order (nothing is written then).
 

@@ -639,7 +639,8 @@ int asterq_paged_attention(const asterq_paged_attention_params* p, void* stream)
  * row (these with *status 1); rows of no sequence are not written.  Offsets that decrease or leave [0, n_rows], and trees of
  * too many nodes, leave the whole call undone with *status 1.
  * Weights enter their product rounded once to dtype, softmax statistics and sums are fp32.  Infinities and NaN in keys and
- * values that a row does not see have no part in it; those it sees reach it as for asterq_paged_attention.
+ * values that a row does not see have no part in it; those it sees reach it as for asterq_paged_attention, but in f16 a weight may count
+ * as zero from 2^-32 of the largest on.
  * head_dim 64, 128 or 256; at most 128 query heads a kv head; page_tokens a multiple of 16; positive strides of q.
  * n_active is for speed alone: how the work is cut goes by the average of rows a sequence, which idle slots make small beside
  * a long prompt.  Outputs of different cuts differ by the rounding of fp32 sums.
