@@ -7,12 +7,14 @@
 // p is the row's place behind the sequence's cached tokens, or positions[row] (a drafted node's place in the
 // pages goes by its number, its position by its depth).
 //
-// Bound by memory: 2 bytes in and 2 out a value, and some ten operations.  A head is held by the lanes of one
+// 2 bytes in and 2 out a value, and some ten operations.  A head is held by the lanes of one
 // group, 16 dims each (two 16-byte vectors whose pairs share eight cos and sin values), so its sum of squares
 // is a few shuffles; a group walks over heads, and CTAs over rows with the weights in shared memory (in registers, 112
 // of them a thread, 16,387 rows took 107 us instead of 84).
-// Measured: 16,387 rows of 32 + 8 + 8 heads of 128 dims, 407 MB in and out: 84 us, 4.84 TB/s (0.74 of the measured copy
-// bandwidth); 32 rows 6.2 us, a launch.
+// Measured: 16,387 rows of 32 + 8 + 8 heads of 128 dims (64 of them turned, interleaved), 407 MB in and out: 84 us, 4.84 TB/s (0.74 of
+// the measured copy bandwidth; the append without norms takes 72).  What bounds it is the pipe of shared memory and loads, busy 133,000 of an SM's
+// 157,000 cycles: lanes of a head read weights 32 or 64 bytes apart, and of 10.8 million accesses to shared memory 8.2 million are repeats for
+// bank conflicts.  32 rows 6.2 us, a launch.
 #include "asterq_internal.h"
 #include "common.cuh"
 #include "launch.cuh"

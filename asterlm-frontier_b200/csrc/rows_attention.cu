@@ -16,16 +16,19 @@
 // and values that TMA brings; a warpgroup takes each, thread t row t, so that maxima and sums need no shuffles, and one's
 // exponentials run under the other's products.  A unit of at most 128 rows has both warpgroups on the same rows and alternate
 // tiles of keys; they join at its end, through tensor memory.
-// S = Q K^T (128 x 128, fp32) lies in tensor memory, its weights as 16-bit values over it, O beside it.  The chain of a tile
+// S = Q K^T (128 x 128, fp32) lies in tensor memory, its weights as 16-bit values over it, O beside it.  Weights are rounded once for
+// their product (csrc/paged_attention.cu takes them in two parts): a second part would double these products, which with the scores' set the
+// pace of long prompts.  Against 64 bits the outputs are 2.1e-3 to 2.3e-3 of their norm off in bf16,
+// where exact sums rounded to bf16 are 1.7e-3, and 2.7e-4 to 2.9e-4 in f16, where those are 2.1e-4.  The chain of a tile
 // (softmax, then product and next scores, 1,024 cycles of the tensor cores, and two waits of some 300 until one side sees
 // the other) is what sets the pace; the weights are handed over in halves to shorten it.  (Tried and slower: a third place for
 // scores of 64 dims, tiles of 64 keys, sixteen softmax warps, a warp of products for each row tile, and a quarter of the
 // exponentials by a polynomial: 5 to 8 % longer, although the softmax alone is 8 % faster so.)
-// Measured, one sequence of 8,192 rows over 24,576 cached, 32 over 8 heads of 128 dims, bf16: 3.1 to 3.4 ms, 1.13 to 1.22 PFLOP/s by
-// the clock that the power limit leaves, 0.67 to 0.73 of the measured burst of matrix products.  9 prompts of 16,393 rows with a
-// window of 1,024 (16 over 8 heads of 64 dims, f16): 161 us, whose 268 million exponentials in whole tiles are 74.  32
-// trees of 16 nodes: 90 us, 4.1 TB/s.  One tree of 8 nodes 19 us, a prompt of 150 tokens 25: one pass through code that no SM has
-// run before, some 5,000 cycles of it until the first copies.
+// Measured, one sequence of 8,192 rows over 24,576 cached, 32 over 8 heads of 128 dims, bf16: 3.1 ms in the first calls, 3.55 to 3.65
+// call after call at the clock that the power limit leaves: 1.05 to 1.24 PFLOP/s, 0.63 to 0.74 of the measured burst of matrix products.  9 prompts
+// of 16,393 rows with a window of 1,024 (16 over 8 heads of 64 dims, f16): 161 us, whose 268 million exponentials in whole tiles are 74.  32
+// trees of 16 nodes: 90 to 104 us over machines, 3.6 to 4.1 TB/s; 24 trees of 61 nodes 290 to 335.  One tree of 8 nodes 19 to 25 us, a prompt of
+// 150 tokens 25 to 27: one pass through code that no SM has run before, some 5,000 cycles of it until the first copies, and the join.
 //
 // Split.  The key tiles of all units laid end to end (with kUnitCost in front of each) are cut into equal contiguous
 // shares, one for each CTA, by sums over lengths and offsets that every CTA does for itself: no planning launch, no

@@ -13,8 +13,9 @@
 // rejection behind which something follows, and to draw; the nodes' own values are gathered at once.  A cluster of CTAs shares a
 // sequence's vocabulary while sequences are few.  Sums are in 64 bits: a border between two tokens among 10^5 is hit
 // by the rounding of a 32-bit sum once in some hundred draws.
-// Measured: 96 trees of 12 over 128,256 tokens (float32) 62 to 77 us: passes of 1 MB a sequence, each of which waits for the decision
-// before it; 4 chains of 6 over 32,000 8.3 us, a launch and reads that wait for one another.
+// Measured: 96 trees of 12 over 128,256 tokens (float32) 62 to 77 us over machines, 80 to 87 a call on new inputs each time: passes of 1 MB a
+// sequence, each of which waits for the decision before it, by 384 CTAs on 296 places; 4 chains of 6 over 32,000 8.3 to 10.5 us, a launch and reads
+// that wait for one another.
 #include <cooperative_groups.h>
 
 #include "asterq_internal.h"
