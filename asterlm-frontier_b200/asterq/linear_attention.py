@@ -67,7 +67,7 @@ def _workspace(device: torch.device, stream: int) -> LinearAttentionWorkspace:
         ws = LinearAttentionWorkspace(device)
         if _capturing(device):
             return ws  # of the graph's own memory
-        _workspaces[(device.index, stream)] = ws
+        ws = _workspaces.setdefault((device.index, stream), ws)  # another host thread's may have come first
     if _quick() is not None:  # whose calls come here until it knows the workspace
         _quick().workspace(1, device.index, stream, ws.buffer.data_ptr(), ws.nbytes)
     return ws

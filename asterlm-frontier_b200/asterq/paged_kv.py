@@ -113,7 +113,7 @@ def _workspace(device: torch.device, stream: int) -> PagedAttentionWorkspace:
         ws = PagedAttentionWorkspace(device)
         if _capturing(device):
             return ws  # of the graph's own memory and zeroed when the graph runs: not for any call but this one
-        _workspaces[(device.index, stream)] = ws
+        ws = _workspaces.setdefault((device.index, stream), ws)  # another host thread's may have come first
     if _quick() is not None:  # whose calls come here until it knows the workspace
         _quick().workspace(0, device.index, stream, ws.buffer.data_ptr(), ws.nbytes)
     return ws
@@ -382,7 +382,8 @@ def _rows_workspace(device: torch.device, stream: int) -> RowsAttentionWorkspace
         return RowsAttentionWorkspace(device)  # of the graph's own memory: graphs may run beside each other and other calls
     ws = _rows_workspaces.get((device.index, stream))
     if ws is None:
-        ws = _rows_workspaces[(device.index, stream)] = RowsAttentionWorkspace(device)
+        # another host thread's may have come first
+        ws = _rows_workspaces.setdefault((device.index, stream), RowsAttentionWorkspace(device))
     if _quick() is not None:  # whose calls come here until it knows the workspace
         _quick().workspace(2, device.index, stream, ws.buffer.data_ptr(), ws.nbytes)
     return ws
